@@ -27,6 +27,7 @@ NP_DTYPE = {"i8": np.int8, "i16": np.int16, "i32": np.int32}
 ITEMSIZE = {"i8": 1, "i16": 2, "i32": 4}
 
 _ERRORS = {1: ValueError, 2: OverflowError, 3: ZeroDivisionError, 4: RuntimeError}
+_CACHE_ERRORS = {5: MemoryError}              # ANVIL_E_MEMORY: a cache without a free page, which the reference has not
 
 # anvil_gemm_i8_ex flags (include/anvil_mi355x.h)
 GEMM_UNCHECKED, GEMM_CAUSAL_SKIP, GEMM_CAUSAL_K, GEMM_MUL24, GEMM_SPLITK = 1, 2, 4, 8, 16
@@ -86,6 +87,13 @@ SIGNATURES = {
     "anvil_copy_strided": [_p, _p, _p, _i, _i, _p, _p],
     "anvil_quantize": [_p, _p, _i, _f64, _i64, _p, _i],
     "anvil_embed_quantize": [_p, _p, _i64, _i, _i, _p, _i, _p, _f64, _p, _i],
+    "anvil_cache_bytes": [_i, _i, _i, _i, C.POINTER(C.c_longlong)],
+    "anvil_cache_append_i4": [_p, _p, _i, _p, _p, _p, _i, _i, _p],
+    "anvil_cache_read_i4": [_p, _p, _i, _p, _p, _p, _i, _i, _p],
+    "anvil_attention_cache_i4": [_p, _p, _i, _p, _p, _p, _i, _i, _i, _p, _i32, _i, _p, _i32, _i32, _i, _i, _i],
+    "anvil_cache_fork": [_p, _p, _p, _p, _p, _i, _i],
+    "anvil_cache_compact": [_p, _p, _p, _p],
+    "anvil_beam_select_i8": [_p, _p],
 }
 
 
@@ -108,6 +116,32 @@ class RowOp(C.Structure):
     _fields_ = [(f, _i32) for f in ("kind", "a", "b", "dst", "n", "k", "table", "m24", "wide", "wide_a", "wide_b", "trans",
                                     "mult", "mult2", "shift", "c", "e", "lut_len")] + [
         ("in", _p), ("lut", _p), ("out", _p), ("ld", _i64), ("kb", _i64)]
+
+
+CACHE_PAGE = 64                              # tokens of a cache page
+
+
+class Cache(C.Structure):
+    """anvil_cache: a pool of 4-bit key and value pages and the tables of a batch of sequences in it (device pointers, which
+    the caller keeps alive)."""
+    _fields_ = [("pool", _p), ("table", _p), ("lens", _p), ("refs", _p), ("seqs", _i32), ("slots", _i32),
+                ("pages", _i32), ("heads", _i32), ("dim", _i32), ("layers", _i32)]
+
+    def __init__(self, pool, table, lens, refs=0, *, seqs, slots, pages, heads, dim, layers=1):
+        super().__init__(_ptr(pool), _ptr(table), _ptr(lens), _ptr(refs) or None, seqs, slots, pages, heads, dim, layers)
+
+    def with_tables(self, table, lens, refs=0, seqs=None) -> "Cache":
+        """The same pool with other tables (what anvil_cache_fork and anvil_cache_compact write)."""
+        return Cache(self.pool, table, lens, refs, seqs=self.seqs if seqs is None else seqs, slots=self.slots,
+                     pages=self.pages, heads=self.heads, dim=self.dim, layers=self.layers)
+
+
+class Beams(C.Structure):
+    """anvil_beams: the arguments of one anvil_beam_select_i8 call."""
+    _fields_ = [("logits", _p), ("ld", _i64), ("scores", _p), ("ended", _p), ("allowed", _p), ("groups", _i32),
+                ("beams", _i32), ("vocab", _i32), ("keep", _i32), ("eos", _i32), ("lut", _p), ("logs", _p),
+                ("nlogs", _i32), ("step", _i32), ("mult", _i32), ("scores_out", _p), ("parent", _p), ("token", _p),
+                ("ended_out", _p)]
 
 
 ROW_LOAD, ROW_NORM, ROW_GEMM, ROW_ADD, ROW_LUT, ROW_LUT_MUL = 1, 2, 3, 4, 5, 6
@@ -136,7 +170,7 @@ class Library:
         rc = getattr(self.cdll, name)(*args)
         if rc:
             msg = self.last_error().decode(errors="replace")
-            raise _ERRORS.get(rc, RuntimeError)(f"{name}: {msg}")
+            raise {**_ERRORS, **_CACHE_ERRORS}.get(rc, RuntimeError)(f"{name}: {msg}")
         return rc
 
 
@@ -151,6 +185,11 @@ def library() -> Library:
 
 def _ptr(x) -> int:
     return x.ptr if isinstance(x, DeviceBuffer) else int(x)
+
+
+def _opt(x):
+    """A pointer argument that may be None."""
+    return None if x is None else _ptr(x)
 
 
 class DeviceBuffer:
@@ -478,6 +517,38 @@ class Device:
         self.lib.call("anvil_embed_quantize", self.ctx, C.c_void_p(_ptr(ids)), int(rows), int(T), int(Cdim),
                       C.c_void_p(_ptr(wte)), int(vocab), C.c_void_p(_ptr(wpe)), float(scale), C.c_void_p(_ptr(out)),
                       DTYPE_CODE[out_dtype])
+
+    # ------------------------------------------------------------------------------------------ decoding
+    def cache_append(self, cache, layer, K, V, starts, rows, max_new, strides):
+        """anvil_cache_append_i4: int8 K and V rows of new tokens into their pages; strides (k row, k head, v row, v head)."""
+        self.lib.call("anvil_cache_append_i4", self.ctx, C.byref(cache), layer, _opt(K), _opt(V), _opt(starts), rows,
+                      max_new, (C.c_int64 * 4)(*strides))
+
+    def cache_read(self, cache, layer, K, V, starts, rows, max_new, strides):
+        """anvil_cache_read_i4: the values that the cache holds for those rows."""
+        self.lib.call("anvil_cache_read_i4", self.ctx, C.byref(cache), layer, _opt(K), _opt(V), _opt(starts), rows,
+                      max_new, (C.c_int64 * 4)(*strides))
+
+    def attention_cache(self, cache, layer, Q, O, starts, rows, max_new, heads, strides, ms, ss, lut, one, mo, so, window=0,
+                        sinks=0):
+        """anvil_attention_cache_i4: the newest tokens' queries over the cache; strides (q row, q head, o row, o head)."""
+        self.lib.call("anvil_attention_cache_i4", self.ctx, C.byref(cache), layer, _opt(Q), _opt(O), _opt(starts), rows,
+                      max_new, heads, (C.c_int64 * 4)(*strides), ms, ss, _opt(lut), one, mo, so, window, sinks)
+
+    def cache_fork(self, cache, out, parent=None, add=None, window=0, sinks=0):
+        """anvil_cache_fork: the tables of the next step into `out`'s."""
+        self.lib.call("anvil_cache_fork", self.ctx, C.byref(cache), C.byref(out), _opt(parent), _opt(add), window, sinks)
+
+    def cache_compact(self, cache, out, moved):
+        """anvil_cache_compact: used pages to the lowest ids; `moved` (pages int32) receives each page's new id."""
+        self.lib.call("anvil_cache_compact", self.ctx, C.byref(cache), C.byref(out), _opt(moved))
+
+    def beam_select(self, logits, ld, scores, ended, allowed, groups, beams, vocab, keep, eos, lut, logs, nlogs, step,
+                    mult, scores_out, parent, token, ended_out):
+        """anvil_beam_select_i8: the best `keep` continuations of each group of beams."""
+        b = Beams(_ptr(logits), ld, _ptr(scores), _opt(ended), _opt(allowed), groups, beams, vocab, keep, eos, _ptr(lut),
+                  _ptr(logs), nlogs, step, mult, _ptr(scores_out), _ptr(parent), _ptr(token), _ptr(ended_out))
+        self.lib.call("anvil_beam_select_i8", self.ctx, C.byref(b))
 
 
 _devices = {}

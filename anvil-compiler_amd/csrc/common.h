@@ -21,6 +21,8 @@ enum : unsigned {
   FLAG_ZERODIV = 4u,    // softmax row sum 0                       -> ZeroDivisionError
   FLAG_RANGE = 8u,      // an operand outside its dtype            -> ValueError
   FLAG_NONFINITE = 16u, // a float input NaN or infinite           -> ValueError
+  FLAG_PAGES = 32u,     // a cache had too few free pages          -> MemoryError
+  FLAG_CACHE = 64u,     // a cache's table, length or start outside its range -> ValueError
 };
 
 constexpr int EVENT_SLOTS = 512;
@@ -39,6 +41,10 @@ struct anvil_ctx {
   long long ws_elems = 0;
   std::vector<int*> ws_retired;
   unsigned* host_flags = nullptr; // page-locked word the flags are fetched into
+  // workspace of the decoding ops, with the same rules; what a call leaves in it no later call reads
+  char* decode_ws = nullptr;
+  size_t decode_ws_bytes = 0;
+  std::vector<char*> decode_ws_retired;
 };
 
 namespace anvil {
@@ -46,6 +52,8 @@ namespace anvil {
 int set_error(int code, const char* fmt, ...);
 int hip_fail(hipError_t e, const char* what);
 int check_ctx(anvil_ctx* ctx);
+// the context's decoding workspace, of at least `bytes` (256-byte aligned)
+int decode_workspace(anvil_ctx* ctx, size_t bytes, char** ptr);
 // zero `bytes` of device memory with a fill kernel on stream s (no memset node: safe inside a captured graph)
 int zero_fill(hipStream_t s, void* dst, size_t bytes);
 // once per device, with that device current: the device address of the GEMM's static split-K scratch

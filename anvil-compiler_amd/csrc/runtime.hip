@@ -183,6 +183,28 @@ int zero_fill(hipStream_t s, void* dst, size_t bytes) {
   return ANVIL_OK;
 }
 
+// Doubled as it grows, so that a cache that gets longer step by step outgrows few buffers.
+int decode_workspace(anvil_ctx* ctx, size_t bytes, char** ptr) {
+  if (ctx->decode_ws_bytes < bytes) {
+    size_t want = 1 << 20;
+    while (want < bytes) want *= 2;
+    char* p = nullptr;
+    ANVIL_HIP(hipMalloc((void**)&p, want));
+    if (ctx->decode_ws) {
+      try {
+        ctx->decode_ws_retired.push_back(ctx->decode_ws);
+      } catch (const std::bad_alloc&) {
+        hipFree(p);
+        return set_error(ANVIL_E_RUNTIME, "out of memory");
+      }
+    }
+    ctx->decode_ws = p;
+    ctx->decode_ws_bytes = want;
+  }
+  *ptr = ctx->decode_ws;
+  return ANVIL_OK;
+}
+
 }  // namespace anvil
 
 using namespace anvil;
@@ -219,10 +241,12 @@ static int report_flags(anvil_ctx* ctx, bool nonfinite_first) {
   ANVIL_HIP(hipMemset(ctx->flags, 0, sizeof(unsigned)));
   const char* nonfinite = "a float input holds NaN or infinite values";
   if (nonfinite_first && (flags & FLAG_NONFINITE)) return set_error(ANVIL_E_VALUE, "%s", nonfinite);
+  if (flags & FLAG_PAGES) return set_error(ANVIL_E_MEMORY, "a cache has too few free pages or slots for its new tokens");
   if (flags & FLAG_OVERFLOW) return set_error(ANVIL_E_OVERFLOW, "an int32 intermediate overflowed on the device");
   if (flags & FLAG_ZERODIV) return set_error(ANVIL_E_ZERODIV, "a softmax row summed to zero");
   if (flags & FLAG_SHIFT) return set_error(ANVIL_E_VALUE, "an rmsnorm shift s + k left [0, 31]");
   if (flags & FLAG_NONFINITE) return set_error(ANVIL_E_VALUE, "%s", nonfinite);
+  if (flags & FLAG_CACHE) return set_error(ANVIL_E_VALUE, "a cache's page table, lengths, starts or parents leave their range");
   return set_error(ANVIL_E_VALUE, "an operand left its dtype range on the device (flags %u)", flags);
 }
 
@@ -277,6 +301,8 @@ int anvil_destroy(anvil_ctx* ctx) {
   if (ctx->host_flags) hipHostFree(ctx->host_flags);
   if (ctx->ws) hipFree(ctx->ws);
   for (int* w : ctx->ws_retired) hipFree(w);
+  if (ctx->decode_ws) hipFree(ctx->decode_ws);
+  for (char* w : ctx->decode_ws_retired) hipFree(w);
   if (ctx->stream) {
     record_drop(ctx->stream);
     hipStreamDestroy(ctx->stream);

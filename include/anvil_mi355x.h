@@ -33,6 +33,7 @@ enum anvil_status {
   ANVIL_E_OVERFLOW = 2,   /* an int32 intermediate left int32: Python OverflowError                */
   ANVIL_E_ZERODIV = 3,    /* a softmax row summed to zero: Python ZeroDivisionError                */
   ANVIL_E_RUNTIME = 4,    /* HIP runtime failure: Python RuntimeError                              */
+  ANVIL_E_MEMORY = 5,     /* a cache has no free page left: Python MemoryError                     */
 };
 
 enum anvil_dtype { ANVIL_I8 = 1, ANVIL_I16 = 2, ANVIL_I32 = 4 };
@@ -387,6 +388,111 @@ int anvil_quantize(anvil_ctx* ctx, const void* x, int x_is_f64, double scale, in
  * anvil_sync as ANVIL_E_VALUE. */
 int anvil_embed_quantize(anvil_ctx* ctx, const int64_t* ids, int64_t rows, int T, int C, const float* wte, int vocab,
                          const float* wpe, double scale, void* out, int out_dtype);
+
+/* ---------------------------------------------------------------------------------------------- decoding */
+/* Token-by-token evaluation. The reference evaluates a whole sequence at once (anvil/interp/graph.py:43-92); these take
+ * the rows of new tokens only and hold the keys and values of the earlier ones in a paged cache of 4-bit codes.
+ *
+ * Rows of new tokens. K, V, Q and O hold the new tokens of every sequence, packed: sequence s owns rows starts[s] ..
+ * starts[s + 1] - 1 (starts: seqs + 1 device int32s, at most `rows` and non-decreasing, at most max_new rows each; NULL:
+ * one row a sequence, rows = seqs and max_new = 1). Row starts[s] + t is the token at position lens[s] - n_s + t: lens
+ * counts the new tokens already (anvil_cache_fork extends it). Rows behind the last sequence's are neither read nor
+ * written. strides are in elements (bytes); one head's channels are contiguous.
+ *
+ * The cache. A page holds ANVIL_CACHE_PAGE tokens of every head, and a pool of `layers` x `pages` pages holds layer l's
+ * page p at byte (l * pages + p) * heads * 68 D, D the head dim (16 is stored as 32 with zero channels). The table's row s names
+ * the page of each 64 tokens of sequence s (-1: none, its tokens are seen by no query). refs counts each page's table
+ * entries (and whatever else the caller holds it by); 0 is free. One head's 68 D bytes of a page, channels in D / 32
+ * groups of 32, NG = D / 32, t the token in the page:
+ *   K codes  64 rows of D / 2 bytes; byte 4 (q NG + g) + i holds channels 32 g + 8 q + i (low four bits) and 32 g + 8 q + 4 + i
+ *            (high), q, i in 0..3 (one dword is eight consecutive channels, a lane's dwords of all groups are adjacent)
+ *   K steps  byte ((t / 4) NG + g) 4 + t % 4
+ *   V codes  byte (16 g + i) 64 + t: channels 32 g + i (low) and 32 g + 16 + i (high), i in 0..15 (a channel's 64 tokens)
+ *   V steps  byte 64 g + t
+ * A group x of 32 channels is held as step = clamp(ceil(max|x| / 7), 1, 18) and signed codes
+ * clamp(floor((2 x + step) / (2 step)), -7, 7); it stands for code x step, an int8. An entry of the table, a length or a start
+ * outside its range is reported by anvil_sync as ANVIL_E_VALUE: its page is not seen, its sequence not evaluated. */
+enum { ANVIL_CACHE_PAGE = 64, ANVIL_CACHE_SLOTS_MAX = 16384, ANVIL_CACHE_ROWS_MAX = 4096 };
+typedef struct anvil_cache {
+  void* pool;                       /* 16-byte aligned */
+  int32_t* table;                   /* seqs x slots */
+  int32_t* lens;                    /* seqs: tokens, at most 64 slots */
+  int32_t* refs;                    /* pages; NULL where only attention, append and read use the cache */
+  int32_t seqs, slots, pages, heads, dim, layers;
+} anvil_cache;
+
+/* The bytes of a pool: layers x pages x heads x 68 D. */
+int anvil_cache_bytes(int layers, int pages, int heads, int dim, long long* bytes);
+
+/* New K and V rows rounded to 4 bits into their pages of one layer. strides = {k row, k head, v row, v head}, multiples
+ * of 16 as are K and V; the pages written belong to their sequence alone (as anvil_cache_fork leaves them). */
+int anvil_cache_append_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, const int8_t* K, const int8_t* V,
+                          const int32_t* starts, int rows, int max_new, const int64_t* strides);
+/* The values that the cache holds for the same rows (append's inverse, up to its rounding; with lens / starts that cover
+ * whole sequences, the whole cache). strides = {k row, k head, v row, v head}, multiples of 16 as are K and V. */
+int anvil_cache_read_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, int8_t* K, int8_t* V, const int32_t* starts,
+                        int rows, int max_new, const int64_t* strides);
+
+/* The attention chain of anvil_attention_i8 (reference anvil/semantics.py:95-103 around the softmax of
+ * anvil/lower/graph_to_tensor.py:352-398) for the rows of new tokens over the cache. Query head h reads cache head
+ * h / (heads_q / cache->heads). The query at position i sees key j iff j <= i and (window = 0, or j > i - window, or j < sinks):
+ *   x_j = clamp_i8((Q . K_j * m_s + 2^(s_s-1)) >> s_s);  m = max x_j;  e_j = lut[x_j - m + 255];  S = sum e_j
+ *   p_j = (e_j * one + S / 2) / S;   O = clamp_i8((sum_j p_j V_j * m_o + 2^(s_o-1)) >> s_o)
+ * S and the products with e_j, one and m_o are held in 64 bits. 1 <= one <= 32767: above 127 the probabilities of a long
+ * context keep more than int8's 7 bits. lut: int32[256], entries below 0 count as 0. A row that sees no key yields
+ * the requantized 0; a row whose S is 0 yields that too and ANVIL_E_ZERODIV at anvil_sync. |m_s| is limited so that
+ * every Q . K_j * m_s + 2^(s_s-1) fits int32 (128 * 126 * D * |m_s| + 2^(s_s-1) < 2^31), else ANVIL_E_OVERFLOW.
+ * strides = {q row, q head, o row, o head}: Q and its strides multiples of 16, O and its strides of 4, o strides >= D. */
+int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, const int8_t* Q, int8_t* O,
+                             const int32_t* starts, int rows, int max_new, int heads_q, const int64_t* strides,
+                             int32_t m_s, int s_s, const int32_t* lut, int32_t one, int32_t m_o, int s_o, int window,
+                             int sinks);
+
+/* Page tables of the next step: row i of `out` continues row parent[i] of `in` (parent NULL: row i; -1: an empty row) by
+ * add[i] >= 0 tokens (add NULL: none). `out` shares in's pool and has its slots; its table, lens and refs are other
+ * memory (in's stay as they are, so that a step can be taken back until its pages are written). Both have at most
+ * ANVIL_CACHE_ROWS_MAX rows. In this order:
+ *   1. the row keeps its parent's pages; with window > 0 not those that no query from its end on sees (every key of
+ *      theirs >= sinks and <= lens - window), whose entries become -1;
+ *   2. refs counts out's entries in place of in's, so pages that no row keeps are free;
+ *   3. row by row, a row that extends into a page which is shared (refs > 1) gets a copy of it in its place (all layers, its
+ *      refs dropping by one: the last row to extend a page nothing else holds keeps it), then its new pages; each is the
+ *      lowest free page, and refs of a new page is 1.
+ * When too few pages are free, or a row would need more than `slots`, every row of `out` is left empty, refs as in `in`, and
+ * anvil_sync returns ANVIL_E_MEMORY. Reserve: parent NULL. Free: parent -1. Fork, beam search's reordering: parent. */
+int anvil_cache_fork(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* out, const int32_t* parent,
+                     const int32_t* add, int window, int sinks);
+/* The used pages (refs > 0) of a pool moved to its lowest ids: with n pages used, the i-th used page of id >= n moves to
+ * the i-th free id below n, all layers. out's table and refs say so (lens is copied), and map[p] is page p's new id, -1
+ * for a free one. out shares in's pool, rows and slots; its table, lens and refs are other memory. */
+int anvil_cache_compact(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* out, int32_t* map);
+
+/* Beam search's selection. Rows groups x beams of int8 logits (row stride ld >= vocab) with their scores (fixed-point log
+ * probabilities so far, INT64_MIN: no beam). With m a row's largest logit, S = sum_v lut[x_v - m + 255] (lut as the softmax's,
+ * int32[256], entries below 0 count as 0) and L(v) = logs[v >> k] + k * step, k the fewest halvings that bring v below
+ * nlogs (v in 64 bits):
+ *   candidate (row, v) = scores[row] + (x_v - m) * mult - (L(S) - L(lut[255]))
+ * A row with ended[row] != 0 (ended NULL: none) has one candidate, the token eos at its score. allowed (vocab bytes, NULL:
+ * all) excludes tokens whose byte is 0 from the candidates, not from S. The best `keep` candidates of each group, by score
+ * descending, then row, then token: score, parent = the row (in groups x beams: what anvil_cache_fork takes), token, and
+ * ended (the row's, or token = eos). Where there are fewer, INT64_MIN, -1, -1, 0. 1 <= beams, keep <= 64; mult >= 1;
+ * nlogs >= 2; eos = -1: none. A row whose S or lut[255] is below 1 has no candidates, and ANVIL_E_ZERODIV is reported. */
+typedef struct anvil_beams {
+  const int8_t* logits;
+  int64_t ld;
+  const int64_t* scores;            /* groups x beams */
+  const uint8_t* ended;             /* groups x beams, or NULL */
+  const uint8_t* allowed;           /* vocab, or NULL */
+  int32_t groups, beams, vocab, keep, eos;
+  const int32_t* lut;
+  const int32_t* logs;
+  int32_t nlogs, step, mult;
+  int64_t* scores_out;              /* groups x keep, as are the next three */
+  int32_t* parent;
+  int32_t* token;
+  uint8_t* ended_out;
+} anvil_beams;
+int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b);
 
 #ifdef __cplusplus
 }
