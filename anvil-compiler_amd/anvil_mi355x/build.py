@@ -23,8 +23,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
           "-packed-fp32-ops", "-Wno-unused-command-line-argument", f"-I{INCLUDE}"]
 # Per-source flags. attention.hip: MFMA accumulators in VGPRs. Its score tiles feed VALU requant code right after
-# each MFMA, and with the accumulators in AGPRs every value would first need a v_accvgpr_read.
-FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# each MFMA, and with the accumulators in AGPRs every value would first need a v_accvgpr_read. cache_attention.hip: the
+# same.
+FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "cache_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def sources():

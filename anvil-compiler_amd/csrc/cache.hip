@@ -10,7 +10,7 @@ int check_cache(const char* who, const anvil_cache* c, bool refs) {
   if (c->dim != 16 && c->dim != 32 && c->dim != 64 && c->dim != 128)
     return set_error(ANVIL_E_VALUE, "%s: head dim %d is not 16, 32, 64 or 128", who, c->dim);
   if (c->seqs < 0 || c->seqs > 65535 || c->slots < 1 || c->slots > ANVIL_CACHE_SLOTS_MAX || c->pages < 1 ||
-      c->pages > (1 << 24) || c->heads < 1 || c->heads > 65535 || c->layers < 1 || c->layers > 65535)
+      c->pages > (1 << 24) || c->heads < 1 || c->heads > 4096 || c->layers < 1 || c->layers > 65535)
     return set_error(ANVIL_E_VALUE, "%s: %d sequences of %d slots, %d pages of %d heads, %d layers", who, c->seqs,
                      c->slots, c->pages, c->heads, c->layers);
   if (!c->pool || (uintptr_t)c->pool % 16) return set_error(ANVIL_E_VALUE, "%s: the pool is null or not 16-byte aligned", who);
@@ -473,7 +473,7 @@ int anvil_cache_bytes(int layers, int pages, int heads, int dim, long long* byte
   *bytes = 0;
   if (dim != 16 && dim != 32 && dim != 64 && dim != 128)
     return set_error(ANVIL_E_VALUE, "anvil_cache_bytes: head dim %d is not 16, 32, 64 or 128", dim);
-  if (layers < 1 || layers > 65535 || pages < 1 || pages > (1 << 24) || heads < 1 || heads > 65535)
+  if (layers < 1 || layers > 65535 || pages < 1 || pages > (1 << 24) || heads < 1 || heads > 4096)
     return set_error(ANVIL_E_VALUE, "anvil_cache_bytes: %d layers of %d pages of %d heads", layers, pages, heads);
   *bytes = (long long)layers * pages * heads * 2176 * groups_of(dim);
   return ANVIL_OK;
