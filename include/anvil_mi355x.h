@@ -475,8 +475,8 @@ int anvil_cache_compact(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache
  * A row with ended[row] != 0 (ended NULL: none) has one candidate, the token eos at its score. allowed (vocab bytes, NULL:
  * all) excludes tokens whose byte is 0 from the candidates, not from S. The best `keep` candidates of each group, by score
  * descending, then row, then token: score, parent = the row (in groups x beams: what anvil_cache_fork takes), token, and
- * ended (the row's, or token = eos). Where there are fewer, INT64_MIN, -1, -1, 0. 1 <= beams, keep <= 64; mult >= 1;
- * nlogs >= 2; eos = -1: none. A row whose S or lut[255] is below 1 has no candidates, and ANVIL_E_ZERODIV is reported. */
+ * ended (the row's, or token = eos). Where there are fewer, INT64_MIN, -1, -1, 0. 1 <= beams, keep <= 64; vocab
+ * at most 2^28; mult >= 1; nlogs >= 2; eos = -1: none. A row whose S or lut[255] is below 1 has no candidates, and ANVIL_E_ZERODIV is reported. */
 typedef struct anvil_beams {
   const int8_t* logits;
   int64_t ld;
