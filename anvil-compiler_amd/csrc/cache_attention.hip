@@ -5,14 +5,16 @@
 // value follow exactly. So a row is evaluated in two passes: its scores (one byte a key, kept) with their histogram, then a
 // 256-entry table of probabilities and the sum of p V, looked up by score. K is read once, V once.
 //
-// Tiles. 16 rows share a pass over a cache head's keys: the query heads of its group, for one token or several. 64 keys (a page)
-// are one step of a wave:
-//   scores  v_mfma_i32_16x16x32_i8 for each 16 keys and group of 32 channels: keys x channels codes (their four bits in a byte's
-//           upper half, so that no sign has to be extended: 16 x the product), channels x rows queries; times the key's step
-//   values  v_mfma_i32_16x16x64_i8 for each 16 channels: channels x keys codes, keys x rows of p x step, which takes 12 to 20
-//           bits and goes through as two or three 7-bit digits
-// The operand row of key 16 q + 4 k + i in the k-th product is 4 q + i, so lane (row, q) receives the scores of keys 16 q .. 16 q + 15
-// in order, which are the keys whose p it supplies to the second product: a lane reads back what it wrote, without a barrier.
+// Tiles. Up to 16 rows share a pass over a cache head's keys: the query heads of its group, for one token or several. 64 keys (a
+// page) are one step of a wave:
+//   scores  keys x channels codes (their four bits in a byte's upper half, so that no sign has to be extended: 16 x the product)
+//           times channels x columns queries, 16 keys a product; each group of 32 channels times the key's step of that group
+//   values  channels x keys codes times keys x columns of p x step, whose 12 to 20 bits go through as 7-bit digits
+// A product has 16 columns. With RP = 4 or 8 row slots the 16 / RP columns of a row are put to use: for the scores each takes
+// groups of its own (zeros elsewhere), which are summed across them after the steps; for the values each takes a digit. So the
+// instructions around the products, which are what bounds the kernel, are shared out over the lanes.
+// The operand rows are ordered so that the lanes of (row, q) receive the scores of keys 16 q .. 16 q + 15 in order, which are the keys
+// whose p they supply to the second product: a wave reads back what it wrote.
 #include <algorithm>
 
 #include "cache.h"
@@ -32,10 +34,10 @@ struct AttendArgs {
   int* sums;                                             //            [unit][tile][split][row][32 NG], 16 x sum p V
 };
 
-constexpr int WAVES = 4, ATTEND_THREADS = 64 * WAVES;
 constexpr int HIST = 257;                                // dwords of a row's histogram in LDS: rows start in different banks
 
-constexpr int ONE_TWO_DIGITS = ((1 << 14) - 1) / STEP_MAX;   // 910: p x step below 2^14
+constexpr int ONE_NARROW = ((1 << 14) - 1) / STEP_MAX;   // 910: p x step is two 7-bit digits
+constexpr int ONE_FIFTEEN = 7 * (1 + 15 + 225 + 3375);   // 25312: four digits of base 15
 
 typedef unsigned short __attribute__((may_alias)) u16_alias;
 
@@ -52,6 +54,8 @@ __device__ __forceinline__ bool find_tile(const CacheView& c, const AttendArgs& 
   t.seq = a.seq0 + t.unit / c.heads, t.head = t.unit % c.heads;
   const int first = (a.tile0 + t.tile) * 16;
   new_rows(c, t.seq, t.r, first == 0 && blockIdx.z == 0 && t.head == 0 && threadIdx.x == 0);
+  t.r.first = __builtin_amdgcn_readfirstlane(t.r.first), t.r.n = __builtin_amdgcn_readfirstlane(t.r.n);   // the same in every lane
+  t.r.len = __builtin_amdgcn_readfirstlane(t.r.len);
   const long long all = (long long)t.r.n * a.group;
   if (first >= all) return false;
   t.rows = (int)min(16ll, all - first);
@@ -65,6 +69,17 @@ __device__ __forceinline__ bool find_tile(const CacheView& c, const AttendArgs& 
 
 __device__ __forceinline__ int slot_of(const Tile& t, int page) {
   return page < t.sink_pages ? page : t.window_page + page - t.sink_pages;
+}
+
+// The table's entry of a page, -1 where it names none. An entry out of range is reported.
+__device__ __forceinline__ int entry_of(const CacheView& c, const Tile& t, int page, int end) {
+  int entry = -1;
+  if (page < end) entry = c.table[(long long)t.seq * c.slots + slot_of(t, page)];
+  if (entry >= c.pages || entry < -1) {
+    raise_flag(c.flags, FLAG_CACHE);
+    entry = -1;
+  }
+  return entry;
 }
 
 // whether every row of the tile sees every key of a page
@@ -94,46 +109,70 @@ template <int N>
 struct Words {
   unsigned w[N];
 };
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 template <int N>
-__device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
+__device__ __forceinline__ Words<N> load_words(__amdgpu_buffer_rsrc_t blk, int at) {
   Words<N> r;
   if constexpr (N == 1) {
-    r.w[0] = *(const unsigned*)p;
+    r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(blk, at, 0, 0);
   } else if constexpr (N == 2) {
-    const uint2 v = *(const uint2*)p;
+    const u2 v = __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(blk, at, 0, 0));
     r.w[0] = v.x, r.w[1] = v.y;
   } else {
-    const uint4 v = *(const uint4*)p;
+    const u4 v = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(blk, at, 0, 0));
     r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
   }
   return r;
 }
 
-// A lane's part of a page's keys: of 16 keys in each of four products the four bits of 8 channels a group, and the steps of the
-// four keys whose scores it receives.
-template <int NG>
+// How a product's 16 columns are shared out: VN columns a row, of which GV hold different groups (NA groups each).
+template <int NG, int RP>
+struct Columns {
+  static constexpr int VN = 16 / RP, GV = VN < NG ? VN : NG, NA = NG / GV, NE = 4 / VN;
+};
+
+// A lane's part of a page's keys: of 16 keys in each of four products the four bits of 8 channels a group, and the steps (of the
+// lane's groups) of the 16 keys whose sums it receives.
+template <int NG, int RP>
 struct KeyPage {
-  Words<NG> code[4], step[4];
-  __device__ __forceinline__ void load(const uint8_t* blk, int lane) {
+  using C = Columns<NG, RP>;
+  Words<NG> code[4];
+  Words<C::NA> step[4];                                  // [i]: keys 16 q + 4 i .. + 3
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t blk, int lane) {
     const int row = lane & 15, q = lane >> 4;
+    const int codes = key_of(row, 0) * Block<NG>::ROW + 4 * q * NG, steps = Block<NG>::K_STEPS + 16 * q * NG + 4 * (row % C::GV);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      code[k] = load_words<NG>(blk + Block<NG>::K + (16 * (row >> 2) + 4 * k + (row & 3)) * Block<NG>::ROW + 4 * q * NG);
-      step[k] = load_words<NG>(blk + Block<NG>::K_STEPS + (4 * q + k) * 4 * NG);
+    for (int k = 0; k < 4; ++k) code[k] = load_words<NG>(blk, codes + k * key_of(0, 1) * Block<NG>::ROW);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (C::GV == 1) {
+        step[e] = load_words<C::NA>(blk, steps + 4 * NG * e);
+      } else {
+#pragma unroll
+        for (int n = 0; n < C::NA; ++n) step[e].w[n] = load_words<1>(blk, steps + 4 * NG * e + 4 * C::GV * n).w[0];
+      }
     }
+  }
+  // the key of operand row `row` in product k. Sum e of product k (operand row 4 q + e) is that of key 16 q + 4 e + k, so that a lane
+  // that keeps one e has four keys in a row; with a column a row, which keeps all, 16 q + 4 k + e: whole cache lines a load.
+  static __device__ __forceinline__ int key_of(int row, int k) { return C::VN > 1 ? 4 * row + k : 16 * (row >> 2) + 4 * k + (row & 3); }
+  __device__ __forceinline__ int step_of(int n, int e, int k) const {
+    return (int)(C::VN > 1 ? (step[e].w[n] >> (8 * k)) & 255u : (step[k].w[n] >> (8 * e)) & 255u);
   }
 };
 
 // A lane's part of a page's values: 16 keys of two channels a group, and their steps.
 template <int NG>
 struct ValuePage {
-  uint4 code[NG], step[NG];
-  __device__ __forceinline__ void load(const uint8_t* blk, int lane) {
+  Words<4> code[NG], step[NG];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t blk, int lane) {
     const int row = lane & 15, q = lane >> 4;
+    const int codes = Block<NG>::V + row * PAGE + 16 * q, steps = Block<NG>::V_STEPS + 16 * q;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      code[g] = *(const uint4*)(blk + Block<NG>::V + (16 * g + row) * PAGE + 16 * q);
-      step[g] = *(const uint4*)(blk + Block<NG>::V_STEPS + PAGE * g + 16 * q);
+      code[g] = load_words<4>(blk, codes + 16 * PAGE * g);
+      step[g] = load_words<4>(blk, steps + PAGE * g);
     }
   }
 };
@@ -148,81 +187,214 @@ struct Requant {
   }
 };
 
-// The lane's 16 scores of a page, a byte each, + 128. The products hold 16 x code: their sum is divided exactly.
-template <int NG>
-__device__ __forceinline__ uint4 score_page(const KeyPage<NG>& k, const long (&q)[NG], const Requant& rq) {
-  unsigned out[4];
+// The query operand: the lane's column holds row column / VN; lane quarter q channels 8 q .. 8 q + 7 of each group that is the
+// column's, zeros for the others (one group a product with VN = 1, two otherwise).
+template <int NG, int RP>
+struct Query {
+  long w[NG];
+  __device__ __forceinline__ void load(const CacheView& c, const AttendArgs& a, const Tile& t, int lane) {
+    using C = Columns<NG, RP>;
+    const int col = lane & 15, row = col / C::VN, r = (a.tile0 + t.tile) * 16 + row, ch = 8 * (lane >> 4);
+    const int8_t* p = a.q + (long long)(t.r.first + r / a.group) * a.q_row + (long long)(t.head * a.group + r % a.group) * a.q_head + ch;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      w[g] = row < t.rows && 32 * g + ch < c.dim && (C::GV == 1 || col % C::GV == g % C::GV) ? *(const long*)(p + 32 * g) : 0;
+  }
+};
+
+// v of lane ^ 1 or lane ^ 2
+template <int X>
+__device__ __forceinline__ int lane_xor(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, X == 1 ? 0xB1 : 0x4E, 0xF, 0xF, false);
+}
+
+// The lane's scores of a page, a byte each, + 128: dword i holds keys 16 q + 4 e + 0..3 with e = NE v + i, v the lane's column of its
+// row. The products hold 16 x code: their sum is divided exactly.
+template <int NG, int RP>
+__device__ __forceinline__ Words<Columns<NG, RP>::NE> score_page(const KeyPage<NG, RP>& k, const Query<NG, RP>& q, const Requant& rq) {
+  using C = Columns<NG, RP>;
+  const int v = threadIdx.x % C::VN;
+  int x[C::NE][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    int acc[4];
+    v4i d[C::NA];
+    if constexpr (NG == 1 || C::VN == 1) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const unsigned w = k.code[i].w[g], st = k.step[i].w[g];
-      const unsigned long low = (w << 4) & 0xF0F0F0F0u, high = w & 0xF0F0F0F0u;
-      const v4i d = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)(high << 32 | low), q[g], v4i{0, 0, 0, 0}, 0, 0, 0);
+      for (int g = 0; g < NG; ++g) {
+        const unsigned long low = (k.code[i].w[g] << 4) & 0xF0F0F0F0u, high = k.code[i].w[g] & 0xF0F0F0F0u;
+        d[g] = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)(high << 32 | low), q.w[g], v4i{0, 0, 0, 0}, 0, 0, 0);
+      }
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int part = __mul24(d[e], (int)((st >> (8 * e)) & 255u));
-        acc[e] = g ? acc[e] + part : part;
+      for (int g = 0; g < NG; g += 2) {
+        const unsigned w0 = k.code[i].w[g], w1 = k.code[i].w[g + 1];
+        const v4i keys = {(int)((w0 << 4) & 0xF0F0F0F0u), (int)(w0 & 0xF0F0F0F0u), (int)((w1 << 4) & 0xF0F0F0F0u), (int)(w1 & 0xF0F0F0F0u)};
+        const v4i rows = {(int)q.w[g], (int)(q.w[g] >> 32), (int)q.w[g + 1], (int)(q.w[g + 1] >> 32)};
+        const bool again = C::GV == 4 && g > 0;          // four columns of a group each: one sum for both products
+        d[g / C::GV] = __builtin_amdgcn_mfma_i32_16x16x64_i8(keys, rows, again ? d[0] : v4i{0, 0, 0, 0}, 0, 0, 0);
       }
     }
-    int x[4];
+    int acc[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = med3i(__mul24(acc[e] >> 4, rq.m) + rq.rnd, rq.lo, rq.hi);
-    out[i] = sra_pack4(x[0], x[1], x[2], x[3], rq.s) ^ 0x80808080u;
+    for (int e = 0; e < 4; ++e) {
+      acc[e] = 0;
+#pragma unroll
+      for (int n = 0; n < C::NA; ++n) acc[e] += __mul24(d[n][e], k.step_of(n, e, i));
+    }
+    // the sum over the row's columns; each keeps its NE of the four keys
+    if constexpr (C::VN == 4) {
+      int a0, a1;
+      if constexpr (C::GV == 4) {
+        a0 = (v & 2 ? acc[2] : acc[0]) + lane_xor<2>(v & 2 ? acc[0] : acc[2]);
+        a1 = (v & 2 ? acc[3] : acc[1]) + lane_xor<2>(v & 2 ? acc[1] : acc[3]);
+      } else {
+        a0 = v & 2 ? acc[2] : acc[0];
+        a1 = v & 2 ? acc[3] : acc[1];
+      }
+      acc[0] = C::GV == 1 ? (v & 1 ? a1 : a0) : (v & 1 ? a1 : a0) + lane_xor<1>(v & 1 ? a0 : a1);
+    } else if constexpr (C::VN == 2) {
+      const int a0 = v ? acc[2] : acc[0], a1 = v ? acc[3] : acc[1];
+      if constexpr (C::GV == 2) {
+        const int b0 = v ? acc[0] : acc[2], b1 = v ? acc[1] : acc[3];
+        acc[0] = a0 + lane_xor<1>(b0), acc[1] = a1 + lane_xor<1>(b1);
+      } else {
+        acc[0] = a0, acc[1] = a1;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < C::NE; ++n) {
+      const int v = med3i(__mul24(acc[n] >> 4, rq.m) + rq.rnd, rq.lo, rq.hi);
+      if constexpr (C::VN > 1) x[n][i] = v;
+      else x[i][n] = v;
+    }
   }
-  return {out[0], out[1], out[2], out[3]};
+  Words<C::NE> out;
+#pragma unroll
+  for (int n = 0; n < C::NE; ++n) out.w[n] = sra_pack4(x[n][0], x[n][1], x[n][2], x[n][3], rq.s) ^ 0x80808080u;
+  return out;
 }
 
 __device__ __forceinline__ unsigned word(const uint4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
-// The scores of a page into the row's histogram.
-__device__ __forceinline__ void count_scores(unsigned* hist, const uint4& sc, unsigned mask) {
+// The scores of a page into the row's histogram: all of them, or with a mask, a bit a key.
+template <int N>
+__device__ __forceinline__ void count_scores(unsigned* hist, const Words<N>& sc) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (mask >> i & 1u) atomicAdd(&hist[(word(sc, i >> 2) >> (8 * (i & 3))) & 255u], 1u);
+  for (int i = 0; i < 4 * N; ++i) atomicAdd(&hist[(sc.w[i >> 2] >> (8 * (i & 3))) & 255u], 1u);
+}
+template <int N>
+__device__ __forceinline__ void count_scores(unsigned* hist, const Words<N>& sc, unsigned mask) {
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i)
+    if (mask >> i & 1u) atomicAdd(&hist[(sc.w[i >> 2] >> (8 * (i & 3))) & 255u], 1u);
 }
 
-// acc[digit][16 channels] += digits of p x step times 16 x code over a page. The table holds 2 p, so that bit 0 of 2 p x step is 0
-// and the low 7-bit digit is its low byte halved. Two digits (p <= 910): below 2^15, two keys a 16-bit packed product. Three:
-// 24-bit products below 2^21.
-template <int NG, int ND>
-__device__ __forceinline__ void add_page(const ValuePage<NG>& v, const uint4& sc, const u16_alias* table, unsigned mask,
-                                         v4i (&acc)[ND][2 * NG]) {
-  unsigned p[8];                                         // 2 p of two keys each
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const unsigned w = word(sc, j >> 1) >> (16 * (j & 1));
-    p[j] = table[w & 255u] | (unsigned)table[(w >> 8) & 255u] << 16;
+// Digits. With four columns a row, p as four digits of base 15 from -7 to 7 (p <= 25312), a column and a table of bytes each: a digit
+// times a step (at most 18) is an int8 as it stands. Else a table entry is 2 p, or 2 (p & 127) and 2 (p >> 7) in two tables (WIDE).
+// Its product with a step is below 2^15 (p <= 910, 127 or 255), so two keys are one 16-bit packed product, whose low byte halved is
+// the low 7-bit digit of p x step (bit 0 is 0) and whose high byte the high one.
+//   RP  4        columns: digits of base 15
+//   RP  8        columns: low and high digit of p x step
+//   RP  8 WIDE   columns: p & 127, p >> 7; a product each for the low and the high digit
+//   RP 16        a product each for the low and the high digit of p x step
+//   RP 16 WIDE   products for both digits of p & 127 and of p >> 7, the middle two into one sum
+enum { TABLE_P = 1, TABLE_SEVEN = 2, TABLE_FIFTEEN = 4 };
+template <int RP, bool WIDE>
+struct Digits {
+  static constexpr int TABLE = RP == 4 ? TABLE_FIFTEEN : (RP == 8 && WIDE ? TABLE_SEVEN : TABLE_P);   // RP 16 takes 2 p apart itself
+  static constexpr int SUMS = RP == 16 ? (WIDE ? 3 : 2) : (RP == 8 && WIDE ? 2 : 1);
+  // the weight of a column's sum n
+  static __device__ __forceinline__ unsigned weight(int v, int n) {
+    if constexpr (RP == 4) return v == 0 ? 1u : (v == 1 ? 15u : (v == 2 ? 225u : 3375u));
+    else if constexpr (RP == 8 && !WIDE) return 1u << (7 * v);
+    else if constexpr (RP == 8) return 1u << (7 * (v + n));
+    else return 1u << (7 * n);
   }
-  if (mask != 0xFFFFu) {
+};
+// byte B of d = a x byte B of st
+template <int B>
+__device__ __forceinline__ void mul_to_byte(unsigned& d, int a, unsigned st) {
+  if constexpr (B == 0)
+    asm("v_mul_i32_i24_sdwa %0, %1, %2 dst_sel:BYTE_0 dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0"
+        : "=v"(d) : "v"(a), "v"(st));
+  else if constexpr (B == 1)
+    asm("v_mul_i32_i24_sdwa %0, %1, %2 dst_sel:BYTE_1 dst_unused:UNUSED_PRESERVE src0_sel:DWORD src1_sel:BYTE_1"
+        : "+v"(d) : "v"(a), "v"(st));
+  else if constexpr (B == 2)
+    asm("v_mul_i32_i24_sdwa %0, %1, %2 dst_sel:BYTE_2 dst_unused:UNUSED_PRESERVE src0_sel:DWORD src1_sel:BYTE_2"
+        : "+v"(d) : "v"(a), "v"(st));
+  else
+    asm("v_mul_i32_i24_sdwa %0, %1, %2 dst_sel:BYTE_3 dst_unused:UNUSED_PRESERVE src0_sel:DWORD src1_sel:BYTE_3"
+        : "+v"(d) : "v"(a), "v"(st));
+}
+typedef unsigned short v2u __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned mul_pair(unsigned a, unsigned b) {
+  return __builtin_bit_cast(unsigned, (v2u)(__builtin_bit_cast(v2u, a) * __builtin_bit_cast(v2u, b)));
+}
+
+// acc += digits of p x step times 16 x code over a page, for the 16 keys of the lane's quarter: sc their scores, a bit of mask a key
+// (`all`: every key, for every lane).
+template <int NG, int RP, bool WIDE>
+__device__ __forceinline__ void add_page(const ValuePage<NG>& v, const uint4& sc, const uint8_t* table, bool all, unsigned mask,
+                                         v4i (&acc)[Digits<RP, WIDE>::SUMS][2 * NG]) {
+  int one[RP == 4 ? 16 : 1];                             // a key's digit
+  unsigned p[8];                                         // or the table entries of two keys each
+  if constexpr (RP == 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] &= (mask >> (2 * j) & 1u ? 0xFFFFu : 0u) | (mask >> (2 * j + 1) & 1u ? 0xFFFF0000u : 0u);
+    for (int i = 0; i < 16; ++i) one[i] = (int8_t)table[(word(sc, i >> 2) >> (8 * (i & 3))) & 255u];
+    if (!all) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) one[i] = mask >> i & 1u ? one[i] : 0;
+    }
+  } else {
+    const u16_alias* t = (const u16_alias*)table;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned w = word(sc, j >> 1) >> (16 * (j & 1));
+      p[j] = t[w & 255u] | (unsigned)t[(w >> 8) & 255u] << 16;
+    }
+    if (!all) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] &= (mask >> (2 * j) & 1u ? 0xFFFFu : 0u) | (mask >> (2 * j + 1) & 1u ? 0xFFFF0000u : 0u);
+    }
   }
+  constexpr unsigned LOW = 0x06040200u, HIGH = 0x07050301u;
+  const bool high = threadIdx.x % (16 / RP);             // RP 8: the digit of the lane's column
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
+    constexpr int ND = RP == 4 || (RP == 8 && !WIDE) ? 1 : (RP == 16 && WIDE ? 4 : 2);
     v4i digit[ND];
+    if constexpr (RP == 4) {
+      unsigned d[4];                                     // byte by byte: a byte's write and the next one's are four apart
+      static_for<4>([&](auto b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned st = word(v.step[g], i);
-      if constexpr (ND == 2) {
-        typedef unsigned short v2u __attribute__((ext_vector_type(2)));
+        for (int i = 0; i < 4; ++i) mul_to_byte<b>(d[i], one[4 * i + b], v.step[g].w[i]);
+      });
+      // a matrix instruction reads a vector register two wait states after its write at the earliest; the compiler sees to that, but
+      // not behind inline assembly
+      asm("s_nop 1" : "+v"(d[0]), "+v"(d[1]), "+v"(d[2]), "+v"(d[3]));
+      digit[0] = {(int)d[0], (int)d[1], (int)d[2], (int)d[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned st = v.step[g].w[i];
         const unsigned s0 = __builtin_amdgcn_perm(0, st, 0x0c010c00u), s1 = __builtin_amdgcn_perm(0, st, 0x0c030c02u);
-        const unsigned y0 = __builtin_bit_cast(unsigned, (v2u)(__builtin_bit_cast(v2u, p[2 * i]) * __builtin_bit_cast(v2u, s0)));
-        const unsigned y1 = __builtin_bit_cast(unsigned, (v2u)(__builtin_bit_cast(v2u, p[2 * i + 1]) * __builtin_bit_cast(v2u, s1)));
-        digit[0][i] = (int)(__builtin_amdgcn_perm(y1, y0, 0x06040200u) >> 1);
-        digit[1][i] = (int)__builtin_amdgcn_perm(y1, y0, 0x07050301u);
-      } else {
-        unsigned y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = (unsigned)__umul24((p[2 * i + (e >> 1)] >> (16 * (e & 1))) & 0xFFFFu, (st >> (8 * e)) & 255u);
-        const unsigned b0 = pack4((int)y[0], (int)y[1], (int)y[2], (int)y[3]);
-        const unsigned b1 = pack4((int)(y[0] >> 8), (int)(y[1] >> 8), (int)(y[2] >> 8), (int)(y[3] >> 8));
-        const unsigned b2 = pack4((int)(y[0] >> 16), (int)(y[1] >> 16), (int)(y[2] >> 16), (int)(y[3] >> 16));
-        digit[0][i] = (int)(b0 >> 1);
-        digit[1][i] = (int)(b1 & 0x7F7F7F7Fu);
-        digit[ND - 1][i] = (int)(b2 << 1 | (b1 >> 7 & 0x01010101u));
+        if constexpr (ND == 4) {
+          const unsigned y0 = mul_pair(p[2 * i] & 0x00FE00FEu, s0), y1 = mul_pair(p[2 * i + 1] & 0x00FE00FEu, s1);
+          const unsigned z0 = mul_pair((p[2 * i] >> 7) & 0x01FE01FEu, s0), z1 = mul_pair((p[2 * i + 1] >> 7) & 0x01FE01FEu, s1);
+          digit[0][i] = (int)(__builtin_amdgcn_perm(y1, y0, LOW) >> 1);
+          digit[1][i] = (int)__builtin_amdgcn_perm(y1, y0, HIGH);
+          digit[2][i] = (int)(__builtin_amdgcn_perm(z1, z0, LOW) >> 1);
+          digit[ND - 1][i] = (int)__builtin_amdgcn_perm(z1, z0, HIGH);
+        } else {
+          const unsigned y0 = mul_pair(p[2 * i], s0), y1 = mul_pair(p[2 * i + 1], s1);
+          if constexpr (ND == 1) {
+            digit[0][i] = (int)(__builtin_amdgcn_perm(y1, y0, high ? HIGH : LOW) >> (high ? 0 : 1));
+          } else {
+            digit[0][i] = (int)(__builtin_amdgcn_perm(y1, y0, LOW) >> 1);
+            digit[ND - 1][i] = (int)__builtin_amdgcn_perm(y1, y0, HIGH);
+          }
+        }
       }
     }
 #pragma unroll
@@ -230,110 +402,152 @@ __device__ __forceinline__ void add_page(const ValuePage<NG>& v, const uint4& sc
       v4i code;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned w = word(v.code[g], i);
+        const unsigned w = v.code[g].w[i];
         code[i] = (int)((half ? w : w << 4) & 0xF0F0F0F0u);
       }
 #pragma unroll
-      for (int n = 0; n < ND; ++n)
-        acc[n][2 * g + half] = __builtin_amdgcn_mfma_i32_16x16x64_i8(code, digit[n], acc[n][2 * g + half], 0, 0, 0);
+      for (int n = 0; n < ND; ++n) {
+        const int sum = ND == 4 && n > 1 ? n - 1 : n;
+        acc[sum][2 * g + half] = __builtin_amdgcn_mfma_i32_16x16x64_i8(code, digit[n], acc[sum][2 * g + half], 0, 0, 0);
+      }
     }
   }
 }
 
-// The query operand: lane (row, q) holds channels 8 q .. 8 q + 7 of each group.
-template <int NG>
-__device__ __forceinline__ void load_query(const CacheView& c, const AttendArgs& a, const Tile& t, int lane, long (&q)[NG]) {
-  const int r = (a.tile0 + t.tile) * 16 + (lane & 15), ch = 8 * (lane >> 4);
-  const int8_t* p = a.q + (long long)(t.r.first + r / a.group) * a.q_row + (long long)(t.head * a.group + r % a.group) * a.q_head + ch;
-#pragma unroll
-  for (int g = 0; g < NG; ++g) q[g] = (lane & 15) < t.rows && 32 * g + ch < c.dim ? *(const long*)(p + 32 * g) : 0;
-}
+// A wave's pages of a tile, begin + wave, begin + wave + waves, .. below end, one after the other, AHEAD of them in flight. One is
+// enough: with two or three, whose steps are unrolled for as many sets of registers, the longer code costs a short walk more (its
+// instructions come from memory too) than the loads in flight bring a long one. 32 x 12 heads over up to 1024 tokens: none
+// 11.9 us, one 11.6, three and two 12.9; 64 x 32 heads over up to 8192: 79.0, 69.7, 70.1. Table entries come 64 at a time, one a lane; the first of
+// them are known when the walk begins (`entry`).
+template <int NG, int AHEAD, typename Page>
+struct Walk {
+  Page ring[AHEAD + 1];
+  const CacheView& c;
+  const Tile& t;
+  const int first, end, waves, lane;
+  int entry, n;
 
-// Pages begin + wave, begin + wave + WAVES, .. below end of a tile, one after the other: step(page, slot, block) for those that the
-// table names, with `ahead` holding what load(block) of the next one returns, issued before step runs on this one. Table
-// entries come 64 at a time, one a lane.
-template <int NG, typename Page, typename Step>
-__device__ __forceinline__ void walk(const CacheView& c, const Tile& t, int begin, int end, bool report, Step&& step) {
-  const int lane = threadIdx.x & 63;
-  const int first = begin + (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long stride = (long long)c.heads * Block<NG>::BYTES;
-  const uint8_t* base = c.pool + (long long)t.head * Block<NG>::BYTES;
-  for (int at = first; at < end; at += 64 * WAVES) {
-    const int mine = at + lane * WAVES;
-    int entry = -1;
-    if (mine < end) entry = c.table[(long long)t.seq * c.slots + slot_of(t, mine)];
-    if (entry >= c.pages || entry < -1) {
-      if (report) raise_flag(c.flags, FLAG_CACHE);
-      entry = -1;
-    }
-    const int n = min(64, (end - at + WAVES - 1) / WAVES);
-    // a page that the table does not name reads page 0's bytes, which step never sees
-    const auto fetch = [&](int i, Page& p) {
-      const int e = __builtin_amdgcn_readlane(entry, i);
-      p.load(base + max(e, 0) * stride, lane);
-    };
-    Page a, b;
-    fetch(0, a);
-    for (int i = 0; i < n; i += 2) {
-      if (i + 1 < n) fetch(i + 1, b);
-      if (__builtin_amdgcn_readlane(entry, i) >= 0) step(a, at + i * WAVES);
-      if (i + 1 >= n) break;
-      if (i + 2 < n) fetch(i + 2, a);
-      if (__builtin_amdgcn_readlane(entry, i + 1) >= 0) step(b, at + (i + 1) * WAVES);
+  __device__ __forceinline__ Walk(const CacheView& view, const Tile& tile, int begin, int stop, int entries)
+      : c(view), t(tile), first(begin + (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), end(stop), waves(blockDim.x >> 6),
+        lane(threadIdx.x & 63), entry(entries) {
+    n = min(64, (end - first + waves - 1) / waves);
+    static_for<AHEAD>([&](auto d) { fetch(d, ring[d]); });
+  }
+  // behind the last page, and where the table names none, an empty descriptor: the loads are issued, so that every step waits for
+  // the same number of them, and touch no memory
+  __device__ __forceinline__ void fetch(int i, Page& p) {
+    const int e = i < n ? __builtin_amdgcn_readlane(entry, i & 63) : -1;
+    const uint8_t* blk = c.pool + ((long long)max(e, 0) * c.heads + t.head) * Block<NG>::BYTES;
+    p.load(uniform_rsrc(blk, e < 0 ? 0 : Block<NG>::BYTES), lane);
+  }
+  // step(page's lane part, page) for those that the table names
+  template <typename Step>
+  __device__ __forceinline__ void run(Step&& step) {
+    for (int at = first; at < end; at += 64 * waves) {
+      if (at != first) {
+        entry = entry_of(c, t, at + lane * waves, end);
+        n = min(64, (end - at + waves - 1) / waves);
+        static_for<AHEAD>([&](auto d) { fetch(d, ring[d]); });
+      }
+      for (int i = 0; i < n; i += AHEAD + 1)
+        static_for<AHEAD + 1>([&](auto d) {
+          if (i + d < n) {
+            fetch(i + d + AHEAD, ring[(d + AHEAD) % (AHEAD + 1)]);
+            if (__builtin_amdgcn_readlane(entry, i + d) >= 0) step(ring[d], at + (i + d) * waves);
+          }
+        });
     }
   }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_add(unsigned long long v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+  return v + ((unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {   // in every lane
+  v = dpp_add<0xB1, 0xF>(v);                             // quad_perm [1,0,3,2]
+  v = dpp_add<0x4E, 0xF>(v);                             // quad_perm [2,3,0,1]
+  v = dpp_add<0x141, 0xF>(v);                            // row_half_mirror
+  v = dpp_add<0x140, 0xF>(v);                            // row_mirror: each row of 16 its sum
+  v = dpp_add<0x142, 0xA>(v);                            // row_bcast:15 into rows 1 and 3
+  v = dpp_add<0x143, 0xC>(v);                            // row_bcast:31 into rows 2 and 3: lane 63 has them all
+  const unsigned lo = __builtin_amdgcn_readlane((int)v, 63), hi = __builtin_amdgcn_readlane((int)(v >> 32), 63);
+  return (unsigned long long)hi << 32 | lo;
 }
 
-// From a row's histogram (counts of scores 4 lane .. 4 lane + 3, less 128) the lane's four probabilities, as pairs of 2 p: every
-// operand is a whole number below 2^53, so double arithmetic is exact but for the quotient, which is put right by its remainder.
-__device__ __forceinline__ uint2 probabilities(const uint4& count, const int* lut, int one, unsigned* flags) {
+// From a row's histogram (counts of scores 4 lane .. 4 lane + 3, less 128) its table in LDS, the lane's four entries: every operand is a whole number below 2^53, so double arithmetic is exact but for the quotient, which is put right by its remainder.
+template <int TABLE>
+__device__ __forceinline__ void probabilities(const uint4& count, const int* lut, int one, unsigned* flags, unsigned* table) {
   const int lane = threadIdx.x & 63;
+  unsigned p[4] = {0, 0, 0, 0};
   const int mine = count.w ? 3 : (count.z ? 2 : (count.y ? 1 : (count.x ? 0 : -1)));
   const unsigned long long any = __ballot(mine >= 0);
-  if (!any) return {0, 0};                               // the row sees nothing
-  const int at = 63 - __builtin_clzll(any), top = 4 * at + __builtin_amdgcn_readlane(mine, at);
-  int e[4];
-  unsigned long long sum = 0;
+  if (any) {                                             // else the row sees nothing
+    const int at = 63 - __builtin_clzll(any), top = 4 * at + __builtin_amdgcn_readlane(mine, at);
+    int e[4];
+    unsigned long long sum = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x = 4 * lane + i;
-    e[i] = x <= top ? max(0, lut[x - top + 255]) : 0;
-    sum += (unsigned long long)e[i] * word(count, i);
-  }
+    for (int i = 0; i < 4; ++i) {
+      const int x = 4 * lane + i;
+      e[i] = x <= top ? max(0, lut[x - top + 255]) : 0;
+      sum += (unsigned long long)(unsigned)e[i] * word(count, i);
+    }
+    sum = wave_sum(sum);
+    if (!sum && lane == 0) raise_flag(flags, FLAG_ZERODIV);
+    if (sum) {
+      // the reciprocal is good to one part in 2^24 at least and the quotient below 2^15: one off at most
+      const double S = (double)sum, half = (double)(sum >> 1), inv = __builtin_amdgcn_rcp(S);
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  if (!sum) {
-    if (lane == 0) raise_flag(flags, FLAG_ZERODIV);
-    return {0, 0};
+      for (int i = 0; i < 4; ++i) {
+        const double n = __builtin_fma((double)e[i], (double)one, half);
+        double k = __builtin_trunc(n * inv);
+        const double rest = __builtin_fma(-k, S, n);
+        k += rest < 0 ? -1.0 : (rest >= S ? 1.0 : 0.0);
+        p[i] = (unsigned)(int)k;
+      }
+    }
   }
-  const double S = (double)sum, half = (double)(sum >> 1), inv = 1.0 / S;
-  unsigned p[4];
+  if constexpr (TABLE == TABLE_FIFTEEN) {                // a byte each of four tables
+    int x[4] = {(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const double n = (double)e[i] * one + half;
-    double k = __builtin_trunc(n * inv);
-    const double rest = __builtin_fma(-k, S, n);
-    k += rest < 0 ? -1.0 : (rest >= S ? 1.0 : 0.0);
-    p[i] = 2u * (unsigned)k;
+    for (int v = 0; v < 4; ++v) {
+      int d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int up = (int)((unsigned)__umul24(x[i] + 7, 34953) >> 19);          // / 15, exact below 2^19 / 7
+        d[i] = x[i] - 15 * up, x[i] = up;
+      }
+      table[64 * v + lane] = pack4(d[0], d[1], d[2], d[3]);
+    }
+  } else if constexpr (TABLE == TABLE_SEVEN) {
+    table[2 * lane] = 2 * (p[0] & 127u) | (p[1] & 127u) << 17, table[2 * lane + 1] = 2 * (p[2] & 127u) | (p[3] & 127u) << 17;
+    table[128 + 2 * lane] = 2 * (p[0] >> 7) | (p[1] >> 7) << 17, table[129 + 2 * lane] = 2 * (p[2] >> 7) | (p[3] >> 7) << 17;
+  } else {
+    table[2 * lane] = 2 * p[0] | p[1] << 17, table[2 * lane + 1] = 2 * p[2] | p[3] << 17;
   }
-  return {p[0] | p[1] << 16, p[2] | p[3] << 16};
 }
 
 // A wave's accumulators as 16 x sums of p V (modulo 2^32, in which the sum itself lies) into row-major int32.
-template <int NG, int ND>
-__device__ __forceinline__ void spill(const v4i (&acc)[ND][2 * NG], int* rows, int stride, int n_rows) {
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  if (r >= n_rows) return;
+template <int NG, int RP, bool WIDE>
+__device__ __forceinline__ void spill(const v4i (&acc)[Digits<RP, WIDE>::SUMS][2 * NG], int* rows, int stride, int n_rows) {
+  using D = Digits<RP, WIDE>;
+  constexpr int VN = 16 / RP;
+  const int lane = threadIdx.x & 63, r = (lane & 15) / VN, v = lane % VN, q = lane >> 4;
 #pragma unroll
   for (int m = 0; m < 2 * NG; ++m) {
     v4i s;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      unsigned x = (unsigned)acc[0][m][e] + ((unsigned)acc[1][m][e] << 7);
-      if constexpr (ND == 3) x += (unsigned)acc[ND - 1][m][e] << 14;
+      unsigned x = 0;
+#pragma unroll
+      for (int n = 0; n < D::SUMS; ++n) x += (unsigned)acc[n][m][e] * D::weight(v, n);
+      if constexpr (VN > 1) x += (unsigned)lane_xor<1>((int)x);
+      if constexpr (VN > 2) x += (unsigned)lane_xor<2>((int)x);
       s[e] = (int)x;
     }
-    *(v4i*)(rows + r * stride + 16 * m + 4 * q) = s;
+    if (v == 0 && r < n_rows) *(v4i*)(rows + r * stride + 16 * m + 4 * q) = s;
   }
 }
 
@@ -353,168 +567,249 @@ __device__ __forceinline__ unsigned* out_word(const AttendArgs& a, const Tile& t
   return (unsigned*)(a.o + (long long)(t.r.first + at / a.group) * a.o_row + (long long)(t.head * a.group + at % a.group) * a.o_head + ch);
 }
 
-// The sum over the workgroup's waves of what each holds, in LDS (`red`: WAVES x rows x stride), then f(row, channel, sum).
-template <int NG, int ND, typename F>
-__device__ __forceinline__ void join_waves(const v4i (&acc)[ND][2 * NG], int* red, const Tile& t, F&& f) {
-  constexpr int STRIDE = 32 * NG + 4;
-  const int wave = threadIdx.x >> 6;
-  spill<NG, ND>(acc, red + wave * t.rows * STRIDE, STRIDE, t.rows);
+// The sum over the workgroup's waves of what each holds, in LDS (`red`: waves x rows x SUM_STRIDE), then f(row, channel, sum).
+template <int NG>
+constexpr int SUM_STRIDE = 32 * NG + 4;
+template <int NG, int RP, bool WIDE, typename F>
+__device__ __forceinline__ void join_waves(const v4i (&acc)[Digits<RP, WIDE>::SUMS][2 * NG], int* red, const Tile& t, F&& f) {
+  constexpr int STRIDE = SUM_STRIDE<NG>;
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  spill<NG, RP, WIDE>(acc, red + wave * t.rows * STRIDE, STRIDE, t.rows);
   __syncthreads();
-  for (int i = threadIdx.x; i < t.rows * 8 * NG; i += ATTEND_THREADS) {
+  for (int i = threadIdx.x; i < t.rows * 8 * NG; i += blockDim.x) {
     const int r = i / (8 * NG), ch = 4 * (i % (8 * NG));
     v4i s = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += *(const v4i*)(red + (w * t.rows + r) * STRIDE + ch);
+    for (int w = 0; w < waves; ++w) s += *(const v4i*)(red + (w * t.rows + r) * STRIDE + ch);
     f(r, ch, s);
   }
 }
 
+constexpr int WAVES_MAX = 8;
+
+
+// Where a lane stands in the first pass: its row, and which of the row's 64 scores of a page are its NE dwords.
+template <int NG, int RP>
+struct Place {
+  using C = Columns<NG, RP>;
+  int r, word, bit;
+  __device__ __forceinline__ Place() {
+    const int lane = threadIdx.x & 63;
+    r = (lane & 15) / C::VN;
+    word = 4 * (lane >> 4) + C::NE * (lane % C::VN);
+    bit = 4 * C::NE * (lane % C::VN);                    // of the quarter's 16 keys
+  }
+};
+
+template <int NG, int RP>
+using KeyWalk = Walk<NG, 1, KeyPage<NG, RP>>;
+template <int NG>
+using ValueWalk = Walk<NG, 1, ValuePage<NG>>;
+
+template <int NG, int RP>
+__device__ __forceinline__ void score_pages(KeyWalk<NG, RP>& walk, const CacheView& c, const AttendArgs& a, const Tile& t,
+                                            unsigned* hist, unsigned* scores, int row_slots) {
+  using C = Columns<NG, RP>;
+  const int lane = threadIdx.x & 63, q = lane >> 4;
+  const Place<NG, RP> at;
+  const Row row(t, a, at.r);
+  Query<NG, RP> query;
+  query.load(c, a, t, lane);
+  const Requant rq(a.m_s, a.s_s);
+  walk.run([&](const KeyPage<NG, RP>& page, int n) {
+    const Words<C::NE> sc = score_page<NG, RP>(page, query, rq);
+    const int slot = slot_of(t, n);
+    if (!row.on) return;
+    unsigned* out = scores + ((long long)n * row_slots + at.r) * (PAGE / 4) + at.word;
+    if constexpr (C::NE == 4) *(uint4*)out = {sc.w[0], sc.w[1], sc.w[2], sc.w[3]};
+    else if constexpr (C::NE == 2) *(uint2*)out = {sc.w[0], sc.w[1]};
+    else *out = sc.w[0];
+    if (whole(t, a, slot)) count_scores(hist + at.r * HIST, sc);
+    else count_scores(hist + at.r * HIST, sc, row.mask(slot * PAGE + 16 * q) >> at.bit);
+  });
+}
+
+template <int NG, int RP, bool WIDE>
+__device__ __forceinline__ void add_pages(ValueWalk<NG>& walk, const AttendArgs& a, const Tile& t, const unsigned* tables,
+                                          const unsigned* scores, int row_slots, v4i (&acc)[Digits<RP, WIDE>::SUMS][2 * NG]) {
+  constexpr int VN = 16 / RP;
+  const int lane = threadIdx.x & 63, q = lane >> 4, v = lane % VN;
+  const Row row(t, a, (lane & 15) / VN);
+  const int r = row.on ? (lane & 15) / VN : 0;
+  const int which = RP == 4 ? 64 * v : (RP == 8 && WIDE ? 128 * v : 0);          // of the row's tables
+  const uint8_t* table = (const uint8_t*)(tables + r * HIST + which);
+  walk.run([&](const ValuePage<NG>& page, int n) {
+    const int slot = slot_of(t, n);
+    const uint4 sc = *(const uint4*)(scores + ((long long)n * row_slots + r) * (PAGE / 4) + 4 * q);
+    add_page<NG, RP, WIDE>(page, sc, table, whole(t, a, slot), row.mask(slot * PAGE + 16 * q), acc);
+  });
+}
+
+// What a workgroup clears and fetches before it knows its tile, whose numbers come from memory themselves: the histograms, the
+// exponentials' table, and without a window the wave's first table entries.
+struct Early {
+  int lut, entry;
+  __device__ __forceinline__ Early(const CacheView& c, const AttendArgs& a, unsigned* hist, bool entries) {
+    lut = threadIdx.x < 256 ? a.lut[threadIdx.x] : 0;
+    entry = -1;
+    const int page = (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 63) * (int)(blockDim.x >> 6);
+    if (entries && !a.window && page < c.slots) entry = c.table[(long long)(a.seq0 + (int)blockIdx.x / c.heads) * c.slots + page];
+    for (int i = threadIdx.x; i < a.rows * HIST; i += blockDim.x) hist[i] = 0;
+  }
+  __device__ __forceinline__ void keep(int* table) const {
+    if (threadIdx.x < 256) table[threadIdx.x] = lut;
+  }
+  // the wave's first entries of a walk over pages begin .. end - 1; `mine`: read ahead
+  __device__ __forceinline__ int entries(const CacheView& c, const AttendArgs& a, const Tile& t, int begin, int end, bool mine) const {
+    const int page = begin + (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 63) * (int)(blockDim.x >> 6);
+    if (!mine || a.window) return entry_of(c, t, page, end);
+    if (page >= end || entry == -1) return -1;
+    if (entry < -1 || entry >= c.pages) {
+      raise_flag(c.flags, FLAG_CACHE);
+      return -1;
+    }
+    return entry;
+  }
+};
+
 // Both passes of a tile in one workgroup, its scores in LDS.
-template <int NG, int ND>
-__global__ __launch_bounds__(ATTEND_THREADS) void attend_tile_kernel(CacheView c, AttendArgs a) {
+template <int NG, int RP, bool WIDE>
+__global__ __launch_bounds__(64 * WAVES_MAX) void attend_tile_kernel(CacheView c, AttendArgs a) {
   extern __shared__ __align__(16) unsigned lds[];
-  __shared__ int lut[256];
+  int* lut = (int*)lds;
+  unsigned* hist = lds + 256;
+  unsigned* scores = hist + (a.rows * HIST + 3) / 4 * 4;
+  const Early early(c, a, hist, true);
   Tile t;
   if (!find_tile(c, a, t)) return;
-  unsigned* hist = lds;
-  uint4* scores = (uint4*)(lds + (a.rows * HIST + 3) / 4 * 4);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
-  const Row row(t, a, r);
-  long query[NG];
-  load_query<NG>(c, a, t, lane, query);
-  lut[tid] = a.lut[tid];
-  for (int i = tid; i < t.rows * HIST; i += ATTEND_THREADS) hist[i] = 0;
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
+  const int entry = early.entries(c, a, t, 0, t.pages, true);
+  {
+    KeyWalk<NG, RP> keys(c, t, 0, t.pages, entry);
+    early.keep(lut);
+    __syncthreads();
+    score_pages<NG, RP>(keys, c, a, t, hist, scores, t.rows);
+  }
+  ValueWalk<NG> values(c, t, 0, t.pages, entry);         // on their way while the tables are made
   __syncthreads();
-  const Requant rq(a.m_s, a.s_s);
-  walk<NG, KeyPage<NG>>(c, t, 0, t.pages, true, [&](const KeyPage<NG>& page, int at) {
-    const uint4 sc = score_page<NG>(page, query, rq);
-    const int slot = slot_of(t, at);
-    if (!row.on) return;
-    scores[(at * t.rows + r) * 4 + q] = sc;
-    if (whole(t, a, slot)) count_scores(hist + r * HIST, sc, 0xFFFFu);
-    else count_scores(hist + r * HIST, sc, row.mask(slot * PAGE + 16 * q));
-  });
-  __syncthreads();
-  for (int i = wave; i < t.rows; i += WAVES) {           // the row's table takes its histogram's place
+  for (int i = tid >> 6; i < t.rows; i += waves) {       // the row's table takes its histogram's place
     unsigned* h = hist + i * HIST;
     const uint4 count = {h[4 * lane], h[4 * lane + 1], h[4 * lane + 2], h[4 * lane + 3]};
-    const uint2 p = probabilities(count, lut, a.one, c.flags);
-    h[2 * lane] = p.x;
-    h[2 * lane + 1] = p.y;
+    probabilities<Digits<RP, WIDE>::TABLE>(count, lut, a.one, c.flags, h);
   }
   __syncthreads();
-  v4i acc[ND][2 * NG] = {};
-  const u16_alias* table = (const u16_alias*)(hist + (row.on ? r : 0) * HIST);
-  walk<NG, ValuePage<NG>>(c, t, 0, t.pages, false, [&](const ValuePage<NG>& page, int at) {
-    const int slot = slot_of(t, at);
-    const uint4 sc = scores[(at * t.rows + (row.on ? r : 0)) * 4 + q];
-    add_page<NG, ND>(page, sc, table, whole(t, a, slot) ? 0xFFFFu : row.mask(slot * PAGE + 16 * q), acc);
-  });
+  v4i acc[Digits<RP, WIDE>::SUMS][2 * NG] = {};
+  add_pages<NG, RP, WIDE>(values, a, t, hist, scores, t.rows, acc);
   __syncthreads();                                       // the scores have been read
-  join_waves<NG, ND>(acc, (int*)scores, t, [&](int i, int ch, const v4i& s) {
+  join_waves<NG, RP, WIDE>(acc, (int*)scores, t, [&](int i, int ch, const v4i& s) {
     if (ch < c.dim) *out_word(a, t, i, ch) = finish4(s, a);
   });
 }
 
 // ---- one tile over several workgroups: scores and histograms, then sums, then their total
 
-__device__ __forceinline__ void split_range(const Tile& t, const AttendArgs& a, int& begin, int& end) {
-  const int per = max(2 * WAVES, (t.pages + a.splits - 1) / a.splits);
-  begin = min((int)blockIdx.z * per, t.pages);
-  end = min(begin + per, t.pages);
-}
+// pages of a part: parts are of equal size, at least a page a wave
+__device__ __forceinline__ int part_pages(const Tile& t, const AttendArgs& a, int waves) { return max(waves, (t.pages + a.splits - 1) / a.splits); }
 
-template <int NG>
-__global__ __launch_bounds__(ATTEND_THREADS) void attend_scores_kernel(CacheView c, AttendArgs a) {
-  __shared__ unsigned hist[16 * HIST];
+template <int NG, int RP>
+__global__ __launch_bounds__(64 * WAVES_MAX) void attend_scores_kernel(CacheView c, AttendArgs a) {
+  __shared__ unsigned hist[RP * HIST];
+  for (int i = threadIdx.x; i < a.rows * HIST; i += blockDim.x) hist[i] = 0;
   Tile t;
   if (!find_tile(c, a, t)) return;
-  int begin, end;
-  split_range(t, a, begin, end);
+  const int per = part_pages(t, a, blockDim.x >> 6), begin = (int)blockIdx.z * per, end = min(begin + per, t.pages);
   if (begin >= end) return;
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
-  const Row row(t, a, r);
-  long query[NG];
-  load_query<NG>(c, a, t, lane, query);
-  for (int i = tid; i < t.rows * HIST; i += ATTEND_THREADS) hist[i] = 0;
+  const int page = begin + (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 63) * (int)(blockDim.x >> 6);
+  KeyWalk<NG, RP> keys(c, t, begin, end, entry_of(c, t, page, end));
   __syncthreads();
-  const Requant rq(a.m_s, a.s_s);
   const long long unit = (long long)t.unit * a.tiles + t.tile;
-  uint4* scores = (uint4*)a.scores + unit * a.bound * a.rows * 4;
-  walk<NG, KeyPage<NG>>(c, t, begin, end, true, [&](const KeyPage<NG>& page, int at) {
-    const uint4 sc = score_page<NG>(page, query, rq);
-    const int slot = slot_of(t, at);
-    if (!row.on) return;
-    scores[((long long)at * a.rows + r) * 4 + q] = sc;
-    if (whole(t, a, slot)) count_scores(hist + r * HIST, sc, 0xFFFFu);
-    else count_scores(hist + r * HIST, sc, row.mask(slot * PAGE + 16 * q));
-  });
+  score_pages<NG, RP>(keys, c, a, t, hist, (unsigned*)a.scores + unit * a.bound * a.rows * (PAGE / 4), a.rows);
   __syncthreads();
   unsigned* out = a.hist + (unit * a.splits + blockIdx.z) * a.rows * 256;
-  for (int i = tid; i < t.rows * 256; i += ATTEND_THREADS) out[i] = hist[(i >> 8) * HIST + (i & 255)];
+  for (int i = threadIdx.x; i < t.rows * 256; i += blockDim.x) out[i] = hist[(i >> 8) * HIST + (i & 255)];
 }
 
-template <int NG, int ND>
-__global__ __launch_bounds__(ATTEND_THREADS) void attend_values_kernel(CacheView c, AttendArgs a) {
-  __shared__ int lut[256];
-  __shared__ __align__(16) unsigned tables[16 * HIST];
-  __shared__ __align__(16) int red[WAVES * 16 * (32 * NG + 4)];
+template <int NG, int RP, bool WIDE>
+__global__ __launch_bounds__(64 * WAVES_MAX) void attend_values_kernel(CacheView c, AttendArgs a) {
+  extern __shared__ __align__(16) unsigned lds[];
+  int* lut = (int*)lds;
+  unsigned* tables = lds + 256;
+  int* red = (int*)(tables + (a.rows * HIST + 3) / 4 * 4);
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
+  for (int i = tid; i < 256; i += blockDim.x) lut[i] = a.lut[i];
+  for (int i = tid; i < a.rows * HIST; i += blockDim.x) tables[i] = 0;
   Tile t;
   if (!find_tile(c, a, t)) return;
-  int begin, end;
-  split_range(t, a, begin, end);
+  const int per = part_pages(t, a, waves), parts = (t.pages + per - 1) / per;
+  const int begin = (int)blockIdx.z * per, end = min(begin + per, t.pages);
   if (begin >= end) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
-  const Row row(t, a, r);
-  lut[tid] = a.lut[tid];
+  ValueWalk<NG> values(c, t, begin, end, entry_of(c, t, begin + (tid >> 6) + lane * waves, end));
   __syncthreads();
   const long long unit = (long long)t.unit * a.tiles + t.tile;
-  const int per = max(2 * WAVES, (t.pages + a.splits - 1) / a.splits), parts = (t.pages + per - 1) / per;
-  for (int i = wave; i < t.rows; i += WAVES) {
-    const uint4* h = (const uint4*)(a.hist + (unit * a.splits * a.rows + i) * 256) + lane;
-    uint4 count = {0, 0, 0, 0};
-    for (int p = 0; p < parts; ++p) {
-      const uint4 x = h[(long long)p * a.rows * 64];
-      count.x += x.x, count.y += x.y, count.z += x.z, count.w += x.w;
+  const uint4* slices = (const uint4*)(a.hist + unit * a.splits * a.rows * 256) + lane;
+  // all parts' histograms: a wave takes a row of every several parts, eight of them at once
+  const int share = max(1, waves / t.rows);
+  for (int i = tid >> 6; i < t.rows * share; i += waves) {
+    const int row = i % t.rows;
+    uint4 sum = {0, 0, 0, 0};
+    for (int p = i / t.rows; p < parts; p += 8 * share) {
+      uint4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = {0, 0, 0, 0};
+        if (p + k * share < parts) x[k] = slices[((long long)(p + k * share) * a.rows + row) * 64];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum.x += x[k].x, sum.y += x[k].y, sum.z += x[k].z, sum.w += x[k].w;
     }
-    const uint2 p = probabilities(count, lut, a.one, c.flags);
-    tables[i * HIST + 2 * lane] = p.x;
-    tables[i * HIST + 2 * lane + 1] = p.y;
+    unsigned* h = tables + row * HIST + 4 * lane;
+    atomicAdd(h, sum.x), atomicAdd(h + 1, sum.y), atomicAdd(h + 2, sum.z), atomicAdd(h + 3, sum.w);
   }
   __syncthreads();
-  v4i acc[ND][2 * NG] = {};
-  const u16_alias* table = (const u16_alias*)(tables + (row.on ? r : 0) * HIST);
-  const uint4* scores = (const uint4*)a.scores + unit * a.bound * a.rows * 4;
-  walk<NG, ValuePage<NG>>(c, t, begin, end, false, [&](const ValuePage<NG>& page, int at) {
-    const int slot = slot_of(t, at);
-    const uint4 sc = scores[((long long)at * a.rows + (row.on ? r : 0)) * 4 + q];
-    add_page<NG, ND>(page, sc, table, whole(t, a, slot) ? 0xFFFFu : row.mask(slot * PAGE + 16 * q), acc);
-  });
+  for (int i = tid >> 6; i < t.rows; i += waves) {
+    unsigned* h = tables + i * HIST;
+    const uint4 count = {h[4 * lane], h[4 * lane + 1], h[4 * lane + 2], h[4 * lane + 3]};
+    probabilities<Digits<RP, WIDE>::TABLE>(count, lut, a.one, c.flags, h);
+  }
+  __syncthreads();
+  v4i acc[Digits<RP, WIDE>::SUMS][2 * NG] = {};
+  add_pages<NG, RP, WIDE>(values, a, t, tables, (const unsigned*)a.scores + unit * a.bound * a.rows * (PAGE / 4), a.rows, acc);
   int* sums = a.sums + (unit * a.splits + blockIdx.z) * a.rows * 32 * NG;
-  join_waves<NG, ND>(acc, red, t, [&](int i, int ch, const v4i& s) { *(v4i*)(sums + i * 32 * NG + ch) = s; });
+  join_waves<NG, RP, WIDE>(acc, red, t, [&](int i, int ch, const v4i& s) { *(v4i*)(sums + i * 32 * NG + ch) = s; });
 }
 
+// One wave a row and 16 channels: four lanes to the channels, 16 to the parts.
+constexpr int JOIN_THREADS = 64;
 template <int NG>
-__global__ __launch_bounds__(ATTEND_THREADS) void attend_join_kernel(CacheView c, AttendArgs a) {
+__global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(CacheView c, AttendArgs a, int waves) {
   Tile t;
   if (!find_tile(c, a, t)) return;
+  const int r = (int)blockIdx.z / (2 * NG), ch = 16 * ((int)blockIdx.z % (2 * NG)) + 4 * (threadIdx.x & 3);
+  if (r >= t.rows || ch >= c.dim) return;
   const long long unit = (long long)t.unit * a.tiles + t.tile;
-  const int per = max(2 * WAVES, (t.pages + a.splits - 1) / a.splits), parts = (t.pages + per - 1) / per;
-  for (int i = threadIdx.x; i < t.rows * 8 * NG; i += ATTEND_THREADS) {
-    const int r = i / (8 * NG), ch = 4 * (i % (8 * NG));
-    if (ch >= c.dim) continue;
-    const int* p = a.sums + (unit * a.splits * a.rows + r) * 32 * NG + ch;
-    v4i s = {0, 0, 0, 0};
-    for (int n = 0; n < parts; ++n) s += *(const v4i*)(p + (long long)n * a.rows * 32 * NG);
-    *out_word(a, t, r, ch) = finish4(s, a);
-  }
+  const int per = part_pages(t, a, waves), parts = (t.pages + per - 1) / per;
+  const int* p = a.sums + (unit * a.splits * a.rows + r) * 32 * NG + ch;
+  v4i s = {0, 0, 0, 0};
+  for (int n = threadIdx.x >> 2; n < parts; n += 16) s += *(const v4i*)(p + (long long)n * a.rows * 32 * NG);
+#pragma unroll
+  for (int d = 4; d < 64; d *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += __shfl_xor(s[e], d);
+  if (threadIdx.x < 4) *out_word(a, t, r, ch) = finish4(s, a);
 }
 
-constexpr int TILE_LDS_MAX = 63 * 1024;                  // a tile's scores and histograms: two workgroups a CU
+constexpr int LDS_MAX = 160 * 1024;                      // of a CU
 constexpr long long SCORES_MAX = 1ll << 30;              // bytes of scores in the workspace, unless one tile has more
-constexpr int FILL = 512;                                // workgroups that fill the card
 
-template <int NG, int ND>
+template <typename K>
+static int launch_lds(K kernel, dim3 grid, int threads, size_t lds, anvil_ctx* ctx, const CacheView& c, const AttendArgs& a) {
+  if (lds > 64 * 1024)
+    ANVIL_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_MAX));
+  ANVIL_LAUNCH(kernel, grid, dim3((unsigned)threads), lds, ctx->stream, c, a);
+  ANVIL_LAUNCHED();
+  return ANVIL_OK;
+}
+
+template <int NG, int RP, bool WIDE>
 static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a, int max_new) {
   const long long all = (long long)max_new * a.group;    // rows of a cache head at most
   a.rows = (int)std::min(16ll, all);
@@ -525,16 +820,20 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a, int max_new)
     const long long seen = ((long long)a.window + tokens + PAGE - 2) / PAGE + 1 + (a.sinks + PAGE - 1) / PAGE;
     a.bound = (int)std::min<long long>(c.slots, seen);
   }
-  const long long units = (long long)c.seqs * c.heads;
-  const size_t lds = sizeof(int) * ((size_t)(a.rows * HIST + 3) / 4 * 4) +
-                     std::max<size_t>((size_t)a.bound * a.rows * PAGE, sizeof(int) * WAVES * a.rows * (32 * NG + 4));
-  const long long wanted = std::min<long long>((FILL + units * tiles - 1) / (units * tiles), (a.bound + 2 * WAVES - 1) / (2 * WAVES));
-  a.splits = (int)std::max(1ll, wanted);
-  if (a.splits == 1 && lds <= TILE_LDS_MAX) {
+  const long long units = (long long)c.seqs * c.heads, groups = units * tiles;
+  const size_t fixed = sizeof(int) * (256 + (size_t)(a.rows * HIST + 3) / 4 * 4), row_sums = sizeof(int) * (size_t)a.rows * SUM_STRIDE<NG>;
+  const size_t scores = (size_t)a.bound * a.rows * PAGE;
+  // Four waves a workgroup where the tiles fill the CUs and two of them fit a CU's LDS, else eight.
+  const int waves = 2 * groups >= 3ll * ctx->num_cu && fixed + std::max(scores, 4 * row_sums) <= LDS_MAX / 2 ? 4 : 8;
+  const size_t sums = waves * row_sums, lds = fixed + std::max(scores, sums);
+  // Parts of a tile only where they bring CUs to work that the tiles leave idle, and where a tile is long: three launches cost what
+  // one does over 32 pages.
+  const bool whole_tiles = a.bound <= 32 || 3 * groups > ctx->num_cu;
+  a.splits = whole_tiles ? 1 : (int)std::min<long long>(ctx->num_cu / groups, (a.bound + 7) / 8);
+  if (a.splits == 1 && lds <= LDS_MAX) {
     for (long long t0 = 0; t0 < tiles; t0 += 65535) {    // a grid dimension's limit
       a.tile0 = (int)t0, a.tiles = (int)std::min<long long>(tiles - t0, 65535);
-      ANVIL_LAUNCH((attend_tile_kernel<NG, ND>), dim3((unsigned)units, (unsigned)a.tiles), dim3(ATTEND_THREADS), lds, ctx->stream, c, a);
-      ANVIL_LAUNCHED();
+      if (int r = launch_lds(attend_tile_kernel<NG, RP, WIDE>, dim3((unsigned)units, (unsigned)a.tiles), 64 * waves, lds, ctx, c, a)) return r;
     }
     return ANVIL_OK;
   }
@@ -554,11 +853,10 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a, int max_new)
       a.tile0 = (int)t0, a.tiles = (int)std::min<long long>(tiles - t0, step);
       const unsigned n = (unsigned)(std::min(seqs, c.seqs - a.seq0) * c.heads);
       const dim3 grid(n, (unsigned)a.tiles, (unsigned)a.splits);
-      ANVIL_LAUNCH(attend_scores_kernel<NG>, grid, dim3(ATTEND_THREADS), 0, ctx->stream, c, a);
-      ANVIL_LAUNCHED();
-      ANVIL_LAUNCH((attend_values_kernel<NG, ND>), grid, dim3(ATTEND_THREADS), 0, ctx->stream, c, a);
-      ANVIL_LAUNCHED();
-      ANVIL_LAUNCH(attend_join_kernel<NG>, dim3(n, (unsigned)a.tiles), dim3(ATTEND_THREADS), 0, ctx->stream, c, a);
+      if (int r = launch_lds(attend_scores_kernel<NG, RP>, grid, 64 * waves, 0, ctx, c, a)) return r;
+      if (int r = launch_lds(attend_values_kernel<NG, RP, WIDE>, grid, 64 * waves, fixed + sums, ctx, c, a)) return r;
+      ANVIL_LAUNCH(attend_join_kernel<NG>, dim3(n, (unsigned)a.tiles, (unsigned)(2 * NG * a.rows)), dim3(JOIN_THREADS), 0, ctx->stream, c,
+                   a, waves);
       ANVIL_LAUNCHED();
     }
   return ANVIL_OK;
@@ -596,7 +894,10 @@ extern "C" int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache
   int r = ANVIL_OK;
   by_groups(c.dim, [&](auto ng) {
     constexpr int NG = decltype(ng)::value;
-    r = one <= ONE_TWO_DIGITS ? attend<NG, 2>(ctx, c, a, max_new) : attend<NG, 3>(ctx, c, a, max_new);
+    const long long rows = (long long)max_new * a.group;
+    if (rows <= 4 && one <= ONE_FIFTEEN) r = attend<NG, 4, false>(ctx, c, a, max_new);
+    else if (rows <= 8) r = one <= ONE_NARROW ? attend<NG, 8, false>(ctx, c, a, max_new) : attend<NG, 8, true>(ctx, c, a, max_new);
+    else r = one <= ONE_NARROW ? attend<NG, 16, false>(ctx, c, a, max_new) : attend<NG, 16, true>(ctx, c, a, max_new);
   });
   return r;
 }
