@@ -12,7 +12,7 @@ constexpr long long NO_SCORE = INT64_MIN;
 constexpr int WAVE_TOKENS = 4096;                        // 64 lanes x 4 blocks x 16 logits
 constexpr int BLOCKS = WAVE_TOKENS / 1024;
 constexpr int PART_WAVES = 4, PART_TOKENS = PART_WAVES * WAVE_TOKENS, PART_THREADS = 64 * PART_WAVES;
-constexpr int PICK_WAVES = 16, PICK_THREADS = 64 * PICK_WAVES;
+constexpr int PICK_WAVES = 8, PICK_THREADS = 64 * PICK_WAVES;
 constexpr int VOCAB_MAX = 1 << 28;                       // 2^14 stretches
 constexpr int KEEP_MAX = 64;                             // of beams too: one a lane
 
@@ -30,130 +30,175 @@ __device__ __forceinline__ uint4 load16(const void* p) {                        
 __device__ __forceinline__ unsigned word(const uint4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 __device__ __forceinline__ unsigned byte(const uint4& v, int i) { return (word(v, i >> 2) >> (8 * (i & 3))) & 255u; }
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
+// a byte by an index that the compiler does not know
+__device__ __forceinline__ unsigned byte_at(const uint4& v, int i) {
+  const unsigned x = v.x, y = v.y, z = v.z, w = v.w;     // values: of lvalues ?: selects an address, which keeps v in memory
+  const unsigned a = i & 4 ? y : x, b = i & 4 ? w : z;
+  return (i & 8 ? b : a) >> (8 * (i & 3)) & 255u;
 }
 
-// One wave's 4096 logits of a row: registers, histogram, and its share of the stretch's k best. W waves share a stretch, each with a
-// histogram of its own (counts of a value below, of its allowed tokens above bit 16).
+template <int W>
+__device__ __forceinline__ void together() {             // what the W waves of a stretch wrote to LDS is there
+  if constexpr (W > 1) __syncthreads();
+  else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// The want-th best of the values that a histogram counts, and how many lie above it; -1 and all of them where there are no more.
+struct Edge {
+  int value, higher;
+  __device__ __forceinline__ Edge(const unsigned* hist, int want) {
+    const int lane = threadIdx.x & 63;
+    const uint4 c = ((const uint4*)hist)[lane];
+    const int mine = (int)(c.x + c.y + c.z + c.w);
+    const int upto = wave_scan(mine), all = __builtin_amdgcn_readlane(upto, 63);
+    const int above = all - upto + mine;                 // of the lane's four values and higher ones
+    value = -1, higher = all;
+    if (higher <= want) return;
+    int e = 3, h = above - mine;
+#pragma unroll
+    for (int i = 3; i > 0; --i) {
+      const int n = (int)word(c, i);
+      if (e == i && h + n < want) h += n, e = i - 1;
+    }
+    const int at = 63 - __builtin_clzll(__ballot(above >= want));
+    value = 4 * at + __builtin_amdgcn_readlane(e, at), higher = __builtin_amdgcn_readlane(h, at);
+  }
+};
+
+// What the W waves of a stretch share: counts of all values, of those of allowed tokens (near the best), and each wave's finds.
+template <int W>
+struct alignas(16) Shared {
+  unsigned hist[256], fit[256];
+  int high[W], equal[W];
+};
+
+// One wave's 4096 logits of a row, in registers, and its share of the stretch's `keep` best.
 template <int W>
 struct Stretch {
   uint4 u[BLOCKS];                                       // logits + 128; block b, lane l: tokens 1024 b + 16 l ..
-  unsigned mask[BLOCKS];                                 // allowed ones
+  int have[BLOCKS];                                      // of them the row has
+  unsigned valid[BLOCKS];                                // the same as `from` says it
 
-  __device__ __forceinline__ void count(const int8_t* x, const uint8_t* allowed, int n, unsigned* hist) {
+  __device__ __forceinline__ Stretch(const int8_t* x, int n) {
     const int lane = threadIdx.x & 63;
-    for (int i = lane; i < 256; i += 64) hist[i] = 0;
-    int have[BLOCKS];
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
+    static_for<BLOCKS>([&](auto b) {
       const int at = 1024 * b + 16 * lane;
       have[b] = min(16, max(0, n - at));
+      valid[b] = 0x0F0F0F0Fu;
       uint4 v = {0, 0, 0, 0};
-      unsigned m = (1u << have[b]) - 1u;
       if (have[b] == 16) {
         v = load16(x + at);
-        if (allowed) {
-          const uint4 ok = load16(allowed + at);
-          m = 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) m |= (byte(ok, i) ? 1u : 0u) << i;
-        }
       } else {
         unsigned w[4] = {0, 0, 0, 0};
+        valid[b] = 0;
         for (int i = 0; i < have[b]; ++i) {
           const unsigned xi = (uint8_t)x[at + i];
+          valid[b] |= 1u << (8 * (i & 3) + (i >> 2));
 #pragma unroll
           for (int j = 0; j < 4; ++j) w[j] |= (i >> 2) == j ? xi << (8 * (i & 3)) : 0u;
-          if (allowed && !allowed[at + i]) m &= ~(1u << i);
         }
         v = {w[0], w[1], w[2], w[3]};
       }
       u[b] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
-      mask[b] = m;
-    }
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < have[b]) atomicAdd(&hist[byte(u[b], i)], 1u + ((mask[b] >> i & 1u) << 16));
+    });
   }
 
-  // The wave's share of the `keep` best of all W waves' tokens into list (keep entries, cleared where there are fewer).
-  __device__ __forceinline__ void collect(const unsigned* hists, int wave, int keep, int token0, u64* list) const {
-    const int lane = threadIdx.x & 63;
-    int c[4], lane_sum = 0;
+  __device__ __forceinline__ void count(unsigned* hist) const {
+    static_for<BLOCKS>([&](auto b) {
+      if (have[b] == 16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[i] = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) c[i] += hists[256 * w + 4 * lane + i] >> 16;
-      lane_sum += c[i];
-    }
-    int above = lane_sum;                                // allowed tokens of this lane's values and higher ones
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int y = __shfl_down(above, d);
-      if (lane + d < 64) above += y;
-    }
-    const int all = __builtin_amdgcn_readfirstlane(above);
-    int edge = -1, higher = all;                         // the k-th best value, and how many lie above it
-    if (all > keep) {
-      int e = 0, h = above - lane_sum;
-      bool found = false;
-#pragma unroll
-      for (int i = 3; i >= 0; --i)
-        if (!found) {
-          if (h + c[i] >= keep) found = true, e = 4 * lane + i;
-          else h += c[i];
+        for (int i = 0; i < 16; ++i) atomicAdd(&hist[byte(u[b], i)], 1u);
+      } else {
+        for (int i = 0; i < have[b]; ++i) {
+          atomicAdd(&hist[byte_at(u[b], i)], 1u);
         }
-      const int at = 63 - __builtin_clzll(__ballot(above >= keep));
-      edge = __builtin_amdgcn_readlane(e, at), higher = __builtin_amdgcn_readlane(h, at);
+      }
+    });
+  }
+
+  // A bit for each of a block's tokens whose value is at least `least`: bit 8 i + j is token 4 j + i, so that four bytes at a time the
+  // carry out of 7 bits and the eighth decide it. Tokens that the row has not are 0 bits.
+  template <int b>
+  __device__ __forceinline__ unsigned from(int least) const {
+    const unsigned add = (0x80u - ((unsigned)least & 0x7Fu)) * 0x01010101u, upper = least >= 128 ? 0u : ~0u;
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned w = word(u[b], j), t = (w & 0x7F7F7F7Fu) + add;
+      const unsigned ge = (w & t) | ((w | t) & upper);   // least >= 128: both bits, else one of them
+      m |= (ge & 0x80808080u) >> (7 - j);
     }
-    int high_at = 0, edge_at = 0;                        // of the waves before this one
+    return least > 255 ? 0 : m & valid[b];
+  }
+  // the tokens of such a mask in order, a bit each
+  static __device__ __forceinline__ unsigned in_order(unsigned m) {
+    unsigned r = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r |= (((m >> j & 0x01010101u) * 0x01020408u) >> 24 & 15u) << (4 * j);
+    return r;
+  }
+
+  // The stretch's `keep` best allowed tokens into list (zeros where there are fewer), the waves' together. s.hist holds the counts.
+  __device__ __forceinline__ void collect(Shared<W>& s, int wave, const uint8_t* allowed, int keep, int token0, u64* list) const {
+    const int lane = threadIdx.x & 63;
+    unsigned mask[BLOCKS];
+    // with forbidden tokens the best 2 keep + 32 of all hold the best `keep` allowed ones, but for the rare row that is looked
+    // through whole
+    Edge edge(s.hist, allowed ? 2 * keep + 32 : keep);
+    for (int least = max(edge.value, 0);; least = 0) {
+      static_for<BLOCKS>([&](auto b) {
+        mask[b] = from<b>(least);
+        if (!allowed) return;
+        for (unsigned todo = mask[b]; todo; todo &= todo - 1) {
+          const int bit = __builtin_ctz(todo), i = 4 * (bit & 3) + (bit >> 3);
+          if (allowed[1024 * b + 16 * lane + i]) atomicAdd(&s.fit[byte_at(u[b], i)], 1u);
+          else mask[b] &= ~(1u << bit);
+        }
+      });
+      if (!allowed) break;
+      together<W>();
+      const Edge fit(s.fit, keep);
+      edge = fit;
+      if (least == 0 || fit.higher >= keep || fit.value >= 0) break;
+      together<W>();                                     // every wave has read the counts
+      for (int i = threadIdx.x & (64 * W - 1); i < 256; i += 64 * W) s.fit[i] = 0;
+      together<W>();
+    }
+    const int at_edge = edge.value < 0 ? 0 : keep - edge.higher;
+    unsigned equal[BLOCKS];
+    int highs = 0, equals = 0;
+    static_for<BLOCKS>([&](auto b) {
+      equal[b] = 0;
+      if (edge.value >= 0 && __ballot(mask[b])) {
+        const unsigned above = mask[b] & from<b>(edge.value + 1);
+        equal[b] = mask[b] & ~above & from<b>(edge.value);
+        mask[b] = above;
+      }
+      highs += __builtin_popcount(mask[b]), equals += __builtin_popcount(equal[b]);
+    });
+    int high_at = 0, equal_at = 0;                       // of the waves before this one
     if constexpr (W > 1) {
-      int before = 0;
-      for (int w = 0; w < wave; ++w) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) before += 4 * lane + i > edge ? (int)(hists[256 * w + 4 * lane + i] >> 16) : 0;
-        if (edge >= 0) edge_at += hists[256 * w + edge] >> 16;
-      }
-      high_at = wave_sum(before);
+      const int high_sum = __builtin_amdgcn_readlane(wave_scan(highs), 63), equal_sum = __builtin_amdgcn_readlane(wave_scan(equals), 63);
+      if (lane == 0) s.high[wave] = high_sum, s.equal[wave] = equal_sum;
+      together<W>();
+      for (int w = 0; w < wave; ++w) high_at += s.high[w], equal_at += s.equal[w];
     }
-    const int at_edge = edge < 0 ? 0 : keep - higher;
     if (wave == 0)
-      for (int i = higher + at_edge + lane; i < keep; i += 64) list[i] = 0;
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
-      unsigned high = 0, equal = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int v = (int)byte(u[b], i);
-        high |= (v > edge ? 1u : 0u) << i;
-        equal |= (v == edge ? 1u : 0u) << i;
+      for (int i = edge.higher + at_edge + lane; i < keep; i += 64) list[i] = 0;
+    int h = high_at + wave_scan(highs) - highs;          // where the lane's higher ones go, in any order
+    static_for<BLOCKS>([&](auto b) {
+      for (unsigned todo = mask[b]; todo; todo &= todo - 1) {
+        const int bit = __builtin_ctz(todo), i = 4 * (bit & 3) + (bit >> 3);
+        list[h++] = key_of(byte_at(u[b], i), token0 + 1024 * b + 16 * lane + i);
       }
-      high &= mask[b], equal &= edge_at < at_edge ? mask[b] : 0;
-      if (!__ballot(high | equal)) continue;
-      const int mine = __builtin_popcount(high) | __builtin_popcount(equal) << 16;
-      int sum = mine;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(sum, d);
-        if (lane >= d) sum += y;
-      }
-      int h = high_at + ((sum - mine) & 0xFFFF), e = edge_at + ((sum - mine) >> 16);
-      const int total = __builtin_amdgcn_readlane(sum, 63);
-      high_at += total & 0xFFFF, edge_at += total >> 16;
-      for (unsigned todo = high | equal; todo; todo &= todo - 1) {
-        const int i = __builtin_ctz(todo);
-        const unsigned v = i < 8 ? (i < 4 ? u[b].x : u[b].y) : (i < 12 ? u[b].z : u[b].w);
-        const u64 key = key_of(v >> (8 * (i & 3)) & 255u, token0 + 1024 * b + 16 * lane + i);
-        if (high >> i & 1u) list[h++] = key;
-        else if (e < at_edge) list[higher + e++] = key;
-      }
-    }
+      const unsigned same = equal_at < at_edge ? equal[b] : 0;                   // those at the edge in token order
+      if (!__ballot(same)) return;
+      const int mine = __builtin_popcount(same), upto = wave_scan(mine);
+      int e = equal_at + upto - mine;
+      equal_at += __builtin_amdgcn_readlane(upto, 63);
+      for (unsigned todo = in_order(same); todo && e < at_edge; todo &= todo - 1)
+        list[edge.higher + e++] = key_of((unsigned)edge.value, token0 + 1024 * b + 16 * lane + __builtin_ctz(todo));
+    });
   }
 };
 
@@ -260,20 +305,19 @@ __device__ __forceinline__ void pick(const anvil_beams& b, int group, const u64*
 
 // One stretch of a row a workgroup (blockIdx: row, stretch).
 __global__ __launch_bounds__(PART_THREADS) void beam_part_kernel(anvil_beams b, u64* lists, unsigned* hists, int parts) {
-  __shared__ unsigned hist[PART_WAVES * 256];
+  __shared__ Shared<PART_WAVES> s;
   const long long row = blockIdx.x;
   const int part = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
+  const int token0 = part * PART_TOKENS + wave * WAVE_TOKENS;
+  const Stretch<PART_WAVES> x(b.logits + row * b.ld + token0, b.vocab - token0);
   const BeamRow r(b, row);
   if (!r.live) return;                                   // the joining workgroup does not read its lists
-  const int token0 = part * PART_TOKENS + wave * WAVE_TOKENS;
-  Stretch<PART_WAVES> s;
-  s.count(b.logits + row * b.ld + token0, b.allowed ? b.allowed + token0 : nullptr, b.vocab - token0, hist + 256 * wave);
+  s.hist[tid] = 0, s.fit[tid] = 0;
   __syncthreads();
-  s.collect(hist, wave, b.keep, token0, lists + (row * parts + part) * b.keep);
-  unsigned sum = 0;
-#pragma unroll
-  for (int w = 0; w < PART_WAVES; ++w) sum += hist[256 * w + tid] & 0xFFFFu;
-  hists[(row * parts + part) * 256 + tid] = sum;
+  x.count(s.hist);
+  __syncthreads();
+  hists[(row * parts + part) * 256 + tid] = s.hist[tid];
+  x.collect(s, wave, b.allowed ? b.allowed + token0 : nullptr, b.keep, token0, lists + (row * parts + part) * b.keep);
 }
 
 // One group a workgroup, a wave a row: its stretches' histograms and lists joined, then the rows'.
@@ -281,24 +325,34 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_join_kernel(anvil_beams b, 
                                                                  unsigned* flags) {
   __shared__ u64 sorted[KEEP_MAX * KEEP_MAX];
   __shared__ long long bases[KEEP_MAX];
-  const int group = blockIdx.x, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x >> 6; i < b.beams; i += PICK_WAVES) {
+  const int group = blockIdx.x, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  for (int i = threadIdx.x >> 6; i < b.beams; i += waves) {
     const long long row = (long long)group * b.beams + i;
     BeamRow r(b, row);
     u64 key = 0;
     if (r.live) {
+      const long long n = (long long)parts * b.keep;
+      const u64* all = lists + row * n;
+      u64 next = lane < n ? all[lane] : 0;               // on its way beside the histograms
       unsigned count[4] = {0, 0, 0, 0};
-      for (int p = 0; p < parts; ++p) {
-        const uint4 x = ((const uint4*)(hists + (row * parts + p) * 256))[lane];
-        count[0] += x.x, count[1] += x.y, count[2] += x.z, count[3] += x.w;
+      for (int p = 0; p < parts; p += 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          x[k] = {0, 0, 0, 0};
+          if (p + k < parts) x[k] = ((const uint4*)(hists + (row * parts + p + k) * 256))[lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) count[0] += x[k].x, count[1] += x[k].y, count[2] += x[k].z, count[3] += x[k].w;
       }
       r.weigh(b, count, flags);
-    }
-    if (r.live) {
-      const long long n = (long long)parts * b.keep;
-      for (long long at = 0; at < n; at += 64) {
-        const u64 next = sort_down(at + lane < n ? lists[row * n + at + lane] : 0);
-        key = at ? merge_down(key, next) : next;
+      if (r.live) {
+        for (long long at = 64;; at += 64) {
+          const u64 now = sort_down(next);
+          key = at > 64 ? merge_down(key, now) : now;
+          if (at >= n) break;
+          next = at + lane < n ? all[at + lane] : 0;
+        }
       }
     } else if (r.ended && lane == 0) {
       key = key_of(128, b.eos);                          // a logit of 0: its own score
@@ -314,25 +368,27 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_join_kernel(anvil_beams b, 
 __global__ __launch_bounds__(PICK_THREADS) void beam_small_kernel(anvil_beams b, unsigned* flags) {
   __shared__ u64 sorted[KEEP_MAX * KEEP_MAX];
   __shared__ long long bases[KEEP_MAX];
-  __shared__ unsigned hists[PICK_WAVES * 256];
-  const int group = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned* hist = hists + 256 * wave;
-  for (int i = wave; i < b.beams; i += PICK_WAVES) {
+  __shared__ Shared<1> shared[PICK_WAVES];
+  const int group = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  Shared<1>& s = shared[wave];
+  for (int i = wave; i < b.beams; i += waves) {
     const long long row = (long long)group * b.beams + i;
     BeamRow r(b, row);
     u64* list = sorted + i * b.keep;
     u64 key = 0;
     if (r.live) {
-      Stretch<1> s;
-      s.count(b.logits + row * b.ld, b.allowed, b.vocab, hist);
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      s.collect(hist, 0, b.keep, 0, list);
-      unsigned count[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) count[j] = hist[4 * lane + j] & 0xFFFFu;
+      const Stretch<1> x(b.logits + row * b.ld, b.vocab);
+      for (int j = lane; j < 256; j += 64) s.hist[j] = 0, s.fit[j] = 0;
+      together<1>();
+      x.count(s.hist);
+      together<1>();
+      const uint4 c = ((const uint4*)s.hist)[lane];
+      const unsigned count[4] = {c.x, c.y, c.z, c.w};
+      x.collect(s, 0, b.allowed, b.keep, 0, list);
+      together<1>();
       r.weigh(b, count, flags);
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       if (r.live) key = sort_down(lane < b.keep ? list[lane] : 0);
+      together<1>();
     }
     if (r.ended && lane == 0) key = key_of(128, b.eos);
     if (lane < b.keep) list[lane] = key;
@@ -363,8 +419,9 @@ extern "C" int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b) {
       (uintptr_t)b->parent % 4 || (uintptr_t)b->token % 4)
     return set_error(ANVIL_E_VALUE, "%s: a pointer is not aligned to its type", who);
   if (int r = check_ctx(ctx)) return r;
+  const unsigned pick_threads = 64u * (unsigned)(b->beams < PICK_WAVES ? b->beams : PICK_WAVES);
   if (b->vocab <= WAVE_TOKENS) {
-    ANVIL_LAUNCH(beam_small_kernel, dim3((unsigned)b->groups), dim3(PICK_THREADS), 0, ctx->stream, *b, ctx->flags);
+    ANVIL_LAUNCH(beam_small_kernel, dim3((unsigned)b->groups), dim3(pick_threads), 0, ctx->stream, *b, ctx->flags);
     ANVIL_LAUNCHED();
     return ANVIL_OK;
   }
@@ -376,7 +433,7 @@ extern "C" int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b) {
   ANVIL_LAUNCH(beam_part_kernel, dim3((unsigned)rows, (unsigned)parts), dim3(PART_THREADS), 0, ctx->stream, *b, (u64*)(ws + bytes),
                (unsigned*)ws, parts);
   ANVIL_LAUNCHED();
-  ANVIL_LAUNCH(beam_join_kernel, dim3((unsigned)b->groups), dim3(PICK_THREADS), 0, ctx->stream, *b, (const u64*)(ws + bytes),
+  ANVIL_LAUNCH(beam_join_kernel, dim3((unsigned)b->groups), dim3(pick_threads), 0, ctx->stream, *b, (const u64*)(ws + bytes),
                (const unsigned*)ws, parts, ctx->flags);
   ANVIL_LAUNCHED();
   return ANVIL_OK;

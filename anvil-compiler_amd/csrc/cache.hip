@@ -200,12 +200,7 @@ constexpr int META = 1024;                               // threads of the workg
 __device__ __forceinline__ int prefix(int v, int& total) {
   __shared__ int sums[META / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  const int x = wave_scan(v);
   __syncthreads();                                       // the last call's sums have been read
   if (lane == 63) sums[wave] = x;
   __syncthreads();

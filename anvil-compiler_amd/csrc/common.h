@@ -317,6 +317,18 @@ __device__ __forceinline__ int lane_group_sum(int v) {                   // sum 
   return v;
 }
 
+// inclusive sums over the lanes of a wave, in data-parallel moves (a shuffle goes through LDS and takes some ten times as long)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_scan_step(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_scan_step<0x111, 0xF>(v);                          // row_shr:1, 2, 4, 8: within rows of 16
+  v = dpp_scan_step<0x112, 0xF>(v);
+  v = dpp_scan_step<0x114, 0xF>(v);
+  v = dpp_scan_step<0x118, 0xF>(v);
+  v = dpp_scan_step<0x142, 0xA>(v);                          // row_bcast:15 into rows 1 and 3
+  return dpp_scan_step<0x143, 0xC>(v);                       // row_bcast:31 into rows 2 and 3
+}
+
 __device__ __forceinline__ unsigned sra_pack4v(int x0, int x1, int x2, int x3, int sh) {   // shift per lane
   unsigned d;
   asm("v_ashrrev_i32_sdwa %0, %1, %2 dst_sel:BYTE_0 dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:DWORD"
