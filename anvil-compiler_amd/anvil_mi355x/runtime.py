@@ -189,7 +189,10 @@ def _ptr(x) -> int:
 
 def _opt(x):
     """A pointer argument that may be None."""
-    return None if x is None else _ptr(x)
+    return x.ptr if isinstance(x, DeviceBuffer) else x
+
+
+_Strides4 = C.c_int64 * 4
 
 
 class DeviceBuffer:
@@ -522,18 +525,18 @@ class Device:
     def cache_append(self, cache, layer, K, V, starts, rows, max_new, strides):
         """anvil_cache_append_i4: int8 K and V rows of new tokens into their pages; strides (k row, k head, v row, v head)."""
         self.lib.call("anvil_cache_append_i4", self.ctx, C.byref(cache), layer, _opt(K), _opt(V), _opt(starts), rows,
-                      max_new, (C.c_int64 * 4)(*strides))
+                      max_new, _Strides4(*strides))
 
     def cache_read(self, cache, layer, K, V, starts, rows, max_new, strides):
         """anvil_cache_read_i4: the values that the cache holds for those rows."""
         self.lib.call("anvil_cache_read_i4", self.ctx, C.byref(cache), layer, _opt(K), _opt(V), _opt(starts), rows,
-                      max_new, (C.c_int64 * 4)(*strides))
+                      max_new, _Strides4(*strides))
 
     def attention_cache(self, cache, layer, Q, O, starts, rows, max_new, heads, strides, ms, ss, lut, one, mo, so, window=0,
                         sinks=0):
         """anvil_attention_cache_i4: the newest tokens' queries over the cache; strides (q row, q head, o row, o head)."""
         self.lib.call("anvil_attention_cache_i4", self.ctx, C.byref(cache), layer, _opt(Q), _opt(O), _opt(starts), rows,
-                      max_new, heads, (C.c_int64 * 4)(*strides), ms, ss, _opt(lut), one, mo, so, window, sinks)
+                      max_new, heads, _Strides4(*strides), ms, ss, _opt(lut), one, mo, so, window, sinks)
 
     def cache_fork(self, cache, out, parent=None, add=None, window=0, sinks=0):
         """anvil_cache_fork: the tables of the next step into `out`'s."""
