@@ -1253,6 +1253,14 @@ class CompiledModel:
                   "hip_graph": bool(graph) and not profile}
         return RunOutput(outs[0], outs, ints, cycles, result, None, self._const_syms, self)
 
+    def decoder(self, rows, max_tokens=None, pages=None, window=0, sinks=0):
+        """A Decoder of this token model (decode.py): up to `rows` sequences token by token over a paged 4-bit cache of up to
+        max_tokens tokens each (default: the position table's), in `pages` pages of 64 tokens (default: enough for every row);
+        window > 0: a token sees the last `window` tokens and the first `sinks`. The reference has no incremental form of
+        CompiledModel.run (anvil/driver.py:305-322)."""
+        from .decode import Decoder
+        return Decoder(self, rows, max_tokens, pages, window, sinks)
+
     def summary(self) -> str:
         plan = self.plan(1)
         return "\n".join(f"{label:>16} {getattr(fn, '__name__', str(fn))}" for label, fn, _ in plan.steps)

@@ -91,6 +91,7 @@ SIGNATURES = {
     "anvil_cache_append_i4": [_p, _p, _i, _p, _p, _p, _i, _i, _p],
     "anvil_cache_read_i4": [_p, _p, _i, _p, _p, _p, _i, _i, _p],
     "anvil_attention_cache_i4": [_p, _p, _i, _p, _p, _p, _i, _i, _i, _p, _i32, _i, _p, _i32, _i32, _i, _i, _i],
+    "anvil_embed_quantize_new": [_p, _p, _p, _p, _i, _i, _i, _p, _i, _p, _i, _f64, _p, _i],
     "anvil_cache_fork": [_p, _p, _p, _p, _p, _i, _i],
     "anvil_cache_compact": [_p, _p, _p, _p],
     "anvil_beam_select_i8": [_p, _p],
@@ -119,6 +120,7 @@ class RowOp(C.Structure):
 
 
 CACHE_PAGE = 64                              # tokens of a cache page
+CACHE_ROWS_MAX = 4096                        # sequences of a cache's tables
 
 
 class Cache(C.Structure):
@@ -522,6 +524,12 @@ class Device:
                       DTYPE_CODE[out_dtype])
 
     # ------------------------------------------------------------------------------------------ decoding
+    def cache_bytes(self, layers, pages, heads, dim) -> int:
+        """anvil_cache_bytes: the bytes of a pool."""
+        n = C.c_longlong()
+        self.lib.call("anvil_cache_bytes", layers, pages, heads, dim, C.byref(n))
+        return n.value
+
     def cache_append(self, cache, layer, K, V, starts, rows, max_new, strides):
         """anvil_cache_append_i4: int8 K and V rows of new tokens into their pages; strides (k row, k head, v row, v head)."""
         self.lib.call("anvil_cache_append_i4", self.ctx, C.byref(cache), layer, _opt(K), _opt(V), _opt(starts), rows,
@@ -537,6 +545,11 @@ class Device:
         """anvil_attention_cache_i4: the newest tokens' queries over the cache; strides (q row, q head, o row, o head)."""
         self.lib.call("anvil_attention_cache_i4", self.ctx, C.byref(cache), layer, _opt(Q), _opt(O), _opt(starts), rows,
                       max_new, heads, _Strides4(*strides), ms, ss, _opt(lut), one, mo, so, window, sinks)
+
+    def embed_quantize_new(self, cache, ids, starts, rows, max_new, Cdim, wte, vocab, wpe, positions, scale, out, out_dtype):
+        """anvil_embed_quantize_new: the quantized embeddings of new tokens (int32 ids) at their positions."""
+        self.lib.call("anvil_embed_quantize_new", self.ctx, C.byref(cache), _opt(ids), _opt(starts), rows, max_new, Cdim,
+                      _opt(wte), vocab, _opt(wpe), positions, float(scale), _opt(out), DTYPE_CODE[out_dtype])
 
     def cache_fork(self, cache, out, parent=None, add=None, window=0, sinks=0):
         """anvil_cache_fork: the tables of the next step into `out`'s."""

@@ -25,7 +25,7 @@ struct CacheView {
   uint8_t* pool;
   const int* table;
   const int* lens;
-  const int* starts;                                     // null: one row a sequence
+  const int* starts;                                     // null: one row a sequence that is not empty
   int seqs, slots, pages, heads, dim, rows, max_new;
   unsigned* flags;
 };
@@ -40,6 +40,7 @@ __device__ __forceinline__ bool new_rows(const CacheView& c, int s, NewRows& r, 
   r.len = c.lens[s];
   r.first = lo;
   r.n = 0;
+  if (!c.starts && r.len == 0) return true;              // an empty sequence has no row
   const bool ok = lo >= 0 && hi >= lo && hi <= c.rows && hi - lo <= c.max_new && r.len >= 0 &&
                   r.len <= c.slots * PAGE && hi - lo <= r.len;
   if (ok) r.n = hi - lo;

@@ -1,5 +1,6 @@
 // The 4-bit paged cache: new rows rounded into their pages, read back, and the page tables of the next step.
 #include <algorithm>
+#include <cmath>
 
 #include "cache.h"
 
@@ -231,6 +232,32 @@ static int rows_call(const char* who, anvil_ctx* ctx, const anvil_cache* cache, 
   });
   ANVIL_LAUNCHED();
   return ANVIL_OK;
+}
+
+// ------------------------------------------------------------------------------------------------- embedding
+
+struct EmbedArgs {
+  const int* ids;
+  const float *wte, *wpe;
+  int C, vocab, positions, lo, hi;
+  double scale;
+};
+
+// One token a workgroup (blockIdx: token of its sequence, striding, and sequence).
+template <typename TO>
+__global__ __launch_bounds__(256) void embed_new_kernel(CacheView c, EmbedArgs e, TO* out) {
+  NewRows r;
+  new_rows(c, blockIdx.y, r, blockIdx.x == 0 && threadIdx.x == 0);
+  for (int t = blockIdx.x; t < r.n; t += gridDim.x) {
+    const int id = e.ids[r.first + t], i = r.len - r.n + t;
+    const bool ok = id >= 0 && id < e.vocab && i < e.positions;
+    if (!ok && threadIdx.x == 0) raise_flag(c.flags, FLAG_RANGE);
+    for (int col = threadIdx.x; col < e.C; col += 256) {
+      double v = 0;
+      if (ok) v = rint(((double)e.wte[(long long)id * e.C + col] + (double)e.wpe[(long long)i * e.C + col]) / e.scale);
+      out[(long long)(r.first + t) * e.C + col] = (TO)(v < e.lo ? e.lo : (v > e.hi ? e.hi : v));
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------- fork and compact
@@ -551,6 +578,28 @@ int anvil_cache_append_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, c
 int anvil_cache_read_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, int8_t* K, int8_t* V, const int32_t* starts,
                         int rows, int max_new, const int64_t* strides) {
   return rows_call("anvil_cache_read_i4", ctx, cache, layer, K, V, starts, rows, max_new, strides, false);
+}
+
+int anvil_embed_quantize_new(anvil_ctx* ctx, const anvil_cache* cache, const int32_t* ids, const int32_t* starts, int rows,
+                             int max_new, int C, const float* wte, int vocab, const float* wpe, int positions, double scale,
+                             void* out, int out_dtype) {
+  const char* who = "anvil_embed_quantize_new";
+  CacheView c;
+  if (int r = cache_view(who, ctx, cache, 0, starts, rows, max_new, &c)) return r;
+  if (C < 1 || vocab < 1 || positions < 1) return set_error(ANVIL_E_VALUE, "%s: C %d, vocab %d, positions %d", who, C, vocab, positions);
+  if (!(scale > 0) || std::isinf(scale)) return set_error(ANVIL_E_VALUE, "%s: scale must be > 0", who);
+  if (out_dtype != ANVIL_I8 && out_dtype != ANVIL_I16) return set_error(ANVIL_E_VALUE, "%s: result dtype must be i8 or i16", who);
+  if (!c.seqs || !rows) return check_ctx(ctx);
+  if (!ids || !wte || !wpe || !out) return set_error(ANVIL_E_VALUE, "%s: null pointer", who);
+  if ((uintptr_t)ids % 4 || (uintptr_t)wte % 4 || (uintptr_t)wpe % 4 || (uintptr_t)out % out_dtype)
+    return set_error(ANVIL_E_VALUE, "%s: a pointer is not aligned to its type", who);
+  if (int r = check_ctx(ctx)) return r;
+  const EmbedArgs e{ids, wte, wpe, C, vocab, positions, dtype_lo(out_dtype), dtype_hi(out_dtype), scale};
+  const dim3 grid((unsigned)std::min(max_new, 4096), (unsigned)c.seqs);
+  if (out_dtype == ANVIL_I8) ANVIL_LAUNCH(embed_new_kernel<int8_t>, grid, dim3(256), 0, ctx->stream, c, e, (int8_t*)out);
+  else ANVIL_LAUNCH(embed_new_kernel<int16_t>, grid, dim3(256), 0, ctx->stream, c, e, (int16_t*)out);
+  ANVIL_LAUNCHED();
+  return ANVIL_OK;
 }
 
 int anvil_cache_fork(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* out, const int32_t* parent,

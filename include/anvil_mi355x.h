@@ -395,9 +395,9 @@ int anvil_embed_quantize(anvil_ctx* ctx, const int64_t* ids, int64_t rows, int T
  *
  * Rows of new tokens. K, V, Q and O hold the new tokens of every sequence, packed: sequence s owns rows starts[s] ..
  * starts[s + 1] - 1 (starts: seqs + 1 device int32s, at most `rows` and non-decreasing, at most max_new rows each; NULL:
- * one row a sequence, rows = seqs and max_new = 1). Row starts[s] + t is the token at position lens[s] - n_s + t: lens
- * counts the new tokens already (anvil_cache_fork extends it). Rows behind the last sequence's are neither read nor
- * written. strides are in elements (bytes); one head's channels are contiguous.
+ * one row a sequence, rows = seqs and max_new = 1, where an empty sequence has none). Row starts[s] + t is the token at
+ * position lens[s] - n_s + t: lens counts the new tokens already (anvil_cache_fork extends it). Rows that no sequence
+ * owns are neither read nor written. strides are in elements (bytes); one head's channels are contiguous.
  *
  * The cache. A page holds ANVIL_CACHE_PAGE tokens of every head, and a pool of `layers` x `pages` pages holds layer l's
  * page p at byte (l * pages + p) * heads * 68 D, D the head dim (16 is stored as 32 with zero channels). The table's row s names
@@ -447,6 +447,14 @@ int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer
                              const int32_t* starts, int rows, int max_new, int heads_q, const int64_t* strides,
                              int32_t m_s, int s_s, const int32_t* lut, int32_t one, int32_t m_o, int s_o, int window,
                              int sinks);
+
+/* anvil_embed_quantize for the rows of new tokens: out[row][c] = clamp_out(rint((wte[ids[row]][c] + wpe[i][c]) / scale))
+ * with i the token's position (reference anvil/driver.py:233-241 on x = wte[ids] + wpe[positions]). ids are int32 (as
+ * anvil_beam_select_i8 writes them), wpe has `positions` rows. An id outside [0, vocab) or a position past the table
+ * stores zeros and is reported by anvil_sync as ANVIL_E_VALUE. */
+int anvil_embed_quantize_new(anvil_ctx* ctx, const anvil_cache* cache, const int32_t* ids, const int32_t* starts, int rows,
+                             int max_new, int C, const float* wte, int vocab, const float* wpe, int positions, double scale,
+                             void* out, int out_dtype);
 
 /* Page tables of the next step: row i of `out` continues row parent[i] of `in` (parent NULL: row i; -1: an empty row) by
  * add[i] >= 0 tokens (add NULL: none). `out` shares in's pool and has its slots; its table, lens and refs are other

@@ -43,8 +43,10 @@ def _check_type(op, val, lead=()):
     return val
 
 
-def run(m, inputs: dict, consts: dict | None = None, *, batch: bool = False, fast: bool = False) -> GraphResult:
-    """Evaluate the graph (reference interp/graph.py:43-92)."""
+def run(m, inputs: dict, consts: dict | None = None, *, batch: bool = False, fast: bool = False,
+        replace: dict | None = None) -> GraphResult:
+    """Evaluate the graph (reference interp/graph.py:43-92). replace: {sym: f}, values that the ops after it see as
+    f(value, values so far by sym)."""
     consts = consts or {}
     env, res = {}, GraphResult([])
     lead, nb, is_const = (), 0, set()
@@ -87,6 +89,8 @@ def run(m, inputs: dict, consts: dict | None = None, *, batch: bool = False, fas
             continue
         else:
             raise NotImplementedError(n)
+        if replace and op.sym_str in replace:
+            val = replace[op.sym_str](val, res.values)
         if n in ("anvil.graph.transpose", "anvil.graph.reshape") and op.x in is_const:
             is_const.add(op.results[0])
         env[op.results[0]] = _check_type(op, val, () if op.results[0] in is_const else lead)

@@ -433,7 +433,7 @@ def test_numbers_that_leave_their_range_are_reported_and_evaluate_nothing():
     pool = seqs.pool()
     q = dev.upload(np.ones((3, 2, 32), np.int8))
     lut = dev.upload(exp_lut().astype(np.int32))
-    for lens, starts, table in (([100, 5000, 70], None, None), ([100, -1, 70], None, None), ([100, 0, 70], None, None),
+    for lens, starts, table in (([100, 5000, 70], None, None), ([100, -1, 70], None, None), ([100, 0, 70], [0, 1, 2, 3], None),
                                 (None, [0, 1, 5, 3], None), (None, [0, 1, 0, 1], None), (None, [0, 1, 3, 4], None),
                                 (None, [-1, 1, 1, 2], None), (None, None, (1, 0, 99)), (None, None, (1, 0, -2))):
         t = seqs.table.copy()
