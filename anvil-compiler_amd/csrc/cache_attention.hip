@@ -461,71 +461,136 @@ struct Walk {
 };
 
 template <int CTRL, int ROWS>
-__device__ __forceinline__ unsigned long long dpp_add(unsigned long long v) {
-  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
-  return v + ((unsigned long long)hi << 32 | lo);
+__device__ __forceinline__ double dpp_add(double v) {     // 0 where the control names no lane
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xF, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
-__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {   // in every lane
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_max(int v) {
+  return max(v, __builtin_amdgcn_update_dpp(INT32_MIN, v, CTRL, ROWS, 0xF, false));
+}
+// over 64 or 16 lanes, in each of them
+template <int LANES>
+__device__ __forceinline__ double lanes_sum(double v) {
   v = dpp_add<0xB1, 0xF>(v);                             // quad_perm [1,0,3,2]
   v = dpp_add<0x4E, 0xF>(v);                             // quad_perm [2,3,0,1]
   v = dpp_add<0x141, 0xF>(v);                            // row_half_mirror
   v = dpp_add<0x140, 0xF>(v);                            // row_mirror: each row of 16 its sum
+  if constexpr (LANES == 16) return v;
   v = dpp_add<0x142, 0xA>(v);                            // row_bcast:15 into rows 1 and 3
   v = dpp_add<0x143, 0xC>(v);                            // row_bcast:31 into rows 2 and 3: lane 63 has them all
-  const unsigned lo = __builtin_amdgcn_readlane((int)v, 63), hi = __builtin_amdgcn_readlane((int)(v >> 32), 63);
-  return (unsigned long long)hi << 32 | lo;
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_readlane((int)u, 63), hi = __builtin_amdgcn_readlane((int)(u >> 32), 63);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+template <int LANES>
+__device__ __forceinline__ int lanes_max(int v) {
+  v = dpp_max<0xB1, 0xF>(v);
+  v = dpp_max<0x4E, 0xF>(v);
+  v = dpp_max<0x141, 0xF>(v);
+  v = dpp_max<0x140, 0xF>(v);
+  if constexpr (LANES == 16) return v;
+  v = dpp_max<0x142, 0xA>(v);
+  v = dpp_max<0x143, 0xC>(v);
+  return __builtin_amdgcn_readlane(v, 63);
 }
 
-// From a row's histogram (counts of scores 4 lane .. 4 lane + 3, less 128) its table in LDS, the lane's four entries: every operand is a whole number below 2^53, so double arithmetic is exact but for the quotient, which is put right by its remainder.
-template <int TABLE>
-__device__ __forceinline__ void probabilities(const uint4& count, const int* lut, int one, unsigned* flags, unsigned* table) {
-  const int lane = threadIdx.x & 63;
-  unsigned p[4] = {0, 0, 0, 0};
-  const int mine = count.w ? 3 : (count.z ? 2 : (count.y ? 1 : (count.x ? 0 : -1)));
-  const unsigned long long any = __ballot(mine >= 0);
-  if (any) {                                             // else the row sees nothing
-    const int at = 63 - __builtin_clzll(any), top = 4 * at + __builtin_amdgcn_readlane(mine, at);
-    int e[4];
-    unsigned long long sum = 0;
+// A row's table in place of its histogram, by LANES lanes (64 or 16, which stay together): lane l has counts 4 (l + LANES i) + j.
+//
+// p = floor(n / S) with n = e one + floor(S / 2), S the sum of e x count; whole numbers below 2^53, so sums in double are exact. For
+// S < 2^34 the quotient is e (one / S) + (floor(S / 2) / S + 2^-35), truncated. Two Newton steps leave 1 / S good to 2^-51 whatever
+// v_rcp_f64 is off by up to 2^-20, and with the roundings (2^-53 each) of a quotient below 2^15 the sum is off by less than
+// 2^15 (2^-51 + 2 2^-53) + 2^-51 < 2^-35: it is not below the quotient, and above it by less than 2^-34 < 1 / S, so no whole number
+// lies between the two. For a larger S the quotient is put right by its remainder.
+template <int TABLE, int LANES>
+__device__ __forceinline__ void probabilities(unsigned* table, const int* lut, int one, unsigned* flags) {
+  constexpr int N = 64 / LANES;
+  const int lane = threadIdx.x & (LANES - 1);
+  uint4 count[N];
+  int top = -1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int x = 4 * lane + i;
-      e[i] = x <= top ? max(0, lut[x - top + 255]) : 0;
-      sum += (unsigned long long)(unsigned)e[i] * word(count, i);
+  for (int i = 0; i < N; ++i) {
+    unsigned* h = table + 4 * (lane + LANES * i);        // rows start at any dword
+    count[i] = {h[0], h[1], h[2], h[3]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (word(count[i], j)) top = 4 * LANES * i + j;
+  }
+  top = lanes_max<LANES>(top < 0 ? -1 : top + 4 * lane);
+  unsigned p[N][4];
+  double e[N][4], S = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int x = min(4 * (lane + LANES * i) + j, max(top, 0)) - max(top, 0) + 255;        // larger scores do not occur
+      e[i][j] = (double)(unsigned)max(0, lut[x]);
+      S = __builtin_fma(e[i][j], (double)word(count[i], j), S);
     }
-    sum = wave_sum(sum);
-    if (!sum && lane == 0) raise_flag(flags, FLAG_ZERODIV);
-    if (sum) {
-      // the reciprocal is good to one part in 2^24 at least and the quotient below 2^15: one off at most
-      const double S = (double)sum, half = (double)(sum >> 1), inv = __builtin_amdgcn_rcp(S);
+  S = lanes_sum<LANES>(S);
+  if (S == 0) {                                          // nothing seen, or nothing but zeros
+    if (top >= 0 && lane == 0) raise_flag(flags, FLAG_ZERODIV);
+    S = 1;
+    one = 0;
+  }
+  const double half = __builtin_trunc(0.5 * S);
+  double inv = __builtin_amdgcn_rcp(S);
+  inv = __builtin_fma(inv, __builtin_fma(-S, inv, 1.0), inv);
+  inv = __builtin_fma(inv, __builtin_fma(-S, inv, 1.0), inv);
+  const double by = (double)one * inv, start = __builtin_fma(half, inv, 0x1p-35);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double n = __builtin_fma((double)e[i], (double)one, half);
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[i][j] = (unsigned)__builtin_fma(e[i][j], by, start);
+  if (S >= 0x1p34) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double n = __builtin_fma(e[i][j], (double)one, half);
         double k = __builtin_trunc(n * inv);
         const double rest = __builtin_fma(-k, S, n);
         k += rest < 0 ? -1.0 : (rest >= S ? 1.0 : 0.0);
-        p[i] = (unsigned)(int)k;
+        p[i][j] = (unsigned)k;
       }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = lane + LANES * i;
+    if constexpr (TABLE == TABLE_FIFTEEN) {              // a byte each of four tables
+      int x[4] = {(int)p[i][0], (int)p[i][1], (int)p[i][2], (int)p[i][3]};
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        int d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int up = (int)((unsigned)__umul24(x[j] + 7, 34953) >> 19);        // / 15, exact below 2^19 / 7
+          d[j] = x[j] - 15 * up, x[j] = up;
+        }
+        table[64 * v + at] = pack4(d[0], d[1], d[2], d[3]);
+      }
+    } else if constexpr (TABLE == TABLE_SEVEN) {
+      table[2 * at] = 2 * (p[i][0] & 127u) | (p[i][1] & 127u) << 17, table[2 * at + 1] = 2 * (p[i][2] & 127u) | (p[i][3] & 127u) << 17;
+      table[128 + 2 * at] = 2 * (p[i][0] >> 7) | (p[i][1] >> 7) << 17;
+      table[129 + 2 * at] = 2 * (p[i][2] >> 7) | (p[i][3] >> 7) << 17;
+    } else {
+      table[2 * at] = 2 * p[i][0] | p[i][1] << 17, table[2 * at + 1] = 2 * p[i][2] | p[i][3] << 17;
     }
   }
-  if constexpr (TABLE == TABLE_FIFTEEN) {                // a byte each of four tables
-    int x[4] = {(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      int d[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int up = (int)((unsigned)__umul24(x[i] + 7, 34953) >> 19);          // / 15, exact below 2^19 / 7
-        d[i] = x[i] - 15 * up, x[i] = up;
-      }
-      table[64 * v + lane] = pack4(d[0], d[1], d[2], d[3]);
-    }
-  } else if constexpr (TABLE == TABLE_SEVEN) {
-    table[2 * lane] = 2 * (p[0] & 127u) | (p[1] & 127u) << 17, table[2 * lane + 1] = 2 * (p[2] & 127u) | (p[3] & 127u) << 17;
-    table[128 + 2 * lane] = 2 * (p[0] >> 7) | (p[1] >> 7) << 17, table[129 + 2 * lane] = 2 * (p[2] >> 7) | (p[3] >> 7) << 17;
+}
+
+// The tables of a tile's rows. A wave takes a row at a time, or four where there are many: the sums over lanes and what is one number a row
+// cost a row less.
+template <int RP, bool WIDE>
+__device__ __forceinline__ void make_tables(unsigned* rows, int n_rows, const int* lut, int one, unsigned* flags) {
+  constexpr int TABLE = Digits<RP, WIDE>::TABLE;
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  if constexpr (RP == 16) {
+    for (int i = 4 * wave + ((threadIdx.x >> 4) & 3); i < n_rows; i += 4 * waves) probabilities<TABLE, 16>(rows + i * HIST, lut, one, flags);
   } else {
-    table[2 * lane] = 2 * p[0] | p[1] << 17, table[2 * lane + 1] = 2 * p[2] | p[3] << 17;
+    for (int i = wave; i < n_rows; i += waves) probabilities<TABLE, 64>(rows + i * HIST, lut, one, flags);
   }
 }
 
@@ -681,7 +746,6 @@ __global__ __launch_bounds__(64 * WAVES_MAX) void attend_tile_kernel(CacheView c
   const Early early(c, a, hist, true);
   Tile t;
   if (!find_tile(c, a, t)) return;
-  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
   const int entry = early.entries(c, a, t, 0, t.pages, true);
   {
     KeyWalk<NG, RP> keys(c, t, 0, t.pages, entry);
@@ -691,11 +755,7 @@ __global__ __launch_bounds__(64 * WAVES_MAX) void attend_tile_kernel(CacheView c
   }
   ValueWalk<NG> values(c, t, 0, t.pages, entry);         // on their way while the tables are made
   __syncthreads();
-  for (int i = tid >> 6; i < t.rows; i += waves) {       // the row's table takes its histogram's place
-    unsigned* h = hist + i * HIST;
-    const uint4 count = {h[4 * lane], h[4 * lane + 1], h[4 * lane + 2], h[4 * lane + 3]};
-    probabilities<Digits<RP, WIDE>::TABLE>(count, lut, a.one, c.flags, h);
-  }
+  make_tables<RP, WIDE>(hist, t.rows, lut, a.one, c.flags);
   __syncthreads();
   v4i acc[Digits<RP, WIDE>::SUMS][2 * NG] = {};
   add_pages<NG, RP, WIDE>(values, a, t, hist, scores, t.rows, acc);
@@ -765,11 +825,7 @@ __global__ __launch_bounds__(64 * WAVES_MAX) void attend_values_kernel(CacheView
     atomicAdd(h, sum.x), atomicAdd(h + 1, sum.y), atomicAdd(h + 2, sum.z), atomicAdd(h + 3, sum.w);
   }
   __syncthreads();
-  for (int i = tid >> 6; i < t.rows; i += waves) {
-    unsigned* h = tables + i * HIST;
-    const uint4 count = {h[4 * lane], h[4 * lane + 1], h[4 * lane + 2], h[4 * lane + 3]};
-    probabilities<Digits<RP, WIDE>::TABLE>(count, lut, a.one, c.flags, h);
-  }
+  make_tables<RP, WIDE>(tables, t.rows, lut, a.one, c.flags);
   __syncthreads();
   v4i acc[Digits<RP, WIDE>::SUMS][2 * NG] = {};
   add_pages<NG, RP, WIDE>(values, a, t, tables, (const unsigned*)a.scores + unit * a.bound * a.rows * (PAGE / 4), a.rows, acc);
