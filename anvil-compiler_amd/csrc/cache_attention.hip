@@ -45,20 +45,21 @@ typedef unsigned short __attribute__((may_alias)) u16_alias;
 // sinks, then from the window's first page on).
 struct Tile {
   NewRows r;
-  int seq, head, unit, tile, rows, lo, hi;               // rows in use; positions of its first and last token
+  int seq, head, unit, tile, first, rows, lo, hi;        // its first row, rows in use; positions of its first and last token
   int sink_pages, window_page, pages;
 };
 
+template <int ROWS = 16>
 __device__ __forceinline__ bool find_tile(const CacheView& c, const AttendArgs& a, Tile& t) {
   t.unit = blockIdx.x, t.tile = (int)blockIdx.y;
   t.seq = a.seq0 + t.unit / c.heads, t.head = t.unit % c.heads;
-  const int first = (a.tile0 + t.tile) * 16;
+  const int first = t.first = (a.tile0 + t.tile) * ROWS;
   new_rows(c, t.seq, t.r, first == 0 && blockIdx.z == 0 && t.head == 0 && threadIdx.x == 0);
   t.r.first = __builtin_amdgcn_readfirstlane(t.r.first), t.r.n = __builtin_amdgcn_readfirstlane(t.r.n);   // the same in every lane
   t.r.len = __builtin_amdgcn_readfirstlane(t.r.len);
   const long long all = (long long)t.r.n * a.group;
   if (first >= all) return false;
-  t.rows = (int)min(16ll, all - first);
+  t.rows = (int)min((long long)ROWS, all - first);
   t.lo = t.r.len - t.r.n + first / a.group;
   t.hi = t.r.len - t.r.n + (first + t.rows - 1) / a.group;
   t.window_page = a.window && t.lo >= a.window ? (t.lo - a.window + 1) >> PAGE_SHIFT : 0;
@@ -88,13 +89,13 @@ __device__ __forceinline__ bool whole(const Tile& t, const AttendArgs& a, int sl
   return last <= t.lo && (!a.window || first > t.hi - a.window || last < a.sinks);
 }
 
-// One row as its lanes know it: row l % 16 of the tile.
+// One row of the tile as its lanes know it.
 struct Row {
   int pos, after, sinks;                                 // sees keys <= pos that are > after or < sinks
   bool on;
   __device__ __forceinline__ Row(const Tile& t, const AttendArgs& a, int r) {
     on = r < t.rows;
-    pos = t.r.len - t.r.n + ((a.tile0 + t.tile) * 16 + r) / a.group;
+    pos = t.r.len - t.r.n + (t.first + r) / a.group;
     after = a.window ? pos - a.window : -1;
     sinks = a.sinks;
   }
@@ -192,9 +193,9 @@ struct Requant {
 template <int NG, int RP>
 struct Query {
   long w[NG];
-  __device__ __forceinline__ void load(const CacheView& c, const AttendArgs& a, const Tile& t, int lane) {
+  __device__ __forceinline__ void load(const CacheView& c, const AttendArgs& a, const Tile& t, int lane, int first = 0) {
     using C = Columns<NG, RP>;
-    const int col = lane & 15, row = col / C::VN, r = (a.tile0 + t.tile) * 16 + row, ch = 8 * (lane >> 4);
+    const int col = lane & 15, row = first + col / C::VN, r = t.first + row, ch = 8 * (lane >> 4);
     const int8_t* p = a.q + (long long)(t.r.first + r / a.group) * a.q_row + (long long)(t.head * a.group + r % a.group) * a.q_head + ch;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
@@ -298,7 +299,7 @@ __device__ __forceinline__ void count_scores(unsigned* hist, const Words<N>& sc,
 //   RP  8 WIDE   columns: p & 127, p >> 7; a product each for the low and the high digit
 //   RP 16        a product each for the low and the high digit of p x step
 //   RP 16 WIDE   products for both digits of p & 127 and of p >> 7, the middle two into one sum
-enum { TABLE_P = 1, TABLE_SEVEN = 2, TABLE_FIFTEEN = 4 };
+enum { TABLE_P = 1, TABLE_SEVEN = 2, TABLE_FIFTEEN = 4, TABLE_BYTES = 5, TABLE_PAIRS = 6 };
 template <int RP, bool WIDE>
 struct Digits {
   static constexpr int TABLE = RP == 4 ? TABLE_FIFTEEN : (RP == 8 && WIDE ? TABLE_SEVEN : TABLE_P);   // RP 16 takes 2 p apart itself
@@ -571,6 +572,13 @@ __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, i
         }
         table[64 * v + at] = pack4(d[0], d[1], d[2], d[3]);
       }
+    } else if constexpr (TABLE == TABLE_BYTES) {
+      table[at] = pack4((int)p[i][0], (int)p[i][1], (int)p[i][2], (int)p[i][3]);
+    } else if constexpr (TABLE == TABLE_PAIRS) {         // a low digit from -128 on and a high one, a byte each
+      unsigned d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = (p[i][j] & 255u) | ((p[i][j] + 128u) & 0xFF00u);
+      table[2 * at] = d[0] | d[1] << 16, table[2 * at + 1] = d[2] | d[3] << 16;
     } else if constexpr (TABLE == TABLE_SEVEN) {
       table[2 * at] = 2 * (p[i][0] & 127u) | (p[i][1] & 127u) << 17, table[2 * at + 1] = 2 * (p[i][2] & 127u) | (p[i][3] & 127u) << 17;
       table[128 + 2 * at] = 2 * (p[i][0] >> 7) | (p[i][1] >> 7) << 17;
@@ -583,11 +591,10 @@ __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, i
 
 // The tables of a tile's rows. A wave takes a row at a time, or four where there are many: the sums over lanes and what is one number a row
 // cost a row less.
-template <int RP, bool WIDE>
+template <int TABLE, bool MANY>
 __device__ __forceinline__ void make_tables(unsigned* rows, int n_rows, const int* lut, int one, unsigned* flags) {
-  constexpr int TABLE = Digits<RP, WIDE>::TABLE;
   const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  if constexpr (RP == 16) {
+  if constexpr (MANY) {
     for (int i = 4 * wave + ((threadIdx.x >> 4) & 3); i < n_rows; i += 4 * waves) probabilities<TABLE, 16>(rows + i * HIST, lut, one, flags);
   } else {
     for (int i = wave; i < n_rows; i += waves) probabilities<TABLE, 64>(rows + i * HIST, lut, one, flags);
@@ -616,19 +623,19 @@ __device__ __forceinline__ void spill(const v4i (&acc)[Digits<RP, WIDE>::SUMS][2
   }
 }
 
-// four results of a row from 16 x its sums
+// four results of a row from its sums
 __device__ __forceinline__ unsigned finish4(const v4i& sum, const AttendArgs& a) {
   int o[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const long long v = ((long long)(sum[e] >> 4) * a.m_o + round_term(a.s_o)) >> a.s_o;
+    const long long v = ((long long)sum[e] * a.m_o + round_term(a.s_o)) >> a.s_o;
     o[e] = v < -128 ? -128 : (v > 127 ? 127 : (int)v);
   }
   return pack4(o[0], o[1], o[2], o[3]);
 }
 
 __device__ __forceinline__ unsigned* out_word(const AttendArgs& a, const Tile& t, int r, int ch) {
-  const int at = (a.tile0 + t.tile) * 16 + r;
+  const int at = t.first + r;
   return (unsigned*)(a.o + (long long)(t.r.first + at / a.group) * a.o_row + (long long)(t.head * a.group + at % a.group) * a.o_head + ch);
 }
 
@@ -755,13 +762,13 @@ __global__ __launch_bounds__(64 * WAVES_MAX) void attend_tile_kernel(CacheView c
   }
   ValueWalk<NG> values(c, t, 0, t.pages, entry);         // on their way while the tables are made
   __syncthreads();
-  make_tables<RP, WIDE>(hist, t.rows, lut, a.one, c.flags);
+  make_tables<Digits<RP, WIDE>::TABLE, RP == 16>(hist, t.rows, lut, a.one, c.flags);
   __syncthreads();
   v4i acc[Digits<RP, WIDE>::SUMS][2 * NG] = {};
   add_pages<NG, RP, WIDE>(values, a, t, hist, scores, t.rows, acc);
   __syncthreads();                                       // the scores have been read
   join_waves<NG, RP, WIDE>(acc, (int*)scores, t, [&](int i, int ch, const v4i& s) {
-    if (ch < c.dim) *out_word(a, t, i, ch) = finish4(s, a);
+    if (ch < c.dim) *out_word(a, t, i, ch) = finish4(s >> 4, a);
   });
 }
 
@@ -825,7 +832,7 @@ __global__ __launch_bounds__(64 * WAVES_MAX) void attend_values_kernel(CacheView
     atomicAdd(h, sum.x), atomicAdd(h + 1, sum.y), atomicAdd(h + 2, sum.z), atomicAdd(h + 3, sum.w);
   }
   __syncthreads();
-  make_tables<RP, WIDE>(tables, t.rows, lut, a.one, c.flags);
+  make_tables<Digits<RP, WIDE>::TABLE, RP == 16>(tables, t.rows, lut, a.one, c.flags);
   __syncthreads();
   v4i acc[Digits<RP, WIDE>::SUMS][2 * NG] = {};
   add_pages<NG, RP, WIDE>(values, a, t, tables, (const unsigned*)a.scores + unit * a.bound * a.rows * (PAGE / 4), a.rows, acc);
@@ -850,10 +857,315 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(CacheView c, 
   for (int d = 4; d < 64; d *= 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += __shfl_xor(s[e], d);
-  if (threadIdx.x < 4) *out_word(a, t, r, ch) = finish4(s, a);
+  if (threadIdx.x < 4) *out_word(a, t, r, ch) = finish4(s >> 4, a);
+}
+
+// ---- many rows: pages made int8 once, in the workspace, then tiles of 32 rows
+//
+// Where a sequence has many rows its pages are worth multiplying out first: a score is then the product itself, a digit of p an
+// operand as it stands, and nothing is left between the products but the requant and the two tables. Scores are not kept but made again
+// in the second pass, so that a tile needs LDS for its histograms alone and has any length. 4 sequences of 32 heads over 8 of 128
+// channels, 1024 new tokens of 16384 each: 3149 us with tiles of 16 rows, 1217 with these; 2 of 512 new of up to 4096: 188 and 92.
+// What bounds it: instructions between the products (half of all cycles) and the LDS's conflicts on histograms and tables (as many).
+// Of that case's time with 16, 32, 48 and 64 rows a tile: 114, 92, 106, 100 us; with 2, 3, 4 and 8 waves 90, 114, 92, 105,
+// and with 2 a third more for short tiles.
+
+constexpr int WIDE_TILES = 2, WIDE_ROWS = 16 * WIDE_TILES, WIDE_WAVES = 4;
+constexpr int ONE_PAIR = 127 * 256 + 127;                // 32639: two digits, the low one from -128 on
+__device__ __forceinline__ unsigned mad_pair(unsigned a, unsigned b, unsigned c) {
+  return __builtin_bit_cast(unsigned, (v2u)(__builtin_bit_cast(v2u, a) * __builtin_bit_cast(v2u, b) + __builtin_bit_cast(v2u, c)));
+}
+
+// A lane's part of a page's keys: of keys 4 row + k, k in 0..3, the codes of 8 channels a group, and the steps.
+template <int NG>
+struct KeyRows {
+  Words<NG> code[4], step;
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t blk, int lane) {
+    const int row = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) code[k] = load_words<NG>(blk, (4 * row + k) * Block<NG>::ROW + 4 * q * NG);
+    step = load_words<NG>(blk, Block<NG>::K_STEPS + 4 * NG * row);
+  }
+  // Key k's values, four bytes a dword: two codes + 8 = u as a number u1 256 + u0, times the step, less 8 x 257 steps and with 128 added,
+  // so that the low byte does not borrow from the high one.
+  template <int k>
+  __device__ __forceinline__ void values(unsigned (&x)[2 * NG]) const {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const unsigned s = __builtin_amdgcn_perm(0, step.w[g], 0x0c000c00u | k << 16 | k), c = mad_pair(s, 0xF7F8F7F8u, 0x00800080u);
+      const unsigned u = code[k].w[g] ^ 0x88888888u;
+      x[2 * g] = mad_pair(u & 0x0F0F0F0Fu, s, c) ^ 0x00800080u;
+      x[2 * g + 1] = mad_pair((u >> 4) & 0x0F0F0F0Fu, s, c) ^ 0x00800080u;
+    }
+  }
+};
+
+// Group g's values, 16 keys of two channels: a product's low byte is that of its operands' low bytes, whatever lies above them.
+template <int NG>
+__device__ __forceinline__ void values_of(const ValuePage<NG>& v, int g, v4i (&x)[2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned u = v.code[g].w[i] ^ 0x88888888u, s0 = v.step[g].w[i], s1 = s0 >> 8;
+    const unsigned c0 = mul_pair(s0, 0xFFF8FFF8u), c1 = mul_pair(s1, 0xFFF8FFF8u);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const unsigned n = (half ? u >> 4 : u) & 0x0F0F0F0Fu;
+      x[half][i] = (int)__builtin_amdgcn_perm(mad_pair(n >> 8, s1, c1), mad_pair(n, s0, c0), 0x06020400u);
+    }
+  }
+}
+
+// A page in the workspace: the operands of its products, a lane's next to the next one's.
+template <int NG>
+struct Wide {
+  static constexpr int KN = NG == 1 ? 1 : NG / 2, KB = NG == 1 ? 8 : 16;         // products and bytes a lane of 16 keys
+  static constexpr int K = 64 * KB, V = 4 * KN * K, BYTES = V + 2 * NG * 1024;
+};
+
+// The pages that some new row of a sequence may see, numbered as a tile's are; a tile's own are among them.
+struct Span {
+  int sink_pages, window_page, pages;
+  __device__ __forceinline__ Span(const NewRows& r, const AttendArgs& a) {
+    const int lo = r.len - r.n;
+    window_page = a.window && lo >= a.window ? (lo - a.window + 1) >> PAGE_SHIFT : 0;
+    sink_pages = min((a.sinks + PAGE - 1) >> PAGE_SHIFT, window_page);
+    pages = sink_pages + ((r.len - 1) >> PAGE_SHIFT) - window_page + 1;
+  }
+  __device__ __forceinline__ int slot(int page) const { return page < sink_pages ? page : window_page + page - sink_pages; }
+  __device__ __forceinline__ int page(int slot) const { return slot < sink_pages ? slot : slot - window_page + sink_pages; }
+};
+
+// blockIdx: cache head of a sequence, page (a wave each, four a workgroup).
+template <int NG>
+__global__ __launch_bounds__(256) void attend_widen_kernel(CacheView c, AttendArgs a) {
+  const int unit = blockIdx.x, seq = a.seq0 + unit / c.heads, head = unit % c.heads, lane = threadIdx.x & 63;
+  const int page = 4 * (int)blockIdx.y + (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  NewRows r;
+  if (!new_rows(c, seq, r, blockIdx.y == 0 && head == 0 && threadIdx.x == 0) || !r.n) return;
+  const Span span(r, a);
+  if (page >= span.pages) return;
+  const uint8_t* blk = page_block<NG>(c, seq, span.slot(page), head, head == 0 && lane == 0);
+  if (!blk) return;
+  KeyRows<NG> k;
+  ValuePage<NG> v;
+  k.load(uniform_rsrc(blk, Block<NG>::BYTES), lane);
+  v.load(uniform_rsrc(blk, Block<NG>::BYTES), lane);
+  uint8_t* out = a.scores + ((long long)unit * a.bound + page) * Wide<NG>::BYTES;
+  static_for<4>([&](auto i) {
+    unsigned x[2 * NG];
+    k.template values<i>(x);
+    uint8_t* o = out + i * Wide<NG>::KN * Wide<NG>::K;
+    if constexpr (NG == 1) {
+      *(uint2*)(o + 8 * lane) = {x[0], x[1]};
+    } else {
+#pragma unroll
+      for (int n = 0; n < NG / 2; ++n) *(uint4*)(o + 1024 * n + 16 * lane) = {x[4 * n], x[4 * n + 1], x[4 * n + 2], x[4 * n + 3]};
+    }
+  });
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    v4i x[2];
+    values_of<NG>(v, g, x);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) *(v4i*)(out + Wide<NG>::V + 1024 * (2 * g + half) + 16 * lane) = x[half];
+  }
+}
+
+template <int NG>
+struct WideKeys {
+  static constexpr int N = Wide<NG>::KN, W = Wide<NG>::KB / 4;
+  Words<W> k[4][N];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t page, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) k[i][n] = load_words<W>(page, (i * N + n) * Wide<NG>::K + 4 * W * lane);
+  }
+};
+template <int NG>
+struct WideValues {
+  Words<4> v[2 * NG];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t page, int lane) {
+#pragma unroll
+    for (int m = 0; m < 2 * NG; ++m) v[m] = load_words<4>(page, Wide<NG>::V + 1024 * m + 16 * lane);
+  }
+};
+
+// A wave's pages of a tile in the workspace, as Walk's in the pool. step(page, its resource, ahead): ahead() when `page` is done with.
+template <int NG, int AHEAD>
+struct WideWalk {
+  WideKeys<NG> ring[AHEAD + 1];
+  const CacheView& c;
+  const Tile& t;
+  const Span span;
+  const uint8_t* base;
+  const int first, waves, lane;
+  int entry, n;
+
+  __device__ __forceinline__ WideWalk(const CacheView& view, const AttendArgs& a, const Tile& tile, int entries)
+      : c(view), t(tile), span(tile.r, a), base(a.scores + (long long)tile.unit * a.bound * Wide<NG>::BYTES),
+        first(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), lane(threadIdx.x & 63), entry(entries) {
+    n = min(64, (t.pages - first + waves - 1) / waves);
+    static_for<AHEAD>([&](auto d) { ring[d].load(page_of(first, d), lane); });
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t page_of(int at, int i) const {
+    const int e = i < n ? __builtin_amdgcn_readlane(entry, i & 63) : -1;
+    const int page = e < 0 ? 0 : span.page(slot_of(t, at + i * waves));
+    return uniform_rsrc(base + (long long)page * Wide<NG>::BYTES, e < 0 ? 0 : Wide<NG>::BYTES);
+  }
+  template <typename Step>
+  __device__ __forceinline__ void run(Step&& step) {
+    for (int at = first; at < t.pages; at += 64 * waves) {
+      if (at != first) {
+        entry = entry_of(c, t, at + lane * waves, t.pages);
+        n = min(64, (t.pages - at + waves - 1) / waves);
+        static_for<AHEAD>([&](auto d) { ring[d].load(page_of(at, d), lane); });
+      }
+      for (int i = 0; i < n; i += AHEAD + 1)
+        static_for<AHEAD + 1>([&](auto d) {
+          if (i + d < n) {
+            ring[(d + AHEAD) % (AHEAD + 1)].load(page_of(at, i + d + AHEAD), lane);
+            if (__builtin_amdgcn_readlane(entry, i + d) >= 0) step(ring[d], at + (i + d) * waves, page_of(at, i + d));
+          }
+        });
+    }
+  }
+};
+
+// f(tile r, e, k, score) for the lane's 16 keys 16 q + 4 e + k of the R rows that are its columns.
+template <int NG, int R, typename F>
+__device__ __forceinline__ void scores_of(const WideKeys<NG>& page, const Query<NG, 16> (&query)[R], const Requant& rq, F&& f) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      v4i d = {0, 0, 0, 0};
+      if constexpr (NG == 1) {
+        d = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((unsigned long)page.k[k][0].w[1] << 32 | page.k[k][0].w[0]), query[r].w[0], d, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NG / 2; ++n) {
+          const Words<4>& w = page.k[k][n];
+          const v4i keys = {(int)w.w[0], (int)w.w[1], (int)w.w[2], (int)w.w[3]};
+          const v4i rows = {(int)query[r].w[2 * n], (int)(query[r].w[2 * n] >> 32), (int)query[r].w[2 * n + 1], (int)(query[r].w[2 * n + 1] >> 32)};
+          d = __builtin_amdgcn_mfma_i32_16x16x64_i8(keys, rows, d, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(r, e, k, med3i(__mul24(d[e], rq.m) + rq.rnd, rq.lo, rq.hi) >> rq.s);
+    }
+}
+
+template <int NG, int ND>
+__global__ __launch_bounds__(64 * WIDE_WAVES) void attend_rows_kernel(CacheView c, AttendArgs a) {
+  constexpr int R = WIDE_TILES;
+  extern __shared__ __align__(16) unsigned lds[];
+  int* lut = (int*)lds;
+  unsigned* hist = lds + 256;
+  const Early early(c, a, hist, true);
+  Tile t;
+  if (!find_tile<WIDE_ROWS>(c, a, t)) return;
+  const int lane = threadIdx.x & 63, col = lane & 15, q = lane >> 4, wave = threadIdx.x >> 6;
+  const int entry = early.entries(c, a, t, 0, t.pages, true);
+  Query<NG, 16> query[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) query[r].load(c, a, t, lane, 16 * r);
+  const Requant rq(a.m_s, a.s_s);
+  {
+    WideWalk<NG, 1> keys(c, a, t, entry);
+    early.keep(lut);
+    __syncthreads();
+    unsigned* mine = hist + col * HIST + 128;            // of a score of 0
+    keys.run([&](const WideKeys<NG>& page, int n, __amdgpu_buffer_rsrc_t) {
+      const int slot = slot_of(t, n);
+      if (whole(t, a, slot)) {
+        scores_of<NG, R>(page, query, rq, [&](int r, int, int, int x) { atomicAdd(mine + 16 * HIST * r + x, 1u); });
+      } else {
+        unsigned mask[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) mask[r] = Row(t, a, 16 * r + col).mask(slot * PAGE + 16 * q);
+        scores_of<NG, R>(page, query, rq,
+                         [&](int r, int e, int k, int x) { atomicAdd(mine + 16 * HIST * r + x, mask[r] >> (4 * e + k) & 1u); });
+      }
+    });
+  }
+  WideWalk<NG, (R * NG * ND > 8 ? 0 : 1)> keys(c, a, t, entry);                  // on their way while the tables are made
+  __syncthreads();
+  make_tables<ND == 1 ? TABLE_BYTES : TABLE_PAIRS, true>(hist, t.rows, lut, a.one, c.flags);
+  __syncthreads();
+  v4i acc[R][2 * NG][ND] = {};
+  keys.run([&](const WideKeys<NG>& page, int n, __amdgpu_buffer_rsrc_t rsrc) {
+    WideValues<NG> v;
+    v.load(rsrc, lane);
+    unsigned p[R][4][ND] = {};                           // digits of 4 keys a dword, or both of two
+    if constexpr (ND == 1) {
+      const uint8_t* mine = (const uint8_t*)(hist + col * HIST) + 128;
+      scores_of<NG, R>(page, query, rq, [&](int r, int i, int k, int x) { p[r][i][0] |= (unsigned)mine[4 * 16 * HIST * r + x] << (8 * k); });
+    } else {
+      const u16_alias* mine = (const u16_alias*)(hist + col * HIST) + 128;
+      scores_of<NG, R>(page, query, rq,
+                       [&](int r, int i, int k, int x) { p[r][i][k >> 1] |= (unsigned)mine[2 * 16 * HIST * r + x] << (16 * (k & 1)); });
+    }
+    v4i digit[R][ND];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (ND == 1) {
+          digit[r][0][i] = (int)p[r][i][0];
+        } else {
+          digit[r][0][i] = (int)__builtin_amdgcn_perm(p[r][i][1], p[r][i][0], 0x06040200u);
+          digit[r][1][i] = (int)__builtin_amdgcn_perm(p[r][i][1], p[r][i][0], 0x07050301u);
+        }
+      }
+    const int slot = slot_of(t, n);
+    if (!whole(t, a, slot)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const unsigned mask = Row(t, a, 16 * r + col).mask(slot * PAGE + 16 * q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                    // a byte of ones a key that is seen
+          const unsigned seen = (((mask >> (4 * i) & 15u) * 0x00204081u) & 0x01010101u) * 255u;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) digit[r][d][i] &= (int)seen;
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < 2 * NG; ++m) {
+      const v4i x = {(int)v.v[m].w[0], (int)v.v[m].w[1], (int)v.v[m].w[2], (int)v.v[m].w[3]};
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[r][m][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, digit[r][d], acc[r][m][d], 0, 0, 0);
+    }
+  });
+  // the waves' sums, 16 rows at a time, where the tables were
+  constexpr int STRIDE = SUM_STRIDE<NG>;
+  int* red = (int*)hist;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    __syncthreads();
+    if (16 * r >= t.rows) break;
+#pragma unroll
+    for (int m = 0; m < 2 * NG; ++m) {
+      v4i s = acc[r][m][0];
+      if constexpr (ND == 2) s += acc[r][m][1] * 256;
+      *(v4i*)(red + (16 * wave + col) * STRIDE + 16 * m + 4 * q) = s;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(16, t.rows - 16 * r) * 8 * NG; i += blockDim.x) {
+      const int row = i / (8 * NG), ch = 4 * (i % (8 * NG));
+      v4i s = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < WIDE_WAVES; ++w) s += *(const v4i*)(red + (16 * w + row) * STRIDE + ch);
+      if (ch < c.dim) *out_word(a, t, 16 * r + row, ch) = finish4(s, a);
+    }
+  }
 }
 
 constexpr int LDS_MAX = 160 * 1024;                      // of a CU
+constexpr long long WIDE_MAX = 2ll << 30;                // bytes of widened pages in the workspace
 constexpr long long SCORES_MAX = 1ll << 30;              // bytes of scores in the workspace, unless one tile has more
 
 template <typename K>
@@ -865,18 +1177,52 @@ static int launch_lds(K kernel, dim3 grid, int threads, size_t lds, anvil_ctx* c
   return ANVIL_OK;
 }
 
+// The pages that the rows of a run of `tokens` tokens can see at most.
+static int pages_seen(const CacheView& c, const AttendArgs& a, int tokens) {
+  if (!a.window) return c.slots;
+  const long long seen = ((long long)a.window + tokens + PAGE - 2) / PAGE + 1 + (a.sinks + PAGE - 1) / PAGE;
+  return (int)std::min<long long>(c.slots, seen);
+}
+
+// As many sequences at once as the workspace holds widened pages of.
+template <int NG, int ND>
+static int attend_rows(anvil_ctx* ctx, const CacheView& c, AttendArgs a, long long all) {
+  const long long tiles = (all + WIDE_ROWS - 1) / WIDE_ROWS, seq_bytes = (long long)c.heads * a.bound * Wide<NG>::BYTES;
+  const int seqs = (int)std::min<long long>(c.seqs, WIDE_MAX / seq_bytes);
+  const size_t lds = sizeof(int) * (256 + std::max<size_t>(WIDE_ROWS * HIST, (size_t)WIDE_WAVES * 16 * SUM_STRIDE<NG>));
+  char* ws;
+  if (int r = decode_workspace(ctx, (size_t)(seqs * seq_bytes), &ws)) return r;
+  a.rows = WIDE_ROWS, a.scores = (uint8_t*)ws;
+  for (a.seq0 = 0; a.seq0 < c.seqs; a.seq0 += seqs) {
+    const unsigned units = (unsigned)(std::min(seqs, c.seqs - a.seq0) * c.heads);
+    ANVIL_LAUNCH(attend_widen_kernel<NG>, dim3(units, (unsigned)(a.bound + 3) / 4), dim3(256), 0, ctx->stream, c, a);
+    ANVIL_LAUNCHED();
+    for (long long t0 = 0; t0 < tiles; t0 += 65535) {
+      a.tile0 = (int)t0, a.tiles = (int)std::min<long long>(tiles - t0, 65535);
+      if (int r = launch_lds(attend_rows_kernel<NG, ND>, dim3(units, (unsigned)a.tiles), 64 * WIDE_WAVES, lds, ctx, c, a)) return r;
+    }
+  }
+  return ANVIL_OK;
+}
+
 template <int NG, int RP, bool WIDE>
 static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a, int max_new) {
   const long long all = (long long)max_new * a.group;    // rows of a cache head at most
   a.rows = (int)std::min(16ll, all);
   const long long tiles = (all + 15) / 16;
   const int tokens = (int)std::min<long long>(max_new, (a.rows - 1) / a.group + 2);
-  a.bound = c.slots;
-  if (a.window) {
-    const long long seen = ((long long)a.window + tokens + PAGE - 2) / PAGE + 1 + (a.sinks + PAGE - 1) / PAGE;
-    a.bound = (int)std::min<long long>(c.slots, seen);
-  }
+  a.bound = pages_seen(c, a, tokens);
   const long long units = (long long)c.seqs * c.heads, groups = units * tiles;
+  if constexpr (RP == 16) {
+    // Widened pages pay where eight or more tiles of 32 rows read each, and where there are enough tiles for the CUs, which a tile of
+    // twice the rows keeps busy twice as long: 2 tiles of 16 rows a CU over 2048 keys or more (1 x 32 x 8 heads of 128, 256 new of 4096: 50.4 us
+    // with 16 rows, 40.2 with 32; of 1024 18.2 and 20.8), 8 over fewer (1024 new of 1024: 47.2 and 37.1). Of few rows: 16 x 12 heads
+    // of 64, 64 new of 4096: 54.4 and 69.6.
+    const AttendArgs wide = [&] { AttendArgs w = a; w.bound = pages_seen(c, a, max_new); return w; }();
+    if (all >= 256 && groups >= 2ll * ctx->num_cu && (a.bound >= 32 || groups >= 8ll * ctx->num_cu) && a.one <= ONE_PAIR &&
+        (long long)c.heads * wide.bound * Wide<NG>::BYTES <= WIDE_MAX)
+      return a.one <= 127 ? attend_rows<NG, 1>(ctx, c, wide, all) : attend_rows<NG, 2>(ctx, c, wide, all);
+  }
   const size_t fixed = sizeof(int) * (256 + (size_t)(a.rows * HIST + 3) / 4 * 4), row_sums = sizeof(int) * (size_t)a.rows * SUM_STRIDE<NG>;
   const size_t scores = (size_t)a.bound * a.rows * PAGE;
   // Four waves a workgroup where the tiles fill the CUs and two of them fit a CU's LDS, else eight.
@@ -942,6 +1288,9 @@ extern "C" int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache
     return set_error(ANVIL_E_VALUE, "%s: strides %lld, %lld, %lld, %lld", who, (long long)strides[0], (long long)strides[1],
                      (long long)strides[2], (long long)strides[3]);
   if (int r = check_ctx(ctx)) return r;
+  max_new = std::min(max_new, rows);
+  if ((long long)max_new * (heads_q / c.heads) > 1 << 30)
+    return set_error(ANVIL_E_VALUE, "%s: %d tokens of %d query heads over %d", who, max_new, heads_q, c.heads);
   AttendArgs a{};
   a.q = Q, a.o = O, a.q_row = strides[0], a.q_head = strides[1], a.o_row = strides[2], a.o_head = strides[3];
   a.lut = lut, a.heads_q = heads_q, a.m_s = m_s, a.s_s = s_s, a.one = one, a.m_o = m_o, a.s_o = s_o;

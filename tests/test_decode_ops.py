@@ -426,6 +426,32 @@ def test_attention_over_long_sequences(dim, heads_q, heads, n, new, one):
     attention_case([n], [new], heads_q, heads, dim, one=one, window=n // 2, sinks=130)
 
 
+MANY = [([2100, 70, 300, 0], [256, 70, 3, 0], 8, 8), ([2111, 129, 64, 1], [128, 128, 1, 1], 16, 4)]    # widened pages: 256 rows a cache head
+
+
+@gpu
+@pytest.mark.parametrize("lens,news,heads_q,heads", MANY)
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("one", [1, 127, 128, 32639, 32640])
+def test_attention_of_many_rows(lens, news, heads_q, heads, dim, one):
+    attention_case(lens, news, heads_q, heads, dim, seed=dim, one=one)
+
+
+@gpu
+@pytest.mark.parametrize("lut", ["large", "random", "signed"])
+@pytest.mark.parametrize("one", [127, 4096])
+def test_attention_of_many_rows_with_tables(lut, one):
+    attention_case(*MANY[0], 32, seed=one, lut=lut, one=one, order="heads")
+    attention_case([190, 64, 1], [9, 12, 1], 4, 2, 32, seed=one, lut=lut, one=one)
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks", [(1, 0), (65, 0), (700, 70), (1900, 4), (64, 640)])
+def test_attention_of_many_rows_through_windows(window, sinks):
+    for case in MANY:                                          # windows under 32 pages take tiles of 16 rows, the others those of 32
+        attention_case(*case, 64, seed=window, window=window, sinks=sinks, drop=[(0, 20), (0, 32)])
+
+
 @gpu
 def test_numbers_that_leave_their_range_are_reported_and_evaluate_nothing():
     dev = rt.device(0)
