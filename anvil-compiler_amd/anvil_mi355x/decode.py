@@ -25,8 +25,7 @@ NO_SCORE = -(1 << 63)
 class KVCache:
     """A pool of pages for `layers` layers of (heads, dim) keys and values, and the tables of up to `rows` sequences of up to
     `max_tokens` tokens. It starts with `rows` empty sequences. A step() takes the tables on (anvil_cache_fork): reserve, fork, free;
-    undo() goes back to those before the last step or compact(), once, and only while nothing has been appended since. Device buffers
-    are this object's; the calls run on the device's stream, in order."""
+    undo() goes back to those before the last one. Device buffers are this object's; the calls run on the device's stream, in order."""
 
     def __init__(self, dev, layers, heads, dim, pages, rows, max_tokens, window=0, sinks=0):
         if rows < 1 or max_tokens < 1:
@@ -42,6 +41,7 @@ class KVCache:
         self._shape = dict(slots=slots, pages=pages, heads=heads, dim=dim, layers=layers)
         self._rows, self._n, self._at = rows, [rows, rows], 0
         self.moved = dev.alloc(4 * pages)                      # compact()'s map
+        self._back = False                                     # the tables before the last step still hold
 
     def _cache(self, which):
         return rt.Cache(self.pool, *self._sets[which], seqs=self._n[which], **self._shape)
@@ -63,22 +63,26 @@ class KVCache:
             raise ValueError(f"{n} rows in a cache of {self._rows}")
         self._n[1 - self._at] = n
         self.dev.cache_fork(self.cache, self._cache(1 - self._at), parent, add, self.window, self.sinks)
-        self._at = 1 - self._at
+        self.stepped(n)
+        self._back = add is None or parent is None and not self.window
 
     def stepped(self, rows):
         """A step that recorded kernels have taken."""
         self._at = 1 - self._at
-        self._n[self._at] = rows
+        self._n[self._at], self._back = rows, False
 
     def compact(self):
         """Used pages to the pool's lowest ids; self.moved then holds each page's new id (-1: free)."""
         self._n[1 - self._at] = self.seqs
         self.dev.cache_compact(self.cache, self._cache(1 - self._at), self.moved)
-        self._at = 1 - self._at
+        self._at, self._back = 1 - self._at, True
 
     def undo(self):
-        """The tables before the last step() or compact()."""
-        self._at = 1 - self._at
+        """The tables before the last compact() or step(), as long as nothing has been appended since. A step that both gives pages
+        back (parents or a window) and adds tokens may have written some of them, and cannot be taken back."""
+        if not self._back:
+            raise ValueError("the last step cannot be taken back")
+        self._at, self._back = 1 - self._at, False
 
     def reset(self, rows=None):
         """`rows` empty sequences (None: as many as the cache has room for)."""
@@ -88,7 +92,7 @@ class KVCache:
             table.upload(np.full(table.nbytes // 4, -1, np.int32))
             lens.upload(np.zeros(lens.nbytes // 4, np.int32))
             refs.upload(np.zeros(refs.nbytes // 4, np.int32))
-        self._at, self._n = 0, [self._rows if rows is None else rows] * 2
+        self._at, self._n, self._back = 0, [self._rows if rows is None else rows] * 2, False
 
     def tables(self):
         """(table, lens, refs) on the host."""

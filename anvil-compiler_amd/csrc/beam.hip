@@ -405,8 +405,8 @@ using namespace anvil;
 extern "C" int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b) {
   const char* who = "anvil_beam_select_i8";
   if (!b) return set_error(ANVIL_E_VALUE, "%s: null arguments", who);
-  if (b->groups < 0 || b->groups > (1 << 24) || b->beams < 1 || b->beams > 64 || b->keep < 1 || b->keep > 64 || b->vocab < 1 || b->vocab > VOCAB_MAX ||
-      b->ld < b->vocab)
+  if (b->groups < 0 || b->beams < 1 || b->beams > KEEP_MAX || (long long)b->groups * b->beams > 1 << 22 || b->keep < 1 ||
+      b->keep > KEEP_MAX || b->vocab < 1 || b->vocab > VOCAB_MAX || b->ld < b->vocab)
     return set_error(ANVIL_E_VALUE, "%s: %d groups of %d beams, %d kept, vocabulary %d, row stride %lld", who, b->groups,
                      b->beams, b->keep, b->vocab, (long long)b->ld);
   if (b->nlogs < 2 || b->mult < 1 || b->step < 0) return set_error(ANVIL_E_VALUE, "%s: %d logs, step %d, mult %d", who, b->nlogs, b->step, b->mult);
@@ -418,6 +418,15 @@ extern "C" int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b) {
   if ((uintptr_t)b->scores % 8 || (uintptr_t)b->scores_out % 8 || (uintptr_t)b->lut % 4 || (uintptr_t)b->logs % 4 ||
       (uintptr_t)b->parent % 4 || (uintptr_t)b->token % 4)
     return set_error(ANVIL_E_VALUE, "%s: a pointer is not aligned to its type", who);
+  const auto apart = [](const void* a, size_t na, const void* b, size_t nb) { return (uintptr_t)a + na <= (uintptr_t)b || (uintptr_t)b + nb <= (uintptr_t)a; };
+  const size_t in = (size_t)b->groups * b->beams, out = (size_t)b->groups * b->keep;
+  const void* const read[2] = {b->scores, b->ended};
+  void* const written[4] = {b->scores_out, b->parent, b->token, b->ended_out};
+  const size_t size[4] = {8, 4, 4, 1};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 2; ++j)                          // a group's rows are read while another's results are written
+      if (read[j] && !apart(read[j], in * (j ? 1 : 8), written[i], out * size[i]))
+        return set_error(ANVIL_E_VALUE, "%s: the results overlap the scores or ended rows that are read", who);
   if (int r = check_ctx(ctx)) return r;
   const unsigned pick_threads = 64u * (unsigned)(b->beams < PICK_WAVES ? b->beams : PICK_WAVES);
   if (b->vocab <= WAVE_TOKENS) {

@@ -34,7 +34,7 @@ int cache_view(const char* who, anvil_ctx* ctx, const anvil_cache* c, int layer,
   v->pool = (uint8_t*)c->pool + (long long)layer * c->pages * c->heads * 2176 * groups_of(c->dim);
   v->table = c->table, v->lens = c->lens, v->starts = starts;
   v->seqs = c->seqs, v->slots = c->slots, v->pages = c->pages, v->heads = c->heads, v->dim = c->dim;
-  v->rows = rows, v->max_new = max_new, v->flags = ctx ? ctx->flags : nullptr;
+  v->rows = rows, v->max_new = std::min(max_new, std::max(rows, 1)), v->flags = ctx ? ctx->flags : nullptr;
   return ANVIL_OK;
 }
 
@@ -225,7 +225,7 @@ static int rows_call(const char* who, anvil_ctx* ctx, const anvil_cache* cache, 
                        (long long)strides[i]);
   if (int r = check_ctx(ctx)) return r;
   const RowPtrs p{(int8_t*)K, (int8_t*)V, strides[0], strides[1], strides[2], strides[3]};
-  const dim3 grid((unsigned)((max_new + PAGE - 2) / PAGE + 1), (unsigned)c.seqs, (unsigned)c.heads);
+  const dim3 grid((unsigned)((c.max_new + PAGE - 2) / PAGE + 1), (unsigned)c.seqs, (unsigned)c.heads);
   by_groups(c.dim, [&](auto ng) {
     constexpr int NG = decltype(ng)::value;
     ANVIL_LAUNCH(write ? append_kernel<NG> : read_kernel<NG>, grid, dim3(ROW_THREADS), 0, ctx->stream, c, p);
@@ -595,7 +595,7 @@ int anvil_embed_quantize_new(anvil_ctx* ctx, const anvil_cache* cache, const int
     return set_error(ANVIL_E_VALUE, "%s: a pointer is not aligned to its type", who);
   if (int r = check_ctx(ctx)) return r;
   const EmbedArgs e{ids, wte, wpe, C, vocab, positions, dtype_lo(out_dtype), dtype_hi(out_dtype), scale};
-  const dim3 grid((unsigned)std::min(max_new, 4096), (unsigned)c.seqs);
+  const dim3 grid((unsigned)std::min(c.max_new, 4096), (unsigned)c.seqs);
   if (out_dtype == ANVIL_I8) ANVIL_LAUNCH(embed_new_kernel<int8_t>, grid, dim3(256), 0, ctx->stream, c, e, (int8_t*)out);
   else ANVIL_LAUNCH(embed_new_kernel<int16_t>, grid, dim3(256), 0, ctx->stream, c, e, (int16_t*)out);
   ANVIL_LAUNCHED();

@@ -1206,11 +1206,11 @@ static int attend_rows(anvil_ctx* ctx, const CacheView& c, AttendArgs a, long lo
 }
 
 template <int NG, int RP, bool WIDE>
-static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a, int max_new) {
-  const long long all = (long long)max_new * a.group;    // rows of a cache head at most
+static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a) {
+  const long long all = (long long)c.max_new * a.group;    // rows of a cache head at most
   a.rows = (int)std::min(16ll, all);
   const long long tiles = (all + 15) / 16;
-  const int tokens = (int)std::min<long long>(max_new, (a.rows - 1) / a.group + 2);
+  const int tokens = (int)std::min<long long>(c.max_new, (a.rows - 1) / a.group + 2);
   a.bound = pages_seen(c, a, tokens);
   const long long units = (long long)c.seqs * c.heads, groups = units * tiles;
   if constexpr (RP == 16) {
@@ -1218,7 +1218,7 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a, int max_new)
     // twice the rows keeps busy twice as long: 2 tiles of 16 rows a CU over 2048 keys or more (1 x 32 x 8 heads of 128, 256 new of 4096: 50.4 us
     // with 16 rows, 40.2 with 32; of 1024 18.2 and 20.8), 8 over fewer (1024 new of 1024: 47.2 and 37.1). Of few rows: 16 x 12 heads
     // of 64, 64 new of 4096: 54.4 and 69.6.
-    const AttendArgs wide = [&] { AttendArgs w = a; w.bound = pages_seen(c, a, max_new); return w; }();
+    const AttendArgs wide = [&] { AttendArgs w = a; w.bound = pages_seen(c, a, c.max_new); return w; }();
     if (all >= 256 && groups >= 2ll * ctx->num_cu && (a.bound >= 32 || groups >= 8ll * ctx->num_cu) && a.one <= ONE_PAIR &&
         (long long)c.heads * wide.bound * Wide<NG>::BYTES <= WIDE_MAX)
       return a.one <= 127 ? attend_rows<NG, 1>(ctx, c, wide, all) : attend_rows<NG, 2>(ctx, c, wide, all);
@@ -1282,15 +1282,14 @@ extern "C" int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache
   if (!strides || !lut || (uintptr_t)lut % 4) return set_error(ANVIL_E_VALUE, "%s: strides or lut null or not aligned", who);
   const long long top = 128ll * 126 * c.dim * (m_s < 0 ? -(long long)m_s : m_s) + (s_s ? 1ll << (s_s - 1) : 0);
   if (top > INT32_MAX) return set_error(ANVIL_E_OVERFLOW, "%s: a score's requant with multiplier %d may leave int32", who, m_s);
+  if ((long long)c.seqs * c.heads > 1 << 22 || (long long)c.max_new * (heads_q / c.heads) > 1 << 30)
+    return set_error(ANVIL_E_VALUE, "%s: %d sequences of %d tokens, %d query heads over %d", who, c.seqs, c.max_new, heads_q, c.heads);
   if (!c.seqs || !rows) return check_ctx(ctx);
   if (!Q || !O || (uintptr_t)Q % 16 || (uintptr_t)O % 4) return set_error(ANVIL_E_VALUE, "%s: Q must be 16- and O 4-byte aligned", who);
   if (strides[0] % 16 || strides[1] % 16 || strides[2] % 4 || strides[3] % 4 || strides[2] < c.dim || strides[3] < c.dim)
     return set_error(ANVIL_E_VALUE, "%s: strides %lld, %lld, %lld, %lld", who, (long long)strides[0], (long long)strides[1],
                      (long long)strides[2], (long long)strides[3]);
   if (int r = check_ctx(ctx)) return r;
-  max_new = std::min(max_new, rows);
-  if ((long long)max_new * (heads_q / c.heads) > 1 << 30)
-    return set_error(ANVIL_E_VALUE, "%s: %d tokens of %d query heads over %d", who, max_new, heads_q, c.heads);
   AttendArgs a{};
   a.q = Q, a.o = O, a.q_row = strides[0], a.q_head = strides[1], a.o_row = strides[2], a.o_head = strides[3];
   a.lut = lut, a.heads_q = heads_q, a.m_s = m_s, a.s_s = s_s, a.one = one, a.m_o = m_o, a.s_o = s_o;
@@ -1299,10 +1298,10 @@ extern "C" int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache
   int r = ANVIL_OK;
   by_groups(c.dim, [&](auto ng) {
     constexpr int NG = decltype(ng)::value;
-    const long long rows = (long long)max_new * a.group;
-    if (rows <= 4 && one <= ONE_FIFTEEN) r = attend<NG, 4, false>(ctx, c, a, max_new);
-    else if (rows <= 8) r = one <= ONE_NARROW ? attend<NG, 8, false>(ctx, c, a, max_new) : attend<NG, 8, true>(ctx, c, a, max_new);
-    else r = one <= ONE_NARROW ? attend<NG, 16, false>(ctx, c, a, max_new) : attend<NG, 16, true>(ctx, c, a, max_new);
+    const long long rows = (long long)c.max_new * a.group;
+    if (rows <= 4 && one <= ONE_FIFTEEN) r = attend<NG, 4, false>(ctx, c, a);
+    else if (rows <= 8) r = one <= ONE_NARROW ? attend<NG, 8, false>(ctx, c, a) : attend<NG, 8, true>(ctx, c, a);
+    else r = one <= ONE_NARROW ? attend<NG, 16, false>(ctx, c, a) : attend<NG, 16, true>(ctx, c, a);
   });
   return r;
 }

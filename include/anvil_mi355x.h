@@ -458,8 +458,8 @@ int anvil_embed_quantize_new(anvil_ctx* ctx, const anvil_cache* cache, const int
 
 /* Page tables of the next step: row i of `out` continues row parent[i] of `in` (parent NULL: row i; -1: an empty row) by
  * add[i] >= 0 tokens (add NULL: none). `out` shares in's pool and has its slots; its table, lens and refs are other
- * memory (in's stay as they are, so that a step can be taken back until its pages are written). Both have at most
- * ANVIL_CACHE_ROWS_MAX rows. In this order:
+ * memory. in's stay as they are, so that a step can be taken back until its pages are written (a page that no row of `out`
+ * keeps may be written at once, as a copy). Both have at most ANVIL_CACHE_ROWS_MAX rows. In this order:
  *   1. the row keeps its parent's pages; with window > 0 not those that no query from its end on sees (every key of
  *      theirs >= sinks and <= lens - window), whose entries become -1;
  *   2. refs counts out's entries in place of in's, so pages that no row keeps are free;
@@ -483,8 +483,9 @@ int anvil_cache_compact(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache
  * A row with ended[row] != 0 (ended NULL: none) has one candidate, the token eos at its score. allowed (vocab bytes, NULL:
  * all) excludes tokens whose byte is 0 from the candidates, not from S. The best `keep` candidates of each group, by score
  * descending, then row, then token: score, parent = the row (in groups x beams: what anvil_cache_fork takes), token, and
- * ended (the row's, or token = eos). Where there are fewer, INT64_MIN, -1, -1, 0. 1 <= beams, keep <= 64; vocab
- * at most 2^28; mult >= 1; nlogs >= 2; eos = -1: none. A row whose S or lut[255] is below 1 has no candidates, and ANVIL_E_ZERODIV is reported. */
+ * ended (the row's, or token = eos). Where there are fewer, INT64_MIN, -1, -1, 0. 1 <= beams, keep <= 64; groups x beams
+ * at most 2^22; vocab at most 2^28; mult >= 1; nlogs >= 2; eos = -1: none. The results are other memory than scores and
+ * ended. A row whose S or lut[255] is below 1 has no candidates, and ANVIL_E_ZERODIV is reported. */
 typedef struct anvil_beams {
   const int8_t* logits;
   int64_t ld;

@@ -118,7 +118,7 @@ GOOD_ATTEND = dict(layer=0, Q=4096, O=4096, starts=None, rows=2, max_new=1, head
                    ms=3, ss=14, lut=4096, one=127, mo=3, so=8, window=0, sinks=0)
 
 
-@pytest.mark.parametrize("bad", [dict(heads=3), dict(heads=0), dict(ss=32), dict(ss=-1), dict(so=32), dict(one=0),
+@pytest.mark.parametrize("bad", [dict(heads=3), dict(heads=0), dict(heads=(1 << 31) - 2), dict(ss=32), dict(ss=-1), dict(so=32), dict(one=0),
                                  dict(one=32768), dict(window=-1), dict(sinks=-1), dict(lut=0), dict(lut=4098), dict(Q=4100),
                                  dict(O=4097), dict(Q=0), dict(strides=None), dict(strides=(C.c_int64 * 4)(256, 8, 256, 64)),
                                  dict(strides=(C.c_int64 * 4)(256, 64, 256, 32)),
@@ -126,6 +126,11 @@ GOOD_ATTEND = dict(layer=0, Q=4096, O=4096, starts=None, rows=2, max_new=1, head
 def test_bad_attention_arguments_are_refused(bad):
     with pytest.raises(ValueError, match="anvil_attention_cache_i4"):
         _call("anvil_attention_cache_i4", C.byref(_cache()), *{**GOOD_ATTEND, **bad}.values())
+
+
+def test_more_sequences_and_heads_than_a_grid_holds_are_refused():
+    with pytest.raises(ValueError, match="65535 sequences"):
+        _call("anvil_attention_cache_i4", C.byref(_cache(seqs=65535, heads=128)), *{**GOOD_ATTEND, "rows": 65535, "heads": 128}.values())
 
 
 def test_a_score_multiplier_past_int32_is_refused():
@@ -169,13 +174,15 @@ def test_bad_step_arguments_are_refused():
 
 
 GOOD_BEAMS = dict(logits=4096, ld=64, scores=4096, ended=None, allowed=None, groups=2, beams=3, vocab=64, keep=3, eos=-1,
-                  lut=4096, logs=4096, nlogs=16, step=4, mult=5, scores_out=4096, parent=4096, token=4096, ended_out=4096)
+                  lut=4096, logs=4096, nlogs=16, step=4, mult=5, scores_out=4144, parent=4144, token=4144, ended_out=4144)
 
 
 @pytest.mark.parametrize("bad", [dict(groups=-1), dict(beams=0), dict(beams=65), dict(keep=0), dict(keep=65), dict(vocab=0),
                                  dict(ld=63), dict(nlogs=1), dict(step=-1), dict(mult=0), dict(eos=64), dict(eos=-2),
                                  dict(ended=4096), dict(logits=0), dict(scores=4100), dict(lut=4098), dict(logs=0),
-                                 dict(scores_out=4100), dict(parent=4097), dict(token=0), dict(ended_out=0)], ids=str)
+                                 dict(scores_out=4100), dict(parent=4097), dict(token=0), dict(ended_out=0),
+                                 dict(groups=1 << 20, beams=5), dict(scores_out=4096), dict(parent=4096 + 44), dict(token=4092),
+                                 dict(ended=8192, ended_out=8197, eos=3), dict(ended_out=4096 + 47)], ids=str)
 def test_bad_beams_are_refused(bad):
     with pytest.raises(ValueError, match="anvil_beam_select_i8"):
         _call("anvil_beam_select_i8", C.byref(rt.Beams(*{**GOOD_BEAMS, **bad}.values())))
@@ -761,3 +768,178 @@ def test_beams_of_any_log_table(n):
     logs = np.rint(np.log(np.maximum(1, np.arange(n))) * 65536).astype(np.int64)
     beams_case(2, 3, 900, 5, logs=logs, lut=exp_lut(0.02, 30))
     beams_case(2, 3, 900, 5, logs=logs, lut=np.random.default_rng(0).integers(-3, 3, 256).clip(max=2) | 1, mult=(1 << 31) - 1)
+
+
+# ------------------------------------------------------------------------------- graphs, contexts and the workspace
+
+class Work:
+    """A call of the attention whose inputs can be changed: run() enqueues it, check() waits and compares."""
+
+    def __init__(self, dev, lens, news, heads_q, heads, dim, seed, one=127):
+        self.dev, self.news, self.heads_q, self.dim = dev, news, heads_q, dim
+        self.seqs = Sequences(lens, heads, dim, seed=seed)
+        self.d = OnDevice(dev, self.seqs, self.seqs.pool())
+        self.rows, self.one = sum(news), one
+        self.ms, self.ss = fixed(0.4 / np.sqrt(dim) / 40, 128 * 126 * dim)
+        self.mo, self.so = fixed(2.0 / one, 126 * (one + max(lens) // 2))
+        self.lut, self.starts = dev.upload(exp_lut().astype(np.int32)), dev.upload(starts_of(news))
+        self.q, self.out = dev.alloc(self.rows * heads_q * dim), dev.alloc(self.rows * heads_q * dim)
+        self.feed(seed)
+
+    def feed(self, seed):
+        q = np.random.default_rng([seed, 5]).integers(-128, 128, (self.rows, self.heads_q, self.dim))
+        self.q.upload(q.astype(np.int8))
+        self.want, _ = attention_want(self.seqs, self.news, q, self.heads_q, self.ms, self.ss, exp_lut(), self.one, self.mo, self.so)
+
+    def run(self):
+        w = self.heads_q * self.dim
+        self.dev.attention_cache(self.d.cache, 0, self.q, self.out, self.starts, self.rows, max(self.news), self.heads_q,
+                                 (w, self.dim, w, self.dim), self.ms, self.ss, self.lut, self.one, self.mo, self.so)
+
+    def check(self):
+        self.dev.sync()
+        got = self.out.download(self.want.shape, np.int8)
+        assert np.array_equal(got, self.want), np.argwhere(got != self.want)[:5]
+
+
+class Choice:
+    """The same for a selection over a vocabulary that takes the workspace."""
+
+    def __init__(self, dev, seed, vocab=20000):
+        self.dev, self.vocab = dev, vocab
+        self.lut = exp_lut(0.05)
+        self.logs = np.rint(np.log(np.maximum(1, np.arange(2048))) * 65536).astype(np.int64)
+        self.d_lut, self.d_logs = dev.upload(self.lut.astype(np.int32)), dev.upload(self.logs.astype(np.int32))
+        self.x, self.scores = dev.alloc(4 * vocab), dev.upload(np.arange(4, dtype=np.int64))
+        self.out = [dev.alloc(6 * n) for n in (8, 4, 4, 1)]
+        self.feed(seed)
+
+    def feed(self, seed):
+        x = np.random.default_rng([seed, 6]).integers(-128, 128, (4, self.vocab))
+        self.x.upload(x.astype(np.int8))
+        self.want = od.beam_select(x, np.arange(4), None, None, 2, 2, 3, -1, self.lut, self.logs, 45426, 3277)[:4]
+
+    def run(self):
+        self.dev.beam_select(self.x, self.vocab, self.scores, None, None, 2, 2, self.vocab, 3, -1, self.d_lut, self.d_logs, 2048, 45426,
+                             3277, *self.out)
+
+    def check(self):
+        self.dev.sync()
+        for buf, w, t in zip(self.out, self.want, (np.int64, np.int32, np.int32, np.uint8)):
+            assert np.array_equal(buf.download((2, 3), t), w)
+
+
+KINDS = {"tiles": lambda dev, seed: Work(dev, [200, 64], [1, 1], 4, 2, 64, seed),
+         "parts": lambda dev, seed: Work(dev, [4200], [1], 4, 1, 128, seed),
+         "many rows": lambda dev, seed: Work(dev, [2100, 300], [64, 1], 64, 16, 32, seed),
+         "beams": Choice}
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["capture", "sequence"])
+def test_replays_with_eager_work_between(kind):
+    """Two recordings share the workspace, each other call of the context takes it too, and one that needs a larger one replaces it."""
+    dev = rt.Device(0)
+    works = [KINDS[k](dev, i) for i, k in enumerate(("parts", "beams", "many rows", "tiles"))]
+    for w in works:
+        w.run()
+        w.check()
+    recorded = [getattr(dev, kind)(lambda: [w.run() for w in pair]) for pair in (works[:2], works[2:])]
+    for seed in range(4):
+        for w in works:
+            w.feed(10 + seed)
+        for r in recorded:
+            r.launch()
+        for w in works:
+            w.check()
+        eager = KINDS["parts" if seed % 2 else "beams"](dev, 20 + seed)
+        for w in works:
+            w.feed(30 + seed)
+        recorded[0].launch()
+        eager.run()
+        recorded[1].launch()
+        recorded[0].launch()
+        for w in (eager, *works):
+            w.check()
+        if seed == 1:                                          # 3 MiB and more of scores, histograms and sums
+            big = Work(dev, [20000], [8], 32, 1, 32, 3)
+            big.run()
+            big.check()
+    del recorded
+    dev.close()
+
+
+@gpu
+def test_a_captured_step_of_tables_rows_and_attention():
+    dev = rt.Device(0)
+    seqs = Sequences([63, 64, 1], 2, 32, extra_slots=1, spare=4)
+    up = lambda x: dev.upload(np.ascontiguousarray(x))                                                # noqa: E731
+    pool, tables = up(seqs.pool()), [up(seqs.table), up(np.array(seqs.lens, np.int32)), up(seqs.refs)]
+    cache = rt.Cache(pool, *tables, seqs=3, slots=seqs.slots, pages=seqs.pages, heads=2, dim=32)
+    outs = [dev.alloc(4 * seqs.table.size), dev.alloc(12), dev.alloc(4 * seqs.refs.size)]
+    stepped = cache.with_tables(*outs)
+    ones, lut = up(np.ones(3, np.int32)), up(exp_lut().astype(np.int32))
+    k, v, q, o = (dev.alloc(3 * 64) for _ in range(4))
+    st = (64, 32, 64, 32)
+
+    def step():
+        dev.cache_fork(cache, stepped, None, ones)
+        dev.cache_append(stepped, 0, k, v, None, 3, 1, st)
+        dev.attention_cache(stepped, 0, q, o, None, 3, 1, 2, st, 3, 10, lut, 127, 1, 7)
+
+    rng = np.random.default_rng(2)
+    step()
+    dev.sync()
+    g = dev.capture(step)
+    for _ in range(4):
+        rows = [rng.integers(-128, 128, (3, 2, 32)) for _ in range(3)]
+        for buf, x in zip((k, v, q), rows):
+            buf.upload(x.astype(np.int8))
+        g.launch()
+        dev.sync()
+        want_t, want_n, want_r, _ = od.fork(seqs.table, seqs.lens, seqs.refs, None, [1, 1, 1])
+        assert np.array_equal(outs[0].download(want_t.shape, np.int32), want_t)
+        assert np.array_equal(outs[1].download((3,), np.int32), want_n)
+        assert np.array_equal(outs[2].download(want_r.shape, np.int32), want_r)
+        got = o.download((3, 2, 32), np.int8)
+        for s, h in np.ndindex(3, 2):
+            keys, vals = (od.held(np.concatenate([old[0][s][:, h], new[s, h][None]])) for old, new in ((seqs.k, rows[0]), (seqs.v, rows[1])))
+            want, _ = od.attend(rows[2][s, h], keys, vals, seqs.lens[s], np.ones(9, bool), 3, 10, exp_lut(), 127, 1, 7)
+            assert np.array_equal(got[s, h], want)
+    del g
+    dev.close()
+
+
+@gpu
+def test_two_contexts_at_once():
+    """Each context has its stream and its workspace: calls from two threads, and interleaved from one."""
+    import threading
+    devs = [rt.Device(0), rt.Device(0)]
+    works = [[KINDS[k](dev, 7 * i + j) for j, k in enumerate(KINDS)] for i, dev in enumerate(devs)]
+    for pair in zip(*works):
+        for _ in range(3):
+            for w in pair:
+                w.run()
+        for w in pair:
+            w.check()
+    errors = []
+
+    def loop(ws):
+        try:
+            for _ in range(5):
+                for w in ws:
+                    w.run()
+                for w in ws:
+                    w.check()
+        except BaseException as e:                             # noqa: BLE001  (reported by the test's thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=loop, args=(ws,)) for ws in works]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    del works
+    for d in devs:
+        d.close()

@@ -195,6 +195,8 @@ def test_a_step_is_taken_back_and_the_pool_compacted():
     dec.cache.undo()
     for x, y in zip(before, dec.cache.tables()):
         np.testing.assert_array_equal(x, y)
+    with pytest.raises(ValueError, match="taken back"):
+        dec.cache.undo()
     parent = count(-1, 1, 2)                                   # a row is freed, its pages are holes, the others move
     dec.cache.step(parent, None)
     dec.cache.compact()
