@@ -4,6 +4,9 @@
 // it: above that value fewer than k tokens lie, and of those at it the first few in token order are taken. Each stretch of
 // 16384 logits is read once into registers by one workgroup, which leaves its histogram and its k best; one workgroup a group then
 // joins them. Rows of at most 4096 logits take a wave each of that last workgroup instead, in one launch.
+//
+// 64 x 8 rows of 100003 logits: 27 us of the stretches (12 of reading, 11 of counting, an LDS atomic a logit at 8.4 clocks a wave's, 5
+// of collecting) and 8 of joining; 8 x 4 rows of 512: 8 us, most of it the launch and one chain.
 #include "common.h"
 
 namespace anvil {
@@ -409,7 +412,8 @@ extern "C" int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b) {
       b->keep > KEEP_MAX || b->vocab < 1 || b->vocab > VOCAB_MAX || b->ld < b->vocab)
     return set_error(ANVIL_E_VALUE, "%s: %d groups of %d beams, %d kept, vocabulary %d, row stride %lld", who, b->groups,
                      b->beams, b->keep, b->vocab, (long long)b->ld);
-  if (b->nlogs < 2 || b->mult < 1 || b->step < 0) return set_error(ANVIL_E_VALUE, "%s: %d logs, step %d, mult %d", who, b->nlogs, b->step, b->mult);
+  if (b->nlogs < 2 || b->mult < 1 || b->step < 0)
+    return set_error(ANVIL_E_VALUE, "%s: %d logs, step %d, mult %d", who, b->nlogs, b->step, b->mult);
   if (b->eos < -1 || b->eos >= b->vocab || (b->ended && b->eos < 0))
     return set_error(ANVIL_E_VALUE, "%s: eos %d of %d (ended rows need one)", who, b->eos, b->vocab);
   if (!b->groups) return check_ctx(ctx);
@@ -418,7 +422,9 @@ extern "C" int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b) {
   if ((uintptr_t)b->scores % 8 || (uintptr_t)b->scores_out % 8 || (uintptr_t)b->lut % 4 || (uintptr_t)b->logs % 4 ||
       (uintptr_t)b->parent % 4 || (uintptr_t)b->token % 4)
     return set_error(ANVIL_E_VALUE, "%s: a pointer is not aligned to its type", who);
-  const auto apart = [](const void* a, size_t na, const void* b, size_t nb) { return (uintptr_t)a + na <= (uintptr_t)b || (uintptr_t)b + nb <= (uintptr_t)a; };
+  const auto apart = [](const void* a, size_t na, const void* b, size_t nb) {
+    return (uintptr_t)a + na <= (uintptr_t)b || (uintptr_t)b + nb <= (uintptr_t)a;
+  };
   const size_t in = (size_t)b->groups * b->beams, out = (size_t)b->groups * b->keep;
   const void* const read[2] = {b->scores, b->ended};
   void* const written[4] = {b->scores_out, b->parent, b->token, b->ended_out};

@@ -26,10 +26,11 @@ struct AttendArgs {
   int8_t* o;
   long long q_row, q_head, o_row, o_head;
   const int* lut;
-  int heads_q, m_s, s_s, one, m_o, s_o, window, sinks;
-  int group, rows;                                       // query heads of a cache head; rows of a tile that can exist (<= 16)
+  int m_s, s_s, one, m_o, s_o, window, sinks;
+  int group, rows;                                       // query heads of a cache head; rows of a tile that can exist
   int seq0, tile0, tiles, splits, bound;                 // this launch's part; pages that a tile can see at most
-  uint8_t* scores;                                       // workspace: [unit][tile][page][row][64], a score + 128
+  uint8_t* scores;                                       // workspace: [unit][tile][page][row][64], a score + 128; or widened
+                                                         //            pages, [unit][page]
   unsigned* hist;                                        //            [unit][tile][split][row][256]
   int* sums;                                             //            [unit][tile][split][row][32 NG], 16 x sum p V
 };
@@ -418,8 +419,8 @@ __device__ __forceinline__ void add_page(const ValuePage<NG>& v, const uint4& sc
 // A wave's pages of a tile, begin + wave, begin + wave + waves, .. below end, one after the other, AHEAD of them in flight. One is
 // enough: with two or three, whose steps are unrolled for as many sets of registers, the longer code costs a short walk more (its
 // instructions come from memory too) than the loads in flight bring a long one. 32 x 12 heads over up to 1024 tokens: none
-// 11.9 us, one 11.6, three and two 12.9; 64 x 32 heads over up to 8192: 79.0, 69.7, 70.1. Table entries come 64 at a time, one a lane; the first of
-// them are known when the walk begins (`entry`).
+// 11.9 us, one 11.6, three and two 12.9; 64 x 32 heads over up to 8192: 79.0, 69.7, 70.1. Table entries come 64 at a time, one a lane;
+// the first of them are known when the walk begins (`entry`).
 template <int NG, int AHEAD, typename Page>
 struct Walk {
   Page ring[AHEAD + 1];
@@ -589,8 +590,8 @@ __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, i
   }
 }
 
-// The tables of a tile's rows. A wave takes a row at a time, or four where there are many: the sums over lanes and what is one number a row
-// cost a row less.
+// The tables of a tile's rows. A wave takes a row at a time, or four where there are many: the sums over lanes and what is one number
+// a row cost a row less.
 template <int TABLE, bool MANY>
 __device__ __forceinline__ void make_tables(unsigned* rows, int n_rows, const int* lut, int one, unsigned* flags) {
   const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -657,7 +658,6 @@ __device__ __forceinline__ void join_waves(const v4i (&acc)[Digits<RP, WIDE>::SU
 }
 
 constexpr int WAVES_MAX = 8;
-
 
 // Where a lane stands in the first pass: its row, and which of the row's 64 scores of a page are its NE dwords.
 template <int NG, int RP>
@@ -867,8 +867,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(CacheView c, 
 // in the second pass, so that a tile needs LDS for its histograms alone and has any length. 4 sequences of 32 heads over 8 of 128
 // channels, 1024 new tokens of 16384 each: 3149 us with tiles of 16 rows, 1217 with these; 2 of 512 new of up to 4096: 188 and 92.
 // What bounds it: instructions between the products (half of all cycles) and the LDS's conflicts on histograms and tables (as many).
-// Of that case's time with 16, 32, 48 and 64 rows a tile: 114, 92, 106, 100 us; with 2, 3, 4 and 8 waves 90, 114, 92, 105,
-// and with 2 a third more for short tiles.
+// The second with 16, 32, 48 and 64 rows a tile: 114, 92, 106, 100 us; with 2, 3, 4 and 8 waves 90, 114, 92, 105, and with 2 a third
+// more where tiles are short (4 x 12 heads of 64, 512 new, the last 1024 seen).
 
 constexpr int WIDE_TILES = 2, WIDE_ROWS = 16 * WIDE_TILES, WIDE_WAVES = 4;
 constexpr int ONE_PAIR = 127 * 256 + 127;                // 32639: two digits, the low one from -128 on
@@ -1215,10 +1215,11 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a) {
   const long long units = (long long)c.seqs * c.heads, groups = units * tiles;
   if constexpr (RP == 16) {
     // Widened pages pay where eight or more tiles of 32 rows read each, and where there are enough tiles for the CUs, which a tile of
-    // twice the rows keeps busy twice as long: 2 tiles of 16 rows a CU over 2048 keys or more (1 x 32 x 8 heads of 128, 256 new of 4096: 50.4 us
-    // with 16 rows, 40.2 with 32; of 1024 18.2 and 20.8), 8 over fewer (1024 new of 1024: 47.2 and 37.1). Of few rows: 16 x 12 heads
-    // of 64, 64 new of 4096: 54.4 and 69.6.
-    const AttendArgs wide = [&] { AttendArgs w = a; w.bound = pages_seen(c, a, c.max_new); return w; }();
+    // twice the rows keeps busy twice as long: 2 tiles of 16 rows a CU over 2048 keys or more (32 heads over 8 of 128, 256 new of
+    // 4096: 50.4 us with 16 rows, 40.2 with 32; of 1024 18.2 and 20.8), 8 over fewer (1024 new of 1024: 47.2 and 37.1). With few rows
+    // (16 x 12 heads of 64, 64 new of 4096): 54.4 and 69.6.
+    AttendArgs wide = a;
+    wide.bound = pages_seen(c, a, c.max_new);
     if (all >= 256 && groups >= 2ll * ctx->num_cu && (a.bound >= 32 || groups >= 8ll * ctx->num_cu) && a.one <= ONE_PAIR &&
         (long long)c.heads * wide.bound * Wide<NG>::BYTES <= WIDE_MAX)
       return a.one <= 127 ? attend_rows<NG, 1>(ctx, c, wide, all) : attend_rows<NG, 2>(ctx, c, wide, all);
@@ -1292,7 +1293,7 @@ extern "C" int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache
   if (int r = check_ctx(ctx)) return r;
   AttendArgs a{};
   a.q = Q, a.o = O, a.q_row = strides[0], a.q_head = strides[1], a.o_row = strides[2], a.o_head = strides[3];
-  a.lut = lut, a.heads_q = heads_q, a.m_s = m_s, a.s_s = s_s, a.one = one, a.m_o = m_o, a.s_o = s_o;
+  a.lut = lut, a.m_s = m_s, a.s_s = s_s, a.one = one, a.m_o = m_o, a.s_o = s_o;
   const int most = c.slots * PAGE;                       // keys; a window that holds them all is none
   a.window = window < most ? window : 0, a.sinks = std::min(sinks, most), a.group = heads_q / c.heads;
   int r = ANVIL_OK;
