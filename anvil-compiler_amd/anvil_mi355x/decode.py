@@ -125,7 +125,7 @@ class Decoder:
         if cm.embedding is None:
             raise ValueError("decoding needs embedding tables: compile(..., embedding=(wte, wpe))")
         if len(cm.output_values) != 1:
-            raise ValueError("decoding needs a graph with one output, the logits")
+            raise ValueError("decoding needs a graph with one output")
         self.cm = cm
         self.T = g.qt(cm.input_ops[0].result).dims[0]
         positions = cm.embedding[1].shape[0]
@@ -139,15 +139,13 @@ class Decoder:
             raise ValueError(f"window {window}, sinks {sinks}")
         self.steps, layers, heads, dim = self._lower()
         self.vocab = cm.embedding[0].shape[0]
-        if self.logits.width > self.vocab:
-            raise ValueError(f"{self.logits.width} logits, but the token table has {self.vocab} rows")
         cm._ensure_device()
         self.dev = cm.dev
         slots = -(-max_tokens // rt.CACHE_PAGE)
         pages = self.rows * (slots + 1) if pages is None else int(pages)
         self.cache = KVCache(self.dev, layers, heads, dim, pages, self.rows, max_tokens, window, sinks)
         self.wte, self.wpe = (self.dev.upload(t) for t in cm.embedding)
-        self._room = 0
+        self._room, self._buffers = 0, []
 
     # ----------------------------------------------------------------------------------------------- lowering
     def _lower(self):
@@ -229,27 +227,27 @@ class Decoder:
         if not layers:
             raise ValueError("decoding needs an attention chain")
         self.logits = rows_of(cm.output_values[0])
-        if self.logits.dtype != "i8":
-            raise ValueError("decoding needs int8 logits")
         self.scale = g.qt(cm.output_values[0]).qscale
         self._values = list(value.values())
         return steps, layers, *shape
 
     def _make_room(self, rows):
         """Buffers of every value for so many rows of tokens. They start as zeros, and only results of the graph's ops follow, so
-        that the rows of empty sequences, which the row-wise ops evaluate with the others, stay in the ranges of the graph's proof."""
+        that the rows of empty sequences, which the row-wise ops evaluate with the others, stay in the ranges of the graph's proof.
+        Smaller ones that came before stay, for launches recorded with them."""
         if rows <= self._room:
             return
-        self._room = rows
+        self._room = max(rows, 2 * self._room)
         for r in self._values:
-            r.buf = self.dev.alloc(rows * r.width * rt.ITEMSIZE[r.dtype])
+            self._buffers.append(r.buf)
+            r.buf = self.dev.alloc(self._room * r.width * rt.ITEMSIZE[r.dtype])
             self.dev.zero(r.buf, r.buf.nbytes)
 
     # ------------------------------------------------------------------------------------------------ forward
     def forward(self, ids, starts, rows, max_new):
-        """The logits (rows, vocab) int8, on the device until the next call, of new tokens: `ids` (device int32s), rows starts[s] ..
-        starts[s + 1] - 1 those of sequence s, at most max_new each (device int32s; None: one a sequence). The cache has been
-        stepped by them. Launches only, once a call of as many rows has run."""
+        """The graph's output (rows, width), on the device until the next call, for new tokens: `ids` (device int32s), rows
+        starts[s] .. starts[s + 1] - 1 those of sequence s, at most max_new each (device int32s; None: one a sequence). The cache has
+        been stepped by them. Launches only, once a call of as many rows has run."""
         dev, cm, cache = self.dev, self.cm, self.cache.cache
         heads, d = cache.heads, cache.dim
         self._make_room(rows)
@@ -310,8 +308,8 @@ class Decoder:
                 raise ValueError(f"token ids outside [0, {self.vocab})")
         if eos is not None and not 0 <= eos < V:
             raise ValueError(f"eos {eos} outside [0, {V})")
-        if self.scale is None:
-            raise ValueError("the logits have no scale")
+        if self.logits.dtype != "i8" or self.scale is None or V > self.vocab:
+            raise ValueError(f"the graph's output is not int8 logits with a scale for {self.vocab} tokens")
         select = Selection.of(self.scale)
         tables = self._tables(select, allowed, V)
         starts = np.cumsum([0] + [p.size for p in prompts]).astype(np.int32)

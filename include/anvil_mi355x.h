@@ -418,7 +418,7 @@ typedef struct anvil_cache {
   int32_t* table;                   /* seqs x slots */
   int32_t* lens;                    /* seqs: tokens, at most 64 slots */
   int32_t* refs;                    /* pages; NULL where only attention, append and read use the cache */
-  int32_t seqs, slots, pages, heads, dim, layers;
+  int32_t seqs, slots, pages, heads, dim, layers;   /* seqs and layers at most 65535, heads 4096, pages 2^24 */
 } anvil_cache;
 
 /* The bytes of a pool: layers x pages x heads x 68 D. */
@@ -442,7 +442,8 @@ int anvil_cache_read_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, int
  * context keep more than int8's 7 bits. lut: int32[256], entries below 0 count as 0. A row that sees no key yields
  * the requantized 0; a row whose S is 0 yields that too and ANVIL_E_ZERODIV at anvil_sync. |m_s| is limited so that
  * every Q . K_j * m_s + 2^(s_s-1) fits int32 (128 * 126 * D * |m_s| + 2^(s_s-1) < 2^31), else ANVIL_E_OVERFLOW.
- * strides = {q row, q head, o row, o head}: Q and its strides multiples of 16, O and its strides of 4, o strides >= D. */
+ * strides = {q row, q head, o row, o head}: Q and its strides multiples of 16, O and its strides of 4, o strides >= D.
+ * O is other memory than Q. seqs x heads at most 2^22, max_new x heads_q / heads at most 2^30. */
 int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, const int8_t* Q, int8_t* O,
                              const int32_t* starts, int rows, int max_new, int heads_q, const int64_t* strides,
                              int32_t m_s, int s_s, const int32_t* lut, int32_t one, int32_t m_o, int s_o, int window,

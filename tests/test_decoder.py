@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import anvil_mi355x
+import helpers
 from anvil_mi355x import decode, models
 from anvil_mi355x import ir as g
 from anvil_mi355x import runtime as rt
@@ -132,6 +133,41 @@ def test_prompts_then_single_tokens_give_the_graphs_logits(name):
 
 
 @gpu
+@pytest.mark.parametrize("name", ["v1", "v2"])
+def test_the_frozen_models_over_an_embedding(name):
+    """Gated MLPs, and in v2 an i16 residual stream with wide norms: the reference's frozen models behind random token tables."""
+    text, consts, _ = helpers.reference_model(name)
+    m = anvil_mi355x.parse_ir(text)
+    rng = np.random.default_rng(4)
+    loud = 1.5 if name == "v1" else 5.0
+    wte, wpe = (rng.normal(0, loud, (n, 32)).astype(np.float32) for n in (40, 16))
+    cm = anvil_mi355x.compile((m, consts), embedding=(wte, wpe))
+    ids = rng.integers(0, 40, (3, 16))
+    lo, hi = (-128, 127) if name == "v1" else (-32768, 32767)
+    x = np.clip(np.rint((wte.astype(np.float64)[ids] + wpe) / cm.scale("x")), lo, hi).astype(np.int64)
+    hold = lambda v, _: od.held(v.reshape(3, 16, 2, 16)).reshape(v.shape)                       # noqa: E731
+    want = interp.run(m, {"x": x}, consts, batch=True, replace={f"L{i}.{n}": hold for i in range(2) for n in "kv"}).outputs[0]
+    dec, dev = cm.decoder(rows=3), cm.dev
+    at = np.zeros(3, int)
+    for n in ([5, 1, 12], [0, 4, 3], *[[1, 1, 0]] * 11):
+        n = np.minimum(n, 16 - at)
+        starts = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+        rows = int(starts[-1])
+        add, new, d_starts = (dev.upload(np.asarray(v, np.int32)) for v in (
+            n, np.concatenate([ids[s, at[s]:at[s] + n[s]] for s in range(3)]), starts))
+        dec.cache.step(None, add)
+        got = dec.forward(new, d_starts, rows, int(max(n))).download((rows, 32), np.int8 if name == "v1" else np.int16)
+        dev.sync()
+        for s in range(3):
+            np.testing.assert_array_equal(got[starts[s]:starts[s + 1]], want[s, at[s]:at[s] + n[s]])
+        at += n
+    assert at.tolist() == [16, 16, 15]
+    if name == "v2":
+        with pytest.raises(ValueError, match="int8 logits"):
+            dec.generate([[1]], 1)
+
+
+@gpu
 @pytest.mark.parametrize("beams,new_tokens", [(1, 1), (1, 9), (2, 2), (4, 7), (3, 4)])
 @pytest.mark.parametrize("name", SPECS)
 def test_generate_equals_the_oracles_beam_search(name, beams, new_tokens):
@@ -210,6 +246,48 @@ def test_a_step_is_taken_back_and_the_pool_compacted():
         dev.sync()
         for s in (1, 2):
             np.testing.assert_array_equal(out[s], want[s][64 + t])
+
+
+@gpu
+def test_recorded_steps_outlive_larger_calls():
+    b = built("heads of 32")
+    cm = anvil_mi355x.compile(b)
+    dec, dev = cm.decoder(rows=2), cm.dev
+    seqs = prompts_of(b.spec, [40, 40], 11)
+    want = Oracle(b).logits(seqs)
+    toks, ones = dev.upload(np.zeros(2, np.int32)), dev.upload(np.ones(2, np.int32))
+
+    def step():
+        dec.cache.step(None, ones)
+        return dec.forward(toks, None, 2, 1)
+
+    def feed(t):
+        toks.upload(np.array([s[t] for s in seqs], np.int32))
+
+    def check(t):
+        dev.sync()
+        got = logits.download((2, b.spec.vocab), np.int8)
+        np.testing.assert_array_equal(got, [w[t] for w in want])
+
+    for t in range(2):                                         # one with each set of tables
+        feed(t)
+        logits = step()
+        check(t)
+    recorded = []
+    for t in range(2, 4):
+        feed(t)
+        recorded.append(dev.sequence(step))
+        check(t)
+    other = cm.decoder(rows=2)
+    prompts = prompts_of(b.spec, [100, 90], 12)
+    for t in range(4, 12):
+        feed(t)
+        recorded[t % 2].launch()
+        dec.cache.stepped(2)
+        check(t)
+        if t == 6:                                             # larger buffers, a larger workspace
+            dec._make_room(500)
+            same(other.generate(prompts, 3, 1), Oracle(b).generate(prompts, 3, 1))
 
 
 @gpu
