@@ -286,13 +286,13 @@ __device__ __forceinline__ int prefix(int v, int& total) {
 struct ForkArgs {
   const int *table, *lens, *refs, *parent, *add;
   int *table_out, *lens_out, *refs_out;
-  int *count, *list;                                     // scratch: references of each page (pages), free pages in order
+  int* list;                                             // scratch: free pages in order
   int2* copies;                                          // scratch: (from, to) page of each row, from = -1: none
   int seqs, seqs_out, slots, pages, window, sinks;
   unsigned* flags;
 };
 
-// A page's references while they are counted: in LDS, or where the pages are too many in scratch memory, past the caches.
+// A page's references while they are counted: in LDS, or with larger tables in refs_out, past the caches.
 template <bool LDS>
 struct Count {
   int* n;
@@ -307,19 +307,64 @@ struct Count {
   __device__ __forceinline__ void add(int p, int v) const { atomicAdd(n + p, v); }
 };
 
+// Entry j of row `row`, which was `was` and continues row par's len tokens (par -1: an empty row): table_out's, and the references of
+// what the entry was and is, where the two differ.
+template <bool LDS>
+__device__ __forceinline__ void carry_entry(const ForkArgs& a, const Count<LDS>& count, int row, int j, int was, int par, int len) {
+  int is = -1;
+  const bool gone = a.window && j * PAGE >= a.sinks && j * PAGE + PAGE - 1 <= len - a.window;
+  if (par >= 0 && j < (len + PAGE - 1) / PAGE && !gone) is = a.table[(long long)par * a.slots + j];
+  if (is < 0 || is >= a.pages) is = -1;
+  if (was < -1 || was >= a.pages) {
+    raise_flag(a.flags, FLAG_CACHE);
+    was = -1;
+  }
+  if (row < a.seqs_out) a.table_out[(long long)row * a.slots + j] = is;
+  if (was == is) return;
+  if (was >= 0) count.add(was, -1);
+  if (is >= 0) count.add(is, 1);
+}
+
+// Larger tables: counts that start as refs, and the entries, by as many workgroups as there are rows or more.
+__global__ __launch_bounds__(256) void fork_refs_kernel(ForkArgs a) {
+  for (int p = (int)blockIdx.x * 256 + (int)threadIdx.x; p < a.pages; p += (int)gridDim.x * 256) a.refs_out[p] = a.refs[p];
+}
+__global__ __launch_bounds__(256) void fork_entries_kernel(ForkArgs a) {
+  const int row = blockIdx.y;
+  int par = -1, len = 0;
+  if (row < a.seqs_out) par = a.parent ? a.parent[row] : row;
+  if (par >= a.seqs) par = -1;
+  if (par >= 0) len = a.lens[par];
+  if (len < 0 || len > a.slots * PAGE) len = 0;          // reported with the rows
+  for (int j = (int)blockIdx.x * 256 + (int)threadIdx.x; j < a.slots; j += (int)gridDim.x * 256)
+    carry_entry(a, Count<false>{a.refs_out}, row, j, row < a.seqs ? a.table[(long long)row * a.slots + j] : -1, par, len);
+}
+
+// Tables of at most so many entries are one workgroup's, with counts in LDS. A step of 64 rows with one workgroup and with many: 8.7 us
+// and 12.9 with 16 entries a row, 16.5 and 13.9 with 256, 60 and 14.2 with 2048.
+constexpr int FORK_LDS_ENTRIES = 8192;
 constexpr int FORK_LDS_PAGES = 12288;                    // 96 KiB of counts and free pages beside 48 KiB of rows
 constexpr int ROWS_EACH = ANVIL_CACHE_ROWS_MAX / META;
 
-// The whole step's tables by one workgroup: a few thousand entries, whose order (references, then copies and new pages row
-// by row, lowest free page first) would need a launch for each step otherwise. A thread's rows stay in its registers. What it takes
-// are the waits for memory one behind the other: parents, lengths, entries, and what is written in the end.
+// A step's tables by one workgroup, or (LDS false) what is left when fork_entries_kernel has carried the entries: copies and new pages
+// row by row, lowest free page first. A thread's rows stay in its registers. What it takes are the waits for memory one behind the
+// other: parents, lengths, entries, and what is written in the end.
 template <bool LDS>
 __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
   extern __shared__ int pages_lds[];
   __shared__ int last[ANVIL_CACHE_ROWS_MAX];             // the shared-candidate page that a row extends into, -1 none
   __shared__ int2 rows[ANVIL_CACHE_ROWS_MAX];            // parent (-1: none), length
   __shared__ int bad;                                    // FLAG_* bits of what rules the step out
-  const Count<LDS> count{LDS ? pages_lds : a.count};
+  constexpr int EACH = LDS ? FORK_LDS_ENTRIES / META : 1;
+  int was[EACH];                                         // on their way beside the rows
+  if constexpr (LDS) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int i = (int)threadIdx.x + k * META;
+      was[k] = i < a.seqs * a.slots ? a.table[i] : -1;
+    }
+  }
+  const Count<LDS> count{LDS ? pages_lds : a.refs_out};
   int* list = LDS ? pages_lds + a.pages : a.list;        // free pages in order
   const int tid = threadIdx.x;
   if (tid == 0) bad = 0;
@@ -333,7 +378,8 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
       add[k] = a.add ? a.add[row] : 0;
     }
   }
-  for (int p = tid; p < a.pages; p += META) count.set(p, a.refs[p]);
+  if constexpr (LDS)
+    for (int p = tid; p < a.pages; p += META) count.set(p, a.refs[p]);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < ROWS_EACH; ++k) {
@@ -357,26 +403,18 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
     last[row] = -1;
     if (add[k] > 0 && len[k] % PAGE) last[row] = a.table[(long long)par[k] * a.slots + len[k] / PAGE];
   }
-  const int in_entries = a.seqs * a.slots, out_entries = a.seqs_out * a.slots;
-  for (int i = tid; i < in_entries; i += META) {
-    const int p = a.table[i];
-    if (p >= 0 && p < a.pages) count.add(p, -1);
-    else if (p != -1) raise_flag(a.flags, FLAG_CACHE);
-  }
+  const int out_entries = a.seqs_out * a.slots;
   __syncthreads();
-  for (int i = tid; i < out_entries; i += META) {
-    const int row = i / a.slots, j = i % a.slots;
-    const int2 r = rows[row];
-    int p = -1;
-    if (r.x >= 0) {
-      const bool gone = a.window && j * PAGE >= a.sinks && j * PAGE + PAGE - 1 <= r.y - a.window;
-      if (j < (r.y + PAGE - 1) / PAGE && !gone) p = a.table[(long long)r.x * a.slots + j];
-      if (p < 0 || p >= a.pages) p = -1;
-      if (p >= 0) count.add(p, 1);
+  if constexpr (LDS) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int i = tid + k * META, row = i / a.slots;
+      if (i >= max(a.seqs, a.seqs_out) * a.slots) break;
+      const int2 r = row < a.seqs_out ? rows[row] : int2{-1, 0};
+      carry_entry(a, count, row, i - row * a.slots, was[k], r.x, r.y);
     }
-    a.table_out[i] = p;
+    __syncthreads();
   }
-  __syncthreads();
   // pages wanted by each row, in order; the copies first
   int wanted = 0, from[ROWS_EACH];
   bool copy[ROWS_EACH];
@@ -396,15 +434,21 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
     from[k] = wanted + prefix((len[k] + add[k] + PAGE - 1) / PAGE - (len[k] + PAGE - 1) / PAGE + copy[k], total);
     wanted += total;
   }
-  // the first `wanted` free pages: each thread its run of pages
-  const int run = (a.pages + META - 1) / META, lo = min(tid * run, a.pages), hi = min(lo + run, a.pages);
-  int free = 0, all;
-  for (int p = lo; p < hi; ++p) free += count.get(p) == 0;
-  int at = prefix(free, all);
-  const bool fail = bad || all < wanted;
-  if (!fail)
-    for (int p = lo; p < hi && at < wanted; ++p)
-      if (count.get(p) == 0) list[at++] = p;
+  // the first `wanted` free pages, a run of RUN a thread at a time
+  constexpr int RUN = LDS ? 2 : 8;
+  int found = 0;
+  if (!bad)
+    for (int p0 = 0; found < wanted && p0 < a.pages; p0 += META * RUN) {
+      int free = 0;
+      const int p = p0 + RUN * tid;
+#pragma unroll
+      for (int k = 0; k < RUN; ++k) free |= (p + k < a.pages && count.get(p + k) == 0) << k;
+      int all;
+      int at = found + prefix(__builtin_popcount(free), all);
+      found += all;
+      for (; free && at < wanted; free &= free - 1) list[at++] = p + __builtin_ctz(free);
+    }
+  const bool fail = bad || found < wanted;
   __syncthreads();
   if (fail) {
     if (tid == 0 && !bad) raise_flag(a.flags, FLAG_PAGES);
@@ -436,8 +480,10 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
     }
     a.lens_out[row] = len[k] + add[k];
   }
-  __syncthreads();
-  for (int p = tid; p < a.pages; p += META) a.refs_out[p] = count.get(p);
+  if constexpr (LDS) {
+    __syncthreads();
+    for (int p = tid; p < a.pages; p += META) a.refs_out[p] = count.get(p);
+  }
 }
 
 struct CompactArgs {
@@ -615,15 +661,22 @@ int anvil_cache_fork(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* o
   if (int r = check_ctx(ctx)) return r;
   char* ws;
   const size_t pairs = (sizeof(int2) * (size_t)out->seqs + 255) / 256 * 256;
-  if (int r = decode_workspace(ctx, pairs + 2 * sizeof(int) * (size_t)in->pages, &ws)) return r;
+  if (int r = decode_workspace(ctx, pairs + sizeof(int) * (size_t)in->pages, &ws)) return r;
   ForkArgs a{in->table, in->lens, in->refs, parent, add, out->table, out->lens, out->refs,
-             (int*)(ws + pairs), (int*)(ws + pairs) + in->pages, (int2*)ws,
+             (int*)(ws + pairs), (int2*)ws,
              in->seqs, out->seqs, in->slots, in->pages, window, sinks, ctx->flags};
-  if (in->pages <= FORK_LDS_PAGES) {
+  const int rows = std::max(in->seqs, out->seqs);
+  if (in->pages <= FORK_LDS_PAGES && (long long)rows * in->slots <= FORK_LDS_ENTRIES) {
     ANVIL_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fork_kernel<true>), hipFuncAttributeMaxDynamicSharedMemorySize,
                                   2 * sizeof(int) * FORK_LDS_PAGES));
     ANVIL_LAUNCH(fork_kernel<true>, dim3(1), dim3(META), 2 * sizeof(int) * in->pages, ctx->stream, a);
   } else {
+    ANVIL_LAUNCH(fork_refs_kernel, dim3((unsigned)std::min(1024, (in->pages + 255) / 256)), dim3(256), 0, ctx->stream, a);
+    ANVIL_LAUNCHED();
+    if (rows) {
+      ANVIL_LAUNCH(fork_entries_kernel, dim3((unsigned)(in->slots + 255) / 256, (unsigned)rows), dim3(256), 0, ctx->stream, a);
+      ANVIL_LAUNCHED();
+    }
     ANVIL_LAUNCH(fork_kernel<false>, dim3(1), dim3(META), 0, ctx->stream, a);
   }
   ANVIL_LAUNCHED();

@@ -613,10 +613,22 @@ def test_a_window_gives_pages_back(window, sinks):
 @pytest.mark.parametrize("seed", range(12))
 def test_random_steps(seed):
     """A batch through several steps: parents, extensions, pages held elsewhere, rows that come and go."""
+    random_steps(seed)
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("more", [dict(extra_slots=2000), dict(spare=13000), dict(extra_slots=400, spare=20000)], ids=str)
+def test_random_steps_of_large_tables(more, seed):
+    """Tables and pools past one workgroup's."""
+    random_steps(seed, **more)
+
+
+def random_steps(seed, **more):
     rng = np.random.default_rng(seed)
     n, slots = int(rng.integers(1, 40)), int(rng.integers(2, 9))
-    seqs = Sequences([int(x) for x in rng.integers(0, 64 * slots // 2, n)], 1, 32, seed, spare=int(rng.integers(0, 60)),
-                     extra_slots=slots, layers=int(rng.integers(1, 3)))
+    seqs = Sequences([int(x) for x in rng.integers(0, 64 * slots // 2, n)], 1, 32, seed,
+                     **{**dict(spare=int(rng.integers(0, 60)), extra_slots=slots, layers=int(rng.integers(1, 3))), **more})
     table, lens, refs = seqs.table, np.array(seqs.lens, np.int32), seqs.refs.copy()
     refs[rng.integers(0, seqs.pages, 2)] += 1
     for _ in range(4):
@@ -657,6 +669,26 @@ def test_parents_and_lengths_out_of_range_are_reported():
             dev.sync()
         got, ln, _ = out.tables()
         assert got.min() >= -1 and got.max() < seqs.pages and ln.min() >= 0 and ln.max() <= 128
+
+
+@gpu
+def test_numbers_out_of_range_in_a_large_table_are_reported():
+    dev = rt.device(0)
+    seqs = Sequences([100, 64], 1, 32, spare=5, extra_slots=9000)
+    pool, most = seqs.pool(), 64 * seqs.slots
+    for parent, add, lens, entry in (([2, 0], [0, 0], None, None), ([-2, 0], [0, 0], None, None), ([0, 1], [-1, 0], None, None),
+                                     ([0, 1], [0, 0], [100, most + 1], None), ([0, 1], [1, 1], [-5, 64], None),
+                                     ([0, 1], [0, 0], None, seqs.pages), ([0, 1], [0, 0], None, -2)):
+        t = seqs.table.copy()
+        if entry is not None:
+            t[0, 0] = entry
+        d = OnDevice(dev, seqs, pool, table=t, lens=lens)
+        out = d.successor()
+        dev.cache_fork(d.cache, out.cache, dev.upload(np.array(parent, np.int32)), dev.upload(np.array(add, np.int32)))
+        with pytest.raises(ValueError, match="parents"):
+            dev.sync()
+        got, ln, _ = out.tables()
+        assert got.min() >= -1 and got.max() < seqs.pages and ln.min() >= 0 and ln.max() <= most
 
 
 @gpu
