@@ -154,6 +154,9 @@ class Decoder:
         cm, T, steps, value = self.cm, self.T, [], {}
         chains = cm._attention_chains("outputs")
         inside = {o for c in chains.values() for o in c}
+        # adds in the epilogue of the product before them, whose own result nothing else reads
+        adds = {op: add for op, add in cm._residual_fusions("outputs").items()
+                if len(cm.users[op.result]) == 1 and g.qt(op.a).dims[-1] % 16 == 0}
         layers, shape = 0, None
 
         def new(v, width=None):
@@ -213,7 +216,17 @@ class Decoder:
             elif isinstance(op, (g.QLinearOp, g.QMatmulOp)):
                 if len(g.qt(op.b).dims) != 2 or op.b not in cm.is_const:
                     raise ValueError(f"decoding: {op.name} {op.sym_str!r} has a computed right operand outside an attention chain")
-                steps.append(("linear", op, rows_of(op.a), new(op.result), None if op.lut is None else table(op.lut)))
+                a, lut, add = rows_of(op.a), None if op.lut is None else table(op.lut), adds.get(op)
+                if add is not None:
+                    inside.add(add)
+                    other = add.b if add.a is op.result else add.a
+                    steps.append(("linear_add", op, a, new(add.result), lut, add, rows_of(other)))
+                    continue
+                call = (op, a, new(op.result), lut)
+                if steps[-1][0] == "linears" and steps[-1][1][0][1] is a and len(steps[-1][1]) < rt.GEMM_GROUP_MAX:
+                    steps[-1][1].append(call)              # of one input: one launch
+                else:
+                    steps.append(("linears", [call]))
             elif isinstance(op, g.RmsNormIntOp):
                 steps.append(("norm", op, rows_of(op.x), new(op.result), table(op.w), table(op.lut)))
             elif isinstance(op, g.AddRequantOp):
@@ -263,14 +276,17 @@ class Decoder:
                 dev.attention_cache(cache, layer, q.buf, o.buf, starts, rows, max_new, heads, (q.width, d, o.width, d),
                                     int(s_op.M), int(s_op.s), const[sm.lut].ptr, int(sm.one), int(op.M), int(op.s),
                                     self.cache.window, self.cache.sinks)
-            elif kind == "linear":
-                a, y, lut = rest
-                flags = rt.GEMM_UNCHECKED
-                if cm.acc_bounds.get(op.result, 1 << 31) < 1 << 23 and abs(int(op.M)) < 1 << 23:
-                    flags |= rt.GEMM_MUL24
-                dev.gemm_i8(a.buf, cm._bt_const(op).ptr, y.buf, 1, 1, rows, y.width, a.width,
-                            [0, 0, a.width, 0, 0, a.width, 0, 0, y.width], int(op.M), int(op.s),
-                            None if lut is None else const[lut].ptr, y.dtype, flags)
+            elif kind == "linears":
+                calls = [self._product(*call, rows, call[2].buf) for call in op]
+                if len(calls) == 1:
+                    dev.gemm_i8(*calls[0])
+                else:
+                    dev.gemm_i8_group(calls)
+            elif kind == "linear_add":
+                a, y, lut, add, r = rest
+                *product, dtype, flags = self._product(op, a, y, lut, rows, None)
+                ma, mb = (add.Mb, add.Ma) if add.a is op.result else (add.Ma, add.Mb)              # residual, product
+                dev.gemm_i8_add(*product, r.buf, int(ma), int(mb), int(add.s), y.buf, [0, 0, y.width, 0, 0, y.width], flags, dtype)
             elif kind == "norm":
                 x, y, w, lut = rest
                 dev.rmsnorm_int(x.buf, x.dtype, const[w].ptr, const[lut].ptr, const[lut].size, int(op.M), int(op.s), op.ss_shift_int,
@@ -286,6 +302,14 @@ class Decoder:
                 x, z, y, lut = rest
                 dev.lut_mul(x.buf, z.buf, const[lut].ptr, int(op.M), int(op.s), rows * y.width, y.buf, rt.OP_UNCHECKED)
         return self.logits.buf
+
+    def _product(self, op, a, y, lut, rows, out):
+        """The arguments of gemm_i8 for rows of a into `out`."""
+        cm, flags = self.cm, rt.GEMM_UNCHECKED
+        if cm.acc_bounds.get(op.result, 1 << 31) < 1 << 23 and abs(int(op.M)) < 1 << 23:
+            flags |= rt.GEMM_MUL24
+        return (a.buf, cm._bt_const(op).ptr, out, 1, 1, rows, y.width, a.width, [0, 0, a.width, 0, 0, a.width, 0, 0, y.width],
+                int(op.M), int(op.s), None if lut is None else cm._const_views[lut].ptr, y.dtype, flags)
 
     # ----------------------------------------------------------------------------------------------- generate
     def generate(self, prompts, new_tokens, beams=1, eos=None, allowed=None) -> Generated:
@@ -354,7 +378,8 @@ class Decoder:
         scores = states[new_tokens % 2]["scores"].download((P, beams), np.int64)
         parent, token = (history[name].download((new_tokens, P, beams), np.int32) for name in ("parent", "token"))
         alive = scores != NO_SCORE
-        tokens = [[_trace(parent, token, p, b, beams, eos) for b in range(beams) if alive[p, b]] for p in range(P)]
+        rows_of = _trace(parent, token)
+        tokens = [[_cut(rows_of[p, b].tolist(), eos) for b in range(beams) if alive[p, b]] for p in range(P)]
         return Generated(tokens, np.where(alive, scores / (1 << Selection.BITS), -np.inf))
 
     def _state(self, rows):
@@ -371,14 +396,20 @@ class Decoder:
         return {"lut": dev.upload(select.lut.astype(np.int32)), "logs": dev.upload(select.logs.astype(np.int32)), "allowed": allowed}
 
 
-def _trace(parent, token, p, b, beams, eos):
-    """A beam's tokens, from the last selection back to the first (whose parents are the prompts)."""
-    out = []
-    for n in range(len(token) - 1, -1, -1):
-        out.append(int(token[n, p, b]))
-        b = int(parent[n, p, b]) - p * beams
-    out.reverse()
-    return out[:out.index(eos) + 1] if eos is not None and eos in out else out
+def _trace(parent, token):
+    """Every beam's tokens (prompts, beams, steps), from the last selection back to the first, whose parents are the prompts. A
+    selection's parents are rows of the one before."""
+    steps, P, beams = token.shape
+    out = np.empty((P, beams, steps), token.dtype)
+    row = np.arange(P * beams)
+    for n in range(steps - 1, -1, -1):
+        out[:, :, n] = token[n].reshape(-1)[row].reshape(P, beams)
+        row = np.maximum(parent[n].reshape(-1)[row], 0)        # -1: of a beam that is none
+    return out
+
+
+def _cut(tokens, eos):
+    return tokens[:tokens.index(eos) + 1] if eos is not None and eos in tokens else tokens
 
 
 @dataclass

@@ -393,6 +393,22 @@ def test_graphs_that_are_not_row_by_row_are_refused():
             graph(build).decoder(rows=1)
 
 
+def test_beams_are_traced_back():
+    rng = np.random.default_rng(0)
+    steps, P, beams = 7, 3, 4
+    parent = np.where(np.arange(steps)[:, None, None] > 0, rng.integers(0, beams, (steps, P, beams)) + beams * np.arange(P)[:, None],
+                      np.arange(P)[:, None] + np.zeros((1, 1, beams), int)).astype(np.int32)
+    token = rng.integers(0, 50, (steps, P, beams)).astype(np.int32)
+    got = decode._trace(parent, token)
+    for p, b in np.ndindex(P, beams):
+        at, want = b, []
+        for n in range(steps - 1, -1, -1):
+            want.append(token[n, p, at])
+            at = parent[n, p, at] - beams * p
+        assert got[p, b].tolist() == want[::-1]
+    assert decode._cut([4, 5, 6], 5) == [4, 5] and decode._cut([4, 5], None) == [4, 5] and decode._cut([4], 9) == [4]
+
+
 def test_selection_tables_are_fixed_point_logs():
     s = decode.Selection.of(0.05)
     assert s.mult == round(0.05 * 65536) and s.step == 45426 and s.lut[255] == 1 << 20
