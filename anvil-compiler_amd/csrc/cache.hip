@@ -287,7 +287,8 @@ struct ForkArgs {
   const int *table, *lens, *refs, *parent, *add;
   int *table_out, *lens_out, *refs_out;
   int* list;                                             // scratch: free pages in order
-  int2* copies;                                          // scratch: (from, to) page of each row, from = -1: none
+  int2* copies;                                          // scratch: (from, to) pages, `*n` of them
+  int* n;
   int seqs, seqs_out, slots, pages, window, sinks;
   unsigned* flags;
 };
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
   extern __shared__ int pages_lds[];
   __shared__ int last[ANVIL_CACHE_ROWS_MAX];             // the shared-candidate page that a row extends into, -1 none
   __shared__ int2 rows[ANVIL_CACHE_ROWS_MAX];            // parent (-1: none), length
-  __shared__ int bad;                                    // FLAG_* bits of what rules the step out
+  __shared__ int bad, copied;                            // FLAG_* bits of what rules the step out; pages copied so far
   constexpr int EACH = LDS ? FORK_LDS_ENTRIES / META : 1;
   int was[EACH];                                         // on their way beside the rows
   if constexpr (LDS) {
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
   const Count<LDS> count{LDS ? pages_lds : a.refs_out};
   int* list = LDS ? pages_lds + a.pages : a.list;        // free pages in order
   const int tid = threadIdx.x;
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = 0, copied = 0;
   int par[ROWS_EACH], len[ROWS_EACH], add[ROWS_EACH];
 #pragma unroll
   for (int k = 0; k < ROWS_EACH; ++k) {
@@ -453,10 +454,8 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
   if (fail) {
     if (tid == 0 && !bad) raise_flag(a.flags, FLAG_PAGES);
     for (int i = tid; i < out_entries; i += META) a.table_out[i] = -1;
-    for (int row = tid; row < a.seqs_out; row += META) {
-      a.lens_out[row] = 0;
-      a.copies[row] = {-1, 0};
-    }
+    for (int row = tid; row < a.seqs_out; row += META) a.lens_out[row] = 0;
+    if (tid == 0) *a.n = 0;
     for (int p = tid; p < a.pages; p += META) a.refs_out[p] = a.refs[p];
     return;
   }
@@ -466,24 +465,23 @@ __global__ __launch_bounds__(META) void fork_kernel(ForkArgs a) {
     if (row >= a.seqs_out) break;
     const int* take = list + from[k];
     int* entries = a.table_out + (long long)row * a.slots;
-    int2 pair = {-1, 0};
     if (copy[k]) {
-      pair = {last[row], *take++};
+      const int2 pair = {last[row], *take++};
       entries[len[k] / PAGE] = pair.y;
       count.add(pair.x, -1);
       count.set(pair.y, 1);
+      a.copies[atomicAdd(&copied, 1)] = pair;            // in any order: no page is in two of them but as a source
     }
-    a.copies[row] = pair;
     for (int j = (len[k] + PAGE - 1) / PAGE; j < (len[k] + add[k] + PAGE - 1) / PAGE; ++j) {
       entries[j] = *take;
       count.set(*take++, 1);
     }
     a.lens_out[row] = len[k] + add[k];
   }
-  if constexpr (LDS) {
-    __syncthreads();
+  __syncthreads();
+  if (tid == 0) *a.n = copied;
+  if constexpr (LDS)
     for (int p = tid; p < a.pages; p += META) a.refs_out[p] = count.get(p);
-  }
 }
 
 struct CompactArgs {
@@ -527,31 +525,32 @@ __global__ __launch_bounds__(META) void compact_map_kernel(CompactArgs a) {
   if (tid == 0) *a.n = movers;
 }
 
-// Pages pairs[i].x -> pairs[i].y of every layer (blockIdx: part of a page, pair, layer).
-// 16 bytes a thread: with four of them, loads before stores, a compaction of 156 MB ran in 76.5 us instead of 63.2 (4.9 TB/s).
+// Pages pairs[i].x -> pairs[i].y of every layer (blockIdx: part of a page, pair, striding, layer).
+// 16 bytes a thread: with four of them, loads before stores, a compaction of 156 MB ran in 76.5 us instead of 63.2.
 constexpr int COPY_THREADS = 256;
 struct CopyArgs {
   uint8_t* pool;
   const int2* pairs;
-  int first, pages, page_bytes;
+  const int* n;
+  int pages, page_bytes, step;                           // step: workgroups of a part and layer
 };
-__device__ __forceinline__ void copy_page(const CopyArgs& a, int2 pair) {
+__device__ __forceinline__ void copy_pages(const CopyArgs& a) {
   const long long layer = (long long)blockIdx.z * a.pages;
-  const uint4* src = (const uint4*)(a.pool + (layer + pair.x) * a.page_bytes);
-  uint4* dst = (uint4*)(a.pool + (layer + pair.y) * a.page_bytes);
-  const int at = (int)blockIdx.x * COPY_THREADS + (int)threadIdx.x;
-  if (at < a.page_bytes / 16) dst[at] = src[at];
+  const int at = (int)blockIdx.x * COPY_THREADS + (int)threadIdx.x, n = *a.n;
+  int2 pair = a.pairs[blockIdx.y];                       // beside n: there is room for a pair each
+  if (at >= a.page_bytes / 16) return;
+  for (int i = blockIdx.y; i < n; i += a.step) {
+    if (i != (int)blockIdx.y) pair = a.pairs[i];
+    ((uint4*)(a.pool + (layer + pair.y) * a.page_bytes))[at] = ((const uint4*)(a.pool + (layer + pair.x) * a.page_bytes))[at];
+  }
 }
 
-__global__ __launch_bounds__(COPY_THREADS) void fork_copy_kernel(CopyArgs a) {
-  const int2 pair = a.pairs[a.first + blockIdx.y];
-  if (pair.x >= 0) copy_page(a, pair);
-}
+__global__ __launch_bounds__(COPY_THREADS) void fork_copy_kernel(CopyArgs a) { copy_pages(a); }
 
-// The moved pages, and by the workgroups behind them (blockIdx.y = pairs) the tables, which the map now tells.
-__global__ __launch_bounds__(COPY_THREADS) void compact_move_kernel(CopyArgs a, CompactArgs t, int pairs) {
-  if ((int)blockIdx.y < pairs) {
-    if (a.first + (int)blockIdx.y < *t.n) copy_page(a, a.pairs[a.first + blockIdx.y]);
+// The moved pages, and by the workgroups behind them (blockIdx.y = step) the tables, which the map now tells.
+__global__ __launch_bounds__(COPY_THREADS) void compact_move_kernel(CopyArgs a, CompactArgs t) {
+  if ((int)blockIdx.y < a.step) {
+    copy_pages(a);
     return;
   }
   const int step = (int)(gridDim.x * gridDim.z) * COPY_THREADS;
@@ -587,17 +586,15 @@ static int check_pair(const char* who, const anvil_cache* in, const anvil_cache*
   return ANVIL_OK;
 }
 
-// launch(arguments, grid) for so many pairs of pages, 32768 at a time (a grid dimension's limit)
-template <typename F>
-static int copy_pages(const anvil_cache* c, const int2* pairs, int n, F&& launch) {
-  CopyArgs a{(uint8_t*)c->pool, pairs, 0, c->pages, c->heads * 2176 * groups_of(c->dim)};
-  const int per = 16 * COPY_THREADS;
-  do {
-    const dim3 grid((unsigned)((a.page_bytes + per - 1) / per), (unsigned)std::min(n - a.first, 32768), (unsigned)c->layers);
-    launch(a, grid);
-    ANVIL_LAUNCHED();
-  } while ((a.first += 32768) < n);
-  return ANVIL_OK;
+// The copies of at most so many pairs, and their grid. A step copies little, and 278000 workgroups that find nothing to do take 60 us
+// (512 rows of 32 layers, 8 heads of 128: 73 us a step, 14 with at most 16384); a compaction of 400 pages of 12 layers takes 63.9 us
+// with 16384 workgroups, 66.3 with half or twice as many, 74 with one a pair.
+constexpr int COPY_GROUPS = 16384;
+static dim3 copy_grid(const anvil_cache* c, const int2* pairs, const int* n, int most, CopyArgs* a) {
+  *a = {(uint8_t*)c->pool, pairs, n, c->pages, c->heads * 2176 * groups_of(c->dim), 0};
+  const int parts = (a->page_bytes + 16 * COPY_THREADS - 1) / (16 * COPY_THREADS);
+  a->step = (int)std::max<long long>(1, std::min<long long>(most, COPY_GROUPS / ((long long)parts * c->layers)));
+  return dim3((unsigned)parts, (unsigned)a->step, (unsigned)c->layers);
 }
 
 }  // namespace anvil
@@ -661,9 +658,11 @@ int anvil_cache_fork(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* o
   if (int r = check_ctx(ctx)) return r;
   char* ws;
   const size_t pairs = (sizeof(int2) * (size_t)out->seqs + 255) / 256 * 256;
-  if (int r = decode_workspace(ctx, pairs + sizeof(int) * (size_t)in->pages, &ws)) return r;
+  if (int r = decode_workspace(ctx, 256 + pairs + sizeof(int) * (size_t)in->pages, &ws)) return r;
+  int* copied = (int*)ws;
+  ws += 256;
   ForkArgs a{in->table, in->lens, in->refs, parent, add, out->table, out->lens, out->refs,
-             (int*)(ws + pairs), (int2*)ws,
+             (int*)(ws + pairs), (int2*)ws, copied,
              in->seqs, out->seqs, in->slots, in->pages, window, sinks, ctx->flags};
   const int rows = std::max(in->seqs, out->seqs);
   if (in->pages <= FORK_LDS_PAGES && (long long)rows * in->slots <= FORK_LDS_ENTRIES) {
@@ -681,9 +680,11 @@ int anvil_cache_fork(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* o
   }
   ANVIL_LAUNCHED();
   if (!add || !out->seqs) return ANVIL_OK;
-  return copy_pages(out, a.copies, out->seqs, [&](const CopyArgs& copy, dim3 grid) {
-    ANVIL_LAUNCH(fork_copy_kernel, grid, dim3(COPY_THREADS), 0, ctx->stream, copy);
-  });
+  CopyArgs copy;
+  const dim3 grid = copy_grid(out, a.copies, copied, out->seqs, &copy);
+  ANVIL_LAUNCH(fork_copy_kernel, grid, dim3(COPY_THREADS), 0, ctx->stream, copy);
+  ANVIL_LAUNCHED();
+  return ANVIL_OK;
 }
 
 int anvil_cache_compact(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache* out, int32_t* map) {
@@ -698,12 +699,12 @@ int anvil_cache_compact(anvil_ctx* ctx, const anvil_cache* in, const anvil_cache
                 in->seqs, in->slots, in->pages, ctx->flags};
   ANVIL_LAUNCH(compact_map_kernel, dim3(1), dim3(META), 0, ctx->stream, a);
   ANVIL_LAUNCHED();
-  // at most half of the pages have a hole before them
-  return copy_pages(in, a.moves, in->pages / 2, [&](const CopyArgs& copy, dim3 grid) {
-    const int pairs = (int)grid.y;
-    if (copy.first == 0) ++grid.y;                       // the tables, once
-    ANVIL_LAUNCH(compact_move_kernel, grid, dim3(COPY_THREADS), 0, ctx->stream, copy, a, pairs);
-  });
+  CopyArgs copy;
+  dim3 grid = copy_grid(in, a.moves, a.n, in->pages / 2, &copy);                 // at most half of the pages have a hole before them
+  ++grid.y;                                              // the tables
+  ANVIL_LAUNCH(compact_move_kernel, grid, dim3(COPY_THREADS), 0, ctx->stream, copy, a);
+  ANVIL_LAUNCHED();
+  return ANVIL_OK;
 }
 
 }  // extern "C"
