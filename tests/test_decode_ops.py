@@ -692,7 +692,8 @@ def test_numbers_out_of_range_in_a_large_table_are_reported():
 
 
 @gpu
-@pytest.mark.parametrize("pages,share", [(1, 1.0), (8, 0.0), (8, 0.5), (64, 1.0), (1000, 0.5), (1025, 0.1), (3000, 0.9)])
+@pytest.mark.parametrize("pages,share", [(1, 1.0), (8, 0.0), (8, 0.5), (64, 1.0), (1000, 0.5), (1025, 0.1), (3000, 0.9),
+                                         (4096, 0.5), (4097, 0.3), (20000, 0.02), (30000, 0.6)])
 @pytest.mark.parametrize("layers,heads,dim", [(1, 1, 32), (3, 2, 64)])
 def test_compact(pages, share, layers, heads, dim):
     dev = rt.device(0)
