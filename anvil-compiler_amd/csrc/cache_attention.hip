@@ -506,6 +506,9 @@ __device__ __forceinline__ int lanes_max(int v) {
 // v_rcp_f64 is off by up to 2^-20, and with the roundings (2^-53 each) of a quotient below 2^15 the sum is off by less than
 // 2^15 (2^-51 + 2 2^-53) + 2^-51 < 2^-35: it is not below the quotient, and above it by less than 2^-34 < 1 / S, so no whole number
 // lies between the two. For a larger S the quotient is put right by its remainder.
+//
+// That p is at most `one`, and so fits its part of a packed entry, holds for the scores that the row has: their e is part of S. A table need
+// not rise, and the entry of a score that no key has may be larger than S by any factor: it counts as 0.
 template <int TABLE, int LANES>
 __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, int one, unsigned* flags) {
   constexpr int N = 64 / LANES;
@@ -528,7 +531,7 @@ __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, i
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int x = min(4 * (lane + LANES * i) + j, max(top, 0)) - max(top, 0) + 255;        // larger scores do not occur
-      e[i][j] = (double)(unsigned)max(0, lut[x]);
+      e[i][j] = word(count[i], j) ? (double)(unsigned)max(0, lut[x]) : 0.0;
       S = __builtin_fma(e[i][j], (double)word(count[i], j), S);
     }
   S = lanes_sum<LANES>(S);
