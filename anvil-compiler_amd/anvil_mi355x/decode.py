@@ -43,8 +43,8 @@ class KVCache:
         self.moved = dev.alloc(4 * pages)                      # compact()'s map
         self._back = False                                     # the tables before the last step still hold
 
-    def _cache(self, which):
-        return rt.Cache(self.pool, *self._sets[which], seqs=self._n[which], **self._shape)
+    def _cache(self, which, seqs=None):
+        return rt.Cache(self.pool, *self._sets[which], seqs=self._n[which] if seqs is None else seqs, **self._shape)
 
     @property
     def cache(self) -> rt.Cache:
@@ -61,8 +61,7 @@ class KVCache:
         n = self.seqs if rows is None else rows
         if not 0 <= n <= self._rows:
             raise ValueError(f"{n} rows in a cache of {self._rows}")
-        self._n[1 - self._at] = n
-        self.dev.cache_fork(self.cache, self._cache(1 - self._at), parent, add, self.window, self.sinks)
+        self.dev.cache_fork(self.cache, self._cache(1 - self._at, n), parent, add, self.window, self.sinks)
         self.stepped(n)
         self._back = add is None or parent is None and not self.window
 
@@ -73,9 +72,10 @@ class KVCache:
 
     def compact(self):
         """Used pages to the pool's lowest ids; self.moved then holds each page's new id (-1: free)."""
-        self._n[1 - self._at] = self.seqs
-        self.dev.cache_compact(self.cache, self._cache(1 - self._at), self.moved)
-        self._at, self._back = 1 - self._at, True
+        n = self.seqs
+        self.dev.cache_compact(self.cache, self._cache(1 - self._at, n), self.moved)
+        self.stepped(n)
+        self._back = True
 
     def undo(self):
         """The tables before the last compact() or step(), as long as nothing has been appended since. A step that both gives pages

@@ -4,6 +4,9 @@ import numpy as np
 import pytest
 
 import test_decode_ops as ops
+from anvil_mi355x import decode
+from anvil_mi355x import runtime as rt
+from host_cache import HostDevice
 
 gpu = pytest.mark.gpu
 
@@ -38,3 +41,51 @@ def test_attention_of_many_rows_with_tables_whose_unseen_entries_are_large(monke
     monkeypatch.setitem(ops.LUTS, "falling", _falling(window, 3))
     for case in ops.MANY:
         ops.attention_case(*case, 32, seed=one, lut="falling", one=one, window=window)
+
+
+# ------------------------------------------------------------------------------- a cache's steps and their undoing
+
+DEVICES = [pytest.param(HostDevice, id="host"), pytest.param(lambda: rt.device(0), id="device", marks=gpu)]
+
+
+def _int32s(dev, *x):
+    return dev.upload(np.array(x, np.int32))
+
+
+def _same(got, want):
+    for g, w in zip(got, want):
+        np.testing.assert_array_equal(g, w)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_refused_step_leaves_the_cache_as_it_was(device):
+    dev = device()
+    cache = decode.KVCache(dev, 1, 1, 32, 12, 4, 200)
+    cache.reset(2)
+    before = cache.tables()
+    add = _int32s(dev, 70, 5)
+    cache.step(None, add)
+    after = cache.tables()
+    for refused in (lambda: cache.step(None, add, rows=4), lambda: cache.step(None, add, rows=1),
+                    lambda: dev.cache_fork(cache.cache, cache.cache), lambda: cache.step(None, add, rows=5)):
+        with pytest.raises(ValueError):
+            refused()
+        assert cache.seqs == 2
+        _same(cache.tables(), after)
+    cache.undo()
+    assert cache.seqs == 2
+    _same(cache.tables(), before)
+
+
+def test_a_refused_compaction_leaves_the_cache_as_it_was():
+    dev = HostDevice()
+    cache = decode.KVCache(dev, 1, 1, 32, 12, 4, 200)
+    cache.step(_int32s(dev, 0, 1), None, rows=2)
+    moved, cache.moved = cache.moved, None
+    with pytest.raises(ValueError, match="map"):
+        cache.compact()
+    cache.moved = moved
+    assert cache.seqs == 2
+    cache.undo()
+    assert cache.seqs == 4
+    dev.sync()
