@@ -41,7 +41,7 @@ class KVCache:
         self._shape = dict(slots=slots, pages=pages, heads=heads, dim=dim, layers=layers)
         self._rows, self._n, self._at = rows, [rows, rows], 0
         self.moved = dev.alloc(4 * pages)                      # compact()'s map
-        self._back = False                                     # the tables before the last step still hold
+        self._back = False                                     # the tables before the last step still hold; None: if it failed
 
     def _cache(self, which, seqs=None):
         return rt.Cache(self.pool, *self._sets[which], seqs=self._n[which] if seqs is None else seqs, **self._shape)
@@ -57,18 +57,20 @@ class KVCache:
 
     def step(self, parent=None, add=None, rows=None):
         """The tables of the next step: row i continues row parent[i] (device int32s; None: row i) by add[i] tokens (device int32s;
-        None: none). rows: how many there are, with parents."""
+        None: none). rows: how many there are, with parents. Too few free pages are reported by the device's sync() as MemoryError, and
+        leave every row empty: undo() then goes back to the rows as they were, if no other step has been taken since."""
         n = self.seqs if rows is None else rows
         if not 0 <= n <= self._rows:
             raise ValueError(f"{n} rows in a cache of {self._rows}")
         self.dev.cache_fork(self.cache, self._cache(1 - self._at, n), parent, add, self.window, self.sinks)
         self.stepped(n)
-        self._back = add is None or parent is None and not self.window
+        if add is None or parent is None and not self.window:
+            self._back = True
 
     def stepped(self, rows):
         """A step that recorded kernels have taken."""
         self._at = 1 - self._at
-        self._n[self._at], self._back = rows, False
+        self._n[self._at], self._back = rows, None
 
     def compact(self):
         """Used pages to the pool's lowest ids; self.moved then holds each page's new id (-1: free)."""
@@ -79,7 +81,11 @@ class KVCache:
 
     def undo(self):
         """The tables before the last compact() or step(), as long as nothing has been appended since. A step that both gives pages
-        back (parents or a window) and adds tokens may have written some of them, and cannot be taken back."""
+        back (parents or a window) and adds tokens may have written some of them, and cannot be taken back unless it failed: its rows
+        are then empty and its references those of before, and it has written nothing (this waits for the device to see that)."""
+        if self._back is None:
+            (_, lens, refs), (_, _, before) = self.tables(), self._tables(1 - self._at)
+            self._back = not lens.any() and np.array_equal(refs, before)
         if not self._back:
             raise ValueError("the last step cannot be taken back")
         self._at, self._back = 1 - self._at, False
@@ -96,8 +102,11 @@ class KVCache:
 
     def tables(self):
         """(table, lens, refs) on the host."""
-        table, lens, refs = self._sets[self._at]
-        n, slots = self.seqs, self._shape["slots"]
+        return self._tables(self._at)
+
+    def _tables(self, which):
+        table, lens, refs = self._sets[which]
+        n, slots = self._n[which], self._shape["slots"]
         return (table.download((n, slots), np.int32), lens.download((n,), np.int32),
                 refs.download((self._shape["pages"],), np.int32))
 

@@ -89,3 +89,54 @@ def test_a_refused_compaction_leaves_the_cache_as_it_was():
     cache.undo()
     assert cache.seqs == 4
     dev.sync()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("window", [0, 10])
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_step_that_runs_out_of_pages_is_taken_back(device, window, recorded):
+    """Parents, added tokens and a window: a step that went well cannot be taken back, one that found too few pages can."""
+    dev = device()
+    cache = decode.KVCache(dev, 2, 1, 32, 5, 3, 256, window=window)
+    cache.reset(2)
+    cache.step(None, _int32s(dev, 64, 60))
+    parent, one, many = _int32s(dev, 0, 1, 1), _int32s(dev, 1, 1, 1), _int32s(dev, 1, 130, 130)
+    cache.step(parent, one, 3)
+    dev.sync()
+    before = cache.tables()
+    with pytest.raises(ValueError, match="taken back"):
+        cache.undo()
+    _same(cache.tables(), before)
+    if recorded:                                               # what KVCache.step calls, then the word that it has run
+        dev.cache_fork(cache.cache, cache._cache(1 - cache._at, 3), None, many, window, 0)
+        cache.stepped(3)
+    else:
+        cache.step(parent, many, 3)
+    with pytest.raises(MemoryError):
+        dev.sync()
+    assert not cache.tables()[1].any()
+    cache.undo()
+    _same(cache.tables(), before)
+    with pytest.raises(ValueError, match="taken back"):        # once
+        cache.undo()
+    cache.step(_int32s(dev, -1, 1, -1), None, 3)               # a row stays, and the step fits
+    cache.step(None, _int32s(dev, 0, 130, 0))
+    dev.sync()
+    assert cache.tables()[1].tolist() == [0, 191, 0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_that_empties_every_row_is_not_mistaken_for_a_failed_one(device):
+    """Rows given back and none extended, with `add` at hand: references tell it from a step that found no pages."""
+    dev = device()
+    cache = decode.KVCache(dev, 1, 1, 32, 5, 2, 256)
+    cache.step(None, _int32s(dev, 64, 60))
+    cache.step(_int32s(dev, -1, -1), _int32s(dev, 1, 1), 2)
+    dev.sync()
+    assert not cache.tables()[1].any() and not cache.tables()[2].any()
+    with pytest.raises(ValueError, match="taken back"):
+        cache.undo()
+    cache.reset()
+    cache.step(_int32s(dev, -1, 1), _int32s(dev, 1, 0), 2)     # nothing was there: nothing is written or given back
+    cache.undo()
+    assert cache.seqs == 2
