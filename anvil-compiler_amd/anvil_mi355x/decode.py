@@ -259,11 +259,14 @@ class Decoder:
         Smaller ones that came before stay, for launches recorded with them."""
         if rows <= self._room:
             return
-        self._room = max(rows, 2 * self._room)
-        for r in self._values:
-            self._buffers.append(r.buf)
-            r.buf = self.dev.alloc(self._room * r.width * rt.ITEMSIZE[r.dtype])
-            self.dev.zero(r.buf, r.buf.nbytes)
+        room = max(rows, 2 * self._room)
+        bufs = [self.dev.alloc(room * r.width * rt.ITEMSIZE[r.dtype]) for r in self._values]
+        for r, buf in zip(self._values, bufs):
+            self.dev.zero(buf, buf.nbytes)
+            if r.buf is not None:
+                self._buffers.append(r.buf)
+            r.buf = buf
+        self._room = room                                      # once all of them are there
 
     # ------------------------------------------------------------------------------------------------ forward
     def forward(self, ids, starts, rows, max_new):

@@ -140,3 +140,46 @@ def test_a_step_that_empties_every_row_is_not_mistaken_for_a_failed_one(device):
     cache.step(_int32s(dev, -1, 1), _int32s(dev, 1, 0), 2)     # nothing was there: nothing is written or given back
     cache.undo()
     assert cache.seqs == 2
+
+
+# ------------------------------------------------------------------------------------------- the decoder's buffers
+
+class _Short(HostDevice):
+    """A device with room for so many more allocations."""
+    left = 1 << 30
+
+    def alloc(self, nbytes):
+        if not self.left:
+            raise RuntimeError("anvil_alloc: out of memory")
+        self.left -= 1
+        return super().alloc(nbytes)
+
+    def zero(self, buf, nbytes):
+        buf.bytes[:nbytes] = 0
+
+
+@pytest.mark.parametrize("left", range(4))
+def test_buffers_that_could_not_grow_are_not_taken_for_grown(left):
+    """A call that runs out of memory while it makes room must leave the next one to make it."""
+    dec = object.__new__(decode.Decoder)
+    dec.dev, dec._room, dec._buffers = _Short(), 0, []
+    dec._values = [decode._Rows(32, "i8"), decode._Rows(48, "i16"), decode._Rows(7, "i8")]
+
+    def holds(rows):
+        return all(v.buf is not None and v.buf.nbytes >= rows * v.width * rt.ITEMSIZE[v.dtype] for v in dec._values)
+
+    dec._make_room(5)
+    assert holds(5)
+    small = [v.buf for v in dec._values]
+    dec.dev.left = left
+    if left < len(dec._values):
+        with pytest.raises(RuntimeError, match="out of memory"):
+            dec._make_room(100)
+    else:
+        dec._make_room(100)
+    dec.dev.left = 1 << 30
+    dec._make_room(5)
+    assert holds(5) and holds(dec._room)
+    dec._make_room(100)
+    assert holds(100) and holds(dec._room)
+    assert all(any(b is x for x in dec._buffers) for b in small)                   # recorded launches may name them
