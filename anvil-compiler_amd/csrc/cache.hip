@@ -563,8 +563,11 @@ __global__ __launch_bounds__(COPY_THREADS) void compact_move_kernel(CopyArgs a, 
     copy_pages(a);
     return;
   }
-  const int step = (int)(gridDim.x * gridDim.z) * COPY_THREADS;
-  for (int i = (int)(blockIdx.x + blockIdx.z * gridDim.x) * COPY_THREADS + (int)threadIdx.x; i < t.seqs * t.slots; i += step) {
+  // parts x layers x COPY_THREADS passes 2^31 in a pool of few large pages
+  const long long step = (long long)gridDim.x * gridDim.z * COPY_THREADS;
+  const int entries = t.seqs * t.slots;
+  for (long long at = ((long long)blockIdx.z * gridDim.x + blockIdx.x) * COPY_THREADS + threadIdx.x; at < entries; at += step) {
+    const int i = (int)at;
     const int p = t.table[i];
     int to = -1;
     if (p >= 0 && p < t.pages) to = t.map[p];

@@ -183,3 +183,35 @@ def test_buffers_that_could_not_grow_are_not_taken_for_grown(left):
     dec._make_room(100)
     assert holds(100) and holds(dec._room)
     assert all(any(b is x for x in dec._buffers) for b in small)                   # recorded launches may name them
+
+
+# ------------------------------------------------------------------------------------------------- large pools
+
+@gpu
+def test_compaction_of_a_pool_of_few_large_pages():
+    """4096 heads of 128 are 8704 workgroups a page and layer: with 1000 layers the launch has more threads than an int holds. Two pages,
+    of which the second moves; the bytes looked at are the first and the last layer's."""
+    dev = rt.Device(0)
+    heads, dim, layers, pages, slots = 4096, 128, 1000, 2, 16384
+    page = heads * 68 * dim
+    pool = dev.alloc(dev.cache_bytes(layers, pages, heads, dim))
+    rng = np.random.default_rng(0)
+    first, last = (rng.integers(0, 256, page).astype(np.uint8) for _ in range(2))
+    pool.upload(first, page)
+    pool.upload(last, (2 * layers - 1) * page)
+    table = np.full((40, slots), -1, np.int32)
+    table[[0, 39], [5, slots - 1]] = 1
+    lens = np.arange(40, dtype=np.int32)
+    cache = rt.Cache(pool, t := dev.upload(table), n := dev.upload(lens), r := dev.upload(np.array([0, 2], np.int32)), seqs=40,
+                     slots=slots, pages=pages, heads=heads, dim=dim, layers=layers)
+    out = [dev.upload(np.full(x, 0x5A5A5A5A, np.int32)) for x in (table.size, 40, pages)]
+    moved = dev.alloc(4 * pages)
+    dev.cache_compact(cache, cache.with_tables(*out), moved)
+    dev.sync()
+    assert np.array_equal(out[0].download(table.shape, np.int32), np.where(table < 0, -1, 0))
+    assert np.array_equal(out[1].download((40,), np.int32), lens)
+    assert out[2].download((2,), np.int32).tolist() == [2, 0] and moved.download((2,), np.int32).tolist() == [-1, 0]
+    assert np.array_equal(pool.download((page,), np.uint8), first)
+    assert np.array_equal(pool.download((page,), np.uint8, (2 * layers - 2) * page), last)
+    del t, n, r
+    dev.close()
