@@ -213,6 +213,9 @@ class Decoder:
                 if n != T or not sm.causal or shape not in (None, (heads, d)):
                     raise ValueError("decoding needs causal attention over the graph's tokens, with every layer's heads alike")
                 shape = (heads, d)
+                # what the attention over the cache takes, whose scores' products are bounded by the values that 4 bits hold
+                if 128 * 126 * d * abs(int(s_op.M)) + (1 << int(s_op.s) >> 1) > 2 ** 31 - 1:
+                    raise OverflowError(f"decoding: {s_op.sym_str!r}'s multiplier {int(s_op.M)} may take scores past int32")
                 split = np.arange(T * heads * d).reshape(T, heads, d).transpose(1, 0, 2)
                 qkv = []
                 for v, want in ((s_op.a, split), (s_op.b, split.transpose(0, 2, 1)), (op.b, split)):

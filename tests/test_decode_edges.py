@@ -3,8 +3,10 @@ integer, so every comparison is exact."""
 import numpy as np
 import pytest
 
+import anvil_mi355x
 import test_decode_ops as ops
 from anvil_mi355x import decode
+from anvil_mi355x import ir as g
 from anvil_mi355x import runtime as rt
 from host_cache import HostDevice
 
@@ -215,3 +217,36 @@ def test_compaction_of_a_pool_of_few_large_pages():
     assert np.array_equal(pool.download((page,), np.uint8, (2 * layers - 2) * page), last)
     del t, n, r
     dev.close()
+
+
+# ------------------------------------------------------------------------------------------ what can be decoded
+
+def _attention_graph(m_s=1, s_s=9):
+    """One head of 32 over 32 tokens, queries within 4 of zero by their table, so that the proof allows a large score multiplier."""
+    bld = g.GraphBuilder("m")
+    x, w, lut = bld.input("x", [32, 32], "i8", 0.1), bld.const("w", [32, 32], "i8"), bld.const("lut", [256], "i32")
+    q = bld.qlinear("q", x, w, 1, 5, lut=bld.const("near", [256], "i8"))
+    k, v = (bld.qlinear(n, x, w, 1, 5) for n in "kv")
+    s = bld.qmatmul("s", q, bld.transpose("kt", k, [1, 0]), m_s, s_s)
+    bld.output(bld.qmatmul("o", bld.softmax_lut("p", s, lut, 127, True), v, 1, 7))
+    consts = {"w": np.eye(32, dtype=int), "near": np.arange(-128, 128) // 32, "lut": np.r_[np.zeros(250, int), 1, 2, 4, 9, 20, 40]}
+    return anvil_mi355x.compile((bld.module(), consts), embedding=(np.zeros((32, 32)), np.zeros((32, 32))))
+
+
+def test_a_score_multiplier_that_the_cache_cannot_take_is_refused_at_once():
+    """128 * 126 * 32 * |m| + 2^(s-1) < 2^31, or the attention over the cache refuses every call."""
+    most = ((1 << 31) - 1 - (1 << 8)) // (128 * 126 * 32)
+    for m in (most + 1, -most - 1):
+        cm = _attention_graph(m)
+        assert cm.proven
+        with pytest.raises(OverflowError, match="multiplier"):
+            cm.decoder(rows=1)
+
+
+@gpu
+def test_the_largest_score_multiplier_is_taken():
+    cm = _attention_graph(((1 << 31) - 1 - (1 << 8)) // (128 * 126 * 32))
+    dec, dev = cm.decoder(rows=1), cm.dev
+    dec.cache.step(None, _int32s(dev, 1))
+    dec.forward(_int32s(dev, 0), None, 1, 1)
+    dev.sync()
