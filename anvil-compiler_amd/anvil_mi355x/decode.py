@@ -161,7 +161,7 @@ class Decoder:
         """The graph's ops as calls on rows: ([(kind, op, ...)], layers, heads, dim). What a row holds is told by the indexes that a
         chain of transposes and reshapes moves its elements by."""
         cm, T, steps, value = self.cm, self.T, [], {}
-        chains = cm._attention_chains("outputs")
+        chains = cm._attention_chains("outputs", rt.CACHE_TOKENS_MAX)
         inside = {o for c in chains.values() for o in c}
         # adds in the epilogue of the product before them, whose own result nothing else reads
         adds = {op: add for op, add in cm._residual_fusions("outputs").items()

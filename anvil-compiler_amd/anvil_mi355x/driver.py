@@ -94,6 +94,7 @@ def _checked_graph(module, consts, prove=True):
     return module, consts
 
 
+ATTENTION_MAX = 1024       # tokens of a sequence that the fused attention of whole sequences takes
 PINNED_MAX = 1 << 28       # read-back buffers up to this size download into page-locked host memory
 # run()'s float inputs and token ids up to this size are read by their kernel where the host wrote them: with the wait
 # 17 us against 35 for 8 KiB through a device copy, 48 against 61 at 1 MiB, no difference at 4 MiB
@@ -218,10 +219,10 @@ class CompiledModel:
                     phys[root] = _swap_last2(len(g.qt(root).dims))
         return phys
 
-    def _chain_of(self, o_op):
+    def _chain_of(self, o_op, longest=ATTENTION_MAX):
         """(scores matmul, softmax) when o_op is the P.V product of a chain the fused attention evaluates (the
         structure only: proven, int8 throughout, q, k and v computed and of one rank, scores and p read by nothing else,
-        square scores with T up to 1024 and a head dim of 16, 32, 64 or 128), else None."""
+        square scores with T up to `longest` and a head dim of 16, 32, 64 or 128), else None."""
         if not self.proven or not isinstance(o_op, g.QMatmulOp) or o_op.lut is not None:
             return None
         if g.qt(o_op.result).dtype != "i8":
@@ -239,7 +240,7 @@ class CompiledModel:
         if any(v in self.is_const or len(g.qt(v).dims) != len(sd) for v in (s_op.a, s_op.b, o_op.b)):
             return None                       # a const has no batch dim, a (K, N) right operand none of the heads'
         T, D = sd[-1], g.qt(s_op.a).dims[-1]
-        if sd[-2] != T or T > 1024 or D not in (16, 32, 64, 128) or od[-1] != D or od[-2] != T:
+        if sd[-2] != T or T > longest or D not in (16, 32, 64, 128) or od[-1] != D or od[-2] != T:
             return None
         return s_op, sm
 
@@ -448,17 +449,17 @@ class CompiledModel:
                                                        t.dtype, rt.OP_UNCHECKED if sure else 0])
         return out
 
-    def _attention_chains(self, keep) -> dict:
+    def _attention_chains(self, keep, longest=ATTENTION_MAX) -> dict:
         """{P.V matmul: (scores matmul, softmax)} for every chain qmatmul -> softmax_lut -> qmatmul whose scores and
         probabilities are read by nothing else, in a proven graph with int8 values throughout, a square (T x T)
-        score matrix with T up to 1024 and one head dim of 16, 32, 64 or 128: the chains
+        score matrix with T up to `longest` and one head dim of 16, 32, 64 or 128: at the default, the chains
         anvil_attention_i8 evaluates without materialising scores or p, or, when the run returns them (keep="all",
         or graph outputs), anvil_attention_i8_keep, which also stores them (_kept_chain)."""
         if not self.proven:
             return {}
         found = {}
         for o_op in self.ops:
-            chain = self._chain_of(o_op)
+            chain = self._chain_of(o_op, longest)
             if chain is not None:
                 found[o_op] = chain
         return found

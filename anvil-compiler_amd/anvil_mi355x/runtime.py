@@ -121,6 +121,7 @@ class RowOp(C.Structure):
 
 CACHE_PAGE = 64                              # tokens of a cache page
 CACHE_ROWS_MAX = 4096                        # sequences of a cache's tables
+CACHE_TOKENS_MAX = 16384 * CACHE_PAGE        # tokens of a sequence
 
 
 class Cache(C.Structure):

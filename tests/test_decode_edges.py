@@ -5,10 +5,11 @@ import pytest
 
 import anvil_mi355x
 import test_decode_ops as ops
-from anvil_mi355x import decode
+from anvil_mi355x import decode, models
 from anvil_mi355x import ir as g
 from anvil_mi355x import runtime as rt
 from host_cache import HostDevice
+from test_decoder import Oracle
 
 gpu = pytest.mark.gpu
 
@@ -250,3 +251,33 @@ def test_the_largest_score_multiplier_is_taken():
     dec.cache.step(None, _int32s(dev, 1))
     dec.forward(_int32s(dev, 0), None, 1, 1)
     dev.sync()
+
+
+def _long_model(seq):
+    return models.build(models.BlockSpec(n_embd=32, n_head=2, seq=seq, layers=1, vocab=40, calib_batches=1, calib_batch=1), 6, stored=False)
+
+
+def test_attention_of_more_tokens_than_the_whole_sequence_kernel_takes_is_decoded():
+    """That kernel's 1024 tokens are no limit of the cache: the lowering finds the chain, and the whole graph's plan still has none."""
+    cm = anvil_mi355x.compile(_long_model(1040))
+    assert cm.proven and not cm._attention_chains("outputs")
+    dec = object.__new__(decode.Decoder)
+    dec.cm, dec.T = cm, 1040
+    steps, layers, heads, dim = dec._lower()
+    assert (layers, heads, dim) == (1, 2, 16) and [s[0] for s in steps].count("attend") == 1
+
+
+@gpu
+def test_a_model_of_1040_tokens_gives_the_graphs_logits():
+    b = _long_model(1040)
+    cm = anvil_mi355x.compile(b)
+    dec, dev = cm.decoder(rows=1), cm.dev
+    seq = np.random.default_rng(3).integers(0, 40, 1040).astype(np.int32)
+    want = Oracle(b).logits([seq])[0]
+    for lo, n in ((0, 1030), (1030, 7), *((t, 1) for t in range(1037, 1040))):
+        dec.cache.step(None, _int32s(dev, n))
+        ids = dev.upload(seq[lo:lo + n])
+        got = dec.forward(ids, starts := _int32s(dev, 0, n), n, n).download((n, 40), np.int8)
+        dev.sync()
+        np.testing.assert_array_equal(got, want[lo:lo + n])
+    del starts
