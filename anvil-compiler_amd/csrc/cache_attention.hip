@@ -1268,6 +1268,28 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a) {
   return ANVIL_OK;
 }
 
+// Whether a head's row of O may share a byte with one of Q: where their extents meet, with row strides alike, each pair of heads
+// settles it (modulo the stride), and strides that differ are taken to meet.
+static bool rows_meet(const AttendArgs& a, int rows, int heads, int dim) {
+  using wide = __int128;
+  const wide apart = (wide)(uintptr_t)a.o - (wide)(uintptr_t)a.q, q_rows = (wide)a.q_row * (rows - 1), q_heads = (wide)a.q_head * (heads - 1),
+             o_last = (wide)a.o_row * (rows - 1) + (wide)a.o_head * (heads - 1);
+  if (apart >= std::max<wide>(q_rows, 0) + std::max<wide>(q_heads, 0) + dim ||
+      apart + o_last + dim <= std::min<wide>(q_rows, 0) + std::min<wide>(q_heads, 0))
+    return false;
+  if (a.q_row != a.o_row || heads > 4096) return true;
+  const wide row = a.o_row;                              // at least dim
+  for (int ho = 0; ho < heads; ++ho)
+    for (int hq = 0; hq < heads; ++hq) {
+      const wide d = apart + (wide)ho * a.o_head - (wide)hq * a.q_head;
+      wide k = d / row;
+      k -= d < k * row;                                  // rounded down
+      const wide rest = d - k * row;
+      if ((rest < dim && k < rows && -k < rows) || (row - rest < dim && k + 1 < rows && -k - 1 < rows)) return true;
+    }
+  return false;
+}
+
 }  // namespace anvil
 
 using namespace anvil;
@@ -1297,6 +1319,8 @@ extern "C" int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache
   AttendArgs a{};
   a.q = Q, a.o = O, a.q_row = strides[0], a.q_head = strides[1], a.o_row = strides[2], a.o_head = strides[3];
   a.lut = lut, a.m_s = m_s, a.s_s = s_s, a.one = one, a.m_o = m_o, a.s_o = s_o;
+  if (rows_meet(a, rows, heads_q, c.dim))
+    return set_error(ANVIL_E_VALUE, "%s: O overlaps Q, which other workgroups still read", who);
   const int most = c.slots * PAGE;                       // keys; a window that holds them all is none
   a.window = window < most ? window : 0, a.sinks = std::min(sinks, most), a.group = heads_q / c.heads;
   int r = ANVIL_OK;

@@ -443,7 +443,8 @@ int anvil_cache_read_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, int
  * the requantized 0; a row whose S is 0 yields that too and ANVIL_E_ZERODIV at anvil_sync. |m_s| is limited so that
  * every Q . K_j * m_s + 2^(s_s-1) fits int32 (128 * 126 * D * |m_s| + 2^(s_s-1) < 2^31), else ANVIL_E_OVERFLOW.
  * strides = {q row, q head, o row, o head}: Q and its strides multiples of 16, O and its strides of 4, o strides >= D.
- * O is other memory than Q. seqs x heads at most 2^22, max_new x heads_q / heads at most 2^30. */
+ * O is other memory than Q: the rows and heads of both (of all `rows`) may lie between each other's only with row strides
+ * alike, else ANVIL_E_VALUE. seqs x heads at most 2^22, max_new x heads_q / heads at most 2^30. */
 int anvil_attention_cache_i4(anvil_ctx* ctx, const anvil_cache* cache, int layer, const int8_t* Q, int8_t* O,
                              const int32_t* starts, int rows, int max_new, int heads_q, const int64_t* strides,
                              int32_t m_s, int s_s, const int32_t* lut, int32_t one, int32_t m_o, int s_o, int window,

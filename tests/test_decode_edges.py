@@ -281,3 +281,44 @@ def test_a_model_of_1040_tokens_gives_the_graphs_logits():
         dev.sync()
         np.testing.assert_array_equal(got, want[lo:lo + n])
     del starts
+
+
+# -------------------------------------------------------------------------------------------- results over queries
+
+def _attend_within(dev, at_q, at_o, strides, rows=3, heads=2, dim=32, size=4096):
+    """An attention call whose queries and results lie in one buffer, at byte offsets; returns (results, expected, the other bytes
+    before and after)."""
+    seqs = ops.Sequences([100, 70, 9][:rows], heads, dim)
+    d = ops.OnDevice(dev, seqs, seqs.pool())
+    raw = np.random.default_rng(1).integers(-128, 128, size).astype(np.int8)
+    buf = dev.upload(raw)
+    where = lambda at, row, head: at + (row * np.arange(rows)[:, None, None] + head * np.arange(heads)[:, None] + np.arange(dim))  # noqa: E731
+    q_at, o_at = where(at_q, *strides[:2]), where(at_o, *strides[2:])
+    lut = dev.upload(ops.exp_lut().astype(np.int32))
+    dev.attention_cache(d.cache, 0, buf.ptr + at_q, buf.ptr + at_o, None, rows, 1, heads, strides, 5, 16, lut, 127, 1, 7)
+    dev.sync()
+    want, _ = ops.attention_want(seqs, [1] * rows, raw[q_at].astype(np.int64), heads, 5, 16, ops.exp_lut(), 127, 1, 7)
+    got = buf.download((size,), np.int8)
+    rest = np.setdiff1d(np.arange(size), o_at)
+    return got[o_at], want, raw[rest], got[rest]
+
+
+@gpu
+@pytest.mark.parametrize("at_q,at_o,strides", [(0, 192, (64, 32, 64, 32)), (256, 0, (64, 32, 64, 32)),          # one behind the other
+                                               (0, 64, (128, 32, 128, 32)), (64, 0, (128, 32, 128, 32)),       # beside each other
+                                               (0, 32, (128, 64, 128, 64)), (128, 32, (512, 256, 512, 64)),    # heads between heads
+                                               (2048, 0, (-64, 32, 64, 32)), (0, 1024, (0, 0, 64, 32))])
+def test_queries_and_results_of_one_buffer(at_q, at_o, strides):
+    got, want, before, after = _attend_within(rt.device(0), at_q, at_o, strides)
+    assert np.array_equal(got, want) and np.array_equal(before, after)
+
+
+@gpu
+@pytest.mark.parametrize("at_q,at_o,strides", [(64, 64, (512, 0, 512, 32)), (0, 0, (64, 32, 64, 32)), (0, 188, (64, 32, 64, 32)), (176, 0, (64, 32, 64, 32)),
+                                               (0, 60, (128, 32, 128, 32)), (64, 4, (128, 32, 128, 32)), (0, 124, (128, 32, 128, 32)),
+                                               (0, 36, (128, 64, 128, 64)), (0, 64, (128, 32, 192, 32)), (256, 0, (-64, 32, 64, 32)),
+                                               (128, 0, (0, 0, 64, 32)), (0, 64, (64, 32, 64, 32)), (1024, 0, (64, 32, 1024, 32))])
+def test_results_over_queries_are_refused(at_q, at_o, strides):
+    """At the ends of both extents, in the rows between, and with strides that differ."""
+    with pytest.raises(ValueError, match="O overlaps Q"):
+        _attend_within(rt.device(0), at_q, at_o, strides)
