@@ -331,7 +331,7 @@ class Decoder:
         """`new_tokens` tokens after each prompt (lists of ids, of any lengths), the best of `beams` beams by their fixed-point log
         probabilities (beams=1: the most likely token each time, the lowest id of equals). eos: a beam that ends with it is done.
         allowed: vocab truth values, tokens to choose from."""
-        dev, cache, V = self.dev, self.cache, self.logits.width
+        V = self.logits.width
         prompts = [np.asarray(p) for p in prompts]
         P, rows = len(prompts), len(prompts) * beams
         if not P or rows > self.rows or not 1 <= beams <= 64:
@@ -349,6 +349,15 @@ class Decoder:
             raise ValueError(f"eos {eos} outside [0, {V})")
         if self.logits.dtype != "i8" or self.scale is None or V > self.vocab:
             raise ValueError(f"the graph's output is not int8 logits with a scale for {self.vocab} tokens")
+        try:
+            return self._generate(prompts, new_tokens, beams, eos, allowed)
+        except BaseException:
+            self.cm._settle()                                  # nothing runs on the call's buffers, and no violation stays behind
+            raise
+
+    def _generate(self, prompts, new_tokens, beams, eos, allowed) -> Generated:
+        dev, cache, V, P = self.dev, self.cache, self.logits.width, len(prompts)
+        rows = P * beams
         select = Selection.of(self.scale)
         tables = self._tables(select, allowed, V)
         starts = np.cumsum([0] + [p.size for p in prompts]).astype(np.int32)

@@ -5,7 +5,7 @@ import pytest
 
 import anvil_mi355x
 import test_decode_ops as ops
-from anvil_mi355x import decode, models
+from anvil_mi355x import decode, driver, models
 from anvil_mi355x import ir as g
 from anvil_mi355x import runtime as rt
 from host_cache import HostDevice
@@ -322,3 +322,39 @@ def test_results_over_queries_are_refused(at_q, at_o, strides):
     """At the ends of both extents, in the rows between, and with strides that differ."""
     with pytest.raises(ValueError, match="O overlaps Q"):
         _attend_within(rt.device(0), at_q, at_o, strides)
+
+
+# ------------------------------------------------------------------------------------------ calls that fail part way
+
+class _Watched(HostDevice):
+    settled = 0
+
+    def fetch(self, items):
+        def call(check=False):
+            self.settled += 1
+            if check:
+                self.sync()
+        return call
+
+
+@pytest.mark.parametrize("error", [RuntimeError("anvil_alloc: out of memory"), KeyboardInterrupt()], ids=["error", "interrupt"])
+def test_a_call_that_fails_part_way_leaves_no_violation_on_the_device(error):
+    """Too few pages, which the call's end would report, and an error before that end: the next call on the device is not the one to
+    report them, and no kernel runs any more when the call's buffers go."""
+    dec = object.__new__(decode.Decoder)
+    dec.dev = dev = _Watched()
+    dec.cm = object.__new__(driver.CompiledModel)
+    dec.cm.dev = dev
+    dec.rows, dec.max_tokens, dec.vocab, dec.logits, dec.scale = 2, 300, 40, decode._Rows(40, "i8"), 0.1
+    dec.cache = decode.KVCache(dev, 1, 1, 32, 3, 2, 300)
+    dec._make_room = lambda rows: None
+
+    def forward(*args):
+        assert isinstance(dev.pending, MemoryError)
+        raise error
+
+    dec.forward = forward
+    with pytest.raises(type(error)):
+        dec.generate([[1] * 200, [2] * 100], 4)
+    assert dev.settled
+    dev.sync()
