@@ -415,7 +415,8 @@ int anvil_embed_quantize(anvil_ctx* ctx, const int64_t* ids, int64_t rows, int T
 enum { ANVIL_CACHE_PAGE = 64, ANVIL_CACHE_SLOTS_MAX = 16384, ANVIL_CACHE_ROWS_MAX = 4096 };
 typedef struct anvil_cache {
   void* pool;                       /* 16-byte aligned */
-  int32_t* table;                   /* seqs x slots */
+  int32_t* table;                   /* seqs x slots. Without a window the attention sizes its parts, its scratch memory and its choice
+                                     * of kernels by slots, which the host knows, not by lens: slots near the longest sequence serve it best */
   int32_t* lens;                    /* seqs: tokens, at most 64 slots */
   int32_t* refs;                    /* pages; NULL where only attention, append and read use the cache */
   int32_t seqs, slots, pages, heads, dim, layers;   /* seqs and layers at most 65535, heads 4096, pages 2^24 */

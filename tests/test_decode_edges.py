@@ -8,6 +8,7 @@ import test_decode_ops as ops
 from anvil_mi355x import decode, driver, models
 from anvil_mi355x import ir as g
 from anvil_mi355x import runtime as rt
+from decode_cases import Sequences
 from host_cache import HostDevice
 from test_decoder import Oracle
 
@@ -358,3 +359,19 @@ def test_a_call_that_fails_part_way_leaves_no_violation_on_the_device(error):
         dec.generate([[1] * 200, [2] * 100], 4)
     assert dev.settled
     dev.sync()
+
+
+# ------------------------------------------------------------------------- short sequences in tables of many slots
+
+@gpu
+@pytest.mark.parametrize("slots", [150, 2100, 16000])
+@pytest.mark.parametrize("lens,news,heads_q,heads,dim", [([130, 1, 0, 65], [1, 1, 0, 1], 4, 2, 64), ([3], [1], 8, 8, 32), ([700], [1], 4, 1, 128),
+                                                         ([190, 70], [6, 1], 4, 4, 64), ([300, 300], [100, 1], 12, 2, 16),
+                                                         ([260, 5], [256, 3], 8, 8, 32)])
+def test_attention_of_short_sequences_in_tables_of_many_slots(monkeypatch, slots, lens, news, heads_q, heads, dim):
+    """What a table could hold decides how a call is split: parts, tiles whose scores lie in memory, many rows, and here most of it is
+    empty."""
+    monkeypatch.setattr(ops, "Sequences", lambda *a, **k: Sequences(*a, **k, extra_slots=slots))
+    ops.attention_case(lens, news, heads_q, heads, dim, one=127)
+    ops.attention_case(lens, news, heads_q, heads, dim, one=4096, window=100, sinks=5)
+    ops.attention_case(lens, news, heads_q, heads, dim, one=911, window=40000, sinks=70)
