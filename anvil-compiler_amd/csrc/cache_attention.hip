@@ -1229,8 +1229,15 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a) {
   }
   const size_t fixed = sizeof(int) * (256 + (size_t)(a.rows * HIST + 3) / 4 * 4), row_sums = sizeof(int) * (size_t)a.rows * SUM_STRIDE<NG>;
   const size_t scores = (size_t)a.bound * a.rows * PAGE;
-  // Four waves a workgroup where the tiles fill the CUs and two of them fit a CU's LDS, else eight.
-  const int waves = 2 * groups >= 3ll * ctx->num_cu && fixed + std::max(scores, 4 * row_sums) <= LDS_MAX / 2 ? 4 : 8;
+  // Four waves a workgroup where there are more tiles than CUs and two such workgroups fit a CU's LDS, else eight. Heads of 128 and 16-row
+  // tiles take more than 128 registers a lane, so that eight waves leave no room for another workgroup: 32 heads over 8 of 128, 1024
+  // tokens, with 256 tiles 12.2 us with four and 11.9 with eight, with 288 15.3 and 20.0, with 704 22.0 and 29.5; 12 heads of 64, 64 new of
+  // 2048, 288 tiles: 20.9 and 24.7 (of 4096, where two do not fit the LDS, 48.5 and 37.5). The others have room for two of either: from 257 to
+  // 512 tiles heads of 64 and 32 take 12.4 and 12.6, 11.3 and 11.0 over 1024 tokens, 29.4 and 28.9, 28.2 and 26.3 over 4096; with 576 tiles
+  // and 1024 tokens 15.5 and 17.7, 14.1 and 14.4.
+  const bool fit = fixed + std::max(scores, 4 * row_sums) <= LDS_MAX / 2;
+  const bool many = NG == 4 || RP == 16 ? groups > ctx->num_cu : 2 * groups >= 3ll * ctx->num_cu;
+  const int waves = many && fit ? 4 : 8;
   const size_t sums = waves * row_sums, lds = fixed + std::max(scores, sums);
   // Parts of a tile only where they bring CUs to work that the tiles leave idle, and where a tile is long: three launches cost what
   // one does over 32 pages.
