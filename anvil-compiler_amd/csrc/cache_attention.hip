@@ -531,7 +531,7 @@ __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, i
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int x = min(4 * (lane + LANES * i) + j, max(top, 0)) - max(top, 0) + 255;        // larger scores do not occur
-      e[i][j] = word(count[i], j) ? (double)(unsigned)max(0, lut[x]) : 0.0;
+      e[i][j] = (double)(unsigned)max(0, lut[x]);
       S = __builtin_fma(e[i][j], (double)word(count[i], j), S);
     }
   S = lanes_sum<LANES>(S);
@@ -563,6 +563,8 @@ __device__ __forceinline__ void probabilities(unsigned* table, const int* lut, i
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[i][j] = word(count[i], j) ? p[i][j] : 0u;
     const int at = lane + LANES * i;
     if constexpr (TABLE == TABLE_FIFTEEN) {              // a byte each of four tables
       int x[4] = {(int)p[i][0], (int)p[i][1], (int)p[i][2], (int)p[i][3]};
