@@ -1257,8 +1257,9 @@ class CompiledModel:
     def decoder(self, rows, max_tokens=None, pages=None, window=0, sinks=0):
         """A Decoder of this token model (decode.py): up to `rows` sequences token by token over a paged 4-bit cache of up to
         max_tokens tokens each (default: the position table's), in `pages` pages of 64 tokens (default: enough for every row);
-        window > 0: a token sees the last `window` tokens and the first `sinks`. The reference has no incremental form of
-        CompiledModel.run (anvil/driver.py:305-322)."""
+        window > 0: a token sees the last `window` tokens and the first `sinks`. The cache rounds keys and values to 4 bits, so
+        logits are those of the graph with the rounded values, and need not be run's. The reference has no incremental form
+        of CompiledModel.run (anvil/driver.py:305-322)."""
         from .decode import Decoder
         return Decoder(self, rows, max_tokens, pages, window, sinks)
 

@@ -100,7 +100,8 @@ __device__ __forceinline__ bool page_rows(const CacheView& c, PageRows& p) {
 // One page of one sequence and head a workgroup (blockIdx: page among those with new rows, sequence, head). Four
 // lanes a group of 32 channels; all of a thread's rows are on their way before the first is rounded. K codes go straight to their
 // rows; V codes, which the page holds channel by channel, meet in LDS and leave as whole 64-byte rows where the page is new from end
-// to end. 8 prompts of up to 2048 tokens, 8 heads of 128: 11.4 us, 1.6 TB/s of rows read and pages written; a chain of waits a page.
+// to end. 8 prompts of up to 2048 tokens, 8 heads of 128: 11.4 us, 1.6 TB/s of rows read and pages written. 36 % of wave cycles wait for
+// memory or the LDS, 40 % for a turn to issue; VALU instructions take 38 % of a SIMD's time.
 template <int NG>
 __global__ __launch_bounds__(ROW_THREADS) void append_kernel(CacheView c, RowPtrs p) {
   using B = Block<NG>;

@@ -870,8 +870,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(CacheView c, 
 // Where a sequence has many rows its pages are worth multiplying out first: a score is then the product itself, a digit of p an
 // operand as it stands, and nothing is left between the products but the requant and the two tables. Scores are not kept but made again
 // in the second pass, so that a tile needs LDS for its histograms alone and has any length. 4 sequences of 32 heads over 8 of 128
-// channels, 1024 new tokens of 16384 each: 3149 us with tiles of 16 rows, 1217 with these; 2 of 512 new of up to 4096: 188 and 92.
-// What bounds it: instructions between the products (half of all cycles) and the LDS's conflicts on histograms and tables (as many).
+// channels, 1024 new tokens of 16384 each: 3134 us with tiles of 16 rows, 1154 with these; 2 of up to 512 new of up to 4096: 188 and 92.
+// Of the latter's time VALU instructions take 28 % on a SIMD, the LDS 30 % (20 % conflicts on histograms and tables), MFMAs 12 %; a wave
+// lives 37 of the 92 us, and of the two workgroups that a CU has room for one is there on average, as the tiles with rows come unevenly.
 // The second with 16, 32, 48 and 64 rows a tile: 114, 92, 106, 100 us; with 2, 3, 4 and 8 waves 90, 114, 92, 105, and with 2 a third
 // more where tiles are short (4 x 12 heads of 64, 512 new, the last 1024 seen).
 
@@ -1222,7 +1223,9 @@ static int attend(anvil_ctx* ctx, const CacheView& c, AttendArgs a) {
     // Widened pages pay where eight or more tiles of 32 rows read each, and where there are enough tiles for the CUs, which a tile of
     // twice the rows keeps busy twice as long: 2 tiles of 16 rows a CU over 2048 keys or more (32 heads over 8 of 128, 256 new of
     // 4096: 50.4 us with 16 rows, 40.2 with 32; of 1024 18.2 and 20.8), 8 over fewer (1024 new of 1024: 47.2 and 37.1). With few rows
-    // (16 x 12 heads of 64, 64 new of 4096): 54.4 and 69.6.
+    // (16 x 12 heads of 64, 64 new of 4096): 54.4 and 69.6. The numbers are those of max_new, as if every sequence had as many. Where one of
+    // many has them, each as long, the two differ by the heads: 1 of 64 sequences with 512 of 8192, the others with one token, 32 heads over
+    // 8 of 128 992 and 994 us, 16 over 4 of 64 613 and 365, but 12 of 64 305 and 541.
     AttendArgs wide = a;
     wide.bound = pages_seen(c, a, c.max_new);
     if (all >= 256 && groups >= 2ll * ctx->num_cu && (a.bound >= 32 || groups >= 8ll * ctx->num_cu) && a.one <= ONE_PAIR &&
