@@ -138,7 +138,7 @@ int launch_kernel(const void* sym, dim3 grid, dim3 block, unsigned lds, hipStrea
     e = hipLaunchKernel(sym, grid, block, args, lds, s);
   }
   if (e == hipSuccess && g_recording.load(std::memory_order_relaxed)) note_launch(sym, grid, block, lds, s, args, sizes, n);
-  return e == hipSuccess ? ANVIL_OK : hip_fail(e, "kernel launch");
+  return e == hipSuccess ? ANVIL_OK : (int)ANVIL_E_RUNTIME;   // the error stays for the caller's ANVIL_LAUNCHED
 }
 
 int set_error(int code, const char* fmt, ...) {
@@ -151,7 +151,9 @@ int set_error(int code, const char* fmt, ...) {
   return code;
 }
 
+// The error is the entry point's own from here on: it does not stay for the next one's ANVIL_LAUNCHED to find.
 int hip_fail(hipError_t e, const char* what) {
+  (void)hipGetLastError();
   return set_error(ANVIL_E_RUNTIME, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
 
@@ -490,9 +492,8 @@ int anvil_graph_launch(anvil_ctx* ctx, void* graph) {
     if (plain) {
       ANVIL_HIP(hipModuleLaunchKernel(r.fn, r.grid.x, r.grid.y, r.grid.z, r.block.x, r.block.y, r.block.z, r.lds,
                                       ctx->stream, r.ptrs.data(), nullptr));
-    } else if (int e = launch_kernel(r.sym, r.grid, r.block, r.lds, ctx->stream, r.ptrs.data(), r.sizes.data(),
-                                     (int)r.sizes.size())) {
-      return e;
+    } else if (launch_kernel(r.sym, r.grid, r.block, r.lds, ctx->stream, r.ptrs.data(), r.sizes.data(), (int)r.sizes.size())) {
+      return hip_fail(hipGetLastError(), "kernel launch");
     }
   }
   return ANVIL_OK;

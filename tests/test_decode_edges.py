@@ -375,3 +375,23 @@ def test_attention_of_short_sequences_in_tables_of_many_slots(monkeypatch, slots
     ops.attention_case(lens, news, heads_q, heads, dim, one=127)
     ops.attention_case(lens, news, heads_q, heads, dim, one=4096, window=100, sinks=5)
     ops.attention_case(lens, news, heads_q, heads, dim, one=911, window=40000, sinks=70)
+
+
+@gpu
+@pytest.mark.parametrize("fails", ["alloc", "workspace"])
+def test_a_call_after_an_allocation_that_failed(fails):
+    """Memory that the device has not is an error of the call that asked for it, and of no later one."""
+    dev = rt.Device(0)
+    work = ops.KINDS["parts"](dev, 1)
+    small = ops.Choice(dev, 2, vocab=300)
+    with pytest.raises(RuntimeError):
+        if fails == "alloc":
+            dev.alloc(1 << 50)
+        else:                                                  # 2^22 rows of 2^28 logits: 2^46 bytes of histograms, before any is read
+            dev.beam_select(small.x, 1 << 28, small.scores, None, None, 1 << 16, 64, 1 << 28, 64, -1, small.d_lut, small.d_logs, 2048, 1, 1,
+                            *[small.x.ptr + (i << 40) for i in (1, 2, 3, 4)])
+    small.run()
+    work.run()
+    work.check()
+    small.check()
+    dev.close()
