@@ -95,8 +95,11 @@ SIGNATURES = {
     "anvil_cache_fork": [_p, _p, _p, _p, _p, _i, _i],
     "anvil_cache_compact": [_p, _p, _p, _p],
     "anvil_beam_select_i8": [_p, _p],
+    "anvil_add_norm_i8": [_p, _p],
+    "anvil_expert_route_i8": [_p, _p],
+    "anvil_expert_gemm_i8": [_p, _p],
+    "anvil_expert_combine_i8": [_p, _p],
 }
-
 
 
 class GemmDesc(C.Structure):
@@ -145,6 +148,39 @@ class Beams(C.Structure):
                 ("beams", _i32), ("vocab", _i32), ("keep", _i32), ("eos", _i32), ("lut", _p), ("logs", _p),
                 ("nlogs", _i32), ("step", _i32), ("mult", _i32), ("scores_out", _p), ("parent", _p), ("token", _p),
                 ("ended_out", _p)]
+
+
+class AddNorm(C.Structure):
+    """anvil_add_norm: the arguments of one anvil_add_norm_i8 call."""
+    _fields_ = [("X", _p), ("Y", _p), ("R", _p), ("x_dtype", _i32), ("y_dtype", _i32), ("r_dtype", _i32), ("ldx", _i64), ("ldy", _i64),
+                ("ldr", _i64), ("ma", _i32), ("mb", _i32), ("shift", _i32), ("w", _p), ("lut", _p), ("lut_len", _i32), ("eps", _i32),
+                ("lut_shift", _i32), ("H", _p), ("ldh", _i64), ("scale", _p), ("rows", _i32), ("cols", _i32)]
+
+
+EXPERTS_MAX = 1024                           # experts of a router or a product
+ROUTE_TOP_MAX = 32                           # experts of a row
+ROUTE_EVERY = 1                              # anvil_route's flag
+
+
+class Route(C.Structure):
+    """anvil_route: the arguments of one anvil_expert_route_i8 call."""
+    _fields_ = [("scores", _p), ("ld", _i64), ("live", _p), ("rows", _i32), ("experts", _i32), ("top", _i32), ("flags", _i32),
+                ("lut", _p), ("one", _i32), ("expert", _p), ("weight", _p), ("slot", _p), ("row", _p), ("starts", _p)]
+
+
+class ExpertGemm(C.Structure):
+    """anvil_expert_gemm: the arguments of one anvil_expert_gemm_i8 call."""
+    _fields_ = [("A", _p), ("lda", _i64), ("row", _p), ("scale", _p), ("B", _p), ("B2", _p), ("ldb", _i64), ("sb", _i64),
+                ("starts", _p), ("rows_a", _i32), ("rows", _i32), ("experts", _i32), ("N", _i32), ("K", _i32), ("mults", _p),
+                ("mults2", _p), ("mult", _i32), ("shift", _i32), ("mult2", _i32), ("shift2", _i32), ("mult3", _i32), ("shift3", _i32),
+                ("lut", _p), ("C", _p), ("ldc", _i64), ("out_dtype", _i32)]
+
+
+class ExpertCombine(C.Structure):
+    """anvil_expert_combine: the arguments of one anvil_expert_combine_i8 call."""
+    _fields_ = [("Y", _p), ("ldy", _i64), ("slot", _p), ("weight", _p), ("positions", _i32), ("rows", _i32), ("top", _i32),
+                ("cols", _i32), ("mult", _i32), ("shift", _i32), ("R", _p), ("ldr", _i64), ("r_dtype", _i32), ("ma", _i32),
+                ("mb", _i32), ("shift2", _i32), ("D", _p), ("ldd", _i64), ("d_dtype", _i32)]
 
 
 ROW_LOAD, ROW_NORM, ROW_GEMM, ROW_ADD, ROW_LUT, ROW_LUT_MUL = 1, 2, 3, 4, 5, 6
@@ -566,6 +602,36 @@ class Device:
         b = Beams(_ptr(logits), ld, _ptr(scores), _opt(ended), _opt(allowed), groups, beams, vocab, keep, eos, _ptr(lut),
                   _ptr(logs), nlogs, step, mult, _ptr(scores_out), _ptr(parent), _ptr(token), _ptr(ended_out))
         self.lib.call("anvil_beam_select_i8", self.ctx, C.byref(b))
+
+    # ------------------------------------------------------------------------------------------ experts
+    def add_norm(self, X, x_dtype, ldx, Y, y_dtype, ldy, ma, mb, shift, R, r_dtype, ldr, w, lut, lut_len, eps, lut_shift, H, ldh,
+                 scale, rows, cols):
+        """anvil_add_norm_i8: R = the sum of X and Y (Y None: X alone, no R), H and scale its norm's codes and rows' scales."""
+        n = AddNorm(_opt(X), _opt(Y), _opt(R), DTYPE_CODE[x_dtype], DTYPE_CODE[y_dtype], DTYPE_CODE[r_dtype], ldx, ldy, ldr, ma, mb,
+                    shift, _opt(w), _opt(lut), lut_len, eps, lut_shift, _opt(H), ldh, _opt(scale), rows, cols)
+        self.lib.call("anvil_add_norm_i8", self.ctx, C.byref(n))
+
+    def expert_route(self, scores, ld, live, rows, experts, top, lut, one, expert, weight, slot, row, starts, every=False):
+        """anvil_expert_route_i8: each row's experts and weights, and the rows sorted by expert. every: weights are shares of all
+        experts' sum, not of the chosen ones'."""
+        r = Route(_opt(scores), ld, _opt(live), rows, experts, top, ROUTE_EVERY if every else 0, _opt(lut), one, _opt(expert),
+                  _opt(weight), _opt(slot), _opt(row), _opt(starts))
+        self.lib.call("anvil_expert_route_i8", self.ctx, C.byref(r))
+
+    def expert_gemm(self, A, lda, rows_a, row, scale, B, B2, ldb, sb, starts, experts, rows, N, K, Cp, ldc, out_dtype, mults=None,
+                    mult=0, shift=0, mults2=None, mult2=0, shift2=0, lut=None, mult3=1, shift3=0):
+        """anvil_expert_gemm_i8: sorted rows times their experts' weights; B2: gated."""
+        g = ExpertGemm(_opt(A), lda, _opt(row), _opt(scale), _opt(B), _opt(B2), ldb, sb, _opt(starts), rows_a, rows, experts, N, K,
+                       _opt(mults), _opt(mults2), mult, shift, mult2, shift2, mult3, shift3, _opt(lut), _opt(Cp), ldc,
+                       DTYPE_CODE[out_dtype])
+        self.lib.call("anvil_expert_gemm_i8", self.ctx, C.byref(g))
+
+    def expert_combine(self, Y, ldy, positions, slot, weight, rows, top, cols, mult, shift, R, r_dtype, ldr, ma, mb, shift2, D, d_dtype,
+                       ldd):
+        """anvil_expert_combine_i8: weighted sums of each row's results, and the residual's addition (R None: none)."""
+        c = ExpertCombine(_opt(Y), ldy, _opt(slot), _opt(weight), positions, rows, top, cols, mult, shift, _opt(R), ldr,
+                          DTYPE_CODE[r_dtype], ma, mb, shift2, _opt(D), ldd, DTYPE_CODE[d_dtype])
+        self.lib.call("anvil_expert_combine_i8", self.ctx, C.byref(c))
 
 
 _devices = {}

@@ -23,6 +23,7 @@ enum : unsigned {
   FLAG_NONFINITE = 16u, // a float input NaN or infinite           -> ValueError
   FLAG_PAGES = 32u,     // a cache had too few free pages          -> MemoryError
   FLAG_CACHE = 64u,     // a cache's table, length or start outside its range -> ValueError
+  FLAG_EXPERTS = 128u,  // a start, row, slot or multiplier of an experts' product outside its range -> ValueError
 };
 
 constexpr int EVENT_SLOTS = 512;

@@ -249,6 +249,7 @@ static int report_flags(anvil_ctx* ctx, bool nonfinite_first) {
   if (flags & FLAG_SHIFT) return set_error(ANVIL_E_VALUE, "an rmsnorm shift s + k left [0, 31]");
   if (flags & FLAG_NONFINITE) return set_error(ANVIL_E_VALUE, "%s", nonfinite);
   if (flags & FLAG_CACHE) return set_error(ANVIL_E_VALUE, "a cache's page table, lengths, starts or parents leave their range");
+  if (flags & FLAG_EXPERTS) return set_error(ANVIL_E_VALUE, "an expert's start, a row, a slot or a multiplier leaves its range");
   return set_error(ANVIL_E_VALUE, "an operand left its dtype range on the device (flags %u)", flags);
 }
 

@@ -506,6 +506,124 @@ typedef struct anvil_beams {
 } anvil_beams;
 int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b);
 
+/* --------------------------------------------------------------------------------------------- experts */
+/* A feed-forward part made of experts, over rows (tokens) whose int8 codes may each have a scale of their own. The reference's
+ * graphs have neither (its feed-forward is one qlinear pair, its scales are constants): these are the same integers with the
+ * row's choice of weights and scale in place of the graph's. One layer is
+ *   anvil_add_norm_i8       the residual's addition and the norm: codes and scales
+ *   anvil_expert_gemm_i8    with one expert: the router's scores
+ *   anvil_expert_route_i8   each row's experts and weights, and the rows sorted by expert
+ *   anvil_expert_gemm_i8    the sorted rows times their experts' weights, up (gated or through a table) and down again
+ *   anvil_expert_combine_i8 weighted sums in the rows' order, and the residual's addition
+ * rq(v, m, s) = (v * m + 2^(s-1)) >> s (2^-1: 0), the product and the sum in 64 bits, before it is clamped to the result's dtype.
+ * Strides (ld...) are in elements, any at least the row's width and below 2^31; an operand is aligned to its type, and 16-byte aligned
+ * operands with strides and widths that are multiples of 16 bytes take the faster kernels. Results are other memory than what
+ * the call reads, unless it says otherwise: rows of both may lie between each other's if their row strides (in bytes) are
+ * alike, else ANVIL_E_VALUE. Nothing behind a row's width, and no row behind the last, is written. */
+
+/* The residual's addition, then a root-mean-square norm of each row into int8 codes with a scale of the row's own:
+ *   r_c = clamp_r(rq(x_c * ma + y_c * mb, 1, shift));  with Y NULL r = x (R is not written, ma, mb and shift are not used)
+ *   t_c = r_c * w_c;  a = max |t_c|;  code_c = sign(t_c) * floor((254 |t_c| + a) / (2 a)), 0 where a = 0
+ *   (i, k) = rsqrt_index(eps + sum r_c^2), the sum in 64 bits (reference anvil/codegen/lower.py:107-113)
+ *   scale = min(32767, rq(a * lut[i], 1, lut_shift + k))
+ * The norm's factor 1 / rms is one for a whole row, so it cancels in the codes and is part of the scale alone: code_c stands
+ * for code_c * scale in units that lut and lut_shift set. x, y and r are i8 or i16; cols at most 65536; ma * x + mb * y +
+ * 2^(shift-1) fits int32 for every x and y of their dtypes, else ANVIL_E_OVERFLOW. lut: lut_len int32s, negative ones count as
+ * 0; 2 <= lut_len <= 65536; eps >= 0; shift and lut_shift in [0, 31]. R may be X or Y itself (of R's dtype and stride). */
+typedef struct anvil_add_norm {
+  const void* X;
+  const void* Y;                    /* NULL: no addition */
+  void* R;                          /* NULL without Y */
+  int32_t x_dtype, y_dtype, r_dtype;
+  int64_t ldx, ldy, ldr;
+  int32_t ma, mb, shift;
+  const int8_t* w;                  /* cols */
+  const int32_t* lut;
+  int32_t lut_len, eps, lut_shift;
+  int8_t* H;                        /* rows x cols codes */
+  int64_t ldh;
+  int16_t* scale;                   /* rows */
+  int32_t rows, cols;
+} anvil_add_norm;
+int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n);
+
+/* The router. scores: rows x experts int8 (row stride ld). Of each row the `top` experts of largest score, the largest first,
+ * the lowest expert of equals; with m the row's largest score and x its chosen ones
+ *   e_j = lut[x_j - m + 255];  S = sum e_j over the chosen (ANVIL_ROUTE_EVERY: over all experts);  weight_j = (e_j * one + S / 2) / S
+ * in 64 bits. A row with live[row] = 0 (live NULL: none; padding of a batch) has experts -1, weights 0 and slots -1. The pairs
+ * (row, expert) sorted by expert, rows in order: expert e has positions starts[e] .. starts[e + 1] - 1, position p is row
+ * row[p], and slot[row][j] is the position of the row's j-th expert. Entries of `row` from starts[experts] on stay as they
+ * were. lut: int32[256], entries below 0 count as 0; a live row whose S is 0 has weights 0, and ANVIL_E_ZERODIV is reported.
+ * 1 <= top <= 32, top <= experts <= 1024, rows * top < 2^30, 1 <= one <= 32767. */
+enum { ANVIL_ROUTE_EVERY = 1, ANVIL_EXPERTS_MAX = 1024, ANVIL_ROUTE_TOP_MAX = 32 };
+typedef struct anvil_route {
+  const int8_t* scores;
+  int64_t ld;
+  const uint8_t* live;              /* rows, or NULL */
+  int32_t rows, experts, top, flags;
+  const int32_t* lut;
+  int32_t one;
+  int32_t* expert;                  /* rows x top */
+  int16_t* weight;                  /* rows x top */
+  int32_t* slot;                    /* rows x top */
+  int32_t* row;                     /* rows * top */
+  int32_t* starts;                  /* experts + 1 */
+} anvil_route;
+int anvil_expert_route_i8(anvil_ctx* ctx, const anvil_route* r);
+
+/* Products of sorted rows with their experts' weights. Position p of expert e (starts[e] <= p < starts[e + 1] <= rows) reads
+ * row i = row[p] of A (row NULL: i = p):
+ *   acc_n = sum_k A[i][k] * B[e][n][k];  m = mult_e * scale[i];  C[p][n] = clamp_out(rq(acc_n, m, shift)) [-> lut[. + 128]]
+ * mult_e is mults[e] (mults NULL: mult), scale[i] is 1 with scale NULL. With B2 (gated; lut given, int8 results)
+ *   g = lut[clamp_i8(rq(acc_n, m, shift)) + 128];  u = clamp_i8(rq(acc2_n, m2, shift2));  C[p][n] = clamp_i8(rq(g * u, mult3, shift3))
+ * acc2 and m2 from B2 and mults2 / mult2. shift, shift2 in [0, 62], shift3 in [0, 31]; 2^14 |mult3| + 2^(shift3-1) < 2^31 and, with scale,
+ * |mult| and |mult2| at most 32767, else ANVIL_E_OVERFLOW (an entry of mults or mults2 that is not, with scale, is reported by anvil_sync as
+ * ANVIL_E_VALUE, and its expert's rows are not written). A start or row outside its range is reported likewise: its expert's rows
+ * are not written, its position's product is that of zeros. B2 has B's strides. N at most 2^20, K at most 2^16, experts at
+ * most ANVIL_EXPERTS_MAX.
+ * With one expert, starts {0, rows} and row NULL this is the product of rows with scales of their own. */
+typedef struct anvil_expert_gemm {
+  const int8_t* A;
+  int64_t lda;
+  const int32_t* row;               /* rows, or NULL */
+  const int16_t* scale;             /* rows_a, or NULL */
+  const int8_t* B;                  /* experts x N rows of K: expert stride sb, row stride ldb */
+  const int8_t* B2;                 /* the same, or NULL */
+  int64_t ldb, sb;
+  const int32_t* starts;            /* experts + 1, non-decreasing */
+  int32_t rows_a, rows, experts, N, K;
+  const int32_t* mults;             /* experts, or NULL */
+  const int32_t* mults2;
+  int32_t mult, shift, mult2, shift2, mult3, shift3;
+  const int8_t* lut;                /* 256, or NULL */
+  void* C;
+  int64_t ldc;
+  int32_t out_dtype;                /* ANVIL_I8; ANVIL_I16 without lut */
+} anvil_expert_gemm;
+int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g);
+
+/* The sorted results back in the rows' order:
+ *   y_c = clamp_i8(rq(sum_j weight[i][j] * Y[slot[i][j]][c], mult, shift)), a slot of -1 adding nothing
+ *   D[i][c] = clamp_d(rq(R[i][c] * ma + y_c * mb, 1, shift2)); with R NULL D = y (int8; ma, mb and shift2 are not used)
+ * Y has `positions` rows. A slot outside [-1, positions) adds nothing and is reported by anvil_sync as ANVIL_E_VALUE. R and D are i8
+ * or i16, and D may be R itself (of R's dtype and stride); R * ma + y * mb + 2^(shift2-1) fits int32 for every R and y of their dtypes, else
+ * ANVIL_E_OVERFLOW; shift in [0, 62], shift2 in [0, 31]; top and rows as the router's, cols at most 2^20. */
+typedef struct anvil_expert_combine {
+  const int8_t* Y;
+  int64_t ldy;
+  const int32_t* slot;              /* rows x top */
+  const int16_t* weight;            /* rows x top */
+  int32_t positions, rows, top, cols;
+  int32_t mult, shift;
+  const void* R;                    /* or NULL */
+  int64_t ldr;
+  int32_t r_dtype, ma, mb, shift2;
+  void* D;
+  int64_t ldd;
+  int32_t d_dtype;
+} anvil_expert_combine;
+int anvil_expert_combine_i8(anvil_ctx* ctx, const anvil_expert_combine* c);
+
 #ifdef __cplusplus
 }
 #endif
