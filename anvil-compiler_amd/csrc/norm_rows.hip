@@ -49,6 +49,183 @@ __device__ __forceinline__ int scale_of(const anvil_add_norm& n, unsigned a, uns
   return (int)min(r, 32767ll);
 }
 
+// floor(u / d) of u < 2^31 for one d in [2, 2^23]: (u m) >> (31 + l) with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d), which lies in
+// [2^31, 2^32) and is too large by less than d / 2^(31+l) of a unit in 2^-(31+l): below 2^31 that is less than 1 / d, so no quotient
+// changes. The quotient in doubles gives m or the number below it, and the remainder shows which.
+struct Divider {
+  unsigned m;
+  int sh;                                                // of the product's upper word
+  __device__ __forceinline__ explicit Divider(unsigned d) {
+    const int l = 32 - __builtin_clz(d - 1);
+    const double p = __builtin_ldexp(1.0, 31 + l);
+    unsigned long long q = (unsigned long long)(p / (double)d);
+    if (q * d < 1ull << (31 + l)) ++q;
+    m = (unsigned)q;
+    sh = l - 1;
+  }
+};
+
+template <int L>
+__device__ __forceinline__ int lane_group_max(int v) {       // maximum over aligned groups of L lanes
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));
+  if constexpr (L > 16) v = max(v, __builtin_amdgcn_ds_swizzle(v, (16 << 10) | 0x1F));
+  if constexpr (L > 32) v = max(v, __shfl_xor(v, 32));
+  return v;
+}
+
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
+// R chunks of eight elements, raw: 16 bytes of i16, or 8 of i8 in a chunk's first half. All loads go out before the first is looked
+// at (unpack), whatever the dtype, and chunks past the row (`off` is OOB there) are zeros.
+template <int R, typename OFF>
+__device__ __forceinline__ void load_chunks(v4i (&v)[R], __amdgpu_buffer_rsrc_t p, int dtype, OFF&& off) {
+  if (dtype == ANVIL_I16) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(p, off(i), 0, 0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(p, off(i), 0, 0));
+      v[i] = v4i{(int)b[0], (int)b[1], 0, 0};
+    }
+  }
+}
+
+// raw chunks as pairs of int16
+template <int R>
+__device__ __forceinline__ void unpack(v4i (&v)[R], int dtype) {
+  if (dtype == ANVIL_I16) return;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const unsigned b0 = (unsigned)v[i][0], b1 = (unsigned)v[i][1];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned b = q < 2 ? b0 : b1;
+      const int lo = (int)(b << (24 - 16 * (q & 1))) >> 24, hi = (int)(b << (16 - 16 * (q & 1))) >> 24;
+      v[i][q] = (int)__builtin_amdgcn_perm((unsigned)hi, (unsigned)lo, 0x05040100u);
+    }
+  }
+}
+
+// Rows of at most 8 L R columns, 16-byte aligned, in registers: L lanes a row (64 / L rows a wave), R chunks of eight elements a lane,
+// and a lane has the same columns of every row it takes, so its weights stay in registers.
+//
+// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 33.7 us, 4.5 TB/s
+// (one workgroup a row, each row read twice: 149). Rows of 768 take 16 lanes of six
+// chunks each: 64 lanes would leave a quarter of the wave idle in the second chunk, and the row's sum and maximum
+// take four data-parallel moves instead of six steps.
+//
+// Codes. floor((254 |t| + a) / 2a) with t's sign is floor((254 t + a - [t < 0]) / 2a); with 256 a added it is 128 larger and its
+// numerator lies in [0, 511 a], below 2^31 (a <= 2^22), so one multiplication by the row's reciprocal (Divider) and a shift
+// straight into the code's byte give it exactly.
+template <int L, int R>
+__global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
+  const anvil_add_norm& n = g.n;
+  const int lane = threadIdx.x & 63, sub = lane & (L - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = n.cols >> 3;
+  const int lo = n.r_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
+  const int rnd = (int)round_term(n.shift), ma = n.ma, mb = n.mb, shift = n.shift;
+  constexpr int ROWS = 64 / L;
+  v2u w[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) w[i] = sub + L * i < chunks ? *reinterpret_cast<const v2u*>(n.w + 8 * (sub + L * i)) : v2u{0, 0};
+  // a lane's first chunk from that of its wave's rows (the launch checks ROWS rows against 2^31); chunk i is i steps on
+  const auto offset = [&](long long ld, int size) { return (unsigned)((lane / L) * ld + 8 * sub) * (unsigned)size; };
+  const unsigned ox = offset(n.ldx, n.x_dtype), oy = n.Y ? offset(n.ldy, n.y_dtype) : 0, oz = n.Y ? offset(n.ldr, n.r_dtype) : 0,
+                 oh = offset(n.ldh, 1);
+  for (long long first = ((long long)blockIdx.x * 4 + wave) * ROWS; first < n.rows; first += (long long)gridDim.x * 4 * ROWS) {
+    const long long row = first + lane / L;
+    const bool live = row < n.rows;
+    const int rows = (int)min((long long)ROWS, n.rows - first);
+    const auto span = [&](const void* p, long long ld, int size) {
+      return uniform_rsrc((const char*)p + first * ld * size, (int)((rows - 1) * ld + n.cols) * size);
+    };
+    const auto at = [&](unsigned o, int size) {
+      return [=](int i) { return live && sub + L * i < chunks ? o + 8 * L * i * size : OOB; };
+    };
+    v4i x[R], y[R];
+    load_chunks(x, span(n.X, n.ldx, n.x_dtype), n.x_dtype, at(ox, n.x_dtype));
+    if (n.Y) {
+      load_chunks(y, span(n.Y, n.ldy, n.y_dtype), n.y_dtype, at(oy, n.y_dtype));
+      unpack(x, n.x_dtype);
+      unpack(y, n.y_dtype);
+#pragma unroll
+      for (int i = 0; i < R; ++i)                        // past the row's end x, y and so r are 0
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int v0 = (__mul24((int)(short)x[i][q], ma) + __mul24((int)(short)y[i][q], mb) + rnd) >> shift;
+          const int v1 = (__mul24(x[i][q] >> 16, ma) + __mul24(y[i][q] >> 16, mb) + rnd) >> shift;
+          x[i][q] = (int)__builtin_amdgcn_perm((unsigned)med3i(v1, lo, hi), (unsigned)med3i(v0, lo, hi), 0x05040100u);
+        }
+      const __amdgpu_buffer_rsrc_t pr = span(n.R, n.ldr, n.r_dtype);
+      const auto off = at(oz, n.r_dtype);
+      if (n.r_dtype == ANVIL_I16) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x[i]), pr, off(i), 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const v2u b = {__builtin_amdgcn_perm((unsigned)x[i][1], (unsigned)x[i][0], 0x06040200u),
+                         __builtin_amdgcn_perm((unsigned)x[i][3], (unsigned)x[i][2], 0x06040200u)};
+          __builtin_amdgcn_raw_buffer_store_b64(b, pr, off(i), 0, 0);
+        }
+      }
+    } else {
+      unpack(x, n.x_dtype);
+    }
+    unsigned long long ss = 0;
+    int top = 0, low = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned p = (unsigned)x[i][q];
+        ss += (unsigned)square_half<0>(p) + (unsigned)square_half<1>(p);       // at most 2^31
+        const unsigned wq = w[i][q >> 1];
+        const int t0 = q & 1 ? mul_half_byte<0, 2>(p, wq) : mul_half_byte<0, 0>(p, wq);
+        const int t1 = q & 1 ? mul_half_byte<1, 3>(p, wq) : mul_half_byte<1, 1>(p, wq);
+        top = max(top, max(t0, t1));
+        low = min(low, min(t0, t1));
+      }
+    }
+    const unsigned a = (unsigned)lane_group_max<L>(max(top, -low));
+    const unsigned s0 = (unsigned)lane_group_sum<L>((int)(ss & 0xFFFFFF)), s1 = (unsigned)lane_group_sum<L>((int)(ss >> 24));
+    // the products t again, rather than held since the sums: 8 R registers of a wave's budget
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(x[i][q]));
+    const Divider div(2 * max(a, 1u));                   // a row of zeros: every code is 257 / 2 - 128
+    const __amdgpu_buffer_rsrc_t ph = span(n.H, n.ldh, 1);
+    const auto to = at(oh, 1);
+    const int bias = 257 * (int)max(a, 1u);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      v2u h;
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        unsigned u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned p = (unsigned)x[i][2 * d + (e >> 1)];
+          const int t = e == 0   ? mul_half_byte<0, 0>(p, w[i][d])
+                        : e == 1 ? mul_half_byte<1, 1>(p, w[i][d])
+                        : e == 2 ? mul_half_byte<0, 2>(p, w[i][d])
+                                 : mul_half_byte<1, 3>(p, w[i][d]);
+          u[e] = __umulhi((unsigned)(mad_i24v(t, 254, bias) + (t >> 31)), div.m);
+        }
+        h[d] = sra_pack4v((int)u[0], (int)u[1], (int)u[2], (int)u[3], div.sh) ^ 0x80808080u;
+      }
+      __builtin_amdgcn_raw_buffer_store_b64(h, ph, to(i), 0, 0);
+    }
+    if (live && sub == 0) n.scale[row] = (int16_t)scale_of(n, a, ((unsigned long long)s1 << 24) + s0, g.nbits);
+  }
+}
+
 // One workgroup a row, any width, stride and alignment; the row is read twice.
 __global__ __launch_bounds__(256) void add_norm_any(NormArgs g) {
   const anvil_add_norm& n = g.n;
@@ -127,6 +304,32 @@ extern "C" int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n) {
   }
   if (int e = check_ctx(ctx)) return e;
   NormArgs g{*n, 32 - __builtin_clz((unsigned)n->lut_len), ctx->flags};
+  // eight elements a load: 16 bytes of i16, 8 of i8; multipliers that a 24-bit product takes
+  const auto even = [&](const void* p, long long ld, int size) { return (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 && ld < 1 << 28; };
+  const auto m24 = [](int m) { return m >= -(1 << 23) && m < 1 << 23; };
+  const int chunks = n->cols / 8;
+  if (n->cols % 8 == 0 && chunks <= 1024 && even(n->X, n->ldx, n->x_dtype) && even(n->H, n->ldh, 1) && even(n->w, 8, 1) &&
+      (!n->Y || (even(n->Y, n->ldy, n->y_dtype) && even(n->R, n->ldr, n->r_dtype) && m24(n->ma) && m24(n->mb)))) {
+    const auto go = [&](auto lanes, auto per) {
+      constexpr int L = decltype(lanes)::value, R = decltype(per)::value;
+      const int groups = (n->rows + 4 * (64 / L) - 1) / (4 * (64 / L));
+      ANVIL_LAUNCH((add_norm_rows<L, R>), dim3((unsigned)std::min(groups, 8 * ctx->num_cu)), dim3(256), 0, ctx->stream, g);
+    };
+    using std::integral_constant;
+    const auto wide = [&](auto lanes) {
+      const int r = (chunks + decltype(lanes)::value - 1) / decltype(lanes)::value;
+      if (r <= 1) go(lanes, integral_constant<int, 1>{});
+      else if (r <= 2) go(lanes, integral_constant<int, 2>{});
+      else if (r <= 4) go(lanes, integral_constant<int, 4>{});
+      else if (r <= 6) go(lanes, integral_constant<int, 6>{});
+      else if (r <= 8) go(lanes, integral_constant<int, 8>{});
+      else if constexpr (decltype(lanes)::value > 16) go(lanes, integral_constant<int, 16>{});
+    };
+    if (chunks <= 128) wide(integral_constant<int, 16>{});
+    else wide(integral_constant<int, 64>{});
+    ANVIL_LAUNCHED();
+    return ANVIL_OK;
+  }
   ANVIL_LAUNCH(add_norm_any, dim3((unsigned)std::min(n->rows, 1 << 20)), dim3(256), 0, ctx->stream, g);
   ANVIL_LAUNCHED();
   return ANVIL_OK;
