@@ -15,8 +15,13 @@ constexpr long long GRID_MAX = (1ll << 24) - 8;          // workgroups of 256: a
 struct ExpertArgs {
   anvil_expert_gemm g;
   int tiles_n;
+  int a_bytes;                                           // of A, as a buffer descriptor takes them: below 2^32
+
   unsigned* flags;
 };
+
+// an offset past an operand's last byte, by more than a row: A and a tile's weights span less
+constexpr unsigned PAST = 0xFFF00000u;
 
 struct ExpertTile {
   int e, p0, rows, n0;                                   // expert, first position, rows of the tile, first column
@@ -35,38 +40,39 @@ __device__ __forceinline__ int expert_rows(const ExpertArgs& a, int e, bool repo
 template <int BM, int BN>
 __device__ __forceinline__ bool find_tile(const ExpertArgs& a, int w, int lane, ExpertTile& t) {
   const int E = a.g.experts;
-  int lo, mt = 0;
+  int lo = 0, n = 0, mt = 0;                             // of the last 64 experts or fewer
   for (int e0 = 0; e0 < E; e0 += 64) {
-    const int n = e0 + lane < E ? expert_rows(a, e0 + lane, w == 0, lo) : 0;
+    n = e0 + lane < E ? expert_rows(a, e0 + lane, w == 0, lo) : 0;
     mt += (n + BM - 1) / BM;
   }
-  const int tiles_m = __builtin_amdgcn_readlane(wave_scan(mt), 63);
-  const long long tiles = (long long)tiles_m * a.tiles_n;
-  const long long per = (tiles + 7) / 8;
-  if ((w >> 3) >= per) return false;
-  const long long pid = (w & 7) * per + (w >> 3);
-  if (pid >= tiles) return false;
-  const int in_group = GROUP_M * a.tiles_n;
+  int incl = wave_scan(mt);
+  const int tiles_m = __builtin_amdgcn_readlane(incl, 63);
+  const unsigned tiles = (unsigned)tiles_m * (unsigned)a.tiles_n;        // at most the grid
+  const unsigned per = (tiles + 7) / 8, pid = (w & 7) * per + (w >> 3);
+  if ((unsigned)(w >> 3) >= per || pid >= tiles) return false;
+  const unsigned in_group = GROUP_M * a.tiles_n;
   const int first_m = (int)(pid / in_group) * GROUP_M, in = (int)(pid % in_group);
   const int gsize = min(tiles_m - first_m, GROUP_M);
   const int gm = first_m + in % gsize;
   t.n0 = in / gsize * BN;
   int before = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    const int n = e0 + lane < E ? expert_rows(a, e0 + lane, false, lo) : 0;
-    const int mine = (n + BM - 1) / BM, incl = wave_scan(mine);
-    const int all = __builtin_amdgcn_readlane(incl, 63);
-    if (gm < before + all) {
-      const int l = __builtin_ctzll(__ballot(gm < before + incl));       // the first expert whose tiles reach past gm
-      const int skip = (gm - before - __builtin_amdgcn_readlane(incl - mine, l)) * BM;
+  for (int e0 = 0;; e0 += 64) {
+    if (E > 64) {
+      n = e0 + lane < E ? expert_rows(a, e0 + lane, false, lo) : 0;
+      mt = (n + BM - 1) / BM;
+      incl = wave_scan(mt);
+    }
+    const unsigned long long past = __ballot(gm < before + incl);
+    if (past || e0 + 64 >= E) {
+      const int l = past ? __builtin_ctzll(past) : 63;   // the first expert whose tiles reach past gm
+      const int skip = (gm - before - __builtin_amdgcn_readlane(incl - mt, l)) * BM;
       t.e = e0 + l;
       t.p0 = __builtin_amdgcn_readlane(lo, l) + skip;
       t.rows = min(BM, __builtin_amdgcn_readlane(n, l) - skip);
-      return true;
+      return past != 0;
     }
-    before += all;
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
-  return false;
 }
 
 // Row i of A for position p; -1 where the caller's number leaves its range.
@@ -85,11 +91,385 @@ __device__ __forceinline__ bool expert_mult(const ExpertArgs& a, const int* mult
   return false;
 }
 
-// Operands at any alignment and stride: 64 x 64 tiles, chunks through registers into LDS.
+// A lane's results: n accumulators of one row (and n of the gate's partner) as n values of the result's dtype.
+template <int n, int OSZ, bool GATED, bool HI, typename V>
+__device__ __forceinline__ void finish_n(const V& acc, const V& acc2, int m, int m2, const Requant& q, const Requant& q2, bool lut,
+                                         const int8_t* lut_s, int mult3, int rnd3, int shift3, int* v) {
+#pragma unroll
+  for (int e = 0; e < n; ++e) {
+    const int x = q.unshifted<HI>(acc[e], m);
+    if (OSZ == 1 && (GATED || lut)) {
+      const int t = lut_s[__builtin_amdgcn_ubfe((unsigned)x, (unsigned)q.rest, 8u)];          // rotated: the entry of v at index v & 255
+      if constexpr (GATED) {
+        const int u = q2.unshifted<HI>(acc2[e], m2) >> q2.rest;
+        v[e] = med3i((__mul24(__mul24(t, u), mult3) + rnd3) >> shift3, -128, 127);
+      } else {
+        v[e] = t;
+      }
+    } else {
+      v[e] = x >> q.rest;
+    }
+  }
+}
+
+// the same address in scalar registers (uniform_rsrc)
+__device__ __forceinline__ void* uniform_ptr(const void* p) {
+  const unsigned long long a = (unsigned long long)p;
+  return (void*)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32)) << 32 |
+                 (unsigned)__builtin_amdgcn_readfirstlane((unsigned)a));
+}
+
+// One workgroup of 2 x 2 waves a BM x BN tile, operands 16-byte aligned, K in stages of BK bytes, NS of them in LDS and NS - 1 on their way.
+//
+// 128 x 256 tiles (waves of 64 x 128, three stages of 64 bytes, two workgroups a CU): 65536 gated positions of 768 to 2048 columns, 412 GOP,
+// 256 to 277 us, 1.5 to 1.6 POPS; 65536 of 2048 to 768, 206 GOP, 122 to 134 us. Without its loads 181 and 80 us, without its matrix
+// instructions 205 and 102, without its epilogue 220 and 111 (239 and 118 without the epilogue's stores): loads from L2 cost most, 2.4 GB in
+// lines of which a stage takes half. 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
+// workgroup's products run beside their epilogue; 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
+// (KFULL): selecting an offset past K for each load instead 261 against 257 us.
+// KFULL: K is a whole number of stages, so a load's offset is its lane's own and the stage's, and stages past K have empty descriptors.
+template <int BM, int BN, int BK, int NS, int OSZ, bool GATED, bool KFULL>
+__global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
+  constexpr int T = 256, NW = 4, WGN = 2, CPR = BK / 16, KS = BK / 32;
+  constexpr int WM = BM / (NW / WGN), WN = BN / WGN, TM = WM / 32, TN = WN / 32;
+  constexpr int COLS = GATED ? BN / 2 : BN;              // columns of the result
+  static_assert(TM >= 1 && TN >= (GATED ? 2 : 1) && (!GATED || TN % 2 == 0) && NS >= 2 && NS <= 4, "wave tile and stages");
+  constexpr int JA = BM * CPR / T, JB = BN * CPR / T, G = JA + JB;       // a wave's loads per stage
+  static_assert(JA * T == BM * CPR && JB * T == BN * CPR && (NS - 2) * G < 64, "whole loads");
+  constexpr int STAGE = (BM + BN) * BK;
+  __shared__ __attribute__((aligned(1024))) int8_t L0[STAGE], L1[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t L2[NS > 2 ? STAGE : 16], L3[NS > 3 ? STAGE : 16];
+  __shared__ int8_t lut_s[256];
+  auto arr = [&](auto u) -> int8_t* {                    // the array of stage u, known at compile time
+    constexpr int U = decltype(u)::value % NS;
+    if constexpr (U == 0) return L0;
+    else if constexpr (U == 1) return L1;
+    else if constexpr (U == 2) return L2;
+    else return L3;
+  };
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = wave / WGN, wn = wave % WGN;
+  const int half = lane >> 5, l32 = lane & 31;
+  const anvil_expert_gemm& g = a.g;
+  ExpertTile tile;
+  if (!find_tile<BM, COLS>(a, blockIdx.x, lane, tile)) return;
+  const int K = g.K;
+
+  // operand rows in LDS: A's as they are; B's in bperm order within each 32, a wave's gate columns before its partner columns
+  const int cols = min(g.N - tile.n0, COLS);
+  const long long b_at = tile.e * g.sb + (long long)tile.n0 * g.ldb;
+  const int b_bytes = __builtin_amdgcn_readfirstlane((int)((cols - 1) * g.ldb + K));
+  void *const pa = uniform_ptr(g.A), *const pb = uniform_ptr(g.B + b_at), *const pb2 = uniform_ptr(GATED ? g.B2 + b_at : g.B);
+  int mult, mult2 = 0, shift = g.shift, shift2 = g.shift2;
+  if (!expert_mult(a, g.mults, g.mult, tile.e, t == 0, mult)) return;
+  if (GATED && !expert_mult(a, g.mults2, g.mult2, tile.e, t == 0, mult2)) return;
+  if (!g.scale) lift_shift(mult, shift), lift_shift(mult2, shift2);
+  // The first loads in the order of what waits for what: the table and the rows' numbers, the first stages of B, and once the numbers
+  // are there the rows' scales and the first stages of A.
+  const int8_t entry = g.lut ? g.lut[t] : (int8_t)0;
+  int rows[JA], mine[TM];
+#pragma unroll
+  for (int j = 0; j < JA; ++j) {
+    const int r = ((wave + NW * j) * 64 + lane) / CPR;
+    rows[j] = r < tile.rows ? row_of(a, tile.p0 + r, tile.n0 == 0) : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const int r = wm * WM + 32 * j + l32;
+    mine[j] = g.scale && r < tile.rows ? row_of(a, tile.p0 + r, false) : -1;
+  }
+  unsigned offa[JA], offb[JB];                           // OOB stays out of range for every k below it: K is at most 2^16
+  int ka[JA], kb[JB];
+#pragma unroll
+  for (int j = 0; j < JB; ++j) {
+    const int P = (wave + NW * j) * 64 + lane, r = P / CPR, c = swz<BK>(r, P % CPR);
+    const int col = GATED ? r / WN * (WN / 2) + (r % (WN / 2) & ~31) + bperm(r & 31) : (r & ~31) + bperm(r & 31);
+    offb[j] = col < cols ? (unsigned)(col * g.ldb + c * 16) : PAST;
+    kb[j] = c * 16;
+  }
+  // chunks past K load zeros; a stage past K is issued all the same, which keeps the wait counts fixed
+  auto load = [&](__amdgpu_buffer_rsrc_t r, int8_t* s, unsigned off, int k, int k0) {
+    if constexpr (KFULL)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)s, 16, off, k0, 0, 0);
+    else
+      dma16(r, s, k0 + k < K ? off + k0 : OOB);
+  };
+  auto within = [&](void* p, int bytes, int k0) {
+    return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, KFULL && k0 >= K ? 0 : bytes, RSRC_DW3);
+  };
+  auto issue_b = [&](int8_t* s, int k0) {
+    const __amdgpu_buffer_rsrc_t r1 = within(pb, b_bytes, k0), r2 = within(pb2, b_bytes, k0);
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+      const bool second = GATED && ((wave + NW * j) * (64 / CPR) % WN) >= WN / 2;
+      load(second ? r2 : r1, s + BM * BK + (wave + NW * j) * 1024, offb[j], kb[j], k0);
+    }
+  };
+  auto issue_a = [&](int8_t* s, int k0) {
+    const __amdgpu_buffer_rsrc_t r = within(pa, a.a_bytes, k0);
+#pragma unroll
+    for (int j = 0; j < JA; ++j) load(r, s + (wave + NW * j) * 1024, offa[j], ka[j], k0);
+  };
+  static_for<NS - 1>([&](auto u) { issue_b(arr(u), decltype(u)::value * BK); });
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < JA; ++j) {
+    const int P = (wave + NW * j) * 64 + lane, r = P / CPR, c = swz<BK>(r, P % CPR);
+    offa[j] = rows[j] >= 0 ? (unsigned)(rows[j] * g.lda + c * 16) : PAST;
+    ka[j] = c * 16;
+  }
+  int scale[TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) scale[j] = !g.scale ? 1 : mine[j] < 0 ? 0 : (int)g.scale[mine[j]];
+  static_for<NS - 1>([&](auto u) { issue_a(arr(u), decltype(u)::value * BK); });
+  lut_s[t ^ 128] = entry;
+
+  v16i acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[i][j] = v16i{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  v4i af[2][TM], bf[2][TN];
+  auto load_frags = [&](int set, const int8_t* s, int ks) {
+    const int ch = ks * 2 + half;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int r = wm * WM + j * 32 + l32;
+      af[set][j] = *reinterpret_cast<const v4i*>(s + r * BK + (swz<BK>(r, ch) << 4));
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const int r = wn * WN + i * 32 + l32;
+      bf[set][i] = *reinterpret_cast<const v4i*>(s + BM * BK + r * BK + (swz<BK>(r, ch) << 4));
+    }
+  };
+  auto mm = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[set][i], af[set][j], acc[i][j], 0, 0, 0);
+  };
+  const int nk = (K + BK - 1) / BK;
+  // stage kt + NS - 1 loads into the array of stage kt - 1; before its last k-step a wave waits for its share of stage kt + 1
+  // and meets the others
+  auto step = [&](int kt, const int8_t* cur, int8_t* nxt, const int8_t* next) {
+    issue_b(nxt, (kt + NS - 1) * BK);
+    issue_a(nxt, (kt + NS - 1) * BK);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < KS - 1; ++ks) {
+      load_frags((ks + 1) & 1, cur, ks + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      mm(ks & 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vm_lgkm0<(NS - 2) * G>();
+    stage_barrier();
+    load_frags(0, next, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    mm((KS - 1) & 1);
+  };
+  wait_vm_lgkm0<(NS - 2) * JA>();                        // all of B's first stages and A's first
+  stage_barrier();
+  load_frags(0, L0, 0);
+#define ANVIL_EXPERT_STEP(u)                                                                               \
+  if constexpr (NS > u) {                                                                                  \
+    step(kt, arr(std::integral_constant<int, u>{}), arr(std::integral_constant<int, u + NS - 1>{}),          \
+         arr(std::integral_constant<int, u + 1>{}));                                                       \
+    if (++kt == nk) break;                                                                                 \
+  }
+  for (int kt = 0;;) {
+    ANVIL_EXPERT_STEP(0) ANVIL_EXPERT_STEP(1) ANVIL_EXPERT_STEP(2) ANVIL_EXPERT_STEP(3)
+  }
+#undef ANVIL_EXPERT_STEP
+
+  Requant q(shift, OSZ == 1 ? -128 : -32768, OSZ == 1 ? 127 : 32767), q2(shift2, -128, 127);
+  const bool high = q.high() && (!GATED || q2.high());
+  if (!high) q.rest = q2.rest = 0;                       // the 64-bit form shifts by all of it
+  const int rnd3 = (int)round_term(g.shift3);
+  constexpr int TC = GATED ? TN / 2 : TN;                // column groups of 32 a wave has of the result
+  auto finish = [&](auto hi_c) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int r = wm * WM + 32 * j + l32;
+      if (r >= tile.rows) continue;
+      const int m = mult * scale[j], m2 = mult2 * scale[j];
+#pragma unroll
+      for (int i = 0; i < TC; ++i) {
+        const int n = tile.n0 + (wn * TC + i) * 32 + 16 * half;
+        if (n >= g.N) continue;
+        int v[16];
+        finish_n<16, OSZ, GATED, decltype(hi_c)::value>(acc[i][j], acc[GATED ? TC + i : i][j], m, m2, q, q2, g.lut != nullptr, lut_s,
+                                                        g.mult3, rnd3, g.shift3, v);
+        char* out = (char*)g.C + ((tile.p0 + r) * g.ldc + n) * OSZ;
+        if (n + 16 <= g.N) {                             // one store at any alignment
+          if constexpr (OSZ == 1) {
+            const v4i w = pack16(v);
+            __builtin_memcpy(out, &w, 16);
+          } else {
+            const v4i w0 = pack8h(v), w1 = pack8h(v + 8);
+            __builtin_memcpy(out, &w0, 16);
+            __builtin_memcpy(out + 16, &w1, 16);
+          }
+        } else {
+          for (int e = 0; e < 16 && n + e < g.N; ++e) {
+            if (OSZ == 1) out[e] = (char)v[e];
+            else ((int16_t*)out)[e] = (int16_t)v[e];
+          }
+        }
+      }
+    }
+  };
+  if (high) finish(std::true_type{});
+  else finish(std::false_type{});
+  wait_vmcnt(0);                                         // the trailing zero loads land before the LDS is released
+}
+
+// Few rows an expert: 16 MT rows x 16 CT columns a workgroup, operands straight from memory into registers.
+//
+// What bounds it is the weights' way from memory, so nothing stands in it: each of the four waves takes every fourth 64 bytes of K, asks
+// for STEPS of them at a time, and its matrix instructions (16 x 16 x 64) take the loads' registers as they are; no LDS, no barrier before
+// the end, where the waves' sums meet in LDS. A lane's results are four consecutive columns of its row.
+template <int MT, int CT, int OSZ, bool GATED>
+__global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
+  constexpr int NB = GATED ? 2 : 1, STEPS = 4, COLS = 16 * CT;
+  __shared__ __attribute__((aligned(16))) v4i sums[4][MT * CT * NB][64];
+  __shared__ int8_t lut_s[256];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r16 = lane & 15, quad = lane >> 4;
+  const anvil_expert_gemm& g = a.g;
+  ExpertTile tile;
+  if (!find_tile<16 * MT, COLS>(a, blockIdx.x, lane, tile)) return;
+  int mult, mult2 = 0, shift = g.shift, shift2 = g.shift2;
+  if (!expert_mult(a, g.mults, g.mult, tile.e, t == 0, mult)) return;
+  if (GATED && !expert_mult(a, g.mults2, g.mult2, tile.e, t == 0, mult2)) return;
+  if (!g.scale) lift_shift(mult, shift), lift_shift(mult2, shift2);
+  const int K = g.K;
+  int row[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = 16 * m + r16;
+    row[m] = r < tile.rows ? row_of(a, tile.p0 + r, tile.n0 == 0 && wave == 0 && quad == 0) : -1;
+  }
+  const int8_t entry = g.lut ? g.lut[t] : (int8_t)0;
+  const int cols = min(g.N - tile.n0, COLS);
+  const long long b_at = tile.e * g.sb + (long long)tile.n0 * g.ldb;
+  const int b_bytes = (int)((cols - 1) * g.ldb + K);
+  const __amdgpu_buffer_rsrc_t ra = uniform_rsrc(g.A, a.a_bytes), rb = uniform_rsrc(g.B + b_at, b_bytes),
+                               rb2 = uniform_rsrc(GATED ? g.B2 + b_at : g.B, GATED ? b_bytes : 0);
+  unsigned offb[CT], offa[MT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) offb[c] = 16 * c + r16 < cols ? (unsigned)((16 * c + r16) * g.ldb + 16 * quad) : PAST;
+  const auto load = [](__amdgpu_buffer_rsrc_t r, unsigned off) {
+    return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+  };
+  v4i acc[NB][CT][MT];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[b][c][m] = v4i{0, 0, 0, 0};
+  v4i fb[STEPS][NB][CT], fa[STEPS][MT];
+  const auto ask_b = [&](int k0) {                       // bytes past K are zeros
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int k = k0 + 256 * s;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const unsigned off = k + 16 * quad < K ? offb[c] + k : OOB;
+        fb[s][0][c] = load(rb, off);
+        if constexpr (GATED) fb[s][NB - 1][c] = load(rb2, off);
+      }
+    }
+  };
+  const auto ask_a = [&](int k0) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int k = k0 + 256 * s;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) fa[s][m] = load(ra, k + 16 * quad < K ? offa[m] + k : OOB);
+    }
+  };
+  ask_b(64 * wave);                                      // before the rows' numbers are there
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) offa[m] = row[m] >= 0 ? (unsigned)(row[m] * g.lda + 16 * quad) : PAST;
+  int scale[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) scale[m] = !g.scale ? 1 : row[m] < 0 ? 0 : (int)g.scale[row[m]];
+  for (int k0 = 64 * wave;;) {
+    ask_a(k0);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            acc[b][c][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[s][b][c], fa[s][m], acc[b][c][m], 0, 0, 0);
+    k0 += 256 * STEPS;
+    if (k0 >= K) break;
+    ask_b(k0);
+  }
+  lut_s[t ^ 128] = entry;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) sums[wave][(m * CT + c) * NB + b][lane] = acc[b][c][m];
+  __syncthreads();
+  Requant q(shift, OSZ == 1 ? -128 : -32768, OSZ == 1 ? 127 : 32767), q2(shift2, -128, 127);
+  const bool high = q.high() && (!GATED || q2.high());
+  if (!high) q.rest = q2.rest = 0;
+  const int rnd3 = (int)round_term(g.shift3);
+#pragma unroll
+  for (int i = 0; i < MT * CT; ++i) {                    // block i of 16 x 16: wave i % 4
+    if (i % 4 != wave) continue;
+    const int r = 16 * (i / CT) + r16, n = tile.n0 + 16 * (i % CT) + 4 * quad;
+    if (r >= tile.rows || n >= g.N) continue;
+    v4i x[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) x[b] = sums[0][i * NB + b][lane] + sums[1][i * NB + b][lane] + sums[2][i * NB + b][lane] + sums[3][i * NB + b][lane];
+    const int sc = scale[i / CT];
+    int v[4];
+    const auto finish = [&](auto hi_c) {
+      finish_n<4, OSZ, GATED, decltype(hi_c)::value>(x[0], x[NB - 1], mult * sc, mult2 * sc, q, q2, g.lut != nullptr, lut_s, g.mult3, rnd3,
+                                                     g.shift3, v);
+    };
+    if (high) finish(std::true_type{});
+    else finish(std::false_type{});
+    char* out = (char*)g.C + ((tile.p0 + r) * g.ldc + n) * OSZ;
+    if (n + 4 <= g.N) {                                  // one store at any alignment
+      if constexpr (OSZ == 1) {
+        const unsigned w = pack4(v[0], v[1], v[2], v[3]);
+        __builtin_memcpy(out, &w, 4);
+      } else {
+        const unsigned w[2] = {__builtin_amdgcn_perm((unsigned)v[1], (unsigned)v[0], 0x05040100u),
+                               __builtin_amdgcn_perm((unsigned)v[3], (unsigned)v[2], 0x05040100u)};
+        __builtin_memcpy(out, w, 8);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < g.N) {
+          if (OSZ == 1) out[e] = (char)v[e];
+          else ((int16_t*)out)[e] = (int16_t)v[e];
+        }
+    }
+  }
+}
+
+// Operands at any alignment and stride, and past 2^32 bytes: 64 x 64 tiles, chunks through registers into LDS, the next stage's on their
+// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 17 us (19.7 with
+// one stage at a time).
 template <int OSZ, bool GATED>
 __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
-  constexpr int BM = 64, BN = 64, BK = 64, NB = GATED ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) int8_t As[BM * BK], Bs[NB][BN * BK];
+  constexpr int BM = 64, BN = 64, BK = 128, NB = GATED ? 2 : 1, PER = BK / 64;
+  __shared__ __attribute__((aligned(16))) int8_t As[2][BM * BK], Bs[2][NB][BN * BK];
   __shared__ int8_t lut_s[256];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = wave >> 1, wn = wave & 1, half = lane >> 5, l32 = lane & 31;
@@ -101,37 +481,53 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   if (GATED && !expert_mult(a, g.mults2, g.mult2, tile.e, t == 0, mult2)) return;
   if (g.lut) lut_s[t] = g.lut[t];
 
-  // thread t stages chunk t % 4 of row t / 4 of each operand
+  // thread t stages chunks t % 4, t % 4 + 4 of row t / 4 of each operand
   const int sr = t >> 2, sc = t & 3;
   const int src = sr < tile.rows ? row_of(a, tile.p0 + sr, tile.n0 == 0 && sc == 0) : -1;
   const int8_t* arow = src < 0 ? nullptr : g.A + (long long)src * g.lda;
   const int n = tile.n0 + sr;
-  const int8_t* brow[2] = {nullptr, nullptr};
-  if (n < g.N) {
-    brow[0] = g.B + tile.e * g.sb + (long long)n * g.ldb;
-    if (GATED) brow[1] = g.B2 + tile.e * g.sb + (long long)n * g.ldb;
-  }
-  const v4i zero = {0, 0, 0, 0};
+  const int8_t* brow[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) brow[b] = n < g.N ? (b ? g.B2 : g.B) + tile.e * g.sb + (long long)n * g.ldb : nullptr;
+  const int K = g.K;
+  const auto chunk = [&](const int8_t* row, int k, bool tail) {
+    v4i v = {0, 0, 0, 0};
+    if (!row) return v;
+    if (tail) return row_chunk(row, k, K);
+    __builtin_memcpy(&v, row + k, 16);
+    return v;
+  };
+  v4i av[PER], bv[NB][PER];
+  const auto ask = [&](int k) {
+    const bool tail = k + BK > K;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      av[i] = chunk(arow, k + 16 * (sc + 4 * i), tail);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) bv[b][i] = chunk(brow[b], k + 16 * (sc + 4 * i), tail);
+    }
+  };
   v16i acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = v16i{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  for (int k = 0; k < g.K; k += BK) {
-    const v4i av = arow ? row_chunk(arow, k + 16 * sc, g.K) : zero;
-    v4i bv[NB];
+  ask(0);
+  for (int k = 0, cur = 0; k < K; k += BK, cur ^= 1) {   // a wave is at most one barrier ahead, so two arrays do
 #pragma unroll
-    for (int b = 0; b < NB; ++b) bv[b] = brow[b] ? row_chunk(brow[b], k + 16 * sc, g.K) : zero;
-    __syncthreads();
-    *reinterpret_cast<v4i*>(As + sr * BK + 16 * swz<BK>(sr, sc)) = av;
+    for (int i = 0; i < PER; ++i) {
+      const int to = sr * BK + 16 * swz<BK>(sr, sc + 4 * i);
+      *reinterpret_cast<v4i*>(As[cur] + to) = av[i];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) *reinterpret_cast<v4i*>(Bs[b] + sr * BK + 16 * swz<BK>(sr, sc)) = bv[b];
+      for (int b = 0; b < NB; ++b) *reinterpret_cast<v4i*>(Bs[cur][b] + to) = bv[b][i];
+    }
     __syncthreads();
+    if (k + BK < K) ask(k + BK);
 #pragma unroll
     for (int ks = 0; ks < BK / 32; ++ks) {
       const int ra = wm * 32 + l32, rb = wn * 32 + bperm(l32), ch = 2 * ks + half;
-      const v4i af = *reinterpret_cast<const v4i*>(As + ra * BK + 16 * swz<BK>(ra, ch));
+      const v4i af = *reinterpret_cast<const v4i*>(As[cur] + ra * BK + 16 * swz<BK>(ra, ch));
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const v4i bf = *reinterpret_cast<const v4i*>(Bs[b] + rb * BK + 16 * swz<BK>(rb, ch));
+        const v4i bf = *reinterpret_cast<const v4i*>(Bs[cur][b] + rb * BK + 16 * swz<BK>(rb, ch));
         acc[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf, af, acc[b], 0, 0, 0);
       }
     }
@@ -140,15 +536,16 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   if (m >= tile.rows) return;
   const int i = row_of(a, tile.p0 + m, false);
   const int scale = g.scale ? (i < 0 ? 0 : (int)g.scale[i]) : 1;
-  const int lo = OSZ == 1 ? -128 : -32768, hi = -lo - 1;
-  const Requant q1(g.shift, lo, hi), q2(g.shift2, -128, 127);
+  const int lo = OSZ == 1 ? -128 : -32768;
+  const Requant q1(g.shift, lo, -lo - 1), q2(g.shift2, -128, 127);
+  const auto of = [](const Requant& q, int acc, int mul) { return q.high() ? q.of<true>(acc, mul) : q.of<false>(acc, mul); };
   const int rnd3 = (int)round_term(g.shift3);
   char* out = (char*)g.C + ((tile.p0 + m) * g.ldc + n0) * OSZ;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    int v = q1.of<false>(acc[0][e], mult * scale);
+    int v = of(q1, acc[0][e], mult * scale);
     if (g.lut) v = lut_s[(v + 128) & 255];
-    if constexpr (GATED) v = min(max((v * q2.of<false>(acc[NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
+    if constexpr (GATED) v = min(max((v * of(q2, acc[NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
     if (n0 + e >= g.N) break;
     if (OSZ == 1) out[e] = (char)v;
     else ((int16_t*)out)[e] = (int16_t)v;
@@ -192,13 +589,71 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
   for (const Span& s : in)
     if (!apart(c, s)) return set_error(ANVIL_E_VALUE, "%s: the result overlaps what is read", who);
   if (int e = check_ctx(ctx)) return e;
-  ExpertArgs a{*g, (g->N + 63) / 64, ctx->flags};
-  const long long tiles = ((long long)g->rows / 64 + std::min(g->experts, g->rows)) * a.tiles_n;
-  if (tiles > GRID_MAX) return set_error(ANVIL_E_VALUE, "%s: %d rows of %d columns are more tiles than a grid has", who, g->rows, g->N);
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
-  if (g->B2) ANVIL_LAUNCH((expert_any<1, true>), grid, dim3(256), 0, ctx->stream, a);
-  else if (g->out_dtype == ANVIL_I8) ANVIL_LAUNCH((expert_any<1, false>), grid, dim3(256), 0, ctx->stream, a);
-  else ANVIL_LAUNCH((expert_any<2, false>), grid, dim3(256), 0, ctx->stream, a);
+  ExpertArgs a{*g, 0, 0, ctx->flags};
+  const auto grid = [&](int bm, int cols) -> unsigned {   // 0: more tiles than a grid has
+    a.tiles_n = (g->N + cols - 1) / cols;
+    const long long tiles = ((long long)g->rows / bm + std::min(g->experts, g->rows)) * a.tiles_n;
+    return tiles > GRID_MAX ? 0 : (unsigned)((tiles + 7) / 8 * 8);
+  };
+  const auto by_type = [&](auto&& f) {
+    if (g->B2) f(std::integral_constant<int, 1>{}, std::true_type{});
+    else if (g->out_dtype == ANVIL_I8) f(std::integral_constant<int, 1>{}, std::false_type{});
+    else f(std::integral_constant<int, 2>{}, std::false_type{});
+  };
+  // 16-byte loads, 32-bit offsets into A and into a tile's weights
+  const long long a_bytes = (g->rows_a - 1) * g->lda + g->K;
+  unsigned wgs = 0;
+  const auto tiles = [&](auto bm, auto bn, auto bk, auto ns) {
+    by_type([&](auto osz, auto gated) {
+      constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, BK = decltype(bk)::value, NS = decltype(ns)::value;
+      constexpr int OSZ = decltype(osz)::value;
+      constexpr bool GATED = decltype(gated)::value;
+      wgs = grid(BM, GATED ? BN / 2 : BN);
+      if (!wgs) return;
+      if (g->K % BK == 0) ANVIL_LAUNCH((expert_tile<BM, BN, BK, NS, OSZ, GATED, true>), dim3(wgs), dim3(256), 0, ctx->stream, a);
+      else ANVIL_LAUNCH((expert_tile<BM, BN, BK, NS, OSZ, GATED, false>), dim3(wgs), dim3(256), 0, ctx->stream, a);
+    });
+  };
+  const auto few = [&](auto mt) {
+    by_type([&](auto osz, auto gated) {
+      constexpr int MT = decltype(mt)::value;
+      constexpr bool GATED = decltype(gated)::value;
+      constexpr int CT = GATED ? 1 : 2;
+      wgs = grid(16 * MT, 16 * CT);
+      if (wgs) ANVIL_LAUNCH((expert_few<MT, CT, decltype(osz)::value, GATED>), dim3(wgs), dim3(256), 0, ctx->stream, a);
+    });
+  };
+  if (aligned16(g->A) && aligned16(g->B) && aligned16(g->B2) && g->K % 16 == 0 && g->lda % 16 == 0 && g->ldb % 16 == 0 && g->sb % 16 == 0 &&
+      a_bytes <= (long long)PAST && g->ldb < 1 << 23) {
+    a.a_bytes = (int)(unsigned)std::max(0ll, a_bytes);
+    using std::integral_constant;
+    const integral_constant<int, 128> i128;
+    const integral_constant<int, 64> i64;
+    // Kernels by size, us on one box (rows x the experts of each):
+    //   few rows / 64 x 128: 16 x 2 of 8 experts, 2048 -> 768, 6.0 / 10.3; 64 x 2 of 8, 2048 -> 768, 7.0 / 10.2; 16 x 4 of 32, gated
+    //     768 -> 1024, 11.4 / 12.1; 8192 of one, 768 -> 16, 4.9 / 6.5; but 64 x 2 of 8, gated 768 -> 2048, 9.7 / 7.5; 64 x 4 of 32, gated
+    //     768 -> 1024, 14.7 / 12.8: every 16 or 32 rows read their weights again
+    //   128 x 256 / 64 x 128: 32768 x 2 of 8, gated 768 -> 2048, 261 / 411; 4096 x 2 of 8, the same, 46 / 55; 8192 x 2 of 16, 2048 -> 768, 41 / 46;
+    //     but 4096 x 2 of 8, 768 -> 2048 (576 tiles), 35 / 30; 2048 x 2 of 8, gated 768 -> 2048 (640), 31 / 31: with few tiles the last round
+    //     of them is half empty, and a short K has little to make up for it
+    const long long width = (long long)g->N * (g->B2 ? 2 : 1);                         // of the operand B, and B2 beside it
+    const long long large = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((width + 255) / 256);
+    if (g->rows * width * g->K <= 1 << 28) {
+      if (g->rows <= 8ll * g->experts) few(integral_constant<int, 1>{});
+      else few(integral_constant<int, 2>{});
+    } else if (large >= (g->K >= 2048 ? 3 : 5) * ctx->num_cu / 2) {
+      tiles(i128, integral_constant<int, 256>{}, i64, integral_constant<int, 3>{});
+    } else {
+      tiles(i64, i128, i128, integral_constant<int, 2>{});
+    }
+  } else {
+    wgs = grid(64, 64);
+    if (wgs)
+      by_type([&](auto osz, auto gated) {
+        ANVIL_LAUNCH((expert_any<decltype(osz)::value, decltype(gated)::value>), dim3(wgs), dim3(256), 0, ctx->stream, a);
+      });
+  }
+  if (!wgs) return set_error(ANVIL_E_VALUE, "%s: %d rows of %d columns are more tiles than a grid has", who, g->rows, g->N);
   ANVIL_LAUNCHED();
   return ANVIL_OK;
 }

@@ -6,29 +6,38 @@
 
 namespace anvil {
 
-// clamp((acc * m + 2^(s-1)) >> s, lo, hi) with the product and the sum in 64 bits. HI: s >= 32, so that all of the result is in
-// the sum's upper word, which is clamped before its shift by s - 32: one 32 x 32 -> 64-bit multiply-add, a clamp and a shift.
-// A product's multiplier is m / 2^s below 1 / 2, so the host and the kernels move a smaller s up to 32 where m has room.
+// clamp((acc * m + 2^(s-1)) >> s, lo, hi) with the product and the sum in 64 bits, left as a clamped int to be shifted right by `rest`.
+// HI: s >= 33, where 2^(s-1) is a whole number of 2^32: the sum's upper word is the product's upper word and 2^(s-33), one
+// multiplication and one addition in 32 bits, clamped before the last s - 32 bits go (|acc| <= 2^30, so neither leaves int32). A product's
+// m / 2^s lies well below 1 / 4, so a smaller s is moved up to 33 where m has room (lift_shift).
 struct Requant {
-  long long rnd;
-  int s, lo, hi;
-  __device__ Requant(int shift, int lo_, int hi_) : rnd(shift ? 1ll << (shift - 1) : 0), s(shift), lo(lo_), hi(hi_) {}
+  int s, rest, add, clo, chi, lo, hi;
+  __host__ __device__ Requant(int shift, int lo_, int hi_) : s(shift), rest(0), add(0), clo(lo_), chi(hi_), lo(lo_), hi(hi_) {
+    if (s < 33) return;
+    rest = s - 32;
+    add = 1 << (rest - 1);
+    const long long a = (long long)lo << rest, b = (((long long)hi + 1) << rest) - 1;
+    clo = a < I32_MIN ? (int)I32_MIN : (int)a;
+    chi = b > I32_MAX ? (int)I32_MAX : (int)b;
+  }
+  __host__ __device__ bool high() const { return s >= 33; }
   template <bool HI>
-  __device__ __forceinline__ int of(int acc, int m) const {
-    const long long v = (long long)acc * m + rnd;
-    if constexpr (HI) return min(max((int)(v >> 32) >> (s - 32), lo), hi);
-    const long long r = v >> s;
+  __device__ __forceinline__ int unshifted(int acc, int m) const {
+    if constexpr (HI) return med3i(__mulhi(acc, m) + add, clo, chi);
+    const long long r = ((long long)acc * m + (s ? 1ll << (s - 1) : 0)) >> s;
     return (int)(r < lo ? lo : r > hi ? hi : r);
   }
+  template <bool HI>
+  __device__ __forceinline__ int of(int acc, int m) const { return unshifted<HI>(acc, m) >> rest; }
 };
 
-// (m, s) with s moved up to 32 where m keeps within int32: the same products and roundings
+// (m, s) with s moved up to 33 where m keeps within int32: the same products and roundings
 __host__ __device__ inline void lift_shift(int& m, int& s) {
-  if (s >= 32) return;
-  const long long w = (long long)m * (1ll << (32 - s));
+  if (s >= 33) return;
+  const long long w = (long long)m * (1ll << (33 - s));
   if (w < I32_MIN || w > I32_MAX) return;
   m = (int)w;
-  s = 32;
+  s = 33;
 }
 
 // Memory of `rows` rows of `width` bytes, `ld` bytes apart.

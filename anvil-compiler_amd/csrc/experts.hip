@@ -245,7 +245,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_place(RouteArgs g) {
 
 struct CombineArgs {
   anvil_expert_combine c;
-  int mult, lifted;                                      // of Requant's upper word, where c.mult / 2^c.shift allows it (c.shift then 32 or more)
+  int mult, lifted;                                      // of Requant's upper word, where c.mult / 2^c.shift allows it (c.shift then 33 or more)
   unsigned* flags;
 };
 
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256) void combine_any(CombineArgs g) {
       if (p >= 0 && p < c.positions) acc += (int)c.weight[i * c.top + j] * (int)c.Y[p * c.ldy + col];
       else if (p != -1) raise_flag(g.flags, FLAG_EXPERTS);
     }
-    int d = rq.of<false>(acc, g.mult);
+    int d = g.lifted ? rq.of<true>(acc, g.mult) : rq.of<false>(acc, g.mult);
     if (c.R) {
       const int r = c.r_dtype == ANVIL_I8 ? (int)((const int8_t*)c.R)[i * c.ldr + col] : (int)((const int16_t*)c.R)[i * c.ldr + col];
       d = min(max((r * c.ma + d * c.mb + (int)round_term(c.shift2)) >> c.shift2, lo), hi);
@@ -448,7 +448,7 @@ extern "C" int anvil_expert_combine_i8(anvil_ctx* ctx, const anvil_expert_combin
   if (int e = check_ctx(ctx)) return e;
   CombineArgs g{*c, c->mult, 0, ctx->flags};
   lift_shift(g.mult, g.c.shift);
-  g.lifted = g.c.shift >= 32;
+  g.lifted = g.c.shift >= 33;
   const long long n = (long long)c->rows * c->cols;
   const auto even = [](const void* p, long long ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; };
   if (c->cols % 16 == 0 && even(c->Y, c->ldy, 1) && even(c->D, c->ldd, c->d_dtype) && (!c->R || even(c->R, c->ldr, c->r_dtype))) {
