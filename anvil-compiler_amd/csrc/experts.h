@@ -40,6 +40,17 @@ __host__ __device__ inline void lift_shift(int& m, int& s) {
   s = 33;
 }
 
+template <int L>
+__device__ __forceinline__ int lane_group_max(int v) {       // maximum over aligned groups of L lanes
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));
+  if constexpr (L > 16) v = max(v, __builtin_amdgcn_ds_swizzle(v, (16 << 10) | 0x1F));
+  if constexpr (L > 32) v = max(v, __shfl_xor(v, 32));
+  return v;
+}
+
 // Memory of `rows` rows of `width` bytes, `ld` bytes apart.
 struct Span {
   const void* p;

@@ -38,17 +38,7 @@ __device__ __forceinline__ int share(long long e, int one, long long S) {
   return (int)q;
 }
 
-// maxima and sums over aligned groups of L lanes
-template <int L>
-__device__ __forceinline__ int group_max(int v) {
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));
-  if constexpr (L > 16) v = max(v, __builtin_amdgcn_ds_swizzle(v, (16 << 10) | 0x1F));
-  if constexpr (L > 32) v = max(v, __shfl_xor(v, 32));
-  return v;
-}
+// sums over aligned groups of L lanes
 template <int L>
 __device__ __forceinline__ long long group_sum(long long v) {
 #pragma unroll
@@ -72,7 +62,7 @@ __device__ __forceinline__ void choose(const RouteArgs& g, long long row, int su
     int m = INT32_MIN;
 #pragma unroll
     for (int i = 0; i < PER; ++i) m = max(m, key[i] < best ? key[i] : INT32_MIN);
-    best = group_max<L>(m);
+    best = lane_group_max<L>(m);
     if (j == 0) top = best >> 10;
     if (sub == j) mine = best;
   }
@@ -260,7 +250,7 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
   const int chunks = c.cols >> 4;
   const long long n = (long long)c.rows * chunks;
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-    const long long i = at / chunks;
+    const long long i = n <= UINT32_MAX ? (unsigned)at / (unsigned)chunks : at / chunks;
     const int col = (int)(at - i * chunks) * 16;
     v4i r0 = {0, 0, 0, 0}, r1 = {0, 0, 0, 0};
     if (c.R) {
@@ -330,7 +320,7 @@ __global__ __launch_bounds__(256) void combine_any(CombineArgs g) {
   const int lo = c.d_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
   const long long n = (long long)c.rows * c.cols;
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-    const long long i = at / c.cols;
+    const long long i = n <= UINT32_MAX ? (unsigned)at / (unsigned)c.cols : at / c.cols;
     const int col = (int)(at - i * c.cols);
     int acc = 0;                                         // 32 x 2^15 x 2^7 at most
     for (int j = 0; j < c.top; ++j) {

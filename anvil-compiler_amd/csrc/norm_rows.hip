@@ -65,17 +65,6 @@ struct Divider {
   }
 };
 
-template <int L>
-__device__ __forceinline__ int lane_group_max(int v) {       // maximum over aligned groups of L lanes
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));
-  if constexpr (L > 16) v = max(v, __builtin_amdgcn_ds_swizzle(v, (16 << 10) | 0x1F));
-  if constexpr (L > 32) v = max(v, __shfl_xor(v, 32));
-  return v;
-}
-
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
@@ -111,13 +100,13 @@ __device__ __forceinline__ void unpack(v4i (&v)[R], int dtype) {
   }
 }
 
-// Rows of at most 8 L R columns, 16-byte aligned, in registers: L lanes a row (64 / L rows a wave), R chunks of eight elements a lane,
-// and a lane has the same columns of every row it takes, so its weights stay in registers.
+// Rows of at most 8 L R columns, 16-byte aligned, in registers: L lanes a row (64 / L rows a wave, or the workgroup's 256), R chunks of
+// eight elements a lane, and a lane has the same columns of every row it takes, so its weights stay in registers.
 //
-// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 33.7 us, 4.5 TB/s
-// (one workgroup a row, each row read twice: 149). Rows of 768 take 16 lanes of six
-// chunks each: 64 lanes would leave a quarter of the wave idle in the second chunk, and the row's sum and maximum
-// take four data-parallel moves instead of six steps.
+// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 27 us of the
+// kernel's own, 33.6 a call in a row of them, 4.5 TB/s (one workgroup a row, each row read twice: 149). Many rows of up to 768 columns take
+// 16 lanes of up to six chunks: 64 lanes would leave a quarter of the wave idle in the second chunk of 768, and the row's
+// sum and maximum take four data-parallel moves instead of six steps.
 //
 // Codes. floor((254 |t| + a) / 2a) with t's sign is floor((254 t + a - [t < 0]) / 2a); with 256 a added it is 128 larger and its
 // numerator lies in [0, 511 a], below 2^31 (a <= 2^22), so one multiplication by the row's reciprocal (Divider) and a shift
@@ -125,20 +114,26 @@ __device__ __forceinline__ void unpack(v4i (&v)[R], int dtype) {
 template <int L, int R>
 __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
   const anvil_add_norm& n = g.n;
-  const int lane = threadIdx.x & 63, sub = lane & (L - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr bool WHOLE = L == 256;                       // a workgroup a row
+  constexpr int ROWS = WHOLE ? 1 : 64 / L;               // of a wave at a time
+  __shared__ unsigned long long sums[2][4];
+  __shared__ int tops[2][4];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x & (L - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int mine = WHOLE ? 0 : lane / L;                 // row of those
   const int chunks = n.cols >> 3;
   const int lo = n.r_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
   const int rnd = (int)round_term(n.shift), ma = n.ma, mb = n.mb, shift = n.shift;
-  constexpr int ROWS = 64 / L;
   v2u w[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) w[i] = sub + L * i < chunks ? *reinterpret_cast<const v2u*>(n.w + 8 * (sub + L * i)) : v2u{0, 0};
   // a lane's first chunk from that of its wave's rows (the launch checks ROWS rows against 2^31); chunk i is i steps on
-  const auto offset = [&](long long ld, int size) { return (unsigned)((lane / L) * ld + 8 * sub) * (unsigned)size; };
+  const auto offset = [&](long long ld, int size) { return (unsigned)(mine * ld + 8 * sub) * (unsigned)size; };
   const unsigned ox = offset(n.ldx, n.x_dtype), oy = n.Y ? offset(n.ldy, n.y_dtype) : 0, oz = n.Y ? offset(n.ldr, n.r_dtype) : 0,
                  oh = offset(n.ldh, 1);
-  for (long long first = ((long long)blockIdx.x * 4 + wave) * ROWS; first < n.rows; first += (long long)gridDim.x * 4 * ROWS) {
-    const long long row = first + lane / L;
+  const long long group = WHOLE ? blockIdx.x : (long long)blockIdx.x * 4 + wave, groups = WHOLE ? gridDim.x : 4ll * gridDim.x;
+  int turn = 0;                                          // a wave is at most one barrier ahead, so two sets of sums do
+  for (long long first = group * ROWS; first < n.rows; first += groups * ROWS, turn ^= 1) {
+    const long long row = first + mine;
     const bool live = row < n.rows;
     const int rows = (int)min((long long)ROWS, n.rows - first);
     const auto span = [&](const void* p, long long ld, int size) {
@@ -192,8 +187,16 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
         low = min(low, min(t0, t1));
       }
     }
-    const unsigned a = (unsigned)lane_group_max<L>(max(top, -low));
-    const unsigned s0 = (unsigned)lane_group_sum<L>((int)(ss & 0xFFFFFF)), s1 = (unsigned)lane_group_sum<L>((int)(ss >> 24));
+    constexpr int W = WHOLE ? 64 : L;
+    unsigned a = (unsigned)lane_group_max<W>(max(top, -low));
+    const unsigned s0 = (unsigned)lane_group_sum<W>((int)(ss & 0xFFFFFF)), s1 = (unsigned)lane_group_sum<W>((int)(ss >> 24));
+    ss = ((unsigned long long)s1 << 24) + s0;
+    if constexpr (WHOLE) {
+      if (lane == 0) sums[turn][wave] = ss, tops[turn][wave] = (int)a;
+      __syncthreads();
+      ss = sums[turn][0] + sums[turn][1] + sums[turn][2] + sums[turn][3];
+      a = (unsigned)max(max(tops[turn][0], tops[turn][1]), max(tops[turn][2], tops[turn][3]));
+    }
     // the products t again, rather than held since the sums: 8 R registers of a wave's budget
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
       }
       __builtin_amdgcn_raw_buffer_store_b64(h, ph, to(i), 0, 0);
     }
-    if (live && sub == 0) n.scale[row] = (int16_t)scale_of(n, a, ((unsigned long long)s1 << 24) + s0, g.nbits);
+    if (live && sub == 0) n.scale[row] = (int16_t)scale_of(n, a, ss, g.nbits);
   }
 }
 
@@ -308,25 +311,38 @@ extern "C" int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n) {
   const auto even = [&](const void* p, long long ld, int size) { return (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 && ld < 1 << 28; };
   const auto m24 = [](int m) { return m >= -(1 << 23) && m < 1 << 23; };
   const int chunks = n->cols / 8;
-  if (n->cols % 8 == 0 && chunks <= 1024 && even(n->X, n->ldx, n->x_dtype) && even(n->H, n->ldh, 1) && even(n->w, 8, 1) &&
+  if (n->cols % 8 == 0 && chunks <= 2048 && even(n->X, n->ldx, n->x_dtype) && even(n->H, n->ldh, 1) && even(n->w, 8, 1) &&
       (!n->Y || (even(n->Y, n->ldy, n->y_dtype) && even(n->R, n->ldr, n->r_dtype) && m24(n->ma) && m24(n->mb)))) {
     const auto go = [&](auto lanes, auto per) {
       constexpr int L = decltype(lanes)::value, R = decltype(per)::value;
-      const int groups = (n->rows + 4 * (64 / L) - 1) / (4 * (64 / L));
+      const int rows = 256 / L, groups = (n->rows + rows - 1) / rows;              // of a workgroup at a time
       ANVIL_LAUNCH((add_norm_rows<L, R>), dim3((unsigned)std::min(groups, 8 * ctx->num_cu)), dim3(256), 0, ctx->stream, g);
     };
     using std::integral_constant;
-    const auto wide = [&](auto lanes) {
-      const int r = (chunks + decltype(lanes)::value - 1) / decltype(lanes)::value;
-      if (r <= 1) go(lanes, integral_constant<int, 1>{});
-      else if (r <= 2) go(lanes, integral_constant<int, 2>{});
-      else if (r <= 4) go(lanes, integral_constant<int, 4>{});
-      else if (r <= 6) go(lanes, integral_constant<int, 6>{});
-      else if (r <= 8) go(lanes, integral_constant<int, 8>{});
-      else if constexpr (decltype(lanes)::value > 16) go(lanes, integral_constant<int, 16>{});
-    };
-    if (chunks <= 128) wide(integral_constant<int, 16>{});
-    else wide(integral_constant<int, 64>{});
+    const integral_constant<int, 1> c1;
+    const integral_constant<int, 2> c2;
+    const integral_constant<int, 4> c4;
+    // Lanes a row, kernel us of an i16 stream with an i8 addend. 16 / 64: 32768 rows of 768 27.4 / 28.8, 8192 9.6 / 10.4, but 2048 5.9 / 5.2 and
+    // 32768 of 1024 34.6 / 32.8 (eight chunks a lane leave two waves a SIMD). 64 / 256: 8192 rows of 1536 17.7 / 20.8, 16384 of 2048 34 / 39,
+    // 8192 of 2560 28.9 / 28.3, 256 of 4096 6.5 / 5.2.
+    const int L = chunks > 256 ? 256 : chunks <= 96 && n->rows > 8 * ctx->num_cu ? 16 : 64;
+    if (L == 256) {
+      const integral_constant<int, 256> l;
+      if (chunks <= 512) go(l, c2);
+      else if (chunks <= 1024) go(l, c4);
+      else go(l, integral_constant<int, 8>{});
+    } else if (L == 16) {
+      const integral_constant<int, 16> l;
+      if (chunks <= 16) go(l, c1);
+      else if (chunks <= 32) go(l, c2);
+      else if (chunks <= 64) go(l, c4);
+      else go(l, integral_constant<int, 6>{});
+    } else {
+      const integral_constant<int, 64> l;
+      if (chunks <= 64) go(l, c1);
+      else if (chunks <= 128) go(l, c2);
+      else go(l, c4);
+    }
     ANVIL_LAUNCHED();
     return ANVIL_OK;
   }
