@@ -358,7 +358,7 @@ def product_case(counts, N, K, kind="plain", gather=True, scaled=True, dtype="i8
     rows = n + behind
     na = (rows_a or max(1, n // 2 + 1)) if gather else max(1, rows)
     A = rng.choice([-128, 127], (na, K)) if extreme else rng.integers(-128, 128, (na, K))
-    B, B2 = rng.integers(-128, 128, (2, E * N, K))
+    B, B2 = rng.integers(-128, 128, (2, E * N, K), dtype=np.int64 if E * N * K < 1 << 22 else np.int8)
     if extreme:
         B = rng.choice([-128, 127], (E * N, K))
         A[0], B[0] = -128, -128
@@ -424,6 +424,33 @@ def test_product_depths(K):
         product_case([40, 0, 70], 96, K, kind, seed=K)
         product_case([200], 160, K, kind, seed=K, gather=False, scaled=False)
         product_case([1, 3, 2], 40, K, kind, seed=K)
+
+
+# Sizes that leave the few-rows kernel (rows x N x K above 2^28) for 64 x 128 tiles, and (at least 640 tiles of 128 x 256, or 384 with a K of
+# 2048 or more on 256 CUs) for those.
+FORMS = [("plain", "i8"), ("plain", "i16"), ("table", "i8"), ("gated", "i8")]
+
+
+@gpu
+@pytest.mark.parametrize("kind,dtype", FORMS)
+@pytest.mark.parametrize("N,K", [(640, 1024), (700, 1040), (1001, 528), (1000, 16 * 41), (513, 2048), (5000, 128)])
+def test_products_by_tiles_of_64_rows(N, K, kind, dtype):
+    counts = [130, 0, 61, 200, 64, 1, 150, 65, 63]
+    product_case(counts, N, K, kind, dtype=dtype, seed=N)
+    product_case(counts, N, K, kind, dtype=dtype, seed=K, gather=False, scaled=False, pads=(16, 32, 1), mults="one")
+
+
+@gpu
+@pytest.mark.parametrize("kind,dtype", FORMS)
+@pytest.mark.parametrize("experts,N,K", [(90, 2048, 80), (90, 2000, 64), (85, 2049, 128), (90, 2048, 192), (80, 2300, 208), (24, 4096, 2064),
+                                         (25, 4100, 2048)])
+def test_products_by_tiles_of_128_rows(experts, N, K, kind, dtype):
+    rng = np.random.default_rng(N)
+    counts = rng.integers(0, 60, experts)
+    counts[[1, 3]] = 0, 300
+    counts[5:8] = 127, 128, 129
+    counts[9] += max(0, (1 << 28) // (N * K) + 1 - counts.sum())
+    product_case(counts.tolist(), N, K, kind, dtype=dtype, seed=K, scaled=K % 128 == 0)
 
 
 @gpu
