@@ -154,6 +154,9 @@ class Decoder:
         pages = self.rows * (slots + 1) if pages is None else int(pages)
         self.cache = KVCache(self.dev, layers, heads, dim, pages, self.rows, max_tokens, window, sinks)
         self.wte, self.wpe = (self.dev.upload(t) for t in cm.embedding)
+        for kind, op, *rest in self.steps:
+            if kind == "experts":
+                rest[-1]["starts"] = self.dev.alloc(4 * (g.qt(op.scores).dims[-1] + 1))
         self._room, self._buffers = 0, []
 
     # ----------------------------------------------------------------------------------------------- lowering
@@ -166,6 +169,7 @@ class Decoder:
         # adds in the epilogue of the product before them, whose own result nothing else reads
         adds = {op: add for op, add in cm._residual_fusions("outputs").items()
                 if len(cm.users[op.result]) == 1 and g.qt(op.a).dims[-1] % 16 == 0}
+        expert_adds, scratch = cm._expert_adds("outputs"), []
         layers, shape = 0, None
 
         def new(v, width=None):
@@ -245,6 +249,15 @@ class Decoder:
                 steps.append(("add", op, rows_of(op.a), rows_of(op.b), new(op.result)))
             elif isinstance(op, g.LutOp):
                 steps.append(("lut", op, rows_of(op.x), new(op.result), table(op.table)))
+            elif isinstance(op, g.ExpertsOp):
+                add = expert_adds.get(op)
+                other = None if add is None else rows_of(add.b if add.a is op.result else add.a)
+                x, scores = rows_of(op.x), rows_of(op.scores)
+                if add is not None:
+                    inside.add(add)
+                buf = {n: _Rows(*what) for n, what in cm._expert_scratch(op).items()}
+                scratch.extend(buf.values())
+                steps.append(("experts", op, x, scores, new(op.result if add is None else add.result), add, other, buf))
             elif isinstance(op, g.LutMulOp):
                 steps.append(("lut_mul", op, rows_of(op.x), rows_of(op.y), new(op.result), table(op.table)))
             else:
@@ -253,7 +266,7 @@ class Decoder:
             raise ValueError("decoding needs an attention chain")
         self.logits = rows_of(cm.output_values[0])
         self.scale = g.qt(cm.output_values[0]).qscale
-        self._values = list(value.values())
+        self._values = list(value.values()) + scratch
         return steps, layers, *shape
 
     def _make_room(self, rows):
@@ -310,6 +323,11 @@ class Decoder:
                 a, b, y = rest
                 dev.add_requant(a.buf, a.dtype, b.buf, b.dtype, int(op.Ma), int(op.Mb), int(op.s), rows * y.width, y.buf, y.dtype,
                                 rt.OP_UNCHECKED)
+            elif kind == "experts":
+                x, scores, y, add, other, buf = rest
+                at = {n: b.buf if isinstance(b, _Rows) else b for n, b in buf.items()}
+                for _, call, args in cm._expert_calls(op, x.buf, scores.buf, rows, {**at, "out": y.buf}, add, other and other.buf):
+                    call(*[a.ptr if hasattr(a, "ptr") else a for a in args])
             elif kind == "lut":
                 x, y, lut = rest
                 dev.lut_i8(x.buf, const[lut].ptr, rows * y.width, y.buf)

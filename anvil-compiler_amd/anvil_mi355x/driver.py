@@ -161,6 +161,8 @@ class CompiledModel:
         self.proven = bool(proven) and bounds.ok
         self.func = g.func_of(module)
         self.ops = [op for op in self.func.ops if not isinstance(op, g.OutputOp)]
+        if not self.proven and any(isinstance(op, g.ExpertsOp) for op in self.ops):
+            raise ValueError("a graph with experts needs a sound int32 proof: their kernels hold 64 bits and check none of 32")
         outs = [op for op in self.func.ops if isinstance(op, g.OutputOp)]
         if len(outs) != 1:
             raise ValueError("the graph needs exactly one output op")
@@ -347,6 +349,9 @@ class CompiledModel:
         first = {}
         if self.row_programs and hasattr(dev, "row_program"):
             first = {prog.ops[0]: prog for prog in rowprog.find(self, nb)}
+        in_programs = {op for prog in first.values() for op in prog.ops}
+        expert_adds = {op: add for op, add in self._expert_adds(keep).items() if add not in in_programs}
+        P.fused_adds |= set(expert_adds.values())
         done = set()
         for op in self.ops:
             if op in first and rowprog.plan(self, P, first[op], views, nb, keep, step):
@@ -384,6 +389,9 @@ class CompiledModel:
                 continue
             if isinstance(op, g.SoftmaxLutOp):
                 views[r] = self._plan_softmax(P, op, views, out_dims, label, dense, step)
+                continue
+            if isinstance(op, g.ExpertsOp):
+                self._plan_experts(P, op, views, out_dims, label, dense, step, expert_adds.get(op))
                 continue
             out = P.kblocked(out_dims, t.dtype, label) if r in P.kb_values else P.dense(out_dims, t.dtype, label)
             views[r] = out
@@ -448,6 +456,82 @@ class CompiledModel:
         step(label, _call_ptrs, self.dev.softmax_lut, [x, lut, int(op.one), bool(op.causal), batch, t1, t2, out,
                                                        t.dtype, rt.OP_UNCHECKED if sure else 0])
         return out
+
+    def _expert_adds(self, keep) -> dict:
+        """{experts: add_requant} where the residual's add is the only reader of an experts' result and its other operand is computed
+        before it: anvil_expert_combine_i8 takes it. Its sum is bounded there by the operands' dtypes."""
+        found, order = {}, {op: i for i, op in enumerate(self.ops)}
+        for op in self.ops:
+            users = self.users.get(op.results[0], []) if isinstance(op, g.ExpertsOp) else []
+            if keep == "all" or len(users) != 1 or not isinstance(users[0], g.AddRequantOp) or op.result in self.output_values:
+                continue
+            u = users[0]
+            other, ma, mb = (u.b, u.Mb, u.Ma) if u.a is op.result else (u.a, u.Ma, u.Mb)
+            bound = Q.DTYPE_MAG[g.qt(other).dtype] * abs(int(ma)) + 128 * abs(int(mb)) + Q.half(int(u.s))
+            if u.a is not u.b and other not in self.is_const and order[other.owner] < order[op] and bound <= Q.INT32_MAX:
+                found[op] = u
+        return found
+
+    def _expert_weights(self, v):
+        """A const (experts, K, N) stored once as (experts, N, K)."""
+        if v not in self._const_bt:
+            vals = np.asarray(self._host_const(v), dtype=np.int64).reshape(g.qt(v).dims)
+            bt = np.ascontiguousarray(vals.transpose(0, 2, 1)).astype(np.int8)
+            b = Buf(bt.nbytes, f"{v.owner.sym_str}.Bt")
+            b.mem = self.dev.upload(bt)
+            self._const_bt[v] = View(b, "i8", bt.shape, contig_strides(bt.shape))
+        return self._const_bt[v]
+
+    def _expert_calls(self, op, x, scores, rows, buf, add=None, residual=None):
+        """The four calls [(name, device method, arguments)] of an experts op over `rows` rows of x and scores, into buf's values:
+        expert, weight, slot, row, starts, hidden, sorted and out, its result or, with `add`, the sum with `residual`."""
+        (E, C, F), N, top = g.qt(op.up).dims, g.qt(op.down).dims[-1], int(op.top)
+        up, down, act = self._expert_weights(op.up), self._expert_weights(op.down), self._const_views[op.act]
+        pairs, dev = rows * top, self.dev
+        if op.gate is None:
+            first = [up, None, C, C * F, buf["starts"], E, pairs, F, C, buf["hidden"], F, "i8", None, int(op.M), int(op.s), None, 0, 0, act]
+        else:
+            first = [self._expert_weights(op.gate), up, C, C * F, buf["starts"], E, pairs, F, C, buf["hidden"], F, "i8", None, int(op.Mg),
+                     int(op.sg), None, int(op.M), int(op.s), act, int(op.Mm), int(op.sm)]
+        ma, mb, s2, dtype = 0, 0, 0, "i8"
+        if add is not None:
+            ma, mb = (int(add.Mb), int(add.Ma)) if add.a is op.result else (int(add.Ma), int(add.Mb))
+            s2, dtype = int(add.s), g.qt(add.result).dtype
+        r_dtype = "i8" if add is None else g.qt(add.b if add.a is op.result else add.a).dtype
+        return [
+            ("route", dev.expert_route, [scores, E, None, rows, E, top, self._const_views[op.exp], int(op.one), buf["expert"], buf["weight"],
+                                         buf["slot"], buf["row"], buf["starts"]]),
+            ("up", dev.expert_gemm, [x, C, rows, buf["row"], None, *first]),
+            ("down", dev.expert_gemm, [buf["hidden"], F, pairs, None, None, down, None, F, F * N, buf["starts"], E, pairs, N, F, buf["sorted"], N,
+                                       "i8", None, int(op.Md), int(op.sd)]),
+            ("combine", dev.expert_combine, [buf["sorted"], N, pairs, buf["slot"], buf["weight"], rows, top, N, int(op.Mc), int(op.sc), residual,
+                                             r_dtype, N, ma, mb, s2, buf["out"], dtype, N])]
+
+    @staticmethod
+    def _expert_scratch(op) -> dict:
+        """{name: (elements a row, dtype)} of what the calls of an experts op leave between each other, `starts` apart."""
+        top = int(op.top)
+        return {"expert": (top, "i32"), "weight": (top, "i16"), "slot": (top, "i32"), "row": (top, "i32"),
+                "hidden": (top * g.qt(op.up).dims[-1], "i8"), "sorted": (top * g.qt(op.down).dims[-1], "i8")}
+
+    def _plan_experts(self, P, op, views, out_dims, label, dense, step, add):
+        """Route, the two products and the weighted sums, with the residual's add where that alone reads them."""
+        def rows_of(v, what):
+            x = dense(views[v], f"{label}.{what}")
+            return _dense_copy_into(P, step, self.dev, x.prepend(out_dims[0]), f"{label}.{what}") if v in self.is_const else x
+
+        x, scores = rows_of(op.x, "x"), rows_of(op.scores, "scores")
+        rows = math.prod(out_dims[:-1])
+        buf = {n: P.dense((rows * width,), dtype, f"{label}.{n}") for n, (width, dtype) in self._expert_scratch(op).items()}
+        buf["starts"] = P.dense((g.qt(op.up).dims[0] + 1,), "i32", f"{label}.starts")
+        residual = None
+        if add is None:
+            views[op.result] = buf["out"] = P.dense(out_dims, "i8", label)
+        else:
+            residual = dense(views[add.b if add.a is op.result else add.a], f"{label}.residual")
+            views[add.result] = buf["out"] = P.dense(out_dims, g.qt(add.result).dtype, add.sym_str or label)
+        for name, fn, args in self._expert_calls(op, x, scores, rows, buf, add, residual):
+            step(label if name == "combine" else f"{label}.{name}", _call_ptrs, fn, args)
 
     def _attention_chains(self, keep, longest=ATTENTION_MAX) -> dict:
         """{P.V matmul: (scores matmul, softmax)} for every chain qmatmul -> softmax_lut -> qmatmul whose scores and
@@ -1349,6 +1433,15 @@ def _work(fn, args):
         return "lut", 0, 2 * a[2] + 256
     if name == "lut_mul":
         return "lut_mul", 0, 3 * a[5] + 256
+    if name == "expert_route":
+        rows, experts, top = a[3], a[4], a[5]
+        return "route", 0, rows * (experts + 14 * top) + 4 * experts + 1024
+    if name == "expert_gemm":                     # every expert's weights, each row once
+        rows_a, twice, experts, rows, N, K = a[2], 1 if a[6] is None else 2, a[10], a[11], a[12], a[13]
+        return "gemm", 2 * rows * N * K * twice, rows_a * K + experts * N * K * twice + rows * N
+    if name == "expert_combine":
+        rows, top, cols = a[5], a[6], a[7]
+        return "combine", 0, rows * (top * (cols + 6) + cols * (isz[a[17]] + (0 if a[10] is None else isz[a[11]])))
     return name or "other", 0, 0
 
 

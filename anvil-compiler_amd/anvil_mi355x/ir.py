@@ -21,6 +21,10 @@ weights and LUTs are `const` ops bound by sym (or carried inline as `value`).
     add_requant (a, b) {Ma, Mb, s}      -> i8|i16
     transpose (x) {perm}, reshape (x)            layout
     output (values...)
+
+and one op that the reference's dialect has not, a feed-forward part made of experts (ExpertsOp):
+
+    experts (x, scores, up, down, exp, act[, gate]) {top, one, M, s, Md, sd, Mc, sc[, Mg, sg, Mm, sm]} -> i8
 """
 from __future__ import annotations
 
@@ -273,6 +277,40 @@ class AddRequantOp(Op):
         self._check_shift("s")
 
 
+class ExpertsOp(Op):
+    """Each row's `top` experts of largest score (the lowest of equals), weighted by a softmax_lut over the chosen scores:
+        e_j = exp[score_j - largest + 255];  w_j = floor((e_j one + S // 2) / S), S = sum e_j
+        h = act[requant(x @ up[expert], M, s) + 128]
+        with gate:  h = requant(act[requant(x @ gate[expert], Mg, sg) + 128] * requant(x @ up[expert], M, s), Mm, sm)
+        y_j = requant(h @ down[expert], Md, sd);  result = requant(sum_j w_j y_j, Mc, sc)
+    No counterpart in the reference."""
+    name = "anvil.graph.experts"
+    OPERANDS = ("x", "scores", "up", "down", "exp", "act", "gate")
+    OPTIONAL = ("gate",)
+    PROPS = ("top", "one", "M", "s", "Md", "sd", "Mc", "sc", "Mg", "sg", "Mm", "sm")
+
+    def verify(self):
+        x, scores, up, down, r = qt(self.x), qt(self.scores), qt(self.up), qt(self.down), qt(self.result)
+        self._expect(x.dtype == scores.dtype == up.dtype == down.dtype == r.dtype == "i8", "rows, scores, weights and result must be i8")
+        self._expect(len(x.dims) >= 2 and scores.dims[:-1] == x.dims[:-1], f"scores {scores.dims} are not those of rows {x.dims}")
+        E, C = scores.dims[-1], x.dims[-1]
+        self._expect(len(up.dims) == 3 and up.dims[:2] == [E, C], f"up {up.dims}: need ({E}, {C}, width)")
+        self._expect(len(down.dims) == 3 and down.dims[:2] == [E, up.dims[2]], f"down {down.dims}: need ({E}, {up.dims[-1]}, columns)")
+        self._expect(r.dims == x.dims[:-1] + [down.dims[2]], f"result {r.dims} != {x.dims[:-1] + [down.dims[-1]]}")
+        self._expect(self.gate is None or (qt(self.gate).dtype == "i8" and qt(self.gate).dims == up.dims), "gate must be as up")
+        for n in ("up", "down", "exp", "act", "gate"):
+            v = self._operands[n]
+            self._expect(v is None or isinstance(v.owner, ConstOp), f"{n} must be an anvil.graph.const")
+        exp = qt(self.exp)
+        self._expect(exp.dims == [256] and exp.dtype == "i32", "exp LUT must be 256 x i32")
+        self._lut256_i8(self.act)
+        self._expect(1 <= int(self.top) <= min(E, 32) and E <= 1024, f"top={int(self.top)} of {E} experts (at most 32 of 1024)")
+        self._expect(1 <= int(self.one) <= 32767, f"one={int(self.one)} outside [1, 32767]")
+        have = [n for n in ("Mg", "sg", "Mm", "sm") if self.props.get(n) is not None]
+        self._expect(len(have) == (0 if self.gate is None else 4), "Mg, sg, Mm and sm go with a gate")
+        self._check_shift("s", "sd", "sc", *(("sg", "sm") if self.gate is not None else ()))
+
+
 class TransposeOp(Op):
     name = "anvil.graph.transpose"
     OPERANDS = ("x",)
@@ -313,7 +351,7 @@ class OutputOp(Op):
 
 
 OPS = {c.name: c for c in (InputOp, ConstOp, QMatmulOp, QLinearOp, LutOp, LutMulOp, RmsNormIntOp, SoftmaxLutOp,
-                           AddRequantOp, TransposeOp, ReshapeOp, OutputOp)}
+                           AddRequantOp, ExpertsOp, TransposeOp, ReshapeOp, OutputOp)}
 
 
 class FuncOp:
@@ -405,6 +443,14 @@ class GraphBuilder:
     def add_requant(self, sym, a, b, ma, mb, s, scale=None, dtype="i8"):
         return self._add(AddRequantOp({"a": a, "b": b}, {"Ma": int(ma), "Mb": int(mb), "s": int(s)},
                                       QTensorType(qt(a).dims, dtype, scale), sym))
+
+    def experts(self, sym, x, scores, up, down, exp, act, top, one, m, s, md, sd, mc, sc, gate=None, mg=None, sg=None, mm=None, sm=None,
+                scale=None):
+        """ExpertsOp: up and gate are consts (experts, C, width), down (experts, width, columns), exp 256 x i32, act 256 x i8."""
+        ints = {"top": top, "one": one, "M": m, "s": s, "Md": md, "sd": sd, "Mc": mc, "sc": sc, "Mg": mg, "sg": sg, "Mm": mm, "sm": sm}
+        out = qt(x).dims[:-1] + [qt(down).dims[-1]]
+        return self._add(ExpertsOp({"x": x, "scores": scores, "up": up, "down": down, "exp": exp, "act": act, "gate": gate},
+                                   {k: int(v) for k, v in ints.items() if v is not None}, QTensorType(out, "i8", scale), sym))
 
     def transpose(self, sym, x, perm=None, scale=None):
         t = qt(x)

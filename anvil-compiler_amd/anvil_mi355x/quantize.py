@@ -236,7 +236,7 @@ class BoundWalker:
             g.InputOp: self._input, g.ConstOp: self._const, g.QMatmulOp: self._matmul, g.QLinearOp: self._matmul,
             g.LutOp: self._lut, g.LutMulOp: self._lut_mul, g.RmsNormIntOp: self._rmsnorm,
             g.SoftmaxLutOp: self._softmax, g.AddRequantOp: self._add, g.TransposeOp: self._view,
-            g.ReshapeOp: self._view,
+            g.ReshapeOp: self._view, g.ExpertsOp: self._experts,
         }
 
     def _m(self, attr) -> int:
@@ -319,6 +319,30 @@ class BoundWalker:
     def _add(self, op):
         num = self.mag[op.a] * self._m(op.Ma) + self.mag[op.b] * self._m(op.Mb) + half(int(op.s))
         return DTYPE_MAG[g.qt(op.result).dtype], [("requant numerator", num)]
+
+    def _experts(self, op):
+        """The weighted sum's weights add up to `one` and half a unit of rounding each; a gated product is bounded by its dtypes, as the
+        kernel takes it."""
+        exp = self.values[op.exp]
+        if exp.min() < 0 or exp[-1] < 1:
+            raise ValueError(f"{op.sym_str or op.name}: the exp table needs entries >= 0 and a last one >= 1")
+        top, one, largest = int(op.top), int(op.one), self.mag[op.exp]
+        terms = [("sum of exps", top * largest), ("numerator", largest * one + top * largest // 2)]
+
+        def product(what, mag, w, m, s):
+            acc = mag * int(np.abs(self.values[w]).sum(axis=-2).max())
+            terms.extend([(f"{what} accumulator", acc), (f"{what} requant numerator", acc * self._m(m) + half(int(s)))])
+
+        product("up", self.mag[op.x], op.up, op.M, op.s)
+        hidden = self.mag[op.act]
+        if op.gate is not None:
+            product("gate", self.mag[op.x], op.gate, op.Mg, op.sg)
+            terms.append(("gated requant numerator", (1 << 14) * self._m(op.Mm) + half(int(op.sm))))
+            hidden = 128
+        product("down", hidden, op.down, op.Md, op.sd)
+        acc = 128 * (one + top)
+        terms.extend([("weighted sum", acc), ("weighted sum's requant numerator", acc * self._m(op.Mc) + half(int(op.sc)))])
+        return 128, terms
 
     def _view(self, op):
         """A const seen through a transpose or reshape. The reference policy keeps the operand's array as it was

@@ -80,3 +80,28 @@ def combine(Y, slot, weight, mult, shift, R, ma, mb, shift2, dtype):
         acc[have] += np.asarray(weight, dtype=np.int64)[have, j][:, None] * np.asarray(Y, dtype=np.int64)[slot[have, j]]
     y = sem.clamp_i8(rq(acc, mult, shift))
     return y if R is None else sem.clamp_dtype(rq(np.asarray(R, dtype=np.int64) * ma + y * mb, 1, shift2), dtype)
+
+
+def graph_op(x, scores, up, down, exp, act, top, one, m, s, md, sd, mc, sc, gate=None, mg=0, sg=0, mm=0, sm=0, fast=False):
+    """The graph's experts op on rows (..., C) with scores (..., E), every intermediate checked against int32 as the other ops' are."""
+    exp = sem.check_i32(exp, "exp table")
+    if exp.shape != (256,) or exp.min() < 0 or exp[-1] < 1:
+        raise ValueError("the exp table needs 256 entries >= 0 and a last one >= 1")
+    lead = x.shape[:-1]
+    x, scores = x.reshape(-1, x.shape[-1]), sem.check_i8(scores, "scores").reshape(-1, scores.shape[-1])
+    expert = np.argsort(-scores, axis=1, kind="stable")[:, :top]
+    mine = np.take_along_axis(scores, expert, 1)
+    e = exp[mine - mine[:, :1] + 255]
+    S = sem.check_i32(e.sum(axis=1, keepdims=True), "sum of exps")
+    weight = sem.check_i32(e * one + S // 2, "e*one + S/2") // S
+    y = np.zeros((len(x), top, down.shape[-1]), dtype=np.int64)
+    for n in range(len(up)):
+        row, j = np.nonzero(expert == n)
+        if not row.size:
+            continue
+        h = sem.qmatmul(x[row], up[n], m, s, act if gate is None else None, fast=fast)
+        if gate is not None:
+            h = sem.swiglu_lut(sem.qmatmul(x[row], gate[n], mg, sg, fast=fast), h, act, mm, sm)
+        y[row, j] = sem.qmatmul(h, down[n], md, sd, fast=fast)
+    acc = sem.check_i32((weight[:, :, None] * y).sum(axis=1), "weighted sum")
+    return sem.requant(acc, mc, sc).reshape(*lead, -1)

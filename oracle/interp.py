@@ -17,6 +17,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
+from . import experts
 from . import semantics as sem
 
 
@@ -78,6 +79,10 @@ def run(m, inputs: dict, consts: dict | None = None, *, batch: bool = False, fas
             val = sem.softmax_lut(v(op.x), v(op.lut), int(op.one), bool(op.causal))
         elif n == "anvil.graph.add_requant":
             val = sem.add_requant(v(op.a), v(op.b), int(op.Ma), int(op.Mb), int(op.s), op.results[0].type.dtype)
+        elif n == "anvil.graph.experts":
+            gate = {} if op.gate is None else {"gate": v(op.gate), **{k.lower(): int(op.props[k]) for k in ("Mg", "sg", "Mm", "sm")}}
+            val = experts.graph_op(v(op.x), v(op.scores), v(op.up), v(op.down), v(op.exp), v(op.act), int(op.top), int(op.one), int(op.M),
+                                   int(op.s), int(op.Md), int(op.sd), int(op.Mc), int(op.sc), fast=fast, **gate)
         elif n == "anvil.graph.transpose":
             k = 0 if op.x in is_const else nb
             val = np.transpose(v(op.x), list(range(k)) + [p + k for p in op.perm_list])
