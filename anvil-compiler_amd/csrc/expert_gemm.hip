@@ -112,6 +112,27 @@ __device__ __forceinline__ void finish_n(const V& acc, const V& acc2, int m, int
   }
 }
 
+// Columns n .. n + 15 of the result's row p, those there are, at any alignment.
+template <int OSZ>
+__device__ __forceinline__ void store16(const anvil_expert_gemm& g, long long p, int n, const int* v) {
+  char* out = (char*)g.C + (p * g.ldc + n) * OSZ;
+  if (n + 16 <= g.N) {
+    const v4i w0 = OSZ == 1 ? pack16(v) : pack8h(v);
+    __builtin_memcpy(out, &w0, 16);
+    if constexpr (OSZ == 2) {
+      const v4i w1 = pack8h(v + 8);
+      __builtin_memcpy(out + 16, &w1, 16);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (n + e < g.N) {
+      if (OSZ == 1) out[e] = (char)v[e];
+      else ((int16_t*)out)[e] = (int16_t)v[e];
+    }
+}
+
 // the same address in scalar registers (uniform_rsrc)
 __device__ __forceinline__ void* uniform_ptr(const void* p) {
   const unsigned long long a = (unsigned long long)p;
@@ -125,7 +146,8 @@ __device__ __forceinline__ void* uniform_ptr(const void* p) {
 // 256 to 277 us, 1.5 to 1.6 POPS; 65536 of 2048 to 768, 206 GOP, 122 to 134 us. Without its loads 181 and 80 us, without its matrix
 // instructions 205 and 102, without its epilogue 220 and 111 (239 and 118 without the epilogue's stores): loads from L2 cost most, 2.4 GB in
 // lines of which a stage takes half. 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
-// workgroup's products run beside their epilogue; 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
+// workgroup's products run beside their epilogue (283 and 136 where a workgroup walks its tiles and the next one's first stages load
+// under the results; 128 x 256 tiles walked that way 298 and 130); 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
 // (KFULL): selecting an offset past K for each load instead 261 against 257 us.
 // KFULL: K is a whole number of stages, so a load's offset is its lane's own and the stage's, and stages past K have empty descriptors.
 template <int BM, int BN, int BK, int NS, int OSZ, bool GATED, bool KFULL>
@@ -302,22 +324,7 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
         int v[16];
         finish_n<16, OSZ, GATED, decltype(hi_c)::value>(acc[i][j], acc[GATED ? TC + i : i][j], m, m2, q, q2, g.lut != nullptr, lut_s,
                                                         g.mult3, rnd3, g.shift3, v);
-        char* out = (char*)g.C + ((tile.p0 + r) * g.ldc + n) * OSZ;
-        if (n + 16 <= g.N) {                             // one store at any alignment
-          if constexpr (OSZ == 1) {
-            const v4i w = pack16(v);
-            __builtin_memcpy(out, &w, 16);
-          } else {
-            const v4i w0 = pack8h(v), w1 = pack8h(v + 8);
-            __builtin_memcpy(out, &w0, 16);
-            __builtin_memcpy(out + 16, &w1, 16);
-          }
-        } else {
-          for (int e = 0; e < 16 && n + e < g.N; ++e) {
-            if (OSZ == 1) out[e] = (char)v[e];
-            else ((int16_t*)out)[e] = (int16_t)v[e];
-          }
-        }
+        store16<OSZ>(g, tile.p0 + r, n, v);
       }
     }
   };
@@ -464,8 +471,8 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
 }
 
 // Operands at any alignment and stride, and past 2^32 bytes: 64 x 64 tiles, chunks through registers into LDS, the next stage's on their
-// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 17 us (19.7 with
-// one stage at a time).
+// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 12.5 us (17
+// with its results stored a byte at a time, 19.7 with one stage at a time as well).
 template <int OSZ, bool GATED>
 __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   constexpr int BM = 64, BN = 64, BK = 128, NB = GATED ? 2 : 1, PER = BK / 64;
@@ -540,16 +547,14 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   const Requant q1(g.shift, lo, -lo - 1), q2(g.shift2, -128, 127);
   const auto of = [](const Requant& q, int acc, int mul) { return q.high() ? q.of<true>(acc, mul) : q.of<false>(acc, mul); };
   const int rnd3 = (int)round_term(g.shift3);
-  char* out = (char*)g.C + ((tile.p0 + m) * g.ldc + n0) * OSZ;
+  int v[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    int v = of(q1, acc[0][e], mult * scale);
-    if (g.lut) v = lut_s[(v + 128) & 255];
-    if constexpr (GATED) v = min(max((v * of(q2, acc[NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
-    if (n0 + e >= g.N) break;
-    if (OSZ == 1) out[e] = (char)v;
-    else ((int16_t*)out)[e] = (int16_t)v;
+    v[e] = of(q1, acc[0][e], mult * scale);
+    if (g.lut) v[e] = lut_s[(v[e] + 128) & 255];
+    if constexpr (GATED) v[e] = min(max((v[e] * of(q2, acc[NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
   }
+  store16<OSZ>(g, tile.p0 + m, n0, v);
 }
 
 }  // namespace anvil
