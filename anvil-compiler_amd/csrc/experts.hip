@@ -6,7 +6,7 @@
 // Sorting. Workgroups count their rows' pairs by expert; the rows of counts meet in a second launch, where every workgroup adds up all of
 // them and those before its own, and places its pairs. Within a workgroup the waves own runs of consecutive pairs, and a pair's
 // rank among the 64 of a step is the number of lower lanes with its expert (ballots over the bits of its number). Atomics add counts, none
-// decides an order: positions are the same each time. 32749 rows, six of 64 experts each: 9.3 + 7.5 us for 5 MB, chains of reductions and of
+// decides an order: positions are the same each time. 32749 rows, six of 64 experts each: 7.3 + 7.5 us for 5 MB, chains of reductions and of
 // waits for counts, not bandwidth.
 #include <algorithm>
 
@@ -14,13 +14,16 @@
 
 namespace anvil {
 
-constexpr int ROUTE_WAVES = 8, ROUTE_THREADS = 64 * ROUTE_WAVES;
-// Rows of a workgroup, at least, and workgroups, at most: each reads the counts of all. 4096 rows over 8, 64 and 256 experts take 8.4, 9.1
-// and 13.6 us with 32 rows, 11.0, 14.1 and 21.6 with 128.
+// Rows of a workgroup, at least, and workgroups, at most: each reads the counts of all. 4096 rows over 8 (two each), 64
+// (six) and 256 experts (eight) take 9.6, 9.6 and 12.8 us with 32 rows, 11.0, 13.0 and 20.4 with 128.
 constexpr int ROUTE_ROWS = 32, ROUTE_BLOCKS = 256;
-// Rows that one workgroup routes and sorts by itself: 64 rows over 8, 64 and 256 experts take it 5.8, 6.7 and 9.8 us, 128 rows 6.8, 8.6 and
-// 14.4; two launches take 256 rows in 7.8, 8.2 and 11.0.
+// Rows that one workgroup routes and sorts by itself: 64 rows over 8, 64 and 256 experts take it 5.8, 6.7 and 9.7 us, 128 rows 6.8, 8.6 and
+// 14.2; two launches take 128 rows in 8.9, 8.9 and 9.9.
 constexpr int ROUTE_ONE = 64;
+
+// Rows of a workgroup that take sixteen waves, not eight: 32768 rows over 8, 64, 256 and 1024 experts (four each) take 12.3, 14.8, 25.0 and
+// 73 us with them, 12.0, 15.9, 27.6 and 99 with eight.
+constexpr int ROUTE_WIDE = 64;
 
 struct RouteArgs {
   anvil_route r;
@@ -190,33 +193,33 @@ __global__ __launch_bounds__(1024) void route_one(RouteArgs g) {
 
 // Many rows, first launch: each workgroup's experts and weights, and its counts.
 template <int L, int PER>
-__global__ __launch_bounds__(ROUTE_THREADS) void route_choose(RouteArgs g) {
+__global__ __launch_bounds__(1024) void route_choose(RouteArgs g) {
   __shared__ int count[L * PER];
-  for (int e = threadIdx.x; e < L * PER; e += ROUTE_THREADS) count[e] = 0;
+  for (int e = threadIdx.x; e < L * PER; e += blockDim.x) count[e] = 0;
   __syncthreads();
   const long long first = (long long)blockIdx.x * g.block_rows;
   choose_rows<L, PER>(g, first, (int)min((long long)g.block_rows, g.r.rows - first), nullptr, count);
   __syncthreads();
-  for (int e = threadIdx.x; e < g.r.experts; e += ROUTE_THREADS) g.counts[(long long)blockIdx.x * g.r.experts + e] = count[e];
+  for (int e = threadIdx.x; e < g.r.experts; e += blockDim.x) g.counts[(long long)blockIdx.x * g.r.experts + e] = count[e];
 }
 
 // Second launch: every workgroup adds up the counts of all, and of those before it, and places its pairs. LDS: totals, those before,
 // bases, a row of experts a wave.
-__global__ __launch_bounds__(ROUTE_THREADS) void route_place(RouteArgs g) {
+__global__ __launch_bounds__(1024) void route_place(RouteArgs g) {
   extern __shared__ int lds[];
-  __shared__ int sums[ROUTE_WAVES];
+  __shared__ int sums[16];
   const anvil_route& r = g.r;
   const int E = r.experts;
   int *total = lds, *before = lds + E, *base = before + E, *at = base + E;
-  for (int e = threadIdx.x; e < (3 + ROUTE_WAVES) * E; e += ROUTE_THREADS) lds[e] = 0;
+  for (int e = threadIdx.x; e < (3 + (int)(blockDim.x >> 6)) * E; e += blockDim.x) lds[e] = 0;
   __syncthreads();
-  // thread t: expert t % pitch, workgroups t / pitch, + ROUTE_THREADS / pitch, ...
-  const int pitch = min(ROUTE_THREADS, (E + 63) / 64 * 64);
-  const int parts = ROUTE_THREADS / pitch, part = threadIdx.x / pitch;
+  // thread t: expert t % pitch, workgroups t / pitch, + blockDim.x / pitch, ...
+  const int pitch = min((int)blockDim.x, (E + 63) / 64 * 64);
+  const int parts = (int)blockDim.x / pitch, part = threadIdx.x / pitch;
   if (part < parts)
     for (int e = threadIdx.x % pitch; e < E; e += pitch) {
       int all = 0, prior = 0;
-#pragma unroll 8
+#pragma unroll 16
       for (int b = part; b < g.blocks; b += parts) {
         const int c = g.counts[(long long)b * E + e];
         all += c;
@@ -376,6 +379,7 @@ extern "C" int anvil_expert_route_i8(anvil_ctx* ctx, const anvil_route* r) {
   const int waves = std::max(1, std::min(16, (r->rows * lanes + 63) / 64));
   const size_t lds_one = (2 + waves) * E + (size_t)r->rows * r->top * sizeof(int);
   const bool one = r->rows <= ROUTE_ONE && lds_one <= 60 << 10;
+  const int wide = block_rows >= ROUTE_WIDE ? 16 : 8, placing = (3 + wide) * E <= 60 << 10 ? wide : 8;
   if (!one) {
     char* ws;
     if (int e = decode_workspace(ctx, g.blocks * E, &ws)) return e;
@@ -387,8 +391,8 @@ extern "C" int anvil_expert_route_i8(anvil_ctx* ctx, const anvil_route* r) {
       ANVIL_LAUNCH((route_one<L, PER>), dim3(1), dim3(64 * waves), lds_one, ctx->stream, g);
       return;
     }
-    ANVIL_LAUNCH((route_choose<L, PER>), dim3((unsigned)g.blocks), dim3(ROUTE_THREADS), 0, ctx->stream, g);
-    ANVIL_LAUNCH(route_place, dim3((unsigned)g.blocks), dim3(ROUTE_THREADS), (3 + ROUTE_WAVES) * E, ctx->stream, g);
+    ANVIL_LAUNCH((route_choose<L, PER>), dim3((unsigned)g.blocks), dim3(64 * wide), 0, ctx->stream, g);
+    ANVIL_LAUNCH(route_place, dim3((unsigned)g.blocks), dim3(64 * placing), (3 + placing) * E, ctx->stream, g);
   };
   using std::integral_constant;
   if (lanes == 16) {
