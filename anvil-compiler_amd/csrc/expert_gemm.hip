@@ -45,6 +45,7 @@ __device__ __forceinline__ bool find_tile(const ExpertArgs& a, int w, int lane, 
     n = e0 + lane < E ? expert_rows(a, e0 + lane, w == 0, lo) : 0;
     mt += (n + BM - 1) / BM;
   }
+  if (__ballot(mt > (int)GRID_MAX)) return false;        // starts that decrease may count positions again, past what the sums hold
   int incl = wave_scan(mt);
   const int tiles_m = __builtin_amdgcn_readlane(incl, 63);
   const unsigned tiles = (unsigned)tiles_m * (unsigned)a.tiles_n;        // at most the grid
@@ -149,7 +150,8 @@ __device__ __forceinline__ void* uniform_ptr(const void* p) {
 // workgroup's products run beside their epilogue (283 and 136 where a workgroup walks its tiles and the next one's first stages load
 // under the results; 128 x 256 tiles walked that way 298 and 130); 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
 // (KFULL): selecting an offset past K for each load instead 261 against 257 us.
-// KFULL: K is a whole number of stages, so a load's offset is its lane's own and the stage's, and stages past K have empty descriptors.
+// KFULL: K is a whole number of stages, so a load's offset is its lane's own and the stage's, which lies within the descriptor's bytes (the range
+// check subtracts it from them); stages past K have empty descriptors and no offset.
 template <int BM, int BN, int BK, int NS, int OSZ, bool GATED, bool KFULL>
 __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
   constexpr int T = 256, NW = 4, WGN = 2, CPR = BK / 16, KS = BK / 32;
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
   // chunks past K load zeros; a stage past K is issued all the same, which keeps the wait counts fixed
   auto load = [&](__amdgpu_buffer_rsrc_t r, int8_t* s, unsigned off, int k, int k0) {
     if constexpr (KFULL)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)s, 16, off, k0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)s, 16, off, k0 < K ? k0 : 0, 0, 0);
     else
       dma16(r, s, k0 + k < K ? off + k0 : OOB);
   };
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
 #undef ANVIL_EXPERT_STEP
 
   Requant q(shift, OSZ == 1 ? -128 : -32768, OSZ == 1 ? 127 : 32767), q2(shift2, -128, 127);
-  const bool high = q.high() && (!GATED || q2.high());
+  const bool high = q.high() && q.rest <= 24 && (!GATED || q2.high());   // 24: the table's index is eight bits of an int
   if (!high) q.rest = q2.rest = 0;                       // the 64-bit form shifts by all of it
   const int rnd3 = (int)round_term(g.shift3);
   constexpr int TC = GATED ? TN / 2 : TN;                // column groups of 32 a wave has of the result
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
       for (int m = 0; m < MT; ++m) sums[wave][(m * CT + c) * NB + b][lane] = acc[b][c][m];
   __syncthreads();
   Requant q(shift, OSZ == 1 ? -128 : -32768, OSZ == 1 ? 127 : 32767), q2(shift2, -128, 127);
-  const bool high = q.high() && (!GATED || q2.high());
+  const bool high = q.high() && q.rest <= 24 && (!GATED || q2.high());   // 24: the table's index is eight bits of an int
   if (!high) q.rest = q2.rest = 0;
   const int rnd3 = (int)round_term(g.shift3);
 #pragma unroll
@@ -628,9 +630,9 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
       if (wgs) ANVIL_LAUNCH((expert_few<MT, CT, decltype(osz)::value, GATED>), dim3(wgs), dim3(256), 0, ctx->stream, a);
     });
   };
-  if (aligned16(g->A) && aligned16(g->B) && aligned16(g->B2) && g->K % 16 == 0 && g->lda % 16 == 0 && g->ldb % 16 == 0 && g->sb % 16 == 0 &&
-      a_bytes <= (long long)PAST && g->ldb < 1 << 23) {
-    a.a_bytes = (int)(unsigned)std::max(0ll, a_bytes);
+  if (aligned16(g->A) && aligned16(g->B) && aligned16(g->B2) && g->K % 16 == 0 && g->lda % 16 == 0 && g->ldb % 16 == 0 &&
+      (g->experts == 1 || g->sb % 16 == 0) && g->rows_a && a_bytes <= (long long)PAST && g->ldb < 1 << 23) {
+    a.a_bytes = (int)(unsigned)a_bytes;
     using std::integral_constant;
     const integral_constant<int, 128> i128;
     const integral_constant<int, 64> i64;
@@ -643,7 +645,7 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
     //     of them is half empty, and a short K has little to make up for it
     const long long width = (long long)g->N * (g->B2 ? 2 : 1);                         // of the operand B, and B2 beside it
     const long long large = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((width + 255) / 256);
-    if (g->rows * width * g->K <= 1 << 28) {
+    if ((double)g->rows * (double)width * g->K <= 1 << 28) {
       if (g->rows <= 8ll * g->experts) few(integral_constant<int, 1>{});
       else few(integral_constant<int, 2>{});
     } else if (large >= (g->K >= 2048 ? 3 : 5) * ctx->num_cu / 2) {

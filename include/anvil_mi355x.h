@@ -527,8 +527,8 @@ int anvil_beam_select_i8(anvil_ctx* ctx, const anvil_beams* b);
  *   (i, k) = rsqrt_index(eps + sum r_c^2), the sum in 64 bits (reference anvil/codegen/lower.py:107-113)
  *   scale = min(32767, rq(a * lut[i], 1, lut_shift + k))
  * The norm's factor 1 / rms is one for a whole row, so it cancels in the codes and is part of the scale alone: code_c stands
- * for code_c * scale in units that lut and lut_shift set. x, y and r are i8 or i16; cols at most 65536; ma * x + mb * y +
- * 2^(shift-1) fits int32 for every x and y of their dtypes, else ANVIL_E_OVERFLOW. lut: lut_len int32s, negative ones count as
+ * for code_c * scale in units that lut and lut_shift set. x, y and r are i8 or i16; cols at most 65536; |ma x| +
+ * |mb y| + 2^(shift-1) < 2^31 for every x and y of their dtypes, else ANVIL_E_OVERFLOW. lut: lut_len int32s, negative ones count as
  * 0; 2 <= lut_len <= 65536; eps >= 0; shift and lut_shift in [0, 31]. R may be X or Y itself (of R's dtype and stride). */
 typedef struct anvil_add_norm {
   const void* X;
@@ -606,7 +606,7 @@ int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g);
  *   y_c = clamp_i8(rq(sum_j weight[i][j] * Y[slot[i][j]][c], mult, shift)), a slot of -1 adding nothing
  *   D[i][c] = clamp_d(rq(R[i][c] * ma + y_c * mb, 1, shift2)); with R NULL D = y (int8; ma, mb and shift2 are not used)
  * Y has `positions` rows. A slot outside [-1, positions) adds nothing and is reported by anvil_sync as ANVIL_E_VALUE. R and D are i8
- * or i16, and D may be R itself (of R's dtype and stride); R * ma + y * mb + 2^(shift2-1) fits int32 for every R and y of their dtypes, else
+ * or i16, and D may be R itself (of R's dtype and stride); |R ma| + |y mb| + 2^(shift2-1) < 2^31 for every R and y of their dtypes, else
  * ANVIL_E_OVERFLOW; shift in [0, 62], shift2 in [0, 31]; top and rows as the router's, cols at most 2^20. */
 typedef struct anvil_expert_combine {
   const int8_t* Y;

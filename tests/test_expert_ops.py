@@ -475,6 +475,60 @@ def test_product_multipliers_and_shifts(mults):
 
 
 @gpu
+@pytest.mark.parametrize("rows,N,K", [(20, 64, 8192), (520, 256, 8192), (300, 70, 8190)], ids=["few", "tiles", "any"])
+@pytest.mark.parametrize("kind", ["table", "gated"])
+def test_tables_behind_the_largest_shifts(rows, N, K, kind):
+    """Sums near 2^27 times multipliers near 2^31: results of a few units either way at shifts up to 58."""
+    dev, rng = device(), np.random.default_rng(K)
+    A, B = rng.integers(100, 128, (rows, K)), rng.integers(90, 128, (2, N, K)) * rng.choice([-1, 1], (2, N, 1))
+    lut = rng.permutation(256) - 128
+    dA, dB, dB2, out = Rows(dev, A, "i8"), Rows(dev, B[0], "i8"), Rows(dev, B[1], "i8"), Rows(dev, np.zeros((rows, N), int), "i8")
+    dt, dl, m, start = flat(dev, [0, rows], "i32"), flat(dev, lut, "i8"), 2 ** 31 - 1, [0, rows]
+    for shift in (55, 56, 57, 58):
+        gated = kind == "gated"
+        want = oe.gemm(np.zeros((rows, N)), A, None, None, B[:1], B[1:] if gated else None, start, [m], shift, [-m], shift, lut, 20, 3, "i8")
+        assert len(np.unique(want)) > 1
+        dev.expert_gemm(dA.ptr, dA.ld, rows, None, None, dB.ptr, dB2.ptr if gated else None, dB.ld, 0, dt.ptr, 1, rows, N, K, out.ptr, out.ld, "i8",
+                        mult=m, shift=shift, mult2=-m, shift2=shift, lut=dl.ptr, mult3=20, shift3=3)
+        dev.sync()
+        out.expect(want, f"shift {shift}")
+
+
+@gpu
+@pytest.mark.parametrize("experts,N,K", [(9, 1024, 1024), (9, 1024, 1040), (90, 2048, 192), (90, 2048, 80)])
+def test_rows_out_of_range_in_tiles_count_as_zeros(experts, N, K):
+    def call(dev, run, args, want, dC, keep):
+        row, want = keep[3].get()[0], want.copy()
+        for p, bad in ((0, -1), (77, args["rows_a"]), (300, 2 ** 31 - 1), (301, -(2 ** 31))):
+            row[p], want[p] = bad, 0
+        dr = flat(dev, row, "i32")
+        dev.expert_gemm(**{**args, "row": dr.ptr})
+        with pytest.raises(ValueError, match="expert"):
+            dev.sync()
+        dev.sync()
+        dC.expect(want)
+
+    product_case([70 + 3 * e for e in range(experts)], N, K, call=call)
+
+
+@gpu
+def test_products_of_no_rows_at_all():
+    """rows_a 0: every position's row leaves its range, and nothing of A is read."""
+    def call(dev, run, args, want, dC, keep):
+        for row in (args["row"], None):
+            dev.expert_gemm(**{**args, "rows_a": 0, "A": None, "row": row})
+            with pytest.raises(ValueError, match="expert"):
+                dev.sync()
+            dev.sync()
+            want = want.copy()
+            want[:sum(counts)] = 0
+            dC.expect(want)
+
+    for counts in ([3, 8], [130, 200, 300]):
+        product_case(counts, 640, 1024, call=call)
+
+
+@gpu
 def test_product_of_large_strides():
     """Weights and rows past 2^32 bytes: the fourth expert lies behind 6 GiB, the last rows behind 5."""
     dev, rng = device(), np.random.default_rng(0)
