@@ -296,6 +296,7 @@ class ExpertsOp(Op):
         E, C = scores.dims[-1], x.dims[-1]
         self._expect(len(up.dims) == 3 and up.dims[:2] == [E, C], f"up {up.dims}: need ({E}, {C}, width)")
         self._expect(len(down.dims) == 3 and down.dims[:2] == [E, up.dims[2]], f"down {down.dims}: need ({E}, {up.dims[-1]}, columns)")
+        self._expect(max(C, up.dims[2]) <= 1 << 16 and down.dims[2] <= 1 << 20, f"sums of {C} and {up.dims[2]} products (at most 65536)")
         self._expect(r.dims == x.dims[:-1] + [down.dims[2]], f"result {r.dims} != {x.dims[:-1] + [down.dims[-1]]}")
         self._expect(self.gate is None or (qt(self.gate).dtype == "i8" and qt(self.gate).dims == up.dims), "gate must be as up")
         for n in ("up", "down", "exp", "act", "gate"):

@@ -87,8 +87,8 @@ def graph_op(x, scores, up, down, exp, act, top, one, m, s, md, sd, mc, sc, gate
     exp = sem.check_i32(exp, "exp table")
     if exp.shape != (256,) or exp.min() < 0 or exp[-1] < 1:
         raise ValueError("the exp table needs 256 entries >= 0 and a last one >= 1")
-    lead = x.shape[:-1]
-    x, scores = x.reshape(-1, x.shape[-1]), sem.check_i8(scores, "scores").reshape(-1, scores.shape[-1])
+    lead = np.broadcast_shapes(x.shape[:-1], scores.shape[:-1])    # a const is the same in every batch
+    x, scores = (np.broadcast_to(v, (*lead, v.shape[-1])).reshape(-1, v.shape[-1]) for v in (x, sem.check_i8(scores, "scores")))
     expert = np.argsort(-scores, axis=1, kind="stable")[:, :top]
     mine = np.take_along_axis(scores, expert, 1)
     e = exp[mine - mine[:, :1] + 255]

@@ -200,3 +200,48 @@ def test_a_token_model_and_its_decoder(gated):
     prompts = prompts_of(SPEC, [1, 20, 7], 3)
     for beams in (1, 2):
         same(dec.generate(prompts, 9, beams=beams), oracle.generate(prompts, 9, beams))
+
+
+@pytest.mark.parametrize("C,width", [(65552, 8), (8, 65537)])
+def test_sums_longer_than_the_kernels_take_are_refused(C, width):
+    b = g.GraphBuilder("long")
+    x, scores, up, down = b.input("x", [1, C], "i8"), b.input("s", [1, 2], "i8"), b.const("u", [2, C, width], "i8"), b.const("d", [2, width, 4], "i8")
+    with pytest.raises(g.VerifyException, match="65536"):
+        b.experts("y", x, scores, up, down, b.const("e", [256], "i32"), b.const("a", [256], "i8"), 1, 127, 1, 20, 1, 20, 1, 7)
+
+
+# --------------------------------------------------------------------------------- operands that are shared
+
+def _shared():
+    """One input as rows and as scores of two experts ops with the same consts, whose results meet in an add; the first is an output
+    too, and its weights are a batch product's right operand as well. A third op's rows and a fourth's scores are consts."""
+    E, C, width, T = 16, 16, 32, 6
+    b, feed = g.GraphBuilder("shared"), eg.Feed("f", C, width, C, E, 3, True, 4)
+    rng = np.random.default_rng(9)
+    consts = {k: v for k, v in feed.values().items() if not k.endswith("router")}
+    consts["rows"] = rng.integers(-128, 128, (T, C))
+    x, each = b.input("x", [T, C], "i8", 0.05), b.input("each", [E, T, C], "i8", 0.05)
+    c = {k: b.const(k, list(v.shape), "i32" if k == "f.exp" else "i8") for k, v in consts.items()}
+
+    def part(sym, x, scores):
+        return b.experts(sym, x, scores, c["f.up"], c["f.down"], c["f.exp"], c["f.act"], 3, feed.one, gate=c["f.gate"], **feed.args)
+
+    y1 = part("y1", x, x)
+    y2 = part("y2", y1, x)
+    y3, y4 = part("y3", c["rows"], x), part("y4", x, c["rows"])
+    m, s = eg.requant(45, 74 * 40 * np.sqrt(C), 128 * int(np.abs(consts["f.up"]).sum(axis=1).max()))
+    z = b.qmatmul("z", each, c["f.up"], m, s)
+    b.output(b.add_requant("both", y1, y2, 60, 70, 6, 0.05), y1, b.add_requant("third", y3, x, 60, 70, 6, 0.05), y4, z)
+    return b.module(), consts
+
+
+@pytest.mark.parametrize("keep", ["outputs", "all"])
+def test_shared_operands_on_the_stand_in(fake, keep):
+    _check(*_shared(), 3, keep)
+
+
+@gpu
+@pytest.mark.parametrize("keep", ["outputs", "all"])
+def test_shared_operands(keep):
+    cm = _check(*_shared(), 3, keep)
+    assert cm.proven
