@@ -662,6 +662,66 @@ def test_slots_out_of_range_are_reported_and_add_nothing():
         assert D.get()[:, :cols].tolist() == [[50] * cols, [50] * cols, [100] * cols]
 
 
+@gpu
+def test_rows_past_four_gib():
+    """Norm, router and weighted sums over rows 5 MiB and more apart: the last of them lie past 2^32 bytes."""
+    dev, rng = device(), np.random.default_rng(0)
+    n, ld, cols = 1000, 5 << 20, 64
+    big = dev.alloc((n - 1) * ld + 4096)
+    some = np.array([0, 1, 409, 410, 819, 820, n - 1])                        # 820 x 5 MiB is the first past 2^32
+
+    def put(values):
+        for i, v in zip(some, values):
+            big.upload(v, int(i) * ld)
+
+    def get(n, dtype):
+        return np.stack([big.download((n,), dtype, int(i) * ld) for i in some]).astype(np.int64)
+
+    big_zero = np.zeros(cols, np.int16)
+    for i in range(n):
+        big.upload(big_zero, i * ld)
+    # the norm, in place: x + y over x
+    x, y, w = np.zeros((n, cols), int), rng.integers(-128, 128, (n, cols)), rng.integers(30, 128, cols)
+    x[some] = rng.integers(-9000, 9000, (len(some), cols))
+    put(x[some].astype(np.int16))
+    dy, dw, dl = Rows(dev, y, "i8"), flat(dev, w, "i8"), flat(dev, roots(), "i32")
+    dh, ds = Rows(dev, np.zeros((n, cols), int), "i8"), flat(dev, np.zeros(n, int), "i16")
+    dev.add_norm(big.ptr, "i16", ld // 2, dy.ptr, "i8", cols, 256, 900, 8, big.ptr, "i16", ld // 2, dw.ptr, dl.ptr, 1024, 7, 10, dh.ptr, cols,
+                 ds.ptr, n, cols)
+    dev.sync()
+    r, h, scale = oe.add_norm(x, y, 256, 900, 8, "i16", w, roots(), 7, 10)
+    dh.expect(h)
+    ds.expect(scale[None])
+    assert np.array_equal(get(cols, np.int16), r[some])
+    # the router
+    scores = np.zeros((n, 8), int)
+    scores[some] = rng.integers(-100, 100, (len(some), 8))
+    for i in range(n):
+        big.upload(scores[i].astype(np.int8), i * ld)
+    expert, weight, slot, row, starts = oe.route(scores, None, 2, exp_lut(), 127)
+    de, dw2, dslot = (Rows(dev, np.zeros((n, 2), int), t) for t in ("i32", "i16", "i32"))
+    dr, dt, de_lut = flat(dev, np.zeros(2 * n, int), "i32"), flat(dev, np.zeros(9, int), "i32"), flat(dev, exp_lut(), "i32")
+    dev.expert_route(big.ptr, ld, None, n, 8, 2, de_lut.ptr, 127, de.ptr, dw2.ptr, dslot.ptr, dr.ptr, dt.ptr)
+    dev.sync()
+    for got, want in ((de, expert), (dw2, weight), (dslot, slot), (dr, row[None]), (dt, starts[None])):
+        got.expect(want)
+    # weighted sums of the rows, and then into them
+    Y = rng.integers(-128, 128, (len(some), cols))
+    put(Y.astype(np.int8))
+    pick = rng.integers(0, len(some), (30, 2))
+    d1, wt = Rows(dev, np.zeros((30, cols), int), "i8"), rng.integers(0, 128, (30, 2))
+    dp, dwt = flat(dev, some[pick], "i32"), flat(dev, wt, "i16")
+    dev.expert_combine(big.ptr, ld, n, dp.ptr, dwt.ptr, 30, 2, cols, 3, 9, None, "i8", 0, 0, 0, 0, d1.ptr, "i8", cols)
+    dev.sync()
+    d1.expect(oe.combine(Y, pick, wt, 3, 9, None, 0, 0, 0, "i8"))
+    slot = rng.integers(0, 30, (n, 2))
+    dp, dwt = flat(dev, slot, "i32"), flat(dev, np.tile(wt, (34, 1))[:n], "i16")
+    y1 = d1.get()
+    dev.expert_combine(d1.ptr, cols, 30, dp.ptr, dwt.ptr, n, 2, cols, 3, 9, None, "i8", 0, 0, 0, 0, big.ptr, "i8", ld)
+    dev.sync()
+    assert np.array_equal(get(cols, np.int8), oe.combine(y1, slot, np.tile(wt, (34, 1))[:n], 3, 9, None, 0, 0, 0, "i8")[some])
+
+
 # ---------------------------------------------------------------------------------- a whole feed-forward (GPU)
 
 class Layer:
