@@ -92,45 +92,63 @@ __device__ __forceinline__ bool expert_mult(const ExpertArgs& a, const int* mult
   return false;
 }
 
-// A lane's results: n accumulators of one row (and n of the gate's partner) as n values of the result's dtype.
+// What follows a product's requants: the table, the gated product and the bounds of its value before its shift.
+struct Epilogue {
+  WideRequant q, q2;
+  bool high, lut;
+  int mult3, rnd3, shift3, clo3, chi3;
+  __device__ __forceinline__ Epilogue(const anvil_expert_gemm& g, int shift, int shift2, int lo)
+      : q(shift, lo, -lo - 1), q2(shift2, -128, 127), lut(g.lut != nullptr), mult3(g.mult3), rnd3((int)round_term(g.shift3)), shift3(g.shift3) {
+    high = q.high() && q.rest <= 24 && (!g.B2 || q2.high());                   // 24: the table's index is eight bits of an int
+    if (!high) q.rest = q2.rest = 0;                     // the 64-bit form shifts by all of it
+    clo3 = shift3 < 24 ? -128 * (1 << shift3) : (int)I32_MIN;
+    chi3 = shift3 < 24 ? 128 * (1 << shift3) - 1 : (int)I32_MAX;
+  }
+};
+
+// A lane's results: n accumulators of one row (and n of the gate's partner) as n values of the result's dtype in words.
 template <int n, int OSZ, bool GATED, bool HI, typename V>
-__device__ __forceinline__ void finish_n(const V& acc, const V& acc2, int m, int m2, const Requant& q, const Requant& q2, bool lut,
-                                         const int8_t* lut_s, int mult3, int rnd3, int shift3, int* v) {
+__device__ __forceinline__ void finish_n(const V& acc, const V& acc2, int m, int m2, const Epilogue& p, const int8_t* lut_s, unsigned* w) {
+  int v[n];
 #pragma unroll
   for (int e = 0; e < n; ++e) {
-    const int x = q.unshifted<HI>(acc[e], m);
-    if (OSZ == 1 && (GATED || lut)) {
-      const int t = lut_s[__builtin_amdgcn_ubfe((unsigned)x, (unsigned)q.rest, 8u)];          // rotated: the entry of v at index v & 255
-      if constexpr (GATED) {
-        const int u = q2.unshifted<HI>(acc2[e], m2) >> q2.rest;
-        v[e] = med3i((__mul24(__mul24(t, u), mult3) + rnd3) >> shift3, -128, 127);
-      } else {
-        v[e] = t;
-      }
+    v[e] = p.q.unshifted<HI>(acc[e], m);
+    if (OSZ == 1 && (GATED || p.lut)) v[e] = lut_s[__builtin_amdgcn_ubfe((unsigned)v[e], (unsigned)p.q.rest, 8u)];      // rotated: v at index v & 255
+    if constexpr (GATED) {
+      const int u = p.q2.unshifted<HI>(acc2[e], m2) >> p.q2.rest;
+      v[e] = med3i(mad_i24v(__mul24(v[e], u), p.mult3, p.rnd3), p.clo3, p.chi3);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < n / 4; ++q) {
+    int* x = v + 4 * q;
+    if constexpr (OSZ == 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[2 * q + h] = __builtin_amdgcn_perm((unsigned)(x[2 * h + 1] >> p.q.rest), (unsigned)(x[2 * h] >> p.q.rest), 0x05040100u);
+    } else if (GATED) {
+      w[q] = sra_pack4(x[0], x[1], x[2], x[3], p.shift3);
+    } else if (p.lut) {
+      w[q] = pack4(x[0], x[1], x[2], x[3]);
     } else {
-      v[e] = x >> q.rest;
+      w[q] = sra_pack4(x[0], x[1], x[2], x[3], p.q.rest);
     }
   }
 }
 
-// Columns n .. n + 15 of the result's row p, those there are, at any alignment.
-template <int OSZ>
-__device__ __forceinline__ void store16(const anvil_expert_gemm& g, long long p, int n, const int* v) {
-  char* out = (char*)g.C + (p * g.ldc + n) * OSZ;
-  if (n + 16 <= g.N) {
-    const v4i w0 = OSZ == 1 ? pack16(v) : pack8h(v);
-    __builtin_memcpy(out, &w0, 16);
-    if constexpr (OSZ == 2) {
-      const v4i w1 = pack8h(v + 8);
-      __builtin_memcpy(out + 16, &w1, 16);
-    }
+// Columns c .. c + n - 1 of the result's row p, those there are, at any alignment: n values in words.
+template <int n, int OSZ>
+__device__ __forceinline__ void store_n(const anvil_expert_gemm& g, long long p, int c, const unsigned* w) {
+  char* out = (char*)g.C + (p * g.ldc + c) * OSZ;
+  if (c + n <= g.N) {
+    __builtin_memcpy(out, w, n * OSZ);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 16; ++e)
-    if (n + e < g.N) {
-      if (OSZ == 1) out[e] = (char)v[e];
-      else ((int16_t*)out)[e] = (int16_t)v[e];
+  for (int e = 0; e < n; ++e)
+    if (c + e < g.N) {
+      if (OSZ == 1) out[e] = (char)(w[e >> 2] >> (8 * (e & 3)));
+      else ((int16_t*)out)[e] = (int16_t)(w[e >> 1] >> (16 * (e & 1)));
     }
 }
 
@@ -163,7 +181,7 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
   constexpr int STAGE = (BM + BN) * BK;
   __shared__ __attribute__((aligned(1024))) int8_t L0[STAGE], L1[STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t L2[NS > 2 ? STAGE : 16], L3[NS > 3 ? STAGE : 16];
-  __shared__ int8_t lut_s[256];
+  __shared__ __attribute__((aligned(2048))) int8_t lut_s[256];            // before the stages, where a read's own offset reaches it
   auto arr = [&](auto u) -> int8_t* {                    // the array of stage u, known at compile time
     constexpr int U = decltype(u)::value % NS;
     if constexpr (U == 0) return L0;
@@ -308,10 +326,7 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
   }
 #undef ANVIL_EXPERT_STEP
 
-  Requant q(shift, OSZ == 1 ? -128 : -32768, OSZ == 1 ? 127 : 32767), q2(shift2, -128, 127);
-  const bool high = q.high() && q.rest <= 24 && (!GATED || q2.high());   // 24: the table's index is eight bits of an int
-  if (!high) q.rest = q2.rest = 0;                       // the 64-bit form shifts by all of it
-  const int rnd3 = (int)round_term(g.shift3);
+  const Epilogue ep(g, shift, shift2, OSZ == 1 ? -128 : -32768);
   constexpr int TC = GATED ? TN / 2 : TN;                // column groups of 32 a wave has of the result
   auto finish = [&](auto hi_c) {
 #pragma unroll
@@ -323,14 +338,13 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
       for (int i = 0; i < TC; ++i) {
         const int n = tile.n0 + (wn * TC + i) * 32 + 16 * half;
         if (n >= g.N) continue;
-        int v[16];
-        finish_n<16, OSZ, GATED, decltype(hi_c)::value>(acc[i][j], acc[GATED ? TC + i : i][j], m, m2, q, q2, g.lut != nullptr, lut_s,
-                                                        g.mult3, rnd3, g.shift3, v);
-        store16<OSZ>(g, tile.p0 + r, n, v);
+        unsigned w[4 * OSZ];
+        finish_n<16, OSZ, GATED, decltype(hi_c)::value>(acc[i][j], acc[GATED ? TC + i : i][j], m, m2, ep, lut_s, w);
+        store_n<16, OSZ>(g, tile.p0 + r, n, w);
       }
     }
   };
-  if (high) finish(std::true_type{});
+  if (ep.high) finish(std::true_type{});
   else finish(std::false_type{});
   wait_vmcnt(0);                                         // the trailing zero loads land before the LDS is released
 }
@@ -431,10 +445,7 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) sums[wave][(m * CT + c) * NB + b][lane] = acc[b][c][m];
   __syncthreads();
-  Requant q(shift, OSZ == 1 ? -128 : -32768, OSZ == 1 ? 127 : 32767), q2(shift2, -128, 127);
-  const bool high = q.high() && q.rest <= 24 && (!GATED || q2.high());   // 24: the table's index is eight bits of an int
-  if (!high) q.rest = q2.rest = 0;
-  const int rnd3 = (int)round_term(g.shift3);
+  const Epilogue ep(g, shift, shift2, OSZ == 1 ? -128 : -32768);
 #pragma unroll
   for (int i = 0; i < MT * CT; ++i) {                    // block i of 16 x 16: wave i % 4
     if (i % 4 != wave) continue;
@@ -444,31 +455,13 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) x[b] = sums[0][i * NB + b][lane] + sums[1][i * NB + b][lane] + sums[2][i * NB + b][lane] + sums[3][i * NB + b][lane];
     const int sc = scale[i / CT];
-    int v[4];
+    unsigned w[OSZ];
     const auto finish = [&](auto hi_c) {
-      finish_n<4, OSZ, GATED, decltype(hi_c)::value>(x[0], x[NB - 1], mult * sc, mult2 * sc, q, q2, g.lut != nullptr, lut_s, g.mult3, rnd3,
-                                                     g.shift3, v);
+      finish_n<4, OSZ, GATED, decltype(hi_c)::value>(x[0], x[NB - 1], mult * sc, mult2 * sc, ep, lut_s, w);
     };
-    if (high) finish(std::true_type{});
+    if (ep.high) finish(std::true_type{});
     else finish(std::false_type{});
-    char* out = (char*)g.C + ((tile.p0 + r) * g.ldc + n) * OSZ;
-    if (n + 4 <= g.N) {                                  // one store at any alignment
-      if constexpr (OSZ == 1) {
-        const unsigned w = pack4(v[0], v[1], v[2], v[3]);
-        __builtin_memcpy(out, &w, 4);
-      } else {
-        const unsigned w[2] = {__builtin_amdgcn_perm((unsigned)v[1], (unsigned)v[0], 0x05040100u),
-                               __builtin_amdgcn_perm((unsigned)v[3], (unsigned)v[2], 0x05040100u)};
-        __builtin_memcpy(out, w, 8);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < g.N) {
-          if (OSZ == 1) out[e] = (char)v[e];
-          else ((int16_t*)out)[e] = (int16_t)v[e];
-        }
-    }
+    store_n<4, OSZ>(g, tile.p0 + r, n, w);
   }
 }
 
@@ -546,8 +539,8 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   const int i = row_of(a, tile.p0 + m, false);
   const int scale = g.scale ? (i < 0 ? 0 : (int)g.scale[i]) : 1;
   const int lo = OSZ == 1 ? -128 : -32768;
-  const Requant q1(g.shift, lo, -lo - 1), q2(g.shift2, -128, 127);
-  const auto of = [](const Requant& q, int acc, int mul) { return q.high() ? q.of<true>(acc, mul) : q.of<false>(acc, mul); };
+  const WideRequant q1(g.shift, lo, -lo - 1), q2(g.shift2, -128, 127);
+  const auto of = [](const WideRequant& q, int acc, int mul) { return q.high() ? q.of<true>(acc, mul) : q.of<false>(acc, mul); };
   const int rnd3 = (int)round_term(g.shift3);
   int v[16];
 #pragma unroll
@@ -556,7 +549,12 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
     if (g.lut) v[e] = lut_s[(v[e] + 128) & 255];
     if constexpr (GATED) v[e] = min(max((v[e] * of(q2, acc[NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
   }
-  store16<OSZ>(g, tile.p0 + m, n0, v);
+  unsigned w[4 * OSZ];
+#pragma unroll
+  for (int q = 0; q < 4 * OSZ; ++q)
+    w[q] = OSZ == 1 ? pack4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3])
+                    : __builtin_amdgcn_perm((unsigned)v[2 * q + 1], (unsigned)v[2 * q], 0x05040100u);
+  store_n<16, OSZ>(g, tile.p0 + m, n0, w);
 }
 
 }  // namespace anvil

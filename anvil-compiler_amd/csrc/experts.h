@@ -7,23 +7,26 @@
 namespace anvil {
 
 // clamp((acc * m + 2^(s-1)) >> s, lo, hi) with the product and the sum in 64 bits, left as a clamped int to be shifted right by `rest`.
-// HI: s >= 33, where 2^(s-1) is a whole number of 2^32: the sum's upper word is the product's upper word and 2^(s-33), one
-// multiplication and one addition in 32 bits, clamped before the last s - 32 bits go (|acc| <= 2^30, so neither leaves int32). A product's
-// m / 2^s lies well below 1 / 4, so a smaller s is moved up to 33 where m has room (lift_shift).
-struct Requant {
-  int s, rest, add, clo, chi, lo, hi;
-  __host__ __device__ Requant(int shift, int lo_, int hi_) : s(shift), rest(0), add(0), clo(lo_), chi(hi_), lo(lo_), hi(hi_) {
+// HI: s >= 33, where the sum's upper word alone is needed: one multiply-add of 32 x 32 + 64 bits, clamped before the last s - 32 bits go. A
+// product's m / 2^s lies well below 1 / 4, so a smaller s is moved up to 33 where m has room (lift_shift). The lower word of 2^(s-1), zero
+// there, comes from where the compiler does not see it: knowing it, it multiplies and adds in two instructions.
+struct WideRequant {
+  int s, rest, clo, chi, lo, hi;
+  long long half;
+  __device__ __forceinline__ WideRequant(int shift, int lo_, int hi_) : s(shift), rest(0), clo(lo_), chi(hi_), lo(lo_), hi(hi_), half(0) {
     if (s < 33) return;
     rest = s - 32;
-    add = 1 << (rest - 1);
+    int zero = 0;
+    asm("" : "+s"(zero));
+    half = (long long)((unsigned long long)(1u << (rest - 1)) << 32 | (unsigned)zero);
     const long long a = (long long)lo << rest, b = (((long long)hi + 1) << rest) - 1;
     clo = a < I32_MIN ? (int)I32_MIN : (int)a;
     chi = b > I32_MAX ? (int)I32_MAX : (int)b;
   }
-  __host__ __device__ bool high() const { return s >= 33; }
+  __device__ __forceinline__ bool high() const { return s >= 33; }
   template <bool HI>
   __device__ __forceinline__ int unshifted(int acc, int m) const {
-    if constexpr (HI) return med3i(__mulhi(acc, m) + add, clo, chi);
+    if constexpr (HI) return med3i((int)(((long long)acc * m + half) >> 32), clo, chi);
     const long long r = ((long long)acc * m + (s ? 1ll << (s - 1) : 0)) >> s;
     return (int)(r < lo ? lo : r > hi ? hi : r);
   }

@@ -238,7 +238,7 @@ __global__ __launch_bounds__(1024) void route_place(RouteArgs g) {
 
 struct CombineArgs {
   anvil_expert_combine c;
-  int mult, lifted;                                      // of Requant's upper word, where c.mult / 2^c.shift allows it (c.shift then 33 or more)
+  int mult, lifted;                                      // of WideRequant's upper word, where c.mult / 2^c.shift allows it (c.shift then 33 or more)
   unsigned* flags;
 };
 
@@ -247,7 +247,7 @@ struct CombineArgs {
 // 32768 rows of 768, two results each: 35.7 us, 4.2 TB/s (an element a thread: 147).
 __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
   const anvil_expert_combine& c = g.c;
-  const Requant rq(c.shift, -128, 127);
+  const WideRequant rq(c.shift, -128, 127);
   const int lo = c.d_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
   const int rnd2 = (int)round_term(c.shift2);
   const int chunks = c.cols >> 4;
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
 // One element a thread, any alignment.
 __global__ __launch_bounds__(256) void combine_any(CombineArgs g) {
   const anvil_expert_combine& c = g.c;
-  const Requant rq(c.shift, -128, 127);
+  const WideRequant rq(c.shift, -128, 127);
   const int lo = c.d_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
   const long long n = (long long)c.rows * c.cols;
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
