@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -150,6 +151,11 @@ class Beams(C.Structure):
                 ("ended_out", _p)]
 
 
+def _packer(cls):
+    """A function from the field values of a ctypes struct of pointers (ints, DeviceBuffers, 0) and integers to its bytes."""
+    return struct.Struct("".join({_p: "P", _i32: "i", _i64: "q"}[t] for _, t in cls._fields_) + "0q").pack
+
+
 class AddNorm(C.Structure):
     """anvil_add_norm: the arguments of one anvil_add_norm_i8 call."""
     _fields_ = [("X", _p), ("Y", _p), ("R", _p), ("x_dtype", _i32), ("y_dtype", _i32), ("r_dtype", _i32), ("ldx", _i64), ("ldy", _i64),
@@ -183,6 +189,9 @@ class ExpertCombine(C.Structure):
                 ("mb", _i32), ("shift2", _i32), ("D", _p), ("ldd", _i64), ("d_dtype", _i32)]
 
 
+_ADD_NORM, _ROUTE, _EXPERT_GEMM, _EXPERT_COMBINE = map(_packer, (AddNorm, Route, ExpertGemm, ExpertCombine))
+
+
 ROW_LOAD, ROW_NORM, ROW_GEMM, ROW_ADD, ROW_LUT, ROW_LUT_MUL = 1, 2, 3, 4, 5, 6
 
 GEMM_GROUP_MAX = 4
@@ -211,6 +220,15 @@ class Library:
             msg = self.last_error().decode(errors="replace")
             raise {**_ERRORS, **_CACHE_ERRORS}.get(rc, RuntimeError)(f"{name}: {msg}")
         return rc
+
+    def call_packed(self, name, ctx, pack, *values):
+        """call(name, ctx, &arguments) with the arguments packed by _packer(their struct): 0.6 us less of host time than a ctypes
+        struct of twenty fields, of the 5 that a small call takes."""
+        try:
+            data = pack(*values)
+        except struct.error as e:
+            raise ValueError(f"{name}: {e}") from None
+        return self.call(name, ctx, data)
 
 
 def library() -> Library:
@@ -242,6 +260,10 @@ class DeviceBuffer:
         out = C.c_void_p()
         dev.lib.call("anvil_alloc", dev.ctx, C.c_size_t(max(1, self.nbytes)), C.byref(out))
         self.ptr = int(out.value)
+
+    def __index__(self):
+        """The device address, where an integer is asked for."""
+        return self.ptr
 
     def upload(self, arr: np.ndarray, offset: int = 0):
         arr = np.ascontiguousarray(arr)
@@ -607,31 +629,28 @@ class Device:
     def add_norm(self, X, x_dtype, ldx, Y, y_dtype, ldy, ma, mb, shift, R, r_dtype, ldr, w, lut, lut_len, eps, lut_shift, H, ldh,
                  scale, rows, cols):
         """anvil_add_norm_i8: R = the sum of X and Y (Y None: X alone, no R), H and scale its norm's codes and rows' scales."""
-        n = AddNorm(_opt(X), _opt(Y), _opt(R), DTYPE_CODE[x_dtype], DTYPE_CODE[y_dtype], DTYPE_CODE[r_dtype], ldx, ldy, ldr, ma, mb,
-                    shift, _opt(w), _opt(lut), lut_len, eps, lut_shift, _opt(H), ldh, _opt(scale), rows, cols)
-        self.lib.call("anvil_add_norm_i8", self.ctx, C.byref(n))
+        self.lib.call_packed("anvil_add_norm_i8", self.ctx, _ADD_NORM, X or 0, Y or 0, R or 0, DTYPE_CODE[x_dtype], DTYPE_CODE[y_dtype],
+                             DTYPE_CODE[r_dtype], ldx, ldy, ldr, ma, mb, shift, w or 0, lut or 0, lut_len, eps, lut_shift, H or 0, ldh,
+                             scale or 0, rows, cols)
 
     def expert_route(self, scores, ld, live, rows, experts, top, lut, one, expert, weight, slot, row, starts, every=False):
         """anvil_expert_route_i8: each row's experts and weights, and the rows sorted by expert. every: weights are shares of all
         experts' sum, not of the chosen ones'."""
-        r = Route(_opt(scores), ld, _opt(live), rows, experts, top, ROUTE_EVERY if every else 0, _opt(lut), one, _opt(expert),
-                  _opt(weight), _opt(slot), _opt(row), _opt(starts))
-        self.lib.call("anvil_expert_route_i8", self.ctx, C.byref(r))
+        self.lib.call_packed("anvil_expert_route_i8", self.ctx, _ROUTE, scores or 0, ld, live or 0, rows, experts, top,
+                             ROUTE_EVERY if every else 0, lut or 0, one, expert or 0, weight or 0, slot or 0, row or 0, starts or 0)
 
     def expert_gemm(self, A, lda, rows_a, row, scale, B, B2, ldb, sb, starts, experts, rows, N, K, Cp, ldc, out_dtype, mults=None,
                     mult=0, shift=0, mults2=None, mult2=0, shift2=0, lut=None, mult3=1, shift3=0):
         """anvil_expert_gemm_i8: sorted rows times their experts' weights; B2: gated."""
-        g = ExpertGemm(_opt(A), lda, _opt(row), _opt(scale), _opt(B), _opt(B2), ldb, sb, _opt(starts), rows_a, rows, experts, N, K,
-                       _opt(mults), _opt(mults2), mult, shift, mult2, shift2, mult3, shift3, _opt(lut), _opt(Cp), ldc,
-                       DTYPE_CODE[out_dtype])
-        self.lib.call("anvil_expert_gemm_i8", self.ctx, C.byref(g))
+        self.lib.call_packed("anvil_expert_gemm_i8", self.ctx, _EXPERT_GEMM, A or 0, lda, row or 0, scale or 0, B or 0, B2 or 0, ldb, sb,
+                             starts or 0, rows_a, rows, experts, N, K, mults or 0, mults2 or 0, mult, shift, mult2, shift2, mult3, shift3,
+                             lut or 0, Cp or 0, ldc, DTYPE_CODE[out_dtype])
 
     def expert_combine(self, Y, ldy, positions, slot, weight, rows, top, cols, mult, shift, R, r_dtype, ldr, ma, mb, shift2, D, d_dtype,
                        ldd):
         """anvil_expert_combine_i8: weighted sums of each row's results, and the residual's addition (R None: none)."""
-        c = ExpertCombine(_opt(Y), ldy, _opt(slot), _opt(weight), positions, rows, top, cols, mult, shift, _opt(R), ldr,
-                          DTYPE_CODE[r_dtype], ma, mb, shift2, _opt(D), ldd, DTYPE_CODE[d_dtype])
-        self.lib.call("anvil_expert_combine_i8", self.ctx, C.byref(c))
+        self.lib.call_packed("anvil_expert_combine_i8", self.ctx, _EXPERT_COMBINE, Y or 0, ldy, slot or 0, weight or 0, positions, rows, top,
+                             cols, mult, shift, R or 0, ldr, DTYPE_CODE[r_dtype], ma, mb, shift2, D or 0, ldd, DTYPE_CODE[d_dtype])
 
 
 _devices = {}

@@ -183,6 +183,28 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert got == [C.sizeof(cls)] + [getattr(cls, f).offset for f in fields]
 
 
+def test_packed_arguments_are_the_structs():
+    class Buffer:
+        def __index__(self):
+            return (1 << 47) + 64
+
+    for cls, pack in ((rt.AddNorm, rt._ADD_NORM), (rt.Route, rt._ROUTE), (rt.ExpertGemm, rt._EXPERT_GEMM), (rt.ExpertCombine, rt._EXPERT_COMBINE)):
+        rng, sizes = np.random.default_rng(1), [t for _, t in cls._fields_]
+        values = [int(rng.integers(0, 1 << 48)) if t is C.c_void_p else int(rng.integers(-2 ** 31, 2 ** 31)) for t in sizes]
+        want, data = bytes(cls(*values)), pack(*values)
+        fields = [(getattr(cls, n).offset, C.sizeof(t)) for n, t in cls._fields_]                     # bytes between fields are nobody's
+        assert len(data) == len(want) and all(data[o:o + n] == want[o:o + n] for o, n in fields)
+        assert pack(*[np.int64(v) for v in values]) == data
+        at = sizes.index(C.c_void_p)
+        values[at] = Buffer()
+        assert pack(*values)[fields[at][0]:][:8] == Buffer().__index__().to_bytes(8, "little")
+    for bad in (dict(rows=1 << 31), dict(ma=-(2 ** 31) - 1), dict(shift=1.5), dict(X="x")):
+        with pytest.raises(ValueError, match="anvil_add_norm_i8"):
+            rt.library().call_packed("anvil_add_norm_i8", None, rt._ADD_NORM, *{**GOOD_NORM, **bad}.values())
+    with pytest.raises(ValueError, match="null context"):
+        rt.library().call_packed("anvil_add_norm_i8", None, rt._ADD_NORM, *GOOD_NORM.values())
+
+
 # ------------------------------------------------------------------------------------------------- norm (GPU)
 
 def norm_case(rows, cols, x="i16", y="i8", r="i16", seed=0, pad=0, off=0, extreme=False, place=None, lut=None, eps=3, lut_shift=15, ma=None,
