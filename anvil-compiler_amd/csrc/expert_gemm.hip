@@ -162,9 +162,10 @@ __device__ __forceinline__ void* uniform_ptr(const void* p) {
 // One workgroup of 2 x 2 waves a BM x BN tile, operands 16-byte aligned, K in stages of BK bytes, NS of them in LDS and NS - 1 on their way.
 //
 // 128 x 256 tiles (waves of 64 x 128, three stages of 64 bytes, two workgroups a CU): 65536 gated positions of 768 to 2048 columns, 412 GOP,
-// 256 to 277 us, 1.5 to 1.6 POPS; 65536 of 2048 to 768, 206 GOP, 122 to 134 us. Without its loads 181 and 80 us, without its matrix
-// instructions 205 and 102, without its epilogue 220 and 111 (239 and 118 without the epilogue's stores): loads from L2 cost most, 2.4 GB in
-// lines of which a stage takes half. 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
+// 271 to 295 us as clocks go, 1.4 to 1.5 POPS; 65536 of 2048 to 768, 206 GOP, 126 to 134 us. At 267 and 126 us it took 181 and 80 without its
+// loads, 205 and 102 without its matrix instructions, 220 and 111 without its epilogue (239 and 118 without the epilogue's stores): loads
+// from L2 cost most, 2.4 GB in lines of which a stage takes half. The epilogue is eleven instructions a gated result (with fifteen 298 us
+// against 293). 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
 // workgroup's products run beside their epilogue (283 and 136 where a workgroup walks its tiles and the next one's first stages load
 // under the results; 128 x 256 tiles walked that way 298 and 130); 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
 // (KFULL): selecting an offset past K for each load instead 261 against 257 us.
