@@ -242,74 +242,81 @@ struct CombineArgs {
   unsigned* flags;
 };
 
-// Sixteen columns a thread, operands 16-byte aligned: a row's slots and weights first, then up to four of its results at a time.
-// What bounds it is memory: top + 4 bytes an element (an i16 residual and result), two instructions a result's element.
-// 32768 rows of 768, two results each: 35.7 us, 4.2 TB/s (an element a thread: 147).
+// Sixteen columns a thread, operands 16-byte aligned: a row's slots and weights first, then up to four of its results at a time. A slot
+// that adds nothing reads row 0 with weight 0, so no load waits for a branch. RSZ, DSZ: bytes of R's (0: none) and D's elements.
+// What bounds it is memory: top + 4 bytes an element (an i16 residual and result), two instructions a result's element and nine more.
+// 32768 rows of 768, two results each: 30.8 us, 4.9 TB/s (with types told apart at run time and a branch a result 37.1, eight columns a thread
+// so 40, an element a thread 147); int8 residual and result 21.8 (31.0), none 15.5 (19.6).
+template <int RSZ, int DSZ>
 __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
   const anvil_expert_combine& c = g.c;
   const WideRequant rq(c.shift, -128, 127);
-  const int lo = c.d_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
-  const int rnd2 = (int)round_term(c.shift2);
+  constexpr int lo = DSZ == 1 ? -128 : -32768, hi = -lo - 1;
+  const int rnd2 = (int)round_term(c.shift2), wide = DSZ == 1 ? 24 : 16;       // a shift from which lo and hi leave int32
+  const int clo = c.shift2 < wide ? lo * (1 << c.shift2) : (int)I32_MIN, chi = c.shift2 < wide ? -lo * (1 << c.shift2) - 1 : (int)I32_MAX;
   const int chunks = c.cols >> 4;
   const long long n = (long long)c.rows * chunks;
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
     const long long i = n <= UINT32_MAX ? (unsigned)at / (unsigned)chunks : at / chunks;
     const int col = (int)(at - i * chunks) * 16;
-    v4i r0 = {0, 0, 0, 0}, r1 = {0, 0, 0, 0};
-    if (c.R) {
-      if (c.r_dtype == ANVIL_I8) {
-        r0 = *reinterpret_cast<const v4i*>((const int8_t*)c.R + i * c.ldr + col);
-      } else {
-        const v4i* p = reinterpret_cast<const v4i*>((const int16_t*)c.R + i * c.ldr + col);
-        r0 = p[0], r1 = p[1];
-      }
+    const int* const slot = c.slot + i * c.top;
+    const int16_t* const weight = c.weight + i * c.top;
+    v4i r[RSZ == 2 ? 2 : 1];
+    if constexpr (RSZ > 0) {
+      const v4i* p = reinterpret_cast<const v4i*>((const char*)c.R + (i * c.ldr + col) * RSZ);
+#pragma unroll
+      for (int q = 0; q < RSZ; ++q) r[q] = p[q];
     }
     int acc[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0;
-    for (int j0 = 0; j0 < c.top; j0 += 4) {
-      int w[4];
-      v4i y[4];
+    const auto add = [&](int j0, auto count) {
+      constexpr int N = decltype(count)::value;
+      int p[N], w[N];
+      v4i y[N];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = j0 + k;
-        int p = -1;
-        w[k] = 0;
-        if (j < c.top) p = c.slot[i * c.top + j], w[k] = c.weight[i * c.top + j];
-        y[k] = v4i{0, 0, 0, 0};
-        if (p >= 0 && p < c.positions) y[k] = *reinterpret_cast<const v4i*>(c.Y + p * c.ldy + col);
-        else if (p != -1) raise_flag(g.flags, FLAG_EXPERTS);
+      for (int k = 0; k < N; ++k) p[k] = slot[j0 + k], w[k] = weight[j0 + k];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const bool in = p[k] >= 0 && p[k] < c.positions;
+        if (!in && p[k] != -1) raise_flag(g.flags, FLAG_EXPERTS);
+        w[k] = in ? w[k] : 0;
+        y[k] = *reinterpret_cast<const v4i*>(c.Y + (in ? p[k] : 0) * c.ldy + col);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (j0 + k < c.top) {
+      for (int k = 0; k < N; ++k)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[e] += __mul24((int)(int8_t)((unsigned)y[k][e >> 2] >> (8 * (e & 3))), w[k]);
-        }
+        for (int e = 0; e < 16; ++e) acc[e] += __mul24((int)(int8_t)((unsigned)y[k][e >> 2] >> (8 * (e & 3))), w[k]);
+    };
+    if (c.positions) {
+      int j = 0;
+      for (; j + 4 <= c.top; j += 4) add(j, std::integral_constant<int, 4>{});
+      if (c.top & 2) add(j, std::integral_constant<int, 2>{}), j += 2;
+      if (c.top & 1) add(j, std::integral_constant<int, 1>{});
     }
     const auto finish = [&](auto hi_c) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] = rq.of<decltype(hi_c)::value>(acc[e], g.mult);
+      for (int e = 0; e < 16; ++e) {
+        acc[e] = rq.of<decltype(hi_c)::value>(acc[e], g.mult);
+        if constexpr (RSZ > 0) {
+          const unsigned h = (unsigned)r[RSZ == 2 ? e >> 3 : 0][RSZ == 2 ? e >> 1 & 3 : e >> 2];
+          const int x = RSZ == 1 ? (int)(int8_t)(h >> (8 * (e & 3))) : e & 1 ? (int)h >> 16 : (int)(int16_t)h;
+          acc[e] = med3i(mad_i24v(x, c.ma, mad_i24v(acc[e], c.mb, rnd2)), clo, chi);
+        }
+      }
     };
     if (g.lifted) finish(std::true_type{});
     else finish(std::false_type{});
-    if (c.R) {
+    const int shift2 = RSZ ? c.shift2 : 0;
+    v4i* const d = reinterpret_cast<v4i*>((char*)c.D + (i * c.ldd + col) * DSZ);
+    if constexpr (DSZ == 1) {
+      v4i w;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        int r;
-        if (c.r_dtype == ANVIL_I8) {
-          r = (int)(int8_t)((unsigned)r0[e >> 2] >> (8 * (e & 3)));
-        } else {
-          const unsigned h = (unsigned)(e < 8 ? r0[e >> 1 & 3] : r1[e >> 1 & 3]);
-          r = e & 1 ? (int)h >> 16 : (int)(int16_t)h;
-        }
-        acc[e] = med3i((r * c.ma + acc[e] * c.mb + rnd2) >> c.shift2, lo, hi);
-      }
-    }
-    if (c.d_dtype == ANVIL_I8) {
-      *reinterpret_cast<v4i*>((int8_t*)c.D + i * c.ldd + col) = pack16(acc);
+      for (int q = 0; q < 4; ++q) w[q] = (int)sra_pack4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3], shift2);
+      d[0] = w;
     } else {
-      v4i* d = reinterpret_cast<v4i*>((int16_t*)c.D + i * c.ldd + col);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] >>= shift2;
       d[0] = pack8h(acc);
       d[1] = pack8h(acc + 8);
     }
@@ -445,8 +452,21 @@ extern "C" int anvil_expert_combine_i8(anvil_ctx* ctx, const anvil_expert_combin
   g.lifted = g.c.shift >= 33;
   const long long n = (long long)c->rows * c->cols;
   const auto even = [](const void* p, long long ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; };
-  if (c->cols % 16 == 0 && even(c->Y, c->ldy, 1) && even(c->D, c->ldd, c->d_dtype) && (!c->R || even(c->R, c->ldr, c->r_dtype))) {
-    ANVIL_LAUNCH(combine_rows, dim3((unsigned)std::min<long long>((n / 16 + 255) / 256, 1 << 20)), dim3(256), 0, ctx->stream, g);
+  const auto m24 = [](int m) { return m >= -(1 << 23) && m < 1 << 23; };         // multipliers that a 24-bit product takes
+  if (c->cols % 16 == 0 && even(c->Y, c->ldy, 1) && even(c->D, c->ldd, c->d_dtype) &&
+      (!c->R || (even(c->R, c->ldr, c->r_dtype) && m24(c->ma) && m24(c->mb)))) {
+    const auto run = [&](auto rsz, auto dsz) {
+      ANVIL_LAUNCH((combine_rows<decltype(rsz)::value, decltype(dsz)::value>), dim3((unsigned)std::min<long long>((n / 16 + 255) / 256, 1 << 20)),
+                   dim3(256), 0, ctx->stream, g);
+    };
+    const std::integral_constant<int, 0> none;
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    if (!c->R) run(none, one);
+    else if (c->r_dtype == ANVIL_I8 && c->d_dtype == ANVIL_I8) run(one, one);
+    else if (c->r_dtype == ANVIL_I8) run(one, two);
+    else if (c->d_dtype == ANVIL_I8) run(two, one);
+    else run(two, two);
     ANVIL_LAUNCHED();
     return ANVIL_OK;
   }
