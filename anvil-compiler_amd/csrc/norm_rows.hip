@@ -100,35 +100,42 @@ __device__ __forceinline__ void unpack(v4i (&v)[R], int dtype) {
   }
 }
 
+// The types of X (and of R) and Y that a kernel is made for: Y 0 none, -1 as the call says.
+template <int X, int Y>
+struct NormTypes {
+  static constexpr int x = X, y = Y;
+};
+
 // Rows of at most 8 L R columns, 16-byte aligned, in registers: L lanes a row (64 / L rows a wave, or the workgroup's 256), R chunks of
 // eight elements a lane, and a lane has the same columns of every row it takes, so its weights stay in registers.
 //
-// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 27 us of the
-// kernel's own, 33.6 a call in a row of them, 4.5 TB/s (one workgroup a row, each row read twice: 149). Many rows of up to 768 columns take
-// 16 lanes of up to six chunks: 64 lanes would leave a quarter of the wave idle in the second chunk of 768, and the row's
-// sum and maximum take four data-parallel moves instead of six steps.
+// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 30.5 us, 4.95
+// TB/s, a copy's rate (one workgroup a row, each row read twice: 149). 32 lanes of three chunks for 768 columns: 64 would leave a quarter of
+// them idle in the second chunk, 16 hold six chunks each and leave room for few waves.
 //
 // Codes. floor((254 |t| + a) / 2a) with t's sign is floor((254 t + a - [t < 0]) / 2a); with 256 a added it is 128 larger and its
 // numerator lies in [0, 511 a], below 2^31 (a <= 2^22), so one multiplication by the row's reciprocal (Divider) and a shift
 // straight into the code's byte give it exactly.
-template <int L, int R>
+template <int L, int R, typename T>
 __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
   const anvil_add_norm& n = g.n;
   constexpr bool WHOLE = L == 256;                       // a workgroup a row
+  const int xt = T::x < 0 ? n.x_dtype : T::x, yt = T::y < 0 ? n.y_dtype : T::y, rt = T::x < 0 ? n.r_dtype : T::x;
+  const bool added = T::y < 0 ? n.Y != nullptr : T::y > 0;
   constexpr int ROWS = WHOLE ? 1 : 64 / L;               // of a wave at a time
   __shared__ unsigned long long sums[2][4];
   __shared__ int tops[2][4];
   const int lane = threadIdx.x & 63, sub = threadIdx.x & (L - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int mine = WHOLE ? 0 : lane / L;                 // row of those
   const int chunks = n.cols >> 3;
-  const int lo = n.r_dtype == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
+  const int lo = rt == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
   const int rnd = (int)round_term(n.shift), ma = n.ma, mb = n.mb, shift = n.shift;
   v2u w[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) w[i] = sub + L * i < chunks ? *reinterpret_cast<const v2u*>(n.w + 8 * (sub + L * i)) : v2u{0, 0};
   // a lane's first chunk from that of its wave's rows (the launch checks ROWS rows against 2^31); chunk i is i steps on
   const auto offset = [&](long long ld, int size) { return (unsigned)(mine * ld + 8 * sub) * (unsigned)size; };
-  const unsigned ox = offset(n.ldx, n.x_dtype), oy = n.Y ? offset(n.ldy, n.y_dtype) : 0, oz = n.Y ? offset(n.ldr, n.r_dtype) : 0,
+  const unsigned ox = offset(n.ldx, xt), oy = added ? offset(n.ldy, yt) : 0, oz = added ? offset(n.ldr, rt) : 0,
                  oh = offset(n.ldh, 1);
   const long long group = WHOLE ? blockIdx.x : (long long)blockIdx.x * 4 + wave, groups = WHOLE ? gridDim.x : 4ll * gridDim.x;
   int turn = 0;                                          // a wave is at most one barrier ahead, so two sets of sums do
@@ -143,11 +150,11 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
       return [=](int i) { return live && sub + L * i < chunks ? o + 8 * L * i * size : OOB; };
     };
     v4i x[R], y[R];
-    load_chunks(x, span(n.X, n.ldx, n.x_dtype), n.x_dtype, at(ox, n.x_dtype));
-    if (n.Y) {
-      load_chunks(y, span(n.Y, n.ldy, n.y_dtype), n.y_dtype, at(oy, n.y_dtype));
-      unpack(x, n.x_dtype);
-      unpack(y, n.y_dtype);
+    load_chunks(x, span(n.X, n.ldx, xt), xt, at(ox, xt));
+    if (added) {
+      load_chunks(y, span(n.Y, n.ldy, yt), yt, at(oy, yt));
+      unpack(x, xt);
+      unpack(y, yt);
 #pragma unroll
       for (int i = 0; i < R; ++i)                        // past the row's end x, y and so r are 0
 #pragma unroll
@@ -156,9 +163,9 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
           const int v1 = (__mul24(x[i][q] >> 16, ma) + __mul24(y[i][q] >> 16, mb) + rnd) >> shift;
           x[i][q] = (int)__builtin_amdgcn_perm((unsigned)med3i(v1, lo, hi), (unsigned)med3i(v0, lo, hi), 0x05040100u);
         }
-      const __amdgpu_buffer_rsrc_t pr = span(n.R, n.ldr, n.r_dtype);
-      const auto off = at(oz, n.r_dtype);
-      if (n.r_dtype == ANVIL_I16) {
+      const __amdgpu_buffer_rsrc_t pr = span(n.R, n.ldr, rt);
+      const auto off = at(oz, rt);
+      if (rt == ANVIL_I16) {
 #pragma unroll
         for (int i = 0; i < R; ++i) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x[i]), pr, off(i), 0, 0);
       } else {
@@ -170,7 +177,7 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
         }
       }
     } else {
-      unpack(x, n.x_dtype);
+      unpack(x, xt);
     }
     unsigned long long ss = 0;
     int top = 0, low = 0;
@@ -313,35 +320,46 @@ extern "C" int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n) {
   const int chunks = n->cols / 8;
   if (n->cols % 8 == 0 && chunks <= 2048 && even(n->X, n->ldx, n->x_dtype) && even(n->H, n->ldh, 1) && even(n->w, 8, 1) &&
       (!n->Y || (even(n->Y, n->ldy, n->y_dtype) && even(n->R, n->ldr, n->r_dtype) && m24(n->ma) && m24(n->mb)))) {
-    const auto go = [&](auto lanes, auto per) {
+    const auto launch = [&](auto lanes, auto per, auto types) {
       constexpr int L = decltype(lanes)::value, R = decltype(per)::value;
-      const int rows = 256 / L, groups = (n->rows + rows - 1) / rows;              // of a workgroup at a time
-      ANVIL_LAUNCH((add_norm_rows<L, R>), dim3((unsigned)std::min(groups, 8 * ctx->num_cu)), dim3(256), 0, ctx->stream, g);
+      const int rows = 256 / L;                          // of a workgroup at a time
+      ANVIL_LAUNCH((add_norm_rows<L, R, decltype(types)>), dim3((unsigned)std::min((n->rows + rows - 1) / rows, 1 << 20)), dim3(256), 0,
+                   ctx->stream, g);
+    };
+    // Streams of one type, alone or with an int8 addend, have kernels of their own: 32768 rows of 768 (i16 and i8) 32.6 us, 34.5 with types
+    // told apart at run time; 8192 of 4096 37.8 and 44.7 (40.0 with workgroups for eight a CU that walk over the rows).
+    const auto go = [&](auto lanes, auto per) {
+      const bool same = n->r_dtype == n->x_dtype;
+      if (same && !n->Y && n->x_dtype == ANVIL_I16) launch(lanes, per, NormTypes<ANVIL_I16, 0>{});
+      else if (same && n->Y && n->x_dtype == ANVIL_I16 && n->y_dtype == ANVIL_I8) launch(lanes, per, NormTypes<ANVIL_I16, ANVIL_I8>{});
+      else if (same && n->Y && n->x_dtype == ANVIL_I8 && n->y_dtype == ANVIL_I8) launch(lanes, per, NormTypes<ANVIL_I8, ANVIL_I8>{});
+      else launch(lanes, per, NormTypes<-1, -1>{});
     };
     using std::integral_constant;
     const integral_constant<int, 1> c1;
     const integral_constant<int, 2> c2;
+    const integral_constant<int, 3> c3;
     const integral_constant<int, 4> c4;
-    // Lanes a row, kernel us of an i16 stream with an i8 addend. 16 / 64: 32768 rows of 768 27.4 / 28.8, 8192 9.6 / 10.4, but 2048 5.9 / 5.2 and
-    // 32768 of 1024 34.6 / 32.8 (eight chunks a lane leave two waves a SIMD). 64 / 256: 8192 rows of 1536 17.7 / 20.8, 16384 of 2048 34 / 39,
-    // 8192 of 2560 28.9 / 28.3, 256 of 4096 6.5 / 5.2.
-    const int L = chunks > 256 ? 256 : chunks <= 96 && n->rows > 8 * ctx->num_cu ? 16 : 64;
-    if (L == 256) {
+    // Lanes a row, us of an i16 stream with an i8 addend. 16 / 32: 32768 rows of 256 10.7 / 11.6, of 512 22.5 / 20.8, of 768 32.7 / 30.5. 32 / 64: 32768
+    // of 768 30.5 / 33.5, 8192 9.5 / 9.8, 2048 5.0 / 5.2. 64 / 256: 32768 of 1024 37.6 / 84.6, 8192 of 1536 15.9 / 23.8, 16384 of 2048 38.6 / 50.0, 8192
+    // of 2560 28.9 / 28.3.
+    if (chunks <= 32) {
+      const integral_constant<int, 16> l;
+      if (chunks <= 16) go(l, c1);
+      else go(l, c2);
+    } else if (chunks <= 96) {
+      const integral_constant<int, 32> l;
+      if (chunks <= 64) go(l, c2);
+      else go(l, c3);
+    } else if (chunks <= 256) {
+      const integral_constant<int, 64> l;
+      if (chunks <= 128) go(l, c2);
+      else go(l, c4);
+    } else {
       const integral_constant<int, 256> l;
       if (chunks <= 512) go(l, c2);
       else if (chunks <= 1024) go(l, c4);
       else go(l, integral_constant<int, 8>{});
-    } else if (L == 16) {
-      const integral_constant<int, 16> l;
-      if (chunks <= 16) go(l, c1);
-      else if (chunks <= 32) go(l, c2);
-      else if (chunks <= 64) go(l, c4);
-      else go(l, integral_constant<int, 6>{});
-    } else {
-      const integral_constant<int, 64> l;
-      if (chunks <= 64) go(l, c1);
-      else if (chunks <= 128) go(l, c2);
-      else go(l, c4);
     }
     ANVIL_LAUNCHED();
     return ANVIL_OK;
