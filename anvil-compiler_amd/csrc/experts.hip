@@ -32,13 +32,14 @@ struct RouteArgs {
   unsigned* flags;
 };
 
-// (e one + S / 2) / S of e <= 2^31 - 1, one <= 2^15 - 1: the quotient of doubles is off by at most one
+// (e one + S / 2) / S of e <= 2^31 - 1, one <= 2^15 - 1, at most 32767: single precision is off by less than 1 / 50 of one, the remainder
+// shows by which way
 __device__ __forceinline__ int share(long long e, int one, long long S) {
   const long long num = e * one + S / 2;
-  long long q = (long long)((double)num / (double)S);
-  if (q * S > num) --q;
-  else if ((q + 1) * S <= num) ++q;
-  return (int)q;
+  int q = (int)((float)num * __builtin_amdgcn_rcpf((float)S));
+  const long long left = num - q * S;
+  q += left < 0 ? -1 : left >= S ? 1 : 0;
+  return q;
 }
 
 // sums over aligned groups of L lanes

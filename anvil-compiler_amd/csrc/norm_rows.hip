@@ -51,16 +51,22 @@ __device__ __forceinline__ int scale_of(const anvil_add_norm& n, unsigned a, uns
 
 // floor(u / d) of u < 2^31 for one d in [2, 2^23]: (u m) >> (31 + l) with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d), which lies in
 // [2^31, 2^32) and is too large by less than d / 2^(31+l) of a unit in 2^-(31+l): below 2^31 that is less than 1 / d, so no quotient
-// changes. The quotient in doubles gives m or the number below it, and the remainder shows which.
+// changes.
+// m comes from single precision and remainders. d is exact there, the hardware's reciprocal off by at most 2^-23 of it and every other
+// step by 2^-24; taken 2^-21 smaller, the first quotient is too small by at most 11 / 2^24 of itself, 2817 units and a fraction, and the second,
+// of what remains, leaves less than 2 d. (With a division in doubles instead some quotients came out units short on the device now
+// and then, when many waves shared a SIMD: codes at exact halves then fell to the next lower one.)
 struct Divider {
   unsigned m;
   int sh;                                                // of the product's upper word
   __device__ __forceinline__ explicit Divider(unsigned d) {
     const int l = 32 - __builtin_clz(d - 1);
-    const double p = __builtin_ldexp(1.0, 31 + l);
-    unsigned long long q = (unsigned long long)(p / (double)d);
-    if (q * d < 1ull << (31 + l)) ++q;
-    m = (unsigned)q;
+    const float r = __builtin_amdgcn_rcpf((float)d) * (1.0f - 0x1p-21f);
+    m = (unsigned)__builtin_ldexpf(r, 31 + l);
+    const unsigned long long whole = 1ull << (31 + l);
+    m += (unsigned)((float)(whole - (unsigned long long)m * d) * r);
+    const unsigned left = (unsigned)(whole - (unsigned long long)m * d);
+    m += (left > 0) + (left > d);
     sh = l - 1;
   }
 };
@@ -323,7 +329,7 @@ extern "C" int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n) {
     const auto launch = [&](auto lanes, auto per, auto types) {
       constexpr int L = decltype(lanes)::value, R = decltype(per)::value;
       const int rows = 256 / L;                          // of a workgroup at a time
-      ANVIL_LAUNCH((add_norm_rows<L, R, decltype(types)>), dim3((unsigned)std::min((n->rows + rows - 1) / rows, 1 << 20)), dim3(256), 0,
+      ANVIL_LAUNCH((add_norm_rows<L, R, decltype(types)>), dim3((unsigned)std::min((n->rows + rows - 1) / rows, 64 * ctx->num_cu)), dim3(256), 0,
                    ctx->stream, g);
     };
     // Streams of one type, alone or with an int8 addend, have kernels of their own: 32768 rows of 768 (i16 and i8) 32.6 us, 34.5 with types

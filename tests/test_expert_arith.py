@@ -5,13 +5,25 @@ import numpy as np
 import pytest
 
 
-def _divider(d):
-    """(m, shift of the upper word) of norm_rows.hip's reciprocal."""
-    l = (d - 1).bit_length()
-    q = int(math.ldexp(1.0, 31 + l) / float(d))
-    if q * d < 1 << (31 + l):
-        q += 1
-    return q, l - 1
+def _divider(d, off=0):
+    """(m, shift of the upper word) of norm_rows.hip's reciprocal. off: of the hardware's single-precision reciprocal, in its units."""
+    l, f = (d - 1).bit_length(), np.float32
+    r = (f(1) / f(d)).view(np.int32) + np.int32(off)
+    r = r.view(f) * f(1 - 2.0 ** -21)
+    m = int(np.ldexp(r, 31 + l))
+    m += int(f((1 << (31 + l)) - m * d) * r)
+    left = (1 << (31 + l)) - m * d
+    assert 0 <= left < 2 * d
+    return m + (left > 0) + (left > d), l - 1
+
+
+def test_reciprocals_of_every_kind():
+    """The smallest m with m d >= 2^(31+l), whatever the last unit of the hardware's reciprocal."""
+    rng = np.random.default_rng(3)
+    for d in {max(2, min(1 << 23, (1 << k) + e)) for k in range(1, 24) for e in range(-3, 4)} | set(rng.integers(2, 1 << 23, 3000).tolist()):
+        for off in (-1, 0, 1):
+            m, sh = _divider(d, off)
+            assert m == -(-(1 << (32 + sh)) // d) and 1 << 31 <= m < 1 << 32
 
 
 def test_codes_by_reciprocal():

@@ -253,6 +253,33 @@ def test_norm_widths(cols):
 
 
 @gpu
+@pytest.mark.parametrize("cols", [64, 128, 200, 256, 400, 512, 768, 1024, 1400, 2048, 4096, 6000, 8192, 16384])
+def test_norm_types_at_every_width(cols):
+    for n, (x, y, r) in enumerate((("i16", "i16", "i16"), ("i8", "i16", "i16"), ("i16", "i8", "i8"), ("i8", None, "i8"), ("i8", "i8", "i8"),
+                                   ("i8", "i8", "i16"))):
+        norm_case(11, cols, x, y, r, seed=cols + n)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(300001, 128), (140003, 512), (70001, 1024), (17003, 2056), (300001, 20)])
+def test_norm_of_more_rows_than_workgroups(rows, cols):
+    """1000 rows over and over, in place, so that a workgroup that walks over rows has them in its registers one after the other."""
+    dev, rng = device(), np.random.default_rng(cols)
+    x, y, w = rng.integers(-9000, 9000, (1000, cols)), rng.integers(-128, 128, (1000, cols)), rng.integers(-128, 128, cols)
+    turns = -(-rows // 1000)
+    tile = lambda a, t: np.tile(a.astype(t), (turns, 1))[:rows]                                       # noqa: E731
+    dx, dy, dw, dl = dev.upload(tile(x, np.int16)), dev.upload(tile(y, np.int8)), flat(dev, w, "i8"), flat(dev, roots(), "i32")
+    dh, ds = dev.alloc(rows * cols), dev.alloc(2 * rows)
+    dev.add_norm(dx.ptr, "i16", cols, dy.ptr, "i8", cols, 256, 900, 8, dx.ptr, "i16", cols, dw.ptr, dl.ptr, 1024, 7, 10, dh.ptr, cols, ds.ptr,
+                 rows, cols)
+    dev.sync()
+    r, h, scale = oe.add_norm(x, y, 256, 900, 8, "i16", w, roots(), 7, 10)
+    assert np.array_equal(dx.download((rows, cols), np.int16), tile(r, np.int16))
+    assert np.array_equal(dh.download((rows, cols), np.int8), tile(h, np.int8))
+    assert np.array_equal(ds.download((rows,), np.int16), np.tile(scale.astype(np.int16), turns)[:rows])
+
+
+@gpu
 @pytest.mark.parametrize("x", ["i8", "i16"])
 @pytest.mark.parametrize("y", [None, "i8", "i16"])
 @pytest.mark.parametrize("r", ["i8", "i16"])
