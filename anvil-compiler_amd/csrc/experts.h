@@ -54,6 +54,46 @@ __device__ __forceinline__ int lane_group_max(int v) {       // maximum over ali
   return v;
 }
 
+// sixteen bytes, at any alignment if ANY
+template <bool ANY>
+__device__ __forceinline__ v4i load16(const void* p) {
+  if constexpr (!ANY) return *reinterpret_cast<const v4i*>(p);
+  v4i v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// The last `bytes` of the 4 N bytes w that would end at `end` (fewer than all): a store for each bit of their number, the largest the
+// last in memory. What is left after each lies in one half of the words before.
+template <int N>
+struct Words {                                           // a vector: an array chosen from at run time would go to memory
+  typedef unsigned type __attribute__((ext_vector_type(N)));
+  typedef type any __attribute__((aligned(1)));
+};
+template <int N>
+__device__ __forceinline__ void store_last(char* end, typename Words<N>::type w, int bytes) {
+  if constexpr (N > 1) {
+    const bool upper = bytes & 2 * N;
+    typename Words<N / 2>::type left, high;
+#pragma unroll
+    for (int q = 0; q < N / 2; ++q) left[q] = upper ? w[q] : w[N / 2 + q], high[q] = w[N / 2 + q];
+    if (upper) {
+      end -= 2 * N;
+      *reinterpret_cast<typename Words<N / 2>::any*>(end) = high;
+    }
+    store_last<N / 2>(end, left, bytes);
+  } else {
+    unsigned v = w[0];
+    if (bytes & 2) {
+      end -= 2;
+      const unsigned short u = (unsigned short)(v >> 16);
+      __builtin_memcpy(end, &u, 2);
+      v <<= 16;
+    }
+    if (bytes & 1) end[-1] = (char)(v >> 24);
+  }
+}
+
 // Memory of `rows` rows of `width` bytes, `ld` bytes apart.
 struct Span {
   const void* p;

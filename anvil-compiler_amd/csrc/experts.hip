@@ -248,25 +248,28 @@ struct CombineArgs {
 // What bounds it is memory: top + 4 bytes an element (an i16 residual and result), two instructions a result's element and nine more.
 // 32768 rows of 768, two results each: 30.8 us, 4.9 TB/s (with types told apart at run time and a branch a result 37.1, eight columns a thread
 // so 40, an element a thread 147); int8 residual and result 21.8 (31.0), none 15.5 (19.6).
-template <int RSZ, int DSZ>
+// ANY: rows at any alignment and of any width from 16 columns on. A row's last thread then takes its last 16 columns and stores those that no
+// other thread has, so it reads no byte past the row, and in place what it has read of another's columns is dropped. 32768 rows of 769: 33.7 us
+// (an element a thread 166).
+template <int RSZ, int DSZ, bool ANY>
 __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
   const anvil_expert_combine& c = g.c;
   const WideRequant rq(c.shift, -128, 127);
   constexpr int lo = DSZ == 1 ? -128 : -32768, hi = -lo - 1;
   const int rnd2 = (int)round_term(c.shift2), wide = DSZ == 1 ? 24 : 16;       // a shift from which lo and hi leave int32
   const int clo = c.shift2 < wide ? lo * (1 << c.shift2) : (int)I32_MIN, chi = c.shift2 < wide ? -lo * (1 << c.shift2) - 1 : (int)I32_MAX;
-  const int chunks = c.cols >> 4;
+  const int chunks = (c.cols + 15) >> 4;
   const long long n = (long long)c.rows * chunks;
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
     const long long i = n <= UINT32_MAX ? (unsigned)at / (unsigned)chunks : at / chunks;
-    const int col = (int)(at - i * chunks) * 16;
+    const int first = (int)(at - i * chunks) * 16, col = ANY ? min(first, c.cols - 16) : first;
     const int* const slot = c.slot + i * c.top;
     const int16_t* const weight = c.weight + i * c.top;
     v4i r[RSZ == 2 ? 2 : 1];
     if constexpr (RSZ > 0) {
-      const v4i* p = reinterpret_cast<const v4i*>((const char*)c.R + (i * c.ldr + col) * RSZ);
+      const char* p = (const char*)c.R + (i * c.ldr + col) * RSZ;
 #pragma unroll
-      for (int q = 0; q < RSZ; ++q) r[q] = p[q];
+      for (int q = 0; q < RSZ; ++q) r[q] = load16<ANY>(p + 16 * q);
     }
     int acc[16];
 #pragma unroll
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
         const bool in = p[k] >= 0 && p[k] < c.positions;
         if (!in && p[k] != -1) raise_flag(g.flags, FLAG_EXPERTS);
         w[k] = in ? w[k] : 0;
-        y[k] = *reinterpret_cast<const v4i*>(c.Y + (in ? p[k] : 0) * c.ldy + col);
+        y[k] = load16<ANY>(c.Y + (in ? p[k] : 0) * c.ldy + col);
       }
 #pragma unroll
       for (int k = 0; k < N; ++k)
@@ -309,22 +312,29 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
     if (g.lifted) finish(std::true_type{});
     else finish(std::false_type{});
     const int shift2 = RSZ ? c.shift2 : 0;
-    v4i* const d = reinterpret_cast<v4i*>((char*)c.D + (i * c.ldd + col) * DSZ);
+    typename Words<4 * DSZ>::type w;
     if constexpr (DSZ == 1) {
-      v4i w;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) w[q] = (int)sra_pack4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3], shift2);
-      d[0] = w;
+      for (int q = 0; q < 4; ++q) w[q] = sra_pack4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3], shift2);
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] >>= shift2;
-      d[0] = pack8h(acc);
-      d[1] = pack8h(acc + 8);
+      for (int q = 0; q < 8; ++q) w[q] = __builtin_amdgcn_perm((unsigned)(acc[2 * q + 1] >> shift2), (unsigned)(acc[2 * q] >> shift2), 0x05040100u);
+    }
+    char* const d = (char*)c.D + (i * c.ldd + col) * DSZ;
+    if (ANY && col != first) {
+      store_last<4 * DSZ>(d + 16 * DSZ, w, (c.cols & 15) * DSZ);
+    } else {
+#pragma unroll
+      for (int q = 0; q < DSZ; ++q) {
+        const v4i v = {(int)w[4 * q], (int)w[4 * q + 1], (int)w[4 * q + 2], (int)w[4 * q + 3]};
+        if constexpr (ANY) __builtin_memcpy(d + 16 * q, &v, 16);
+        else *reinterpret_cast<v4i*>(d + 16 * q) = v;
+      }
     }
   }
 }
 
-// One element a thread, any alignment.
+// One element a thread: rows of fewer than 16 columns, multipliers of more than 24 bits.
 __global__ __launch_bounds__(256) void combine_any(CombineArgs g) {
   const anvil_expert_combine& c = g.c;
   const WideRequant rq(c.shift, -128, 127);
@@ -454,11 +464,14 @@ extern "C" int anvil_expert_combine_i8(anvil_ctx* ctx, const anvil_expert_combin
   const long long n = (long long)c->rows * c->cols;
   const auto even = [](const void* p, long long ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; };
   const auto m24 = [](int m) { return m >= -(1 << 23) && m < 1 << 23; };         // multipliers that a 24-bit product takes
-  if (c->cols % 16 == 0 && even(c->Y, c->ldy, 1) && even(c->D, c->ldd, c->d_dtype) &&
-      (!c->R || (even(c->R, c->ldr, c->r_dtype) && m24(c->ma) && m24(c->mb)))) {
+  if (c->cols >= 16 && (!c->R || (m24(c->ma) && m24(c->mb)))) {
+    const bool aligned = c->cols % 16 == 0 && even(c->Y, c->ldy, 1) && even(c->D, c->ldd, c->d_dtype) && (!c->R || even(c->R, c->ldr, c->r_dtype));
+    const long long threads = (long long)c->rows * ((c->cols + 15) / 16);
+    const dim3 grid((unsigned)std::min<long long>((threads + 255) / 256, 1 << 20));
     const auto run = [&](auto rsz, auto dsz) {
-      ANVIL_LAUNCH((combine_rows<decltype(rsz)::value, decltype(dsz)::value>), dim3((unsigned)std::min<long long>((n / 16 + 255) / 256, 1 << 20)),
-                   dim3(256), 0, ctx->stream, g);
+      constexpr int RSZ = decltype(rsz)::value, DSZ = decltype(dsz)::value;
+      if (aligned) ANVIL_LAUNCH((combine_rows<RSZ, DSZ, false>), grid, dim3(256), 0, ctx->stream, g);
+      else ANVIL_LAUNCH((combine_rows<RSZ, DSZ, true>), grid, dim3(256), 0, ctx->stream, g);
     };
     const std::integral_constant<int, 0> none;
     const std::integral_constant<int, 1> one;

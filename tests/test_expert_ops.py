@@ -695,6 +695,12 @@ def test_combine_types_strides_and_extremes(R, D):
 def test_combine_in_place_and_many_rows():
     combine_case(70, 2, 256, "i16", "i16", place=True)
     combine_case(70, 2, 250, "i8", "i8", place=True, pad=2)
+    for cols in range(16, 50):                                                # every number of columns behind the last sixteen
+        combine_case(40, 2, cols, "i16", "i16", place=True, off=1, seed=cols)
+        combine_case(40, 3, cols, "i8", "i8", place=True, off=3, pad=1, seed=cols)
+        combine_case(40, 1, cols, "i8", "i16", seed=cols, off=1)
+        combine_case(40, 5, cols, None, seed=cols)
+    combine_case(20011, 2, 769, "i16", "i16", place=True, seed=2)
     combine_case(30001, 2, 48, seed=1)
 
 
