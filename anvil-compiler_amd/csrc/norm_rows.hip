@@ -122,7 +122,10 @@ struct NormTypes {
 // Codes. floor((254 |t| + a) / 2a) with t's sign is floor((254 t + a - [t < 0]) / 2a); with 256 a added it is 128 larger and its
 // numerator lies in [0, 511 a], below 2^31 (a <= 2^22), so one multiplication by the row's reciprocal (Divider) and a shift
 // straight into the code's byte give it exactly.
-template <int L, int R, typename T>
+//
+// ANY: rows at any alignment and of any width from eight columns on. The last chunk is the row's last eight columns, of which those that the
+// chunk before has count as zeros and are not stored. 32768 x 769: 43 us (a workgroup a row that reads it twice 167).
+template <int L, int R, typename T, bool ANY>
 __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
   const anvil_add_norm& n = g.n;
   constexpr bool WHOLE = L == 256;                       // a workgroup a row
@@ -133,12 +136,21 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
   __shared__ int tops[2][4];
   const int lane = threadIdx.x & 63, sub = threadIdx.x & (L - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int mine = WHOLE ? 0 : lane / L;                 // row of those
-  const int chunks = n.cols >> 3;
+  const int chunks = (n.cols + 7) >> 3, over = ANY ? 8 * chunks - n.cols : 0;  // columns that the last two chunks share
+  const int last = ANY ? (chunks - 1) / L : -1;          // its number with its lane
+  const bool shares = ANY && over && sub == (chunks - 1) % L;
+  const unsigned back = shares ? over : 0;
   const int lo = rt == ANVIL_I8 ? -128 : -32768, hi = -lo - 1;
   const int rnd = (int)round_term(n.shift), ma = n.ma, mb = n.mb, shift = n.shift;
   v2u w[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) w[i] = sub + L * i < chunks ? *reinterpret_cast<const v2u*>(n.w + 8 * (sub + L * i)) : v2u{0, 0};
+  for (int i = 0; i < R; ++i) {
+    w[i] = v2u{0, 0};
+    if (sub + L * i < chunks) __builtin_memcpy(&w[i], __builtin_assume_aligned(n.w + 8 * (sub + L * i) - (i == last ? back : 0), ANY ? 1 : 8), 8);
+  }
+  v4i keep;                                              // of the last chunk's pairs
+#pragma unroll
+  for (int q = 0; q < 4; ++q) keep[q] = (back <= 2 * q ? 0xFFFF : 0) | (back <= 2 * q + 1 ? ~0xFFFF : 0);
   // a lane's first chunk from that of its wave's rows (the launch checks ROWS rows against 2^31); chunk i is i steps on
   const auto offset = [&](long long ld, int size) { return (unsigned)(mine * ld + 8 * sub) * (unsigned)size; };
   const unsigned ox = offset(n.ldx, xt), oy = added ? offset(n.ldy, yt) : 0, oz = added ? offset(n.ldr, rt) : 0,
@@ -153,7 +165,11 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
       return uniform_rsrc((const char*)p + first * ld * size, (int)((rows - 1) * ld + n.cols) * size);
     };
     const auto at = [&](unsigned o, int size) {
-      return [=](int i) { return live && sub + L * i < chunks ? o + 8 * L * i * size : OOB; };
+      return [=](int i) { return live && sub + L * i < chunks ? o + (8 * L * i - (ANY && i == last ? back : 0)) * size : OOB; };
+    };
+    const auto but = [&](unsigned o, int size) {         // the same without a chunk that shares columns
+      const auto f = at(o, size);
+      return [=](int i) { return ANY && i == last && shares ? OOB : f(i); };
     };
     v4i x[R], y[R];
     load_chunks(x, span(n.X, n.ldx, xt), xt, at(ox, xt));
@@ -170,7 +186,7 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
           x[i][q] = (int)__builtin_amdgcn_perm((unsigned)med3i(v1, lo, hi), (unsigned)med3i(v0, lo, hi), 0x05040100u);
         }
       const __amdgpu_buffer_rsrc_t pr = span(n.R, n.ldr, rt);
-      const auto off = at(oz, rt);
+      const auto off = but(oz, rt);
       if (rt == ANVIL_I16) {
 #pragma unroll
         for (int i = 0; i < R; ++i) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x[i]), pr, off(i), 0, 0);
@@ -182,8 +198,23 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
           __builtin_amdgcn_raw_buffer_store_b64(b, pr, off(i), 0, 0);
         }
       }
+      if constexpr (ANY) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (i == last && shares && live) {
+            char* const end = (char*)n.R + (row * n.ldr + n.cols) * rt;
+            const v4u v = __builtin_bit_cast(v4u, x[i]);
+            if (rt == ANVIL_I16) store_last<4>(end, v, 2 * (8 - over));
+            else store_last<2>(end, v2u{__builtin_amdgcn_perm(v[1], v[0], 0x06040200u), __builtin_amdgcn_perm(v[3], v[2], 0x06040200u)}, 8 - over);
+          }
+      }
     } else {
       unpack(x, xt);
+    }
+    if constexpr (ANY) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (i == last) x[i] &= keep;
     }
     unsigned long long ss = 0;
     int top = 0, low = 0;
@@ -217,7 +248,7 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
       for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(x[i][q]));
     const Divider div(2 * max(a, 1u));                   // a row of zeros: every code is 257 / 2 - 128
     const __amdgpu_buffer_rsrc_t ph = span(n.H, n.ldh, 1);
-    const auto to = at(oh, 1);
+    const auto to = but(oh, 1);
     const int bias = 257 * (int)max(a, 1u);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -237,12 +268,15 @@ __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
         h[d] = sra_pack4v((int)u[0], (int)u[1], (int)u[2], (int)u[3], div.sh) ^ 0x80808080u;
       }
       __builtin_amdgcn_raw_buffer_store_b64(h, ph, to(i), 0, 0);
+      if constexpr (ANY) {
+        if (i == last && shares && live) store_last<2>((char*)n.H + row * n.ldh + n.cols, h, 8 - over);
+      }
     }
     if (live && sub == 0) n.scale[row] = (int16_t)scale_of(n, a, ss, g.nbits);
   }
 }
 
-// One workgroup a row, any width, stride and alignment; the row is read twice.
+// One workgroup a row, which is read twice: rows of fewer than 8 or more than 16384 columns, multipliers of more than 24 bits, rows far apart.
 __global__ __launch_bounds__(256) void add_norm_any(NormArgs g) {
   const anvil_add_norm& n = g.n;
   __shared__ unsigned long long sums[4];
@@ -320,26 +354,30 @@ extern "C" int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n) {
   }
   if (int e = check_ctx(ctx)) return e;
   NormArgs g{*n, 32 - __builtin_clz((unsigned)n->lut_len), ctx->flags};
-  // eight elements a load: 16 bytes of i16, 8 of i8; multipliers that a 24-bit product takes
-  const auto even = [&](const void* p, long long ld, int size) { return (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 && ld < 1 << 28; };
+  // eight elements a load: 16 bytes of i16, 8 of i8; multipliers that a 24-bit product takes; four rows within 32-bit offsets
+  const auto even = [&](const void* p, long long ld, int size) { return (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0; };
   const auto m24 = [](int m) { return m >= -(1 << 23) && m < 1 << 23; };
-  const int chunks = n->cols / 8;
-  if (n->cols % 8 == 0 && chunks <= 2048 && even(n->X, n->ldx, n->x_dtype) && even(n->H, n->ldh, 1) && even(n->w, 8, 1) &&
-      (!n->Y || (even(n->Y, n->ldy, n->y_dtype) && even(n->R, n->ldr, n->r_dtype) && m24(n->ma) && m24(n->mb)))) {
-    const auto launch = [&](auto lanes, auto per, auto types) {
+  const auto near = [](long long ld) { return ld < 1 << 28; };
+  const int chunks = (n->cols + 7) / 8;
+  if (n->cols >= 8 && chunks <= 2048 && near(n->ldx) && near(n->ldh) && (!n->Y || (near(n->ldy) && near(n->ldr) && m24(n->ma) && m24(n->mb)))) {
+    const bool aligned = n->cols % 8 == 0 && even(n->X, n->ldx, n->x_dtype) && even(n->H, n->ldh, 1) && even(n->w, 8, 1) &&
+                         (!n->Y || (even(n->Y, n->ldy, n->y_dtype) && even(n->R, n->ldr, n->r_dtype)));
+    const auto launch = [&](auto lanes, auto per, auto types, auto any) {
       constexpr int L = decltype(lanes)::value, R = decltype(per)::value;
       const int rows = 256 / L;                          // of a workgroup at a time
-      ANVIL_LAUNCH((add_norm_rows<L, R, decltype(types)>), dim3((unsigned)std::min((n->rows + rows - 1) / rows, 64 * ctx->num_cu)), dim3(256), 0,
+      ANVIL_LAUNCH((add_norm_rows<L, R, decltype(types), decltype(any)::value>), dim3((unsigned)std::min((n->rows + rows - 1) / rows, 64 * ctx->num_cu)), dim3(256), 0,
                    ctx->stream, g);
     };
     // Streams of one type, alone or with an int8 addend, have kernels of their own: 32768 rows of 768 (i16 and i8) 32.6 us, 34.5 with types
     // told apart at run time; 8192 of 4096 37.8 and 44.7 (40.0 with workgroups for eight a CU that walk over the rows).
     const auto go = [&](auto lanes, auto per) {
       const bool same = n->r_dtype == n->x_dtype;
-      if (same && !n->Y && n->x_dtype == ANVIL_I16) launch(lanes, per, NormTypes<ANVIL_I16, 0>{});
-      else if (same && n->Y && n->x_dtype == ANVIL_I16 && n->y_dtype == ANVIL_I8) launch(lanes, per, NormTypes<ANVIL_I16, ANVIL_I8>{});
-      else if (same && n->Y && n->x_dtype == ANVIL_I8 && n->y_dtype == ANVIL_I8) launch(lanes, per, NormTypes<ANVIL_I8, ANVIL_I8>{});
-      else launch(lanes, per, NormTypes<-1, -1>{});
+      const std::false_type whole;
+      if (!aligned) launch(lanes, per, NormTypes<-1, -1>{}, std::true_type{});
+      else if (same && !n->Y && n->x_dtype == ANVIL_I16) launch(lanes, per, NormTypes<ANVIL_I16, 0>{}, whole);
+      else if (same && n->Y && n->x_dtype == ANVIL_I16 && n->y_dtype == ANVIL_I8) launch(lanes, per, NormTypes<ANVIL_I16, ANVIL_I8>{}, whole);
+      else if (same && n->Y && n->x_dtype == ANVIL_I8 && n->y_dtype == ANVIL_I8) launch(lanes, per, NormTypes<ANVIL_I8, ANVIL_I8>{}, whole);
+      else launch(lanes, per, NormTypes<-1, -1>{}, whole);
     };
     using std::integral_constant;
     const integral_constant<int, 1> c1;

@@ -261,7 +261,21 @@ def test_norm_types_at_every_width(cols):
 
 
 @gpu
-@pytest.mark.parametrize("rows,cols", [(300001, 128), (140003, 512), (70001, 1024), (17003, 2056), (300001, 20)])
+@pytest.mark.parametrize("cols", [*range(8, 34), 129, 255, 257, 263, 383, 511, 513, 519, 765, 767, 769, 1023, 1025, 2047, 2049, 2055, 4095, 4097, 8191,
+                                  8193, 16383, 16377])
+def test_norm_of_odd_widths(cols):
+    """Every number of columns that a row's last two chunks share, beside each other's rows, in place, at any alignment."""
+    rows = 37 if cols < 3000 else 3
+    norm_case(rows, cols, seed=cols, place="x")
+    norm_case(rows, cols, "i16", "i16", "i16", seed=cols + 1, place="y", off=3)
+    norm_case(rows, cols, "i8", "i8", "i8", seed=cols + 2, place="x", off=1, pad=1)
+    norm_case(rows, cols, "i16", None, seed=cols + 3, pad=5)
+    norm_case(rows, cols, "i8", None, "i8", seed=cols + 4, off=7)
+    norm_case(rows, cols, "i8", "i16", "i16", seed=cols + 5, extreme=True)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(300001, 128), (140003, 512), (70001, 1024), (17003, 2056), (300001, 20), (140003, 517), (17003, 2049)])
 def test_norm_of_more_rows_than_workgroups(rows, cols):
     """1000 rows over and over, in place, so that a workgroup that walks over rows has them in its registers one after the other."""
     dev, rng = device(), np.random.default_rng(cols)
