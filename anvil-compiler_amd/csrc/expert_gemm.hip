@@ -152,6 +152,13 @@ __device__ __forceinline__ void store_n(const anvil_expert_gemm& g, long long p,
     }
 }
 
+// sixteen bytes with the first n, if any, zeros
+__device__ __forceinline__ v4i without_first(v4i v, int n) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] &= n >= 4 * q + 4 ? 0 : n <= 4 * q ? -1 : -1 << (8 * (n - 4 * q));
+  return v;
+}
+
 // the same address in scalar registers (uniform_rsrc)
 __device__ __forceinline__ void* uniform_ptr(const void* p) {
   const unsigned long long a = (unsigned long long)p;
@@ -355,7 +362,9 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
 // What bounds it is the weights' way from memory, so nothing stands in it: each of the four waves takes every fourth 64 bytes of K, asks
 // for STEPS of them at a time, and its matrix instructions (16 x 16 x 64) take the loads' registers as they are; no LDS, no barrier before
 // the end, where the waves' sums meet in LDS. A lane's results are four consecutive columns of its row.
-template <int MT, int CT, int OSZ, bool GATED>
+//
+// ANY: rows at any alignment and K from 16 on. K's last chunk is the rows' last 16 bytes, of which those that the chunk before has are zeros in A.
+template <int MT, int CT, int OSZ, bool GATED, bool ANY>
 __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
   constexpr int NB = GATED ? 2 : 1, STEPS = 4, COLS = 16 * CT;
   __shared__ __attribute__((aligned(16))) v4i sums[4][MT * CT * NB][64];
@@ -384,7 +393,7 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
                                rb2 = uniform_rsrc(GATED ? g.B2 + b_at : g.B, GATED ? b_bytes : 0);
   unsigned offb[CT], offa[MT];
 #pragma unroll
-  for (int c = 0; c < CT; ++c) offb[c] = 16 * c + r16 < cols ? (unsigned)((16 * c + r16) * g.ldb + 16 * quad) : PAST;
+  for (int c = 0; c < CT; ++c) offb[c] = 16 * c + r16 < cols ? (unsigned)((16 * c + r16) * g.ldb) : PAST;
   const auto load = [](__amdgpu_buffer_rsrc_t r, unsigned off) {
     return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
   };
@@ -396,13 +405,17 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) acc[b][c][m] = v4i{0, 0, 0, 0};
   v4i fb[STEPS][NB][CT], fa[STEPS][MT];
-  const auto ask_b = [&](int k0) {                       // bytes past K are zeros
+  const auto within = [&](unsigned off, int k) {         // of the lane's chunk of the 64 bytes from k on; chunks past K are zeros
+    const int at = k + 16 * quad;
+    return at < K ? off + (ANY ? min(at, K - 16) : at) : OOB;
+  };
+  const auto ask_b = [&](int k0) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       const int k = k0 + 256 * s;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const unsigned off = k + 16 * quad < K ? offb[c] + k : OOB;
+        const unsigned off = within(offb[c], k);
         fb[s][0][c] = load(rb, off);
         if constexpr (GATED) fb[s][NB - 1][c] = load(rb2, off);
       }
@@ -413,18 +426,28 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
     for (int s = 0; s < STEPS; ++s) {
       const int k = k0 + 256 * s;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) fa[s][m] = load(ra, k + 16 * quad < K ? offa[m] + k : OOB);
+      for (int m = 0; m < MT; ++m) fa[s][m] = load(ra, within(offa[m], k));
     }
   };
   ask_b(64 * wave);                                      // before the rows' numbers are there
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) offa[m] = row[m] >= 0 ? (unsigned)(row[m] * g.lda + 16 * quad) : PAST;
+  for (int m = 0; m < MT; ++m) offa[m] = row[m] >= 0 ? (unsigned)(row[m] * g.lda) : PAST;
   int scale[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) scale[m] = !g.scale ? 1 : row[m] < 0 ? 0 : (int)g.scale[row[m]];
   for (int k0 = 64 * wave;;) {
     ask_a(k0);
+    if constexpr (ANY) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int k = k0 + 256 * s;
+        if (k < K && k + 64 > K) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) fa[s][m] = without_first(fa[s][m], k + 16 * quad - (K - 16));
+        }
+      }
+    }
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
@@ -467,7 +490,7 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
 }
 
 // Operands at any alignment and stride, and past 2^32 bytes: 64 x 64 tiles, chunks through registers into LDS, the next stage's on their
-// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 12.5 us (17
+// way while one is multiplied (more of them on their way: no faster). 3001 rows of 500, three of 11 experts each, to 333 columns: 12.5 us (17
 // with its results stored a byte at a time, 19.7 with one stage at a time as well).
 template <int OSZ, bool GATED>
 __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
@@ -489,25 +512,27 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   const int src = sr < tile.rows ? row_of(a, tile.p0 + sr, tile.n0 == 0 && sc == 0) : -1;
   const int8_t* arow = src < 0 ? nullptr : g.A + (long long)src * g.lda;
   const int n = tile.n0 + sr;
-  const int8_t* brow[NB];
+  const int8_t* brow[NB];                                // past the last column some other row: what it gives is not stored
 #pragma unroll
-  for (int b = 0; b < NB; ++b) brow[b] = n < g.N ? (b ? g.B2 : g.B) + tile.e * g.sb + (long long)n * g.ldb : nullptr;
+  for (int b = 0; b < NB; ++b) brow[b] = (b ? g.B2 : g.B) + tile.e * g.sb + (long long)min(n, g.N - 1) * g.ldb;
   const int K = g.K;
-  const auto chunk = [&](const int8_t* row, int k, bool tail) {
-    v4i v = {0, 0, 0, 0};
-    if (!row) return v;
-    if (tail) return row_chunk(row, k, K);
-    __builtin_memcpy(&v, row + k, 16);
-    return v;
-  };
   v4i av[PER], bv[NB][PER];
-  const auto ask = [&](int k) {
-    const bool tail = k + BK > K;
+  // K's last chunk is the rows' last 16 bytes, of which those that the chunk before has are zeros in A, as are chunks past K
+  const auto ask = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      av[i] = chunk(arow, k + 16 * (sc + 4 * i), tail);
+      const int k = k0 + 16 * (sc + 4 * i), at = min(k, K - 16);
+      av[i] = v4i{0, 0, 0, 0};
+      if (K >= 16) {
+        if (arow) __builtin_memcpy(&av[i], arow + at, 16);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) bv[b][i] = chunk(brow[b], k + 16 * (sc + 4 * i), tail);
+        for (int b = 0; b < NB; ++b) __builtin_memcpy(&bv[b][i], brow[b] + at, 16);
+        if (k0 + BK > K) av[i] = without_first(av[i], k - (K - 16));
+      } else {
+        if (arow) av[i] = row_chunk(arow, k, K);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) bv[b][i] = row_chunk(brow[b], k, K);
+      }
     }
   };
   v16i acc[NB];
@@ -620,19 +645,26 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
       else ANVIL_LAUNCH((expert_tile<BM, BN, BK, NS, OSZ, GATED, false>), dim3(wgs), dim3(256), 0, ctx->stream, a);
     });
   };
-  const auto few = [&](auto mt) {
-    by_type([&](auto osz, auto gated) {
-      constexpr int MT = decltype(mt)::value;
-      constexpr bool GATED = decltype(gated)::value;
-      constexpr int CT = GATED ? 1 : 2;
-      wgs = grid(16 * MT, 16 * CT);
-      if (wgs) ANVIL_LAUNCH((expert_few<MT, CT, decltype(osz)::value, GATED>), dim3(wgs), dim3(256), 0, ctx->stream, a);
-    });
+  using std::integral_constant;
+  const auto few = [&](auto any) {
+    const auto go = [&](auto mt) {
+      by_type([&](auto osz, auto gated) {
+        constexpr int MT = decltype(mt)::value;
+        constexpr bool GATED = decltype(gated)::value;
+        constexpr int CT = GATED ? 1 : 2;
+        wgs = grid(16 * MT, 16 * CT);
+        if (wgs) ANVIL_LAUNCH((expert_few<MT, CT, decltype(osz)::value, GATED, decltype(any)::value>), dim3(wgs), dim3(256), 0, ctx->stream, a);
+      });
+    };
+    if (g->rows <= 8ll * g->experts) go(integral_constant<int, 1>{});
+    else go(integral_constant<int, 2>{});
   };
-  if (aligned16(g->A) && aligned16(g->B) && aligned16(g->B2) && g->K % 16 == 0 && g->lda % 16 == 0 && g->ldb % 16 == 0 &&
-      (g->experts == 1 || g->sb % 16 == 0) && g->rows_a && a_bytes <= (long long)PAST && g->ldb < 1 << 23) {
-    a.a_bytes = (int)(unsigned)a_bytes;
-    using std::integral_constant;
+  const bool near = g->rows_a && g->K >= 16 && a_bytes <= (long long)PAST && g->ldb < 1 << 23;
+  const bool aligned = aligned16(g->A) && aligned16(g->B) && aligned16(g->B2) && g->K % 16 == 0 && g->lda % 16 == 0 && g->ldb % 16 == 0 &&
+                       (g->experts == 1 || g->sb % 16 == 0);
+  const long long width = (long long)g->N * (g->B2 ? 2 : 1);                           // of the operand B, and B2 beside it
+  a.a_bytes = near ? (int)(unsigned)a_bytes : 0;
+  if (near && aligned) {
     const integral_constant<int, 128> i128;
     const integral_constant<int, 64> i64;
     // Kernels by size, us on one box (rows x the experts of each):
@@ -642,16 +674,19 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
     //   128 x 256 / 64 x 128: 32768 x 2 of 8, gated 768 -> 2048, 261 / 411; 4096 x 2 of 8, the same, 46 / 55; 8192 x 2 of 16, 2048 -> 768, 41 / 46;
     //     but 4096 x 2 of 8, 768 -> 2048 (576 tiles), 35 / 30; 2048 x 2 of 8, gated 768 -> 2048 (640), 31 / 31: with few tiles the last round
     //     of them is half empty, and a short K has little to make up for it
-    const long long width = (long long)g->N * (g->B2 ? 2 : 1);                         // of the operand B, and B2 beside it
     const long long large = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((width + 255) / 256);
     if ((double)g->rows * (double)width * g->K <= 1 << 28) {
-      if (g->rows <= 8ll * g->experts) few(integral_constant<int, 1>{});
-      else few(integral_constant<int, 2>{});
+      few(std::false_type{});
     } else if (large >= (g->K >= 2048 ? 3 : 5) * ctx->num_cu / 2) {
       tiles(i128, integral_constant<int, 256>{}, i64, integral_constant<int, 3>{});
     } else {
       tiles(i64, i128, i128, integral_constant<int, 2>{});
     }
+  } else if (near && g->rows <= 64ll * g->experts && ((long long)g->rows / 64 + std::min(g->experts, g->rows)) * ((g->N + 63) / 64) < 3 * ctx->num_cu) {
+    // Rows at any alignment, us. Few rows / 64 x 64: 200 x 2 of 8, gated 700 -> 1001, 9.3 / 12.4; 64 x 4 of 16, 1001 -> 333, 7.0 / 8.9; 30 x 4 of 40, gated
+    // 1500 -> 1001, 25 / 32; but 40 x 4 of 100, 2001 -> 700 (1120 tiles of 64 x 64), 35 / 25.5; 600 x 2 of 8, gated 700 -> 1001 (150 rows an expert),
+    // 18.7 / 14.6: more rows read their weights again, and many tiles hide their stages' waits behind each other's.
+    few(std::true_type{});
   } else {
     wgs = grid(64, 64);
     if (wgs)

@@ -517,6 +517,16 @@ def test_products_by_tiles_of_128_rows(experts, N, K, kind, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("kind,dtype", FORMS)
+@pytest.mark.parametrize("K", [*range(16, 34), 47, 63, 65, 79, 127, 129, 1000, 1023, 1025, 1041, 2047, 4097])
+def test_products_of_odd_depths(K, kind, dtype):
+    """Every number of bytes that K's last two chunks share: few rows, tiles of 64 by 64, at any alignment."""
+    product_case([3, 0, 20, 1, 40], 37, K, kind, dtype=dtype, seed=K)
+    product_case([3, 0, 20, 1, 40], 37, K, kind, dtype=dtype, seed=K, off=5, pads=(1, 3, 2), gather=False, scaled=False, mults="one")
+    product_case([300, 5, 0, 130], 70, K, kind, dtype=dtype, seed=K, off=1)
+
+
+@gpu
 @pytest.mark.parametrize("kind", ["plain", "gated"])
 def test_product_strides_and_alignment(kind):
     for pads, off in (((16, 16, 16), 0), ((64, 0, 0), 16), ((0, 0, 0), 1), ((1, 0, 0), 0), ((0, 3, 0), 0), ((0, 0, 5), 0), ((0, 0, 0), 4)):
