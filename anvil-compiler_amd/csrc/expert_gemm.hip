@@ -646,6 +646,7 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
     });
   };
   using std::integral_constant;
+  const bool once = g->rows <= 8ll * g->experts;         // most experts have one tile of 16 rows and read their weights once
   const auto few = [&](auto any) {
     const auto go = [&](auto mt) {
       by_type([&](auto osz, auto gated) {
@@ -656,26 +657,30 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
         if (wgs) ANVIL_LAUNCH((expert_few<MT, CT, decltype(osz)::value, GATED, decltype(any)::value>), dim3(wgs), dim3(256), 0, ctx->stream, a);
       });
     };
-    if (g->rows <= 8ll * g->experts) go(integral_constant<int, 1>{});
+    if (once) go(integral_constant<int, 1>{});
     else go(integral_constant<int, 2>{});
   };
   const bool near = g->rows_a && g->K >= 16 && a_bytes <= (long long)PAST && g->ldb < 1 << 23;
   const bool aligned = aligned16(g->A) && aligned16(g->B) && aligned16(g->B2) && g->K % 16 == 0 && g->lda % 16 == 0 && g->ldb % 16 == 0 &&
                        (g->experts == 1 || g->sb % 16 == 0);
-  const long long width = (long long)g->N * (g->B2 ? 2 : 1);                           // of the operand B, and B2 beside it
   a.a_bytes = near ? (int)(unsigned)a_bytes : 0;
   if (near && aligned) {
     const integral_constant<int, 128> i128;
     const integral_constant<int, 64> i64;
-    // Kernels by size, us on one box (rows x the experts of each):
-    //   few rows / 64 x 128: 16 x 2 of 8 experts, 2048 -> 768, 6.0 / 10.3; 64 x 2 of 8, 2048 -> 768, 7.0 / 10.2; 16 x 4 of 32, gated
-    //     768 -> 1024, 11.4 / 12.1; 8192 of one, 768 -> 16, 4.9 / 6.5; but 64 x 2 of 8, gated 768 -> 2048, 9.7 / 7.5; 64 x 4 of 32, gated
-    //     768 -> 1024, 14.7 / 12.8: every 16 or 32 rows read their weights again
-    //   128 x 256 / 64 x 128: 32768 x 2 of 8, gated 768 -> 2048, 261 / 411; 4096 x 2 of 8, the same, 46 / 55; 8192 x 2 of 16, 2048 -> 768, 41 / 46;
-    //     but 4096 x 2 of 8, 768 -> 2048 (576 tiles), 35 / 30; 2048 x 2 of 8, gated 768 -> 2048 (640), 31 / 31: with few tiles the last round
+    // Kernels by size, us on one box (rows x the experts of each). Few rows / 64 x 128, by the few rows' workgroups (more than five a CU wait for each
+    // other; past half of that only where they read the weights once):
+    //   16 x 2 of 8, 2048 -> 768 (240), 6.0 / 10.3; 64 x 2 of 4, 4096 -> 1024 (256), 12.8 / 22; 200 x 2 of 8, 2048 -> 768 (480), 11.6 / 13.9; 2048 of one,
+    //     4096 -> 256 (520), 18.7 / 22.4; once: 16 x 2 of 8, 4096 -> 4096 (1280), 32 / 36; 2 of 8, gated 4096 -> 8192 (1024), 31 / 36
+    //   but 30000 of one, 768 -> 16 (938), 9.4 / 9.1; 4096 of one, 1024 -> 256 (1032), 11.2 / 7.9; 64 x 2 of 8, gated 768 -> 2048 (1536), 9.7 / 7.5; 16 x 4 of
+    //     32, gated 768 -> 1024 (2304), 12.3 / 11.5; 1000 x 2 of 8, 64 -> 1024 (2240), 12 / 6.3; 40 x 4 of 100, 1024 -> 1408 (4840), 24 / 20.5
+    // 128 x 256 / 64 x 128:
+    //   32768 x 2 of 8, gated 768 -> 2048, 261 / 411; 4096 x 2 of 8, the same, 46 / 55; 8192 x 2 of 16, 2048 -> 768, 41 / 46;
+    //   but 4096 x 2 of 8, 768 -> 2048 (576 tiles), 35 / 30; 2048 x 2 of 8, gated 768 -> 2048 (640), 31 / 31: with few tiles the last round
     //     of them is half empty, and a short K has little to make up for it
+    const long long shares = ((long long)g->rows / (once ? 16 : 32) + std::min(g->experts, g->rows)) * (g->B2 ? (g->N + 15) / 16 : (g->N + 31) / 32);
+    const long long width = (long long)g->N * (g->B2 ? 2 : 1);                         // of the operand B, and B2 beside it
     const long long large = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((width + 255) / 256);
-    if ((double)g->rows * (double)width * g->K <= 1 << 28) {
+    if (2 * shares <= (once ? 10 : 5) * ctx->num_cu) {
       few(std::false_type{});
     } else if (large >= (g->K >= 2048 ? 3 : 5) * ctx->num_cu / 2) {
       tiles(i128, integral_constant<int, 256>{}, i64, integral_constant<int, 3>{});

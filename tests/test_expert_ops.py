@@ -496,7 +496,7 @@ FORMS = [("plain", "i8"), ("plain", "i16"), ("table", "i8"), ("gated", "i8")]
 
 @gpu
 @pytest.mark.parametrize("kind,dtype", FORMS)
-@pytest.mark.parametrize("N,K", [(640, 1024), (700, 1040), (1001, 528), (1000, 16 * 41), (513, 2048), (5000, 128)])
+@pytest.mark.parametrize("N,K", [(640, 1024), (700, 1040), (1001, 528), (1000, 16 * 41), (513, 2048), (5000, 128), (960, 1024), (736, 2048), (1300, 384)])
 def test_products_by_tiles_of_64_rows(N, K, kind, dtype):
     counts = [130, 0, 61, 200, 64, 1, 150, 65, 63]
     product_case(counts, N, K, kind, dtype=dtype, seed=N)
@@ -548,7 +548,8 @@ def test_product_multipliers_and_shifts(mults):
 
 
 @gpu
-@pytest.mark.parametrize("rows,N,K", [(20, 64, 8192), (520, 256, 8192), (300, 70, 8190)], ids=["few", "tiles", "any"])
+@pytest.mark.parametrize("rows,N,K", [(20, 64, 8192), (520, 256, 8192), (300, 70, 8190), (700, 1500, 8192), (700, 1500, 8190)],
+                         ids=["few", "tiles", "any", "wide tiles", "wide, any"])
 @pytest.mark.parametrize("kind", ["table", "gated"])
 def test_tables_behind_the_largest_shifts(rows, N, K, kind):
     """Sums near 2^27 times multipliers near 2^31: results of a few units either way at shifts up to 58."""
