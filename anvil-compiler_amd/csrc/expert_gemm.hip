@@ -489,13 +489,14 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
   }
 }
 
-// Operands at any alignment and stride, and past 2^32 bytes: 64 x 64 tiles, chunks through registers into LDS, the next stage's on their
-// way while one is multiplied (more of them on their way: no faster). 3001 rows of 500, three of 11 experts each, to 333 columns: 12.5 us (17
-// with its results stored a byte at a time, 19.7 with one stage at a time as well).
-template <int OSZ, bool GATED>
+// Operands at any alignment and stride, and past 2^32 bytes: 64 TM x 64 tiles, chunks through registers into LDS, the next stage's on their
+// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 11.6 us (12.4 with 64 bytes of a row a load, for
+// which unaligned rows' lines are asked twice as often, 17 with results stored a byte at a time as well). One array of LDS and two barriers
+// a stage, for more workgroups a CU: 20000 x 2 rows of 700 to 1001, gated, 136 us, 150 with two arrays. More stages on their way: no faster.
+template <int TM, int OSZ, bool GATED>
 __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
-  constexpr int BM = 64, BN = 64, BK = 128, NB = GATED ? 2 : 1, PER = BK / 64;
-  __shared__ __attribute__((aligned(16))) int8_t As[2][BM * BK], Bs[2][NB][BN * BK];
+  constexpr int BM = 64 * TM, BN = 64, BK = 128, NB = GATED ? 2 : 1, PER = 2, PA = PER * TM;
+  __shared__ __attribute__((aligned(16))) int8_t As[BM * BK], Bs[NB][BN * BK];
   __shared__ int8_t lut_s[256];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = wave >> 1, wn = wave & 1, half = lane >> 5, l32 = lane & 31;
@@ -507,80 +508,101 @@ __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   if (GATED && !expert_mult(a, g.mults2, g.mult2, tile.e, t == 0, mult2)) return;
   if (g.lut) lut_s[t] = g.lut[t];
 
-  // thread t stages chunks t % 4, t % 4 + 4 of row t / 4 of each operand
-  const int sr = t >> 2, sc = t & 3;
-  const int src = sr < tile.rows ? row_of(a, tile.p0 + sr, tile.n0 == 0 && sc == 0) : -1;
-  const int8_t* arow = src < 0 ? nullptr : g.A + (long long)src * g.lda;
-  const int n = tile.n0 + sr;
-  const int8_t* brow[NB];                                // past the last column some other row: what it gives is not stored
+  // thread t stages chunk t % 8 of rows t / 8 and t / 8 + 32 of each operand: 128 bytes of a row an eighth of a wave
+  const int sr = t >> 3, sc = t & 7;
+  const int8_t *arow[PA], *brow[NB][PER];                // past the last column some other row: what it gives is not stored
 #pragma unroll
-  for (int b = 0; b < NB; ++b) brow[b] = (b ? g.B2 : g.B) + tile.e * g.sb + (long long)min(n, g.N - 1) * g.ldb;
+  for (int i = 0; i < PA; ++i) {
+    const int r = sr + 32 * i, src = r < tile.rows ? row_of(a, tile.p0 + r, tile.n0 == 0 && sc == 0) : -1;
+    arow[i] = src < 0 ? nullptr : g.A + (long long)src * g.lda;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) brow[b][i] = (b ? g.B2 : g.B) + tile.e * g.sb + (long long)min(tile.n0 + sr + 32 * i, g.N - 1) * g.ldb;
   const int K = g.K;
-  v4i av[PER], bv[NB][PER];
+  v4i av[PA], bv[NB][PER];
   // K's last chunk is the rows' last 16 bytes, of which those that the chunk before has are zeros in A, as are chunks past K
   const auto ask = [&](int k0) {
+    const int k = k0 + 16 * sc, at = min(k, K - 16);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int k = k0 + 16 * (sc + 4 * i), at = min(k, K - 16);
+    for (int i = 0; i < PA; ++i) {
       av[i] = v4i{0, 0, 0, 0};
-      if (K >= 16) {
-        if (arow) __builtin_memcpy(&av[i], arow + at, 16);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) __builtin_memcpy(&bv[b][i], brow[b] + at, 16);
-        if (k0 + BK > K) av[i] = without_first(av[i], k - (K - 16));
-      } else {
-        if (arow) av[i] = row_chunk(arow, k, K);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) bv[b][i] = row_chunk(brow[b], k, K);
+      if (arow[i]) {
+        if (K >= 16) __builtin_memcpy(&av[i], arow[i] + at, 16);
+        else av[i] = row_chunk(arow[i], k, K);
       }
     }
-  };
-  v16i acc[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = v16i{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  ask(0);
-  for (int k = 0, cur = 0; k < K; k += BK, cur ^= 1) {   // a wave is at most one barrier ahead, so two arrays do
+    for (int i = 0; i < PER; ++i)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int to = sr * BK + 16 * swz<BK>(sr, sc + 4 * i);
-      *reinterpret_cast<v4i*>(As[cur] + to) = av[i];
+      for (int b = 0; b < NB; ++b) {
+        if (K >= 16) __builtin_memcpy(&bv[b][i], brow[b][i] + at, 16);
+        else bv[b][i] = row_chunk(brow[b][i], k, K);
+      }
+    if (k0 + BK > K && K >= 16) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) *reinterpret_cast<v4i*>(Bs[cur][b] + to) = bv[b][i];
+      for (int i = 0; i < PA; ++i) av[i] = without_first(av[i], k - (K - 16));
     }
+  };
+  v16i acc[TM][NB];
+#pragma unroll
+  for (int j = 0; j < TM; ++j)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[j][b] = v16i{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  ask(0);
+  for (int k = 0; k < K; k += BK) {
+    if (k) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PA; ++i) *reinterpret_cast<v4i*>(As + (sr + 32 * i) * BK + 16 * swz<BK>(sr + 32 * i, sc)) = av[i];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) *reinterpret_cast<v4i*>(Bs[b] + (sr + 32 * i) * BK + 16 * swz<BK>(sr + 32 * i, sc)) = bv[b][i];
     __syncthreads();
     if (k + BK < K) ask(k + BK);
 #pragma unroll
     for (int ks = 0; ks < BK / 32; ++ks) {
-      const int ra = wm * 32 + l32, rb = wn * 32 + bperm(l32), ch = 2 * ks + half;
-      const v4i af = *reinterpret_cast<const v4i*>(As[cur] + ra * BK + 16 * swz<BK>(ra, ch));
+      const int rb = wn * 32 + bperm(l32), ch = 2 * ks + half;
+      v4i af[TM];
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const int ra = wm * 32 * TM + 32 * j + l32;
+        af[j] = *reinterpret_cast<const v4i*>(As + ra * BK + 16 * swz<BK>(ra, ch));
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const v4i bf = *reinterpret_cast<const v4i*>(Bs[cur][b] + rb * BK + 16 * swz<BK>(rb, ch));
-        acc[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf, af, acc[b], 0, 0, 0);
+        const v4i bf = *reinterpret_cast<const v4i*>(Bs[b] + rb * BK + 16 * swz<BK>(rb, ch));
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[j][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf, af[j], acc[j][b], 0, 0, 0);
       }
     }
   }
-  const int m = wm * 32 + l32, n0 = tile.n0 + wn * 32 + 16 * half;       // this lane's row and its 16 columns
-  if (m >= tile.rows) return;
-  const int i = row_of(a, tile.p0 + m, false);
-  const int scale = g.scale ? (i < 0 ? 0 : (int)g.scale[i]) : 1;
+  const int n0 = tile.n0 + wn * 32 + 16 * half;          // this lane's 16 columns
   const int lo = OSZ == 1 ? -128 : -32768;
   const WideRequant q1(g.shift, lo, -lo - 1), q2(g.shift2, -128, 127);
   const auto of = [](const WideRequant& q, int acc, int mul) { return q.high() ? q.of<true>(acc, mul) : q.of<false>(acc, mul); };
   const int rnd3 = (int)round_term(g.shift3);
-  int v[16];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    v[e] = of(q1, acc[0][e], mult * scale);
-    if (g.lut) v[e] = lut_s[(v[e] + 128) & 255];
-    if constexpr (GATED) v[e] = min(max((v[e] * of(q2, acc[NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
+  for (int j = 0; j < TM; ++j) {
+    const int m = wm * 32 * TM + 32 * j + l32;
+    if (m >= tile.rows) continue;
+    const int i = row_of(a, tile.p0 + m, false);
+    const int scale = g.scale ? (i < 0 ? 0 : (int)g.scale[i]) : 1;
+    int v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      v[e] = of(q1, acc[j][0][e], mult * scale);
+      if (g.lut) v[e] = lut_s[(v[e] + 128) & 255];
+      if constexpr (GATED) v[e] = min(max((v[e] * of(q2, acc[j][NB - 1][e], mult2 * scale) * g.mult3 + rnd3) >> g.shift3, -128), 127);
+    }
+    unsigned w[4 * OSZ];
+#pragma unroll
+    for (int q = 0; q < 4 * OSZ; ++q)
+      w[q] = OSZ == 1 ? pack4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3])
+                      : __builtin_amdgcn_perm((unsigned)v[2 * q + 1], (unsigned)v[2 * q], 0x05040100u);
+    store_n<16, OSZ>(g, tile.p0 + m, n0, w);
   }
-  unsigned w[4 * OSZ];
-#pragma unroll
-  for (int q = 0; q < 4 * OSZ; ++q)
-    w[q] = OSZ == 1 ? pack4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3])
-                    : __builtin_amdgcn_perm((unsigned)v[2 * q + 1], (unsigned)v[2 * q], 0x05040100u);
-  store_n<16, OSZ>(g, tile.p0 + m, n0, w);
 }
 
 }  // namespace anvil
@@ -693,11 +715,18 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
     // 18.7 / 14.6: more rows read their weights again, and many tiles hide their stages' waits behind each other's.
     few(std::true_type{});
   } else {
-    wgs = grid(64, 64);
-    if (wgs)
-      by_type([&](auto osz, auto gated) {
-        ANVIL_LAUNCH((expert_any<decltype(osz)::value, decltype(gated)::value>), dim3(wgs), dim3(256), 0, ctx->stream, a);
-      });
+    const auto go = [&](auto tm) {
+      wgs = grid(64 * decltype(tm)::value, 64);
+      if (wgs)
+        by_type([&](auto osz, auto gated) {
+          ANVIL_LAUNCH((expert_any<decltype(tm)::value, decltype(osz)::value, decltype(gated)::value>), dim3(wgs), dim3(256), 0, ctx->stream, a);
+        });
+    };
+    // 128 rows / 64, us: 20000 x 2 of 8, gated 700 -> 1001, 121 / 133; 6000 x 2 of 16, 1501 -> 1501, 83 / 97; but 2000 x 2 of 8, 700 -> 1001 (624 tiles of
+    // 128), 16.2 / 15.7; 300 x 4 of 100, 2001 -> 700, 51 / 43
+    const long long tall = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((g->N + 63) / 64);
+    if (tall >= 8 * ctx->num_cu && g->rows >= 128ll * g->experts) go(integral_constant<int, 2>{});
+    else go(integral_constant<int, 1>{});
   }
   if (!wgs) return set_error(ANVIL_E_VALUE, "%s: %d rows of %d columns are more tiles than a grid has", who, g->rows, g->N);
   ANVIL_LAUNCHED();

@@ -489,8 +489,8 @@ def test_product_depths(K):
         product_case([1, 3, 2], 40, K, kind, seed=K)
 
 
-# Sizes that leave the few-rows kernel (rows x N x K above 2^28) for 64 x 128 tiles, and (at least 640 tiles of 128 x 256, or 384 with a K of
-# 2048 or more on 256 CUs) for those.
+# Sizes that leave the few-rows kernel (640 workgroups, or 1280 where rows are at most 8 an expert) for 64 x 128 tiles, and (at least 640 tiles of
+# 128 x 256, or 384 with a K of 2048 or more) for those, on 256 CUs.
 FORMS = [("plain", "i8"), ("plain", "i16"), ("table", "i8"), ("gated", "i8")]
 
 
@@ -524,6 +524,15 @@ def test_products_of_odd_depths(K, kind, dtype):
     product_case([3, 0, 20, 1, 40], 37, K, kind, dtype=dtype, seed=K)
     product_case([3, 0, 20, 1, 40], 37, K, kind, dtype=dtype, seed=K, off=5, pads=(1, 3, 2), gather=False, scaled=False, mults="one")
     product_case([300, 5, 0, 130], 70, K, kind, dtype=dtype, seed=K, off=1)
+
+
+@gpu
+@pytest.mark.parametrize("kind,dtype", FORMS)
+@pytest.mark.parametrize("N,K", [(1400, 33), (1401, 129), (1409, 150)])
+def test_products_of_many_rows_at_any_alignment(N, K, kind, dtype):
+    """At least 2048 tiles of 128 x 64 (8 a CU)."""
+    product_case([4000, 0, 129, 127, 128, 5900, 1, 2000], N, K, kind, dtype=dtype, seed=K)
+    product_case([6000, 3, 6200], N, K, kind, dtype=dtype, seed=N, off=3, pads=(1, 0, 5), scaled=False, gather=False)
 
 
 @gpu
