@@ -15,7 +15,8 @@
 namespace anvil {
 
 // Rows of a workgroup, at least, and workgroups, at most: each reads the counts of all. 4096 rows over 8 (two each), 64
-// (six) and 256 experts (eight) take 9.6, 9.6 and 12.8 us with 32 rows, 11.0, 13.0 and 20.4 with 128.
+// (six) and 256 experts (eight) take 9.6, 9.6 and 12.8 us with 32 rows, 11.0, 13.0 and 20.4 with 128. 32768 rows
+// over 64: 14.4 us by 256 workgroups, 20.4 by 128, 24.8 by 512.
 constexpr int ROUTE_ROWS = 32, ROUTE_BLOCKS = 256;
 // Rows that one workgroup routes and sorts by itself: 64 rows over 8, 64 and 256 experts take it 5.8, 6.7 and 9.7 us, 128 rows 6.8, 8.6 and
 // 14.2; two launches take 128 rows in 8.9, 8.9 and 9.9.
