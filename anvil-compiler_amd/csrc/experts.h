@@ -34,9 +34,10 @@ struct WideRequant {
   __device__ __forceinline__ int of(int acc, int m) const { return unshifted<HI>(acc, m) >> rest; }
 };
 
-// (m, s) with s moved up to 33 where m keeps within int32: the same products and roundings
+// (m, s) with s moved up to 33 where m keeps within int32: the same products and roundings. From below 2 only m = 0 would keep, and the product
+// here leaves 64 bits (-2^31 from 0).
 __host__ __device__ inline void lift_shift(int& m, int& s) {
-  if (s >= 33) return;
+  if (s >= 33 || s < 2) return;
   const long long w = (long long)m * (1ll << (33 - s));
   if (w < I32_MIN || w > I32_MAX) return;
   m = (int)w;
