@@ -54,8 +54,7 @@ __device__ __forceinline__ int scale_of(const anvil_add_norm& n, unsigned a, uns
 // changes.
 // m comes from single precision and remainders. d is exact there, the hardware's reciprocal off by at most 2^-23 of it and every other
 // step by 2^-24; taken 2^-21 smaller, the first quotient is too small by at most 11 / 2^24 of itself, 2817 units and a fraction, and the second,
-// of what remains, leaves less than 2 d. (With a division in doubles instead some quotients came out units short on the device now
-// and then, when many waves shared a SIMD: codes at exact halves then fell to the next lower one.)
+// of what remains, leaves less than 2 d.
 struct Divider {
   unsigned m;
   int sh;                                                // of the product's upper word
