@@ -298,6 +298,9 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
       for (; j + 4 <= c.top; j += 4) add(j, std::integral_constant<int, 4>{});
       if (c.top & 2) add(j, std::integral_constant<int, 2>{}), j += 2;
       if (c.top & 1) add(j, std::integral_constant<int, 1>{});
+    } else {                                             // no row to read, so a slot adds nothing and only -1 is none
+      for (int j = 0; j < c.top; ++j)
+        if (slot[j] != -1) raise_flag(g.flags, FLAG_EXPERTS);
     }
     const auto finish = [&](auto hi_c) {
 #pragma unroll

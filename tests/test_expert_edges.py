@@ -74,3 +74,28 @@ def test_products_at_the_ends_of_the_multiplier(counts, N, K, kind, dtype):
                             mult3=13, shift3=9)
             dev.sync()
             out.expect(want, f"{mult} >> {shift}")
+
+
+# ----------------------------------------------------------------------------------- numbers out of their range
+
+@gpu
+@pytest.mark.parametrize("cols", [15, 16, 17, 64])
+@pytest.mark.parametrize("R", [None, "i16"])
+def test_slots_of_no_positions_are_reported(cols, R):
+    """Y has no rows: a slot of -1 is none, every other one is out of range, adds nothing and is reported."""
+    dev, rng = device(), np.random.default_rng(cols)
+    res = None if R is None else rng.integers(-3000, 3000, (9, cols))
+    want = np.zeros((9, cols), int) if R is None else oe.rq(res * 256, 1, 8)
+    dR, out = None if R is None else Rows(dev, res, R), Rows(dev, np.ones((9, cols), int), R or "i8")
+    dw = flat(dev, np.full((9, 5), 7), "i16")
+    for at, bad in ((None, -1), (0, 0), (44, -2), (22, 2 ** 31 - 1), (7, -(2 ** 31))):
+        slot = np.full(45, -1)
+        if at is not None:
+            slot[at] = bad
+        ds = flat(dev, slot, "i32")
+        dev.expert_combine(None, cols, 0, ds.ptr, dw.ptr, 9, 5, cols, 3, 4, dR and dR.ptr, R or "i8", cols, 256, 9, 8, out.ptr, R or "i8", cols)
+        if at is not None:
+            with pytest.raises(ValueError, match="slot"):
+                dev.sync()
+        dev.sync()
+        out.expect(want, f"slot {bad}")
