@@ -298,9 +298,6 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
       for (; j + 4 <= c.top; j += 4) add(j, std::integral_constant<int, 4>{});
       if (c.top & 2) add(j, std::integral_constant<int, 2>{}), j += 2;
       if (c.top & 1) add(j, std::integral_constant<int, 1>{});
-    } else {                                             // no row to read, so a slot adds nothing and only -1 is none
-      for (int j = 0; j < c.top; ++j)
-        if (slot[j] != -1) raise_flag(g.flags, FLAG_EXPERTS);
     }
     const auto finish = [&](auto hi_c) {
 #pragma unroll
@@ -336,6 +333,14 @@ __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {
       }
     }
   }
+}
+
+// Slots of a Y without rows, which combine_rows does not look at: every one but -1 is out of range. (Looked at there, they cost it four registers and
+// with them a wave a SIMD.)
+__global__ __launch_bounds__(256) void report_slots(CombineArgs g) {
+  const long long n = (long long)g.c.rows * g.c.top;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256)
+    if (g.c.slot[i] != -1) raise_flag(g.flags, FLAG_EXPERTS);
 }
 
 // One element a thread: rows of fewer than 16 columns, multipliers of more than 24 bits.
@@ -472,6 +477,10 @@ extern "C" int anvil_expert_combine_i8(anvil_ctx* ctx, const anvil_expert_combin
     const bool aligned = c->cols % 16 == 0 && even(c->Y, c->ldy, 1) && even(c->D, c->ldd, c->d_dtype) && (!c->R || even(c->R, c->ldr, c->r_dtype));
     const long long threads = (long long)c->rows * ((c->cols + 15) / 16);
     const dim3 grid((unsigned)std::min<long long>((threads + 255) / 256, 1 << 20));
+    if (!c->positions) {
+      ANVIL_LAUNCH(report_slots, dim3((unsigned)std::min<long long>((pairs + 255) / 256, 1 << 16)), dim3(256), 0, ctx->stream, g);
+      ANVIL_LAUNCHED();
+    }
     const auto run = [&](auto rsz, auto dsz) {
       constexpr int RSZ = decltype(rsz)::value, DSZ = decltype(dsz)::value;
       if (aligned) ANVIL_LAUNCH((combine_rows<RSZ, DSZ, false>), grid, dim3(256), 0, ctx->stream, g);
