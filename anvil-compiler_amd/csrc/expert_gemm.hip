@@ -15,8 +15,8 @@ constexpr long long GRID_MAX = (1ll << 24) - 8;          // workgroups of 256: a
 struct ExpertArgs {
   anvil_expert_gemm g;
   int tiles_n;
+  unsigned tiles;                                        // at most: of row tiles that `rows` rows of ascending starts can have
   int a_bytes;                                           // of A, as a buffer descriptor takes them: below 2^32
-
   unsigned* flags;
 };
 
@@ -36,7 +36,8 @@ __device__ __forceinline__ int expert_rows(const ExpertArgs& a, int e, bool repo
   return 0;
 }
 
-// Tile number `w` of a grid of row tiles of BM x column tiles of BN; false past the last.
+// Tile number `w` of a grid of row tiles of BM x column tiles of BN; false past the last. Starts that decrease (expert_rows reports them) may count
+// positions again; where that gives more tiles than the grid was made for there is none at all, rather than those that it reaches.
 template <int BM, int BN>
 __device__ __forceinline__ bool find_tile(const ExpertArgs& a, int w, int lane, ExpertTile& t) {
   const int E = a.g.experts;
@@ -45,10 +46,11 @@ __device__ __forceinline__ bool find_tile(const ExpertArgs& a, int w, int lane, 
     n = e0 + lane < E ? expert_rows(a, e0 + lane, w == 0, lo) : 0;
     mt += (n + BM - 1) / BM;
   }
-  if (__ballot(mt > (int)GRID_MAX)) return false;        // starts that decrease may count positions again, past what the sums hold
+  if (__ballot(mt > (int)GRID_MAX)) return false;        // past what the sums hold
   int incl = wave_scan(mt);
   const int tiles_m = __builtin_amdgcn_readlane(incl, 63);
-  const unsigned tiles = (unsigned)tiles_m * (unsigned)a.tiles_n;        // at most the grid
+  if ((unsigned long long)tiles_m * (unsigned)a.tiles_n > a.tiles) return false;
+  const unsigned tiles = (unsigned)tiles_m * (unsigned)a.tiles_n;
   const unsigned per = (tiles + 7) / 8, pid = (w & 7) * per + (w >> 3);
   if ((unsigned)(w >> 3) >= per || pid >= tiles) return false;
   const unsigned in_group = GROUP_M * a.tiles_n;
@@ -642,11 +644,12 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
   for (const Span& s : in)
     if (!apart(c, s)) return set_error(ANVIL_E_VALUE, "%s: the result overlaps what is read", who);
   if (int e = check_ctx(ctx)) return e;
-  ExpertArgs a{*g, 0, 0, ctx->flags};
+  ExpertArgs a{*g, 0, 0, 0, ctx->flags};
   const auto grid = [&](int bm, int cols) -> unsigned {   // 0: more tiles than a grid has
     a.tiles_n = (g->N + cols - 1) / cols;
     const long long tiles = ((long long)g->rows / bm + std::min(g->experts, g->rows)) * a.tiles_n;
-    return tiles > GRID_MAX ? 0 : (unsigned)((tiles + 7) / 8 * 8);
+    a.tiles = tiles > GRID_MAX ? 0 : (unsigned)tiles;
+    return (a.tiles + 7) / 8 * 8;
   };
   const auto by_type = [&](auto&& f) {
     if (g->B2) f(std::integral_constant<int, 1>{}, std::true_type{});

@@ -580,7 +580,8 @@ int anvil_expert_route_i8(anvil_ctx* ctx, const anvil_route* r);
  * acc2 and m2 from B2 and mults2 / mult2. shift, shift2 in [0, 62], shift3 in [0, 31]; 2^14 |mult3| + 2^(shift3-1) < 2^31 and, with scale,
  * |mult| and |mult2| at most 32767, else ANVIL_E_OVERFLOW (an entry of mults or mults2 that is not, with scale, is reported by anvil_sync as
  * ANVIL_E_VALUE, and its expert's rows are not written). A start or row outside its range is reported likewise: its expert's rows
- * are not written, its position's product is that of zeros. B2 has B's strides. N at most 2^20, K at most 2^16, experts at
+ * are not written, its position's product is that of zeros. Starts that decrease are reported too; positions that two experts then share
+ * hold either one's results, and where the experts' rows come to more tiles than `rows` positions can have nothing is written. B2 has B's strides. N at most 2^20, K at most 2^16, experts at
  * most ANVIL_EXPERTS_MAX.
  * With one expert, starts {0, rows} and row NULL this is the product of rows with scales of their own. */
 typedef struct anvil_expert_gemm {

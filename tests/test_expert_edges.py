@@ -99,3 +99,90 @@ def test_slots_of_no_positions_are_reported(cols, R):
                 dev.sync()
         dev.sync()
         out.expect(want, f"slot {bad}")
+
+
+def _products(starts, rows, N, K, kind, call, seed=0, experts_mult=None, unaligned=False, oracle=True):
+    """(result before, the oracle's rows of each expert alone, the device's result) of a product whose starts need not ascend; call(dev, args) runs it."""
+    dev, rng, E = device(), np.random.default_rng(seed), len(starts) - 1
+    A, B = rng.integers(-128, 128, (rows, K)), rng.integers(-128, 128, (2, E, N, K), dtype=np.int8)
+    scale, mults, shift = rng.integers(1000, 32768, rows), rng.integers(200, 900, E), 31
+    lut = None if kind == "plain" else act_lut()
+    before, alone = rng.integers(-100, 100, (rows, N)), {}
+    for e in range(E):
+        lo, hi = starts[e], starts[e + 1]
+        if oracle and 0 <= lo <= hi <= rows:
+            one = slice(e, e + 1)
+            alone[e] = oe.gemm(np.zeros((rows, N)), A, None, scale, B[0][one], B[1][one] if kind == "gated" else None, [lo, hi], mults[one], shift,
+                               mults[one], shift, lut, 13, 9, "i8")[lo:hi]
+    pad = 1 if unaligned else 0
+    dA, dB, dB2 = Rows(dev, A, "i8", pad), *(Rows(dev, b.reshape(-1, K), "i8", pad) for b in B)
+    out, ds, dt, dl = Rows(dev, before, "i8", 5), flat(dev, scale, "i16"), flat(dev, starts, "i32"), flat(dev, act_lut(), "i8")
+    given = mults if experts_mult is None else experts_mult(mults)
+    dm, dm2 = flat(dev, given, "i32"), flat(dev, mults, "i32")
+    call(dev, dict(A=dA.ptr, lda=dA.ld, rows_a=rows, row=None, scale=ds.ptr, B=dB.ptr, B2=dB2.ptr if kind == "gated" else None, ldb=dB.ld, sb=N * dB.ld,
+                   starts=dt.ptr, experts=E, rows=rows, N=N, K=K, Cp=out.ptr, ldc=out.ld, out_dtype="i8", mults=dm.ptr, mults2=dm2.ptr,
+                   shift=shift, shift2=shift, lut=None if lut is None else dl.ptr, mult3=13, shift3=9))
+    return before, alone, out
+
+
+def _reported(dev, args):
+    dev.expert_gemm(**args)
+    with pytest.raises(ValueError, match="expert"):
+        dev.sync()
+    dev.sync()
+
+
+def _either(starts, before, alone, out):
+    """Each element is that of an expert whose rows are there, or what it was; nothing around the rows is written."""
+    got, count = out.get(), np.zeros(len(before), int)
+    right = np.zeros(before.shape, bool)
+    for e, v in alone.items():
+        at = slice(starts[e], starts[e + 1])
+        count[at] += 1
+        right[at] |= got[at] == v
+    right[count == 0] = got[count == 0] == before[count == 0]
+    assert right.all(), np.argwhere(~right)[:5]
+    out.expect(got, "around the rows")
+    return count
+
+
+# columns, depth, alignment: few rows, tiles of 64 x 128, tiles of 64 x 64 at any alignment
+FORMS = [(64, 64, False), (1024, 1024, False), (1000, 1001, True)]
+
+
+@gpu
+@pytest.mark.parametrize("N,K,unaligned", FORMS, ids=["few", "tiles", "any"])
+@pytest.mark.parametrize("kind", ["plain", "gated"])
+@pytest.mark.parametrize("starts,rows", [([0, 5, 3, 9], 9), ([0, 4, 8, 99], 9), ([-1, 4, 8, 9], 9), ([0, 10, 10, 10], 9), ([0, 100, 90, 100], 100),
+                                         ([0, 300, 300, 200, 500, 2 ** 31 - 1, 500], 500), ([-(2 ** 31), 0, 40, 30, 64], 64)], ids=str)
+def test_starts_out_of_range_write_what_the_other_experts_have(starts, rows, N, K, unaligned, kind):
+    before, alone, out = _products(starts, rows, N, K, kind, _reported, unaligned=unaligned)
+    count = _either(starts, before, alone, out)
+    assert len(alone) < len(starts) - 1 and (count.max() == 2) == (starts in ([0, 5, 3, 9], [0, 100, 90, 100], [0, 300, 300, 200, 500, 2 ** 31 - 1, 500],
+                                                                              [-(2 ** 31), 0, 40, 30, 64]))
+
+
+@gpu
+@pytest.mark.parametrize("N,K,unaligned", FORMS, ids=["few", "tiles", "any"])
+@pytest.mark.parametrize("experts", [3, 9, 129, 1023])
+def test_starts_that_count_more_tiles_than_a_call_has_write_nothing(experts, N, K, unaligned):
+    """Up and down again: half of the experts have all rows each. 1100 rows are 17 to 35 whole tiles, and one more an expert at most."""
+    rows = 1100
+    starts = [0 if e % 2 == 0 else rows for e in range(experts + 1)]
+    N, K = (N, K) if experts < 100 else (N // 4, K // 4)
+    before, _, out = _products(starts, rows, N, K, "plain", _reported, unaligned=unaligned, oracle=False)
+    out.expect(before)
+
+
+@gpu
+@pytest.mark.parametrize("N,K,unaligned", FORMS, ids=["few", "tiles", "any"])
+@pytest.mark.parametrize("kind", ["plain", "gated"])
+@pytest.mark.parametrize("bad", [32768, -32768, 2 ** 31 - 1, -(2 ** 31)])
+def test_multipliers_out_of_range_leave_their_experts_rows(bad, N, K, unaligned, kind):
+    starts = [0, 30, 93, 100, 190]
+    before, alone, out = _products(starts, 200, N, K, kind, _reported, unaligned=unaligned, experts_mult=lambda m: np.where(np.arange(4) == 1, bad, m))
+    want = before.copy()
+    for e, v in alone.items():
+        if e != 1:
+            want[starts[e]:starts[e + 1]] = v
+    out.expect(want)
