@@ -76,6 +76,32 @@ def test_products_at_the_ends_of_the_multiplier(counts, N, K, kind, dtype):
             out.expect(want, f"{mult} >> {shift}")
 
 
+# ------------------------------------------------------------------------------------------- the router's weights
+
+def test_shares_by_a_reciprocal_in_single_precision():
+    """The router's (e one + S / 2) / S as its kernel takes it: num and S rounded to single precision, the hardware's reciprocal with its last unit
+    off either way, their product cut off, one step by the remainder. The quotient before that step is off by at most 4 roundings of 2^-23 of
+    at most 32767.5, 1/64, so it is the right one or next to it. Sums up to 2^41 (1024 experts of 2^31 - 1), and quotients at whole numbers."""
+    rng, f, n = np.random.default_rng(5), np.float32, 400000
+    one = np.where(rng.random(n) < 0.5, 32767, rng.integers(1, 32768, n))
+    S = np.maximum(1, (2.0 ** rng.uniform(0, 41, n)).astype(np.int64) + rng.integers(-2, 3, n))
+    S[:200] = np.r_[np.arange(1, 101), (1 << 41) - np.arange(1024, 1124)]
+    most = np.minimum(S, (1 << 31) - 1)
+    e = (rng.random(n) * (most + 1)).astype(np.int64)
+    near = np.clip((rng.integers(0, 1 << 15, n) % (one + 1) * S - S // 2) // one + rng.integers(-1, 2, n), 0, most)     # e one + S / 2 at a multiple of S
+    e = np.where(rng.random(n) < 0.6, near, np.where(rng.random(n) < 0.1, most, e))
+    num = e * one + S // 2
+    assert num.max() < 1 << 47
+    for off in (-1, 0, 1):
+        r = ((f(1) / S.astype(f)).view(np.int32) + np.int32(off)).view(f)
+        q = (num.astype(f) * r).astype(np.int64)
+        assert np.abs(q - num // S).max() <= 1
+        left = num - q * S
+        q += np.where(left < 0, -1, np.where(left >= S, 1, 0))
+        assert np.array_equal(q, num // S) and q.max() <= 32767
+    assert (num % S == 0).sum() > 1000 and (num % S == S - 1).sum() > 1000
+
+
 # ----------------------------------------------------------------------------------- numbers out of their range
 
 @gpu
