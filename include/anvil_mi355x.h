@@ -553,8 +553,9 @@ int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n);
  * in 64 bits. A row with live[row] = 0 (live NULL: none; padding of a batch) has experts -1, weights 0 and slots -1. The pairs
  * (row, expert) sorted by expert, rows in order: expert e has positions starts[e] .. starts[e + 1] - 1, position p is row
  * row[p], and slot[row][j] is the position of the row's j-th expert. Entries of `row` from starts[experts] on stay as they
- * were. Calls of many rows count in the context's workspace (the first one allocates it). lut: int32[256], entries below 0
- * count as 0; a live row whose S is 0 has weights 0, and ANVIL_E_ZERODIV is reported.
+ * were. Calls of more than 64 rows count in the context's workspace, as do calls of fewer whose counts are more than 60 KiB (of 1024
+ * experts from 13 rows on); the first one allocates it. lut: int32[256], entries below 0 count as 0; a live row whose S is 0
+ * has weights 0, and ANVIL_E_ZERODIV is reported.
  * 1 <= top <= 32, top <= experts <= 1024, rows * top < 2^30, 1 <= one <= 32767. */
 enum { ANVIL_ROUTE_EVERY = 1, ANVIL_EXPERTS_MAX = 1024, ANVIL_ROUTE_TOP_MAX = 32 };
 typedef struct anvil_route {
