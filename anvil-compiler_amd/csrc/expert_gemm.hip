@@ -185,19 +185,17 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
   constexpr int T = 256, NW = 4, WGN = 2, CPR = BK / 16, KS = BK / 32;
   constexpr int WM = BM / (NW / WGN), WN = BN / WGN, TM = WM / 32, TN = WN / 32;
   constexpr int COLS = GATED ? BN / 2 : BN;              // columns of the result
-  static_assert(TM >= 1 && TN >= (GATED ? 2 : 1) && (!GATED || TN % 2 == 0) && NS >= 2 && NS <= 4, "wave tile and stages");
+  static_assert(TM >= 1 && TN >= (GATED ? 2 : 1) && (!GATED || TN % 2 == 0) && NS >= 2 && NS <= 3, "wave tile and stages");
   constexpr int JA = BM * CPR / T, JB = BN * CPR / T, G = JA + JB;       // a wave's loads per stage
   static_assert(JA * T == BM * CPR && JB * T == BN * CPR && (NS - 2) * G < 64, "whole loads");
   constexpr int STAGE = (BM + BN) * BK;
-  __shared__ __attribute__((aligned(1024))) int8_t L0[STAGE], L1[STAGE];
-  __shared__ __attribute__((aligned(1024))) int8_t L2[NS > 2 ? STAGE : 16], L3[NS > 3 ? STAGE : 16];
+  __shared__ __attribute__((aligned(1024))) int8_t L0[STAGE], L1[STAGE], L2[NS > 2 ? STAGE : 16];
   __shared__ __attribute__((aligned(2048))) int8_t lut_s[256];            // before the stages, where a read's own offset reaches it
   auto arr = [&](auto u) -> int8_t* {                    // the array of stage u, known at compile time
     constexpr int U = decltype(u)::value % NS;
     if constexpr (U == 0) return L0;
     else if constexpr (U == 1) return L1;
-    else if constexpr (U == 2) return L2;
-    else return L3;
+    else return L2;
   };
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wm = wave / WGN, wn = wave % WGN;
@@ -332,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void expert_tile(ExpertArgs a) {
     if (++kt == nk) break;                                                                                 \
   }
   for (int kt = 0;;) {
-    ANVIL_EXPERT_STEP(0) ANVIL_EXPERT_STEP(1) ANVIL_EXPERT_STEP(2) ANVIL_EXPERT_STEP(3)
+    ANVIL_EXPERT_STEP(0) ANVIL_EXPERT_STEP(1) ANVIL_EXPERT_STEP(2)
   }
 #undef ANVIL_EXPERT_STEP
 
