@@ -15,7 +15,7 @@ constexpr long long GRID_MAX = (1ll << 24) - 8;          // workgroups of 256: a
 struct ExpertArgs {
   anvil_expert_gemm g;
   int tiles_n;
-  unsigned tiles;                                        // at most: of row tiles that `rows` rows of ascending starts can have
+  int tiles_m;                                           // as many as `rows` rows of ascending starts can have
   int a_bytes;                                           // of A, as a buffer descriptor takes them: below 2^32
   unsigned* flags;
 };
@@ -49,7 +49,7 @@ __device__ __forceinline__ bool find_tile(const ExpertArgs& a, int w, int lane, 
   if (__ballot(mt > (int)GRID_MAX)) return false;        // past what the sums hold
   int incl = wave_scan(mt);
   const int tiles_m = __builtin_amdgcn_readlane(incl, 63);
-  if ((unsigned long long)tiles_m * (unsigned)a.tiles_n > a.tiles) return false;
+  if (tiles_m > a.tiles_m) return false;
   const unsigned tiles = (unsigned)tiles_m * (unsigned)a.tiles_n;
   const unsigned per = (tiles + 7) / 8, pid = (w & 7) * per + (w >> 3);
   if ((unsigned)(w >> 3) >= per || pid >= tiles) return false;
@@ -645,9 +645,9 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
   ExpertArgs a{*g, 0, 0, 0, ctx->flags};
   const auto grid = [&](int bm, int cols) -> unsigned {   // 0: more tiles than a grid has
     a.tiles_n = (g->N + cols - 1) / cols;
-    const long long tiles = ((long long)g->rows / bm + std::min(g->experts, g->rows)) * a.tiles_n;
-    a.tiles = tiles > GRID_MAX ? 0 : (unsigned)tiles;
-    return (a.tiles + 7) / 8 * 8;
+    a.tiles_m = g->rows / bm + std::min(g->experts, g->rows);
+    const long long tiles = (long long)a.tiles_m * a.tiles_n;
+    return tiles > GRID_MAX ? 0 : (unsigned)((tiles + 7) / 8 * 8);
   };
   const auto by_type = [&](auto&& f) {
     if (g->B2) f(std::integral_constant<int, 1>{}, std::true_type{});
