@@ -1,4 +1,5 @@
-"""The check of the built device code for 64-bit shifts by a kernel's last vector register, and the norm whose codes such a shift once made wrong."""
+"""The check of the built device code for 64-bit shifts by a kernel's last vector register, the norm whose codes such a shift once made wrong, and
+other quotients at whole numbers, where a unit too little shows, in calls that keep every SIMD busy."""
 import subprocess
 
 import numpy as np
@@ -6,8 +7,10 @@ import pytest
 
 from anvil_mi355x import device_code
 from anvil_mi355x.build import ARCH, LIB
+from anvil_mi355x import runtime as rt
 from expert_cases import device, flat, roots
 from oracle import experts as oe
+from oracle import semantics as sem
 
 
 def _planted(tmp_path, kernels):
@@ -64,3 +67,37 @@ def test_codes_at_exact_halves_of_many_rows(cols, y):
         dev.sync()
         assert np.array_equal(dh.download((rows, cols), np.int8), want)
         assert np.array_equal(ds.download((rows,), np.int16), np.tile(scale.astype(np.int16), turns)[:rows])
+
+
+def _halves(rows, rng):
+    """Rows of 64 scores (a largest, m, once) and a factor: with the table g (127 - 2 (255 - d)) every e 127 + S // 2 is a multiple of S. The
+    odd numbers 127 and 63 others that add up to 127 give S = 254 g."""
+    odd = np.ones((rows, 63), int)
+    np.add.at(odd, (np.repeat(np.arange(rows), 32), rng.integers(0, 63, 32 * rows)), 2)
+    m = rng.integers(-60, 128, (rows, 1))
+    scores = np.concatenate([m, m - (127 - odd) // 2], axis=1)
+    return np.take_along_axis(scores, rng.permuted(np.tile(np.arange(64), (rows, 1)), axis=1), 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [1, 3, 1001, 77777, 132104])
+def test_probabilities_at_whole_numbers_of_many_rows(g):
+    """softmax_lut by itself, into int8 and int32, and fused: with K and V unit matrices and no rounding between, the attention's result is the
+    probabilities."""
+    dev, rng, heads = device(), np.random.default_rng(g), 2048
+    x = _halves(64 * heads, rng)
+    lut = g * np.maximum(0, 127 - 2 * (255 - np.arange(256)))
+    want = sem.softmax_lut(x, lut, 127, False)
+    e = lut[x - x.max(1, keepdims=True) + 255]
+    assert ((e * 127 + 127 * g) % (254 * g) == 0).all() and np.array_equal(want, (e // g + 1) // 2)
+    dx, dl, unit = dev.upload(x.astype(np.int8)), dev.upload(lut.astype(np.int32)), dev.upload(np.tile(np.eye(64, dtype=np.int8), (heads, 1)))
+    for _ in range(3):
+        for dtype, np_type, flags in (("i8", np.int8, rt.OP_UNCHECKED), ("i32", np.int32, rt.OP_UNCHECKED), ("i8", np.int8, 0)):
+            out = dev.alloc(x.size * np.dtype(np_type).itemsize)
+            dev.softmax_lut(dx, dl, 127, False, heads, 64, 64, out, dtype, flags)
+            dev.sync()
+            assert np.array_equal(out.download(x.shape, np_type), want), (dtype, flags)
+        out = dev.alloc(x.size)
+        dev.attention_i8(dx, unit, unit, out, heads, 1, 64, 64, [4096, 0, 64] * 4, 1, 0, dl, 127, False, 1, 0, rt.OP_UNCHECKED)
+        dev.sync()
+        assert np.array_equal(out.download(x.shape, np.int8), want)
