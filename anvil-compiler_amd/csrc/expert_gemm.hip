@@ -171,13 +171,13 @@ __device__ __forceinline__ void* uniform_ptr(const void* p) {
 // One workgroup of 2 x 2 waves a BM x BN tile, operands 16-byte aligned, K in stages of BK bytes, NS of them in LDS and NS - 1 on their way.
 //
 // 128 x 256 tiles (waves of 64 x 128, three stages of 64 bytes, two workgroups a CU): 65536 gated positions of 768 to 2048 columns, 412 GOP,
-// 271 to 295 us as clocks go, 1.4 to 1.5 POPS; 65536 of 2048 to 768, 206 GOP, 126 to 134 us. At 267 and 126 us it took 181 and 80 without its
+// 270 to 275 us in a row of calls, 1.5 POPS (ten from rest 296, as clocks go); 65536 of 2048 to 768, 206 GOP, 132 to 134. On a box where these were 267 and 126 it took 181 and 80 without its
 // loads, 205 and 102 without its matrix instructions, 220 and 111 without its epilogue (239 and 118 without the epilogue's stores): loads
-// from L2 cost most, 2.4 GB in lines of which a stage takes half. The epilogue is eleven instructions a gated result (with fifteen 298 us
-// against 293). 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
+// from L2 cost most, 2.4 GB in lines of which a stage takes half. The epilogue is eleven instructions a gated result (with fifteen the
+// call took 2 % longer). 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
 // workgroup's products run beside their epilogue (283 and 136 where a workgroup walks its tiles and the next one's first stages load
 // under the results; 128 x 256 tiles walked that way 298 and 130); 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
-// (KFULL): selecting an offset past K for each load instead 261 against 257 us.
+// (KFULL): selecting an offset past K for each load instead took 2 % longer.
 // KFULL: K is a whole number of stages, so a load's offset is its lane's own and the stage's, which lies within the descriptor's bytes (the range
 // check subtracts it from them); stages past K have empty descriptors and no offset.
 template <int BM, int BN, int BK, int NS, int OSZ, bool GATED, bool KFULL>
@@ -490,9 +490,10 @@ __global__ __launch_bounds__(256) void expert_few(ExpertArgs a) {
 }
 
 // Operands at any alignment and stride, and past 2^32 bytes: 64 TM x 64 tiles, chunks through registers into LDS, the next stage's on their
-// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 11.6 us (12.4 with 64 bytes of a row a load, for
+// way while one is multiplied. 3001 rows of 500, three of 11 experts each, to 333 columns: 11.3 us (12.4 with 64 bytes of a row a load, for
 // which unaligned rows' lines are asked twice as often, 17 with results stored a byte at a time as well). One array of LDS and two barriers
-// a stage, for more workgroups a CU: 20000 x 2 rows of 700 to 1001, gated, 136 us, 150 with two arrays. More stages on their way: no faster.
+// a stage, for more workgroups a CU: 20000 x 2 rows of 700 to 1001, gated, by 64 x 64 tiles 133 us (150 with two arrays), by 128 x 64 122. More
+// stages on their way: no faster.
 template <int TM, int OSZ, bool GATED>
 __global__ __launch_bounds__(256) void expert_any(ExpertArgs a) {
   constexpr int BM = 64 * TM, BN = 64, BK = 128, NB = GATED ? 2 : 1, PER = 2, PA = PER * TM;
@@ -692,14 +693,15 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
     const integral_constant<int, 64> i64;
     // Kernels by size, us on one box (rows x the experts of each). Few rows / 64 x 128, by the few rows' workgroups (more than five a CU wait for each
     // other; past half of that only where they read the weights once):
-    //   16 x 2 of 8, 2048 -> 768 (240), 6.0 / 10.3; 64 x 2 of 4, 4096 -> 1024 (256), 12.8 / 22; 200 x 2 of 8, 2048 -> 768 (480), 11.6 / 13.9; 2048 of one,
-    //     4096 -> 256 (520), 18.7 / 22.4; once: 16 x 2 of 8, 4096 -> 4096 (1280), 32 / 36; 2 of 8, gated 4096 -> 8192 (1024), 31 / 36
-    //   but 30000 of one, 768 -> 16 (938), 9.4 / 9.1; 4096 of one, 1024 -> 256 (1032), 11.2 / 7.9; 64 x 2 of 8, gated 768 -> 2048 (1536), 9.7 / 7.5; 16 x 4 of
-    //     32, gated 768 -> 1024 (2304), 12.3 / 11.5; 1000 x 2 of 8, 64 -> 1024 (2240), 12 / 6.3; 40 x 4 of 100, 1024 -> 1408 (4840), 24 / 20.5
+    //   16 x 2 of 8, 2048 -> 768 (240), 6.9 / 14; 64 x 2 of 4, 4096 -> 1024 (256), 13.0 / 22.5; 200 x 2 of 8, 2048 -> 768 (480), 11.6 / 14; 2048 of one,
+    //     4096 -> 256 (520), 18.8 / 22.7; once: 16 x 2 of 8, 4096 -> 4096 (1280), 33 / 36; 2 x 2 of 8, gated 4096 -> 8192 (1024), 48 / 57
+    //   but 30000 of one, 768 -> 16 (938), 9.4 / 9.2; 4096 of one, 1024 -> 256 (1032), 11.4 / 7.9; 64 x 2 of 8, gated 768 -> 2048 (1536), 11.2 / 9.6; 16 x 4 of
+    //     32, gated 768 -> 1024 (2304), 12.3 / 11.6; 1000 x 2 of 8, 64 -> 1024 (2240), 12.1 / 6.4; 40 x 4 of 100, 1024 -> 1408 (4840), 24 / 20.5
     // 128 x 256 / 64 x 128:
-    //   32768 x 2 of 8, gated 768 -> 2048, 261 / 411; 4096 x 2 of 8, the same, 46 / 55; 8192 x 2 of 16, 2048 -> 768, 41 / 46;
-    //   but 4096 x 2 of 8, 768 -> 2048 (576 tiles), 35 / 30; 2048 x 2 of 8, gated 768 -> 2048 (640), 31 / 31: with few tiles the last round
-    //     of them is half empty, and a short K has little to make up for it
+    //   32768 x 2 of 8, gated 768 -> 2048, 271 / 382; 32768 x 2 of 8, 2048 -> 768, 133 / 161; 4096 x 2 of 8, gated 768 -> 2048, 46 / 55; 8192 x 2 of 16,
+    //     2048 -> 768, 41 / 47; 2048 x 2 of 8, gated 768 -> 2048 (640 tiles), 29 / 31;
+    //   but 4096 x 2 of 8, 768 -> 2048 (576), 34 / 30: with few tiles the last round of them is half empty, and a short K has little to make up
+    //     for it
     const long long shares = ((long long)g->rows / (once ? 16 : 32) + std::min(g->experts, g->rows)) * (g->B2 ? (g->N + 15) / 16 : (g->N + 31) / 32);
     const long long width = (long long)g->N * (g->B2 ? 2 : 1);                         // of the operand B, and B2 beside it
     const long long large = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((width + 255) / 256);
@@ -711,9 +713,9 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
       tiles(i64, i128, i128, integral_constant<int, 2>{});
     }
   } else if (near && g->rows <= 64ll * g->experts && ((long long)g->rows / 64 + std::min(g->experts, g->rows)) * ((g->N + 63) / 64) < 3 * ctx->num_cu) {
-    // Rows at any alignment, us. Few rows / 64 x 64: 200 x 2 of 8, gated 700 -> 1001, 9.3 / 12.4; 64 x 4 of 16, 1001 -> 333, 7.0 / 8.9; 30 x 4 of 40, gated
-    // 1500 -> 1001, 25 / 32; but 40 x 4 of 100, 2001 -> 700 (1120 tiles of 64 x 64), 35 / 25.5; 600 x 2 of 8, gated 700 -> 1001 (150 rows an expert),
-    // 18.7 / 14.6: more rows read their weights again, and many tiles hide their stages' waits behind each other's.
+    // Rows at any alignment, us. Few rows / 64 x 64: 200 x 2 of 8, gated 700 -> 1001, 9.5 / 11.8; 64 x 4 of 16, 1001 -> 333, 7.3 / 9.0; 30 x 4 of 40, gated
+    // 1500 -> 1001, 26 / 28; but 40 x 4 of 100, 2001 -> 700 (1120 tiles of 64 x 64), 35 / 24.5; 600 x 2 of 8, gated 700 -> 1001 (150 rows an expert),
+    // 18.7 / 13.2: more rows read their weights again, and many tiles hide their stages' waits behind each other's.
     few(std::true_type{});
   } else {
     const auto go = [&](auto tm) {
@@ -723,8 +725,8 @@ extern "C" int anvil_expert_gemm_i8(anvil_ctx* ctx, const anvil_expert_gemm* g) 
           ANVIL_LAUNCH((expert_any<decltype(tm)::value, decltype(osz)::value, decltype(gated)::value>), dim3(wgs), dim3(256), 0, ctx->stream, a);
         });
     };
-    // 128 rows / 64, us: 20000 x 2 of 8, gated 700 -> 1001, 121 / 133; 6000 x 2 of 16, 1501 -> 1501, 83 / 97; but 2000 x 2 of 8, 700 -> 1001 (624 tiles of
-    // 128), 16.2 / 15.7; 300 x 4 of 100, 2001 -> 700, 51 / 43
+    // 128 rows / 64, us: 20000 x 2 of 8, gated 700 -> 1001, 122 / 133; 6000 x 2 of 16, 1501 -> 1501, 84 / 96; but 300 x 4 of 100, 2001 -> 700, 51 / 44; 3001 x
+    // 3 of 11, 500 -> 333, 12.1 / 11.3. Between them little is lost either way: 2000 x 2 of 8, gated 700 -> 1001 (624 tiles of 128), 23.1 / 24.5
     const long long tall = ((long long)g->rows / 128 + std::min(g->experts, g->rows)) * ((g->N + 63) / 64);
     if (tall >= 8 * ctx->num_cu && g->rows >= 128ll * g->experts) go(integral_constant<int, 2>{});
     else go(integral_constant<int, 1>{});

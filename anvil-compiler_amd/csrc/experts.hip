@@ -6,7 +6,7 @@
 // Sorting. Workgroups count their rows' pairs by expert; the rows of counts meet in a second launch, where every workgroup adds up all of
 // them and those before its own, and places its pairs. Within a workgroup the waves own runs of consecutive pairs, and a pair's
 // rank among the 64 of a step is the number of lower lanes with its expert (ballots over the bits of its number). Atomics add counts, none
-// decides an order: positions are the same each time. 32749 rows, six of 64 experts each: 7.3 + 7.5 us for 5 MB, chains of reductions and of
+// decides an order: positions are the same each time. 32749 rows, six of 64 experts each: 7.2 + 8.0 us for 5 MB, chains of reductions and of
 // waits for counts, not bandwidth.
 #include <algorithm>
 
@@ -247,10 +247,10 @@ struct CombineArgs {
 // Sixteen columns a thread, operands 16-byte aligned: a row's slots and weights first, then up to four of its results at a time. A slot
 // that adds nothing reads row 0 with weight 0, so no load waits for a branch. RSZ, DSZ: bytes of R's (0: none) and D's elements.
 // What bounds it is memory: top + 4 bytes an element (an i16 residual and result), two instructions a result's element and nine more.
-// 32768 rows of 768, two results each: 30.8 us, 4.9 TB/s (with types told apart at run time and a branch a result 37.1, eight columns a thread
-// so 40, an element a thread 147); int8 residual and result 21.8 (31.0), none 15.5 (19.6).
+// 32768 rows of 768, two results each: 30.7 us, 4.9 TB/s (with types told apart at run time and a branch a result 37.1, eight columns a thread
+// so 40, an element a thread 147); int8 residual and result 21.0 (31.0), none 15.7 (19.6).
 // ANY: rows at any alignment and of any width from 16 columns on. A row's last thread then takes its last 16 columns and stores those that no
-// other thread has, so it reads no byte past the row, and in place what it has read of another's columns is dropped. 32768 rows of 769: 33.7 us
+// other thread has, so it reads no byte past the row, and in place what it has read of another's columns is dropped. 32768 rows of 769: 33.3 us
 // (an element a thread 166).
 template <int RSZ, int DSZ, bool ANY>
 __global__ __launch_bounds__(256) void combine_rows(CombineArgs g) {

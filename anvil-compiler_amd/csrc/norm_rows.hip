@@ -114,7 +114,7 @@ struct NormTypes {
 // Rows of at most 8 L R columns, 16-byte aligned, in registers: L lanes a row (64 / L rows a wave, or the workgroup's 256), R chunks of
 // eight elements a lane, and a lane has the same columns of every row it takes, so its weights stay in registers.
 //
-// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 30.5 us, 4.95
+// What bounds it is memory: 6 bytes an element (an i16 stream and an i8 addend), some 22 instructions. 32768 x 768: 30.4 us, 4.97
 // TB/s, a copy's rate (one workgroup a row, each row read twice: 149). 32 lanes of three chunks for 768 columns: 64 would leave a quarter of
 // them idle in the second chunk, 16 hold six chunks each and leave room for few waves.
 //
@@ -123,7 +123,7 @@ struct NormTypes {
 // straight into the code's byte give it exactly.
 //
 // ANY: rows at any alignment and of any width from eight columns on. The last chunk is the row's last eight columns, of which those that the
-// chunk before has count as zeros and are not stored. 32768 x 769: 43 us (a workgroup a row that reads it twice 167).
+// chunk before has count as zeros and are not stored. 32768 x 769: 41 us (a workgroup a row that reads it twice 167).
 template <int L, int R, typename T, bool ANY>
 __global__ __launch_bounds__(256) void add_norm_rows(NormArgs g) {
   const anvil_add_norm& n = g.n;
@@ -367,8 +367,8 @@ extern "C" int anvil_add_norm_i8(anvil_ctx* ctx, const anvil_add_norm* n) {
       ANVIL_LAUNCH((add_norm_rows<L, R, decltype(types), decltype(any)::value>), dim3((unsigned)std::min((n->rows + rows - 1) / rows, 64 * ctx->num_cu)), dim3(256), 0,
                    ctx->stream, g);
     };
-    // Streams of one type, alone or with an int8 addend, have kernels of their own: 32768 rows of 768 (i16 and i8) 32.6 us, 34.5 with types
-    // told apart at run time; 8192 of 4096 37.8 and 44.7 (40.0 with workgroups for eight a CU that walk over the rows).
+    // Streams of one type, alone or with an int8 addend, have kernels of their own: 32768 rows of 768 (i16 and i8) 30.4 us, 32.4 with types
+    // told apart at run time; 8192 of 4096 37.5 and 41.0 (40.0 with workgroups for eight a CU that walk over the rows).
     const auto go = [&](auto lanes, auto per) {
       const bool same = n->r_dtype == n->x_dtype;
       const std::false_type whole;
