@@ -8,6 +8,7 @@ import pytest
 
 from expert_cases import Rows, act_lut, device, flat
 from oracle import experts as oe
+from test_expert_ops import route_case
 
 gpu = pytest.mark.gpu
 CSRC = Path(__file__).resolve().parents[1] / "anvil-compiler_amd" / "csrc"
@@ -100,6 +101,16 @@ def test_shares_by_a_reciprocal_in_single_precision():
         q += np.where(left < 0, -1, np.where(left >= S, 1, 0))
         assert np.array_equal(q, num // S) and q.max() <= 32767
     assert (num % S == 0).sum() > 1000 and (num % S == S - 1).sum() > 1000
+
+
+@gpu
+@pytest.mark.parametrize("experts", [896, 960, 1000, 1024])
+def test_route_where_one_workgroup_no_longer_holds_the_counts(experts):
+    """A row of counts a wave and two more, and the pairs, in 60 KiB: up to 12 rows of 1024 experts, 13 of 960, 13 of 1000 with one choice each and
+    12 with 32, 15 and 14 of 896."""
+    for rows in range(11, 18):
+        for top in (1, 32):
+            route_case(rows, experts, top, seed=rows, live=0.9, pad=1)
 
 
 # ----------------------------------------------------------------------------------- numbers out of their range
