@@ -171,13 +171,13 @@ __device__ __forceinline__ void* uniform_ptr(const void* p) {
 // One workgroup of 2 x 2 waves a BM x BN tile, operands 16-byte aligned, K in stages of BK bytes, NS of them in LDS and NS - 1 on their way.
 //
 // 128 x 256 tiles (waves of 64 x 128, three stages of 64 bytes, two workgroups a CU): 65536 gated positions of 768 to 2048 columns, 412 GOP,
-// 270 to 275 us in a row of calls, 1.5 POPS (ten from rest 296, as clocks go); 65536 of 2048 to 768, 206 GOP, 132 to 134. On a card where these were 267 and 126 it took 181 and 80 without its
-// loads, 205 and 102 without its matrix instructions, 220 and 111 without its epilogue (239 and 118 without the epilogue's stores): loads
-// from L2 cost most, 2.4 GB in lines of which a stage takes half. The epilogue is eleven instructions a gated result (with fifteen the
-// call took 2 % longer). 256 x 256 tiles of eight waves, one workgroup a CU, load a third less and take 300 and 133 us, as no other
-// workgroup's products run beside their epilogue (283 and 136 where a workgroup walks its tiles and the next one's first stages load
-// under the results; 128 x 256 tiles walked that way 298 and 130); 128 x 128 tiles 316 and 138. A load's offset is one register and the stage's scalar
-// (KFULL): selecting an offset past K for each load instead took 2 % longer.
+// 270 to 275 us in a row of calls, 1.5 POPS (ten from rest 296, as clocks go); 65536 of 2048 to 768, 206 GOP, 132 to 134. On a card where these
+// were 267 and 126 it took 181 and 80 without its loads, 205 and 102 without its matrix instructions, 220 and 111 without its epilogue (239 and
+// 118 without the epilogue's stores): loads from L2 cost most, 2.4 GB in lines of which a stage takes half. The epilogue is eleven
+// instructions a gated result (with fifteen the call took 2 % longer). 256 x 256 tiles of eight waves, one workgroup a CU, load a third less
+// and take 300 and 133 us, as no other workgroup's products run beside their epilogue (283 and 136 where a workgroup walks its tiles and the
+// next one's first stages load under the results; 128 x 256 tiles walked that way 298 and 130); 128 x 128 tiles 316 and 138. A load's offset
+// is one register and the stage's scalar (KFULL): selecting an offset past K for each load instead took 2 % longer.
 // KFULL: K is a whole number of stages, so a load's offset is its lane's own and the stage's, which lies within the descriptor's bytes (the range
 // check subtracts it from them); stages past K have empty descriptors and no offset.
 template <int BM, int BN, int BK, int NS, int OSZ, bool GATED, bool KFULL>
